@@ -27,6 +27,8 @@ typedef void* viola_stream_t; /* hipStream_t */
 
 enum { VIOLA_F32 = 0, VIOLA_BF16 = 1, VIOLA_F16 = 2, VIOLA_E4M3 = 3, VIOLA_E5M2 = 4 };
 enum { VIOLA_SILU = 0, VIOLA_GELU = 1, VIOLA_RELU = 2 };
+enum { VIOLA_NORM_NONE = 0, VIOLA_NORM_RMS = 1, VIOLA_NORM_LAYER = 2 };
+enum { VIOLA_SOFTMAX = 0, VIOLA_SIGMOID = 1 };
 enum { VIOLA_NEAREST = 0, VIOLA_STOCHASTIC = 1 };
 /* group scales: FP32 values, or E8M0 bytes (power-of-two scale 2^(byte - 127), the `native` / mxfp8 recipe) */
 enum { VIOLA_SCALE_F32 = 0, VIOLA_SCALE_E8M0 = 1 };
@@ -496,6 +498,66 @@ int viola_comm_unpack_table(const int64_t* table, int64_t buckets, int64_t max_e
 /* dst[0 .. count) on the device = host_words, carried in kernel arguments (no staging buffer; host_words may be reused at
  * once). For tables of a few hundred words: offsets of variable groups. */
 int viola_store_words(int64_t* dst, const int64_t* host_words, int64_t count, viola_stream_t stream);
+/* ---------------------------------------------------------------- norms around a block
+ * No counterpart in the reference. The norm that a block reads, and the norm, gate and residual sum of what it gives:
+ *   out = residual_scale x + branch_scale gate (n(y) after_weight + after_bias)      (n(y) = y with after = VIOLA_NORM_NONE)
+ *   h   = (n(out) weight + bias) (1 + scale) + shift
+ * with n(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps) over a row (VIOLA_NORM_LAYER) or the same without the mean (VIOLA_NORM_RMS).
+ * Three forms: y and out null: h from x alone; h null and before = VIOLA_NORM_NONE: out alone; both, where h is computed from out before out is
+ * rounded. x and out: [rows, cols] of x_dtype; y and h of branch_dtype; rows of x and y `pitch` elements apart, out and h contiguous.
+ * after_weight .. bias: [cols] of weight_dtype. gate, scale, shift: [cols] of vector_dtype (pitch 0), or one such vector for each group of
+ * group_rows rows, `pitch` elements apart. Null: ones, or zeros for biases, scale and shift. stats (16-byte aligned; null: not wanted):
+ * float[rows][4] for the backward pass.
+ *
+ * Backward: dout of x_dtype, dh and dy of branch_dtype, dx of x_dtype, all contiguous; a null dout is zeros, a null output is not wanted.
+ * A call without dh (then before = VIOLA_NORM_NONE) is that of the form without h. Gradients of the vectors: [cols], or [groups][cols] where
+ * the vector has a pitch, of the vector's type. parts: viola_norm_portions(rows, group_rows) * 4 * cols floats (fewer where fewer of the gradients are
+ * wanted). Sums over rows are added in an order of their own that does not change from call to call. */
+int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols,
+                       int after, const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
+                       const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch,
+                       int vector_dtype, int64_t group_rows, float residual_scale, float branch_scale, float eps, void* out, void* h, float* stats,
+                       viola_stream_t stream);
+int64_t viola_norm_portions(int64_t rows, int64_t group_rows);
+int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols,
+                        int after, const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
+                        const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch,
+                        int vector_dtype, int64_t group_rows, float residual_scale, float branch_scale, const float* stats, const void* dout,
+                        const void* dh, void* dx, void* dy, float* parts, int64_t parts_floats, void* d_after_weight, void* d_after_bias,
+                        void* d_weight, void* d_bias, void* d_gate, void* d_scale, void* d_shift, viola_stream_t stream);
+
+/* ---------------------------------------------------------------- routing of a mixture of experts
+ * No counterpart in the reference. viola_route_forward: of logits [tokens, experts] (rows `pitch` apart, f32 / bf16 / f16) the top_k largest of
+ * each row (ties to the lowest index, NaN above all numbers, -inf never), their gates under score VIOLA_SOFTMAX or VIOLA_SIGMOID (normalize: over the chosen;
+ * all times scale), the place of each choice among all in the order of experts and then of tokens, the counts of the experts, offsets [experts + 1]
+ * (where each expert's places begin), and the balance loss: the mean over sequences of `sequence` tokens of
+ * experts * sum_e (choices of e / (tokens top_k)) (mean probability of e). chosen, positions, gates: [tokens, top_k]; a choice that is not there is
+ * -1, -1 and a gate of 0. mask (null: all): 0 for a token that is left out, of choices, counts and loss. cost: float[tokens / sequence][experts],
+ * stats: float[tokens][2] (8-byte aligned), both for the backward pass (stats null: not wanted). workspace: viola_route_workspace words of 4 bytes. experts <= 1024,
+ * top_k <= 32 (VIOLA_EUNSUPPORTED beyond).
+ * viola_balance_forward: loss and counts for choices made elsewhere (int32, or int64 with chosen_wide; indices out of range count nowhere).
+ * viola_route_backward: dlogits [tokens, experts], contiguous, of the logits' type from the gates' and / or the loss's gradient (null: none). */
+int64_t viola_route_workspace(int64_t tokens, int64_t experts, int64_t sequence);
+int viola_route_forward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
+                        const uint8_t* mask, int64_t sequence, int32_t* chosen, float* gates, int32_t* positions, int32_t* counts, int32_t* offsets,
+                        float* loss, float* cost, float* stats, int32_t* workspace, int64_t workspace_words, viola_stream_t stream);
+int viola_balance_forward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, const uint8_t* mask,
+                          int64_t sequence, const void* chosen, int chosen_wide, int32_t* counts, float* loss, float* cost, float* stats,
+                          int32_t* workspace, int64_t workspace_words, viola_stream_t stream);
+int viola_route_backward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
+                         int64_t sequence, const int32_t* chosen, const float* cost, const float* stats, const float* dgates, const float* dloss,
+                         void* dlogits, viola_stream_t stream);
+
+/* Rows of tokens to the experts and back (f32 / bf16 / f16, sums in f32). positions [tokens, top_k]: a row, or negative for none; no row twice.
+ * viola_rows_gather: out[t] = sum_j gates[t, j] rows[positions[t, j]] (gates null: ones), out [tokens, cols] contiguous.
+ * viola_rows_scatter: rows[positions[t, j]] = gates[t, j] x[t], rows [row_count, cols] contiguous, and zeros in the rows from *total (on the device) on;
+ * dots (null: not wanted): dots[t, j] = sum_c x[t, c] values[positions[t, j], c]. rows may be null when only dots are wanted.
+ * Positions of row_count and beyond are read as none. */
+int viola_rows_gather(const void* rows, int64_t pitch, int64_t row_count, int dtype, int64_t cols, const int32_t* positions, const float* gates, int64_t tokens,
+                      int top_k, void* out, viola_stream_t stream);
+int viola_rows_scatter(const void* x, int64_t pitch, int dtype, int64_t cols, const int32_t* positions, const float* gates, int64_t tokens, int top_k,
+                       const int32_t* total, void* rows, int64_t row_count, const void* values, int64_t values_pitch, float* dots, viola_stream_t stream);
+
 /* ---------------------------------------------------------------- self checks (test support)
  * Compare the hardware FP8 conversion instructions with the software codecs over every fp32 bit
  * pattern of magnitude <= the format's clamp range (encode) and all 256 codes (decode); writes

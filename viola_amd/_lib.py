@@ -17,6 +17,8 @@ F32, BF16, F16, E4M3, E5M2 = range(5)
 DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
          torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
 ACTIVATION = {"silu": 0, "gelu": 1, "relu": 2}
+NORM = {None: 0, "rms": 1, "layer": 2}
+SCORE = {"softmax": 0, "sigmoid": 1}
 ROUNDING = {"nearest": 0, "stochastic": 1}
 LIBRARY = Path(__file__).resolve().parent / "csrc" / "libviola_hip.so"
 
@@ -81,11 +83,18 @@ _SIGNATURES = {
     "viola_comm_pack_table": [_p, _l, _l, _i, _i, _p],
     "viola_comm_unpack_table": [_p, _l, _l, _i, _i, _i, _p],
     "viola_store_words": [_p, _p, _l, _p],
+    "viola_norm_forward": [_p, _l, _i, _p, _l, _i, _l, _l, _i, _p, _p, _i, _p, _p, _i, _p, _l, _p, _l, _p, _l, _i, _l, _f, _f, _f, _p, _p, _p, _p],
+    "viola_norm_backward": [_p, _l, _i, _p, _l, _i, _l, _l, _i, _p, _p, _i, _p, _p, _i, _p, _l, _p, _l, _p, _l, _i, _l, _f, _f, _p, _p, _p, _p, _p, _p, _l, _p, _p, _p, _p, _p, _p, _p, _p],
+    "viola_route_forward": [_p, _l, _i, _l, _l, _i, _i, _i, _f, _p, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p, _l, _p],
+    "viola_balance_forward": [_p, _l, _i, _l, _l, _i, _i, _p, _l, _p, _i, _p, _p, _p, _p, _p, _l, _p],
+    "viola_route_backward": [_p, _l, _i, _l, _l, _i, _i, _i, _f, _l, _p, _p, _p, _p, _p, _p, _p],
+    "viola_rows_gather": [_p, _l, _l, _i, _l, _p, _p, _l, _i, _p, _p],
+    "viola_rows_scatter": [_p, _l, _i, _l, _p, _p, _l, _i, _p, _p, _l, _p, _l, _p, _p],
     "viola_selftest_fp8": [_p, _p],
     "viola_selftest_philox": [_p, _p, _l, _p],
 }
 EXPORTS = tuple(_SIGNATURES) + ("viola_abi_version", "viola_error_string", "viola_ns_plan", "viola_ns_plan_many", "viola_tensor_encode_slices", "viola_group_gemm_parts",
-                                "viola_group_gemm_form", "viola_scaled_gemm_form")
+                                "viola_group_gemm_form", "viola_scaled_gemm_form", "viola_norm_portions", "viola_route_workspace")
 
 _lib = None
 
@@ -107,6 +116,8 @@ def library():
         lib.viola_group_gemm_parts.argtypes, lib.viola_group_gemm_parts.restype = [_l, _l, _l], ctypes.c_int
         lib.viola_group_gemm_form.argtypes, lib.viola_group_gemm_form.restype = [_l, _l, _l, _i, _i, _i], ctypes.c_int
         lib.viola_scaled_gemm_form.argtypes, lib.viola_scaled_gemm_form.restype = [_l, _l, _l], ctypes.c_int
+        lib.viola_norm_portions.argtypes, lib.viola_norm_portions.restype = [_l, _l], ctypes.c_int64
+        lib.viola_route_workspace.argtypes, lib.viola_route_workspace.restype = [_l, _l, _l], ctypes.c_int64
         lib.viola_ns_plan.argtypes, lib.viola_ns_plan.restype = [_l, _l, _l, _l, _i, _i, _i, ctypes.POINTER(ctypes.c_int)], ctypes.c_int
         lib.viola_ns_plan_many.argtypes, lib.viola_ns_plan_many.restype = [_p, _i, ctypes.POINTER(ctypes.c_int)], ctypes.c_int
         assert lib.viola_abi_version() == 1

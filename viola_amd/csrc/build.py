@@ -19,7 +19,8 @@ ARCH = "gfx950"
 # scale with an explicit fmaf.
 COMMON = ["-O3", f"--offload-arch={ARCH}", "-fPIC", "-std=c++17", "-ffp-contract=off", "-fno-fast-math",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-command-line-argument"]
-SOURCES = ["gemm_generic.hip", "gemm_fast.hip", "gemm_fast_mx.hip", "gemm_fast_tensor.hip", "gemm_pingpong_grouped.hip", "gemm_pingpong_mx.hip", "gemm_pingpong_tensor.hip", "gemm.hip", "gemm_skinny.hip", "quantize.hip", "ns.hip", "ns_fast.hip", "optim.hip", "misc.hip", "tensor.hip"]
+SOURCES = ["gemm_generic.hip", "gemm_fast.hip", "gemm_fast_mx.hip", "gemm_fast_tensor.hip", "gemm_pingpong_grouped.hip", "gemm_pingpong_mx.hip", "gemm_pingpong_tensor.hip", "gemm.hip", "gemm_skinny.hip", "quantize.hip", "ns.hip", "ns_fast.hip", "optim.hip", "misc.hip", "tensor.hip",
+           "norm.hip", "route.hip", "rows.hip"]
 
 
 def hipcc():
@@ -33,7 +34,7 @@ def _filter(text):
     return "\n".join(line for line in text.splitlines() if "is not a recognized feature for this target" not in line)
 
 
-HOST_SOURCES = ["host.cpp", "host_optim.cpp"]
+HOST_SOURCES = ["host.cpp", "host_optim.cpp", "host_blocks.cpp"]
 
 
 def _host_flags():

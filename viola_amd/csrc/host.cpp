@@ -16,7 +16,6 @@
 #include "host.hpp"
 
 #include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/saved_variable.h>
 
 using namespace viola_host;
 using torch::autograd::Node;
@@ -74,19 +73,12 @@ struct Layer {
 };
 enum { WEIGHT = 0, INPUT = 1, GRAD = 2 };
 
-bool holds(const Tensor& t, const at::Device& device, at::ScalarType type, at::IntArrayRef sizes) {
-    return t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == sizes && t.is_contiguous();
-}
-
 // Whether a framework transform is at work that sees operators and autograd functions, not these kernels: vmap, grad and the like
 // (functorch), tracing, a dispatch mode written in Python.
 bool transformed() {
     static const c10::DispatchKeySet keys({c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::Tracer, c10::DispatchKey::Python});
     return c10::impl::tls_local_dispatch_key_set().included_.has_any(keys);
 }
-
-// A tensor subclass with its own dispatch, or a dual number of forward-mode differentiation, whose tangent would be lost here.
-bool plain(const Tensor& t) { return !t.defined() || (!t.unsafeGetTensorImpl()->is_python_dispatch() && !t._fw_grad(0).defined()); }
 
 // Whether a layer's tensors are what the kernels here read by raw pointer: the recipe's formats and shapes, contiguous, on x's
 // device, and plain. Any other call is the general path's (nn/_grouped_linear.py, nn/_tensor_linear.py), which copies a weight whose rows
@@ -124,13 +116,6 @@ struct Place {
         return q < 0 ? Codes{} : Codes{p + q, p + s, pitch};
     }
 };
-
-// A tensor that was saved for backward, as it comes back: a saved-tensor hook may have moved it or made another of it.
-Tensor restored(const SavedVariable& saved, const at::Device& device, at::ScalarType type, at::IntArrayRef sizes) {
-    const Tensor t = saved.unpack();
-    TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == sizes, "a tensor saved by a viola module came back changed");
-    return t.contiguous();
-}
 
 // What a projection's backward needs. All of it is saved the way autograd saves tensors, so that saved-tensor hooks (save_on_cpu,
 // checkpointing) see it, in-place changes are noticed and it is freed with the graph; no address outlives the forward pass.
@@ -1061,6 +1046,7 @@ PYBIND11_MODULE(_host, m) {
         recording.store(!list.is_none());
     });
     register_optimizer(m);
+    register_blocks(m);
     m.def("segment_offsets", torch::wrap_pybind_function([](const std::vector<int64_t>& counts, const at::Device& device) {
         Groups g;
         make_groups(g, counts, device, c10::hip::getCurrentHIPStream(device.index()).stream());

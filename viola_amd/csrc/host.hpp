@@ -1,7 +1,8 @@
-// Shared by the two native host files (host.cpp: modules, host_optim.cpp: optimizer and wire codec): calling the library's
-// entry points, tensor helpers, arenas.
+// Shared by the native host files (host.cpp: modules, host_blocks.cpp: norms around a block and routing, host_optim.cpp: optimizer and
+// wire codec): calling the library's entry points, tensor helpers, arenas.
 #pragma once
 #include <torch/extension.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <c10/hip/HIPStream.h>
 
@@ -82,6 +83,21 @@ private:
     Tensor buffer_;
 };
 
+inline bool holds(const Tensor& t, const at::Device& device, at::ScalarType type, at::IntArrayRef sizes) {
+    return t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == sizes && t.is_contiguous();
+}
+
+// A tensor subclass with its own dispatch, or a dual number of forward-mode differentiation, whose tangent would be lost here.
+inline bool plain(const Tensor& t) { return !t.defined() || (!t.unsafeGetTensorImpl()->is_python_dispatch() && !t._fw_grad(0).defined()); }
+
+// A tensor that was saved for backward, as it comes back: a saved-tensor hook may have moved it or made another of it.
+inline Tensor restored(const torch::autograd::SavedVariable& saved, const at::Device& device, at::ScalarType type, at::IntArrayRef sizes) {
+    const Tensor t = saved.unpack();
+    TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == sizes, "a tensor saved by a viola module came back changed");
+    return t.contiguous();
+}
+
 void register_optimizer(py::module_& m);                         // host_optim.cpp
+void register_blocks(py::module_& m);                            // host_blocks.cpp
 
 }  // namespace viola_host

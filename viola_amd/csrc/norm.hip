@@ -1,0 +1,309 @@
+// Norms before and after a block with its gate and residual sum (norm.hpp), and the gradients of the vectors along the row.
+#include "norm.hpp"
+
+using namespace viola;
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------- any width, type and address
+// A block for each row at a time, element by element; what a row needs twice is read again, from cache. Columns stay with their thread, so
+// sums over the rows of a portion can be kept in the portion's own slots.
+struct Columns {
+    const NormArgs& a;
+    int64_t row, group;
+    float4 stat;                                                             // mu_y, r_y, mu_x, r_x as far as they are known
+    __device__ __forceinline__ float vector(const void* data, int64_t at, int dtype, int c, float absent) const { return data ? load_float(data, at + c, dtype) : absent; }
+    __device__ __forceinline__ float y_hat(int c) const { return (load_float(a.y, row * a.y_pitch + c, a.branch_dtype) - stat.x) * stat.y; }
+    __device__ __forceinline__ float gate(int c) const { return a.alpha * vector(a.gate.data, group * a.gate.pitch, a.vector_dtype, c, 1.0f); }
+    __device__ __forceinline__ float after_weight(int c) const { return vector(a.after_weight, 0, a.weight_dtype, c, 1.0f); }
+    __device__ __forceinline__ float out(int c) const {
+        const float x = load_float(a.x, row * a.x_pitch + c, a.x_dtype);
+        if (!a.y) return x;
+        return fmaf(a.rho, x, gate(c) * fmaf(y_hat(c), after_weight(c), vector(a.after_bias, 0, a.weight_dtype, c, 0.0f)));
+    }
+    __device__ __forceinline__ float scale(int c) const { return 1.0f + vector(a.scale.data, group * a.scale.pitch, a.vector_dtype, c, 0.0f); }
+    __device__ __forceinline__ float weight(int c) const { return vector(a.weight, 0, a.weight_dtype, c, 1.0f); }
+};
+
+// mu and r of a row given by its columns. The mean first and the deviations from it after that: a row far from zero keeps its digits.
+template <typename F> __device__ __forceinline__ float2 statistics(const NormArgs& a, int kind, BlockSums& sums, F&& value) {
+    float mean = 0.0f, s = 0.0f;
+    if (kind == VIOLA_NORM_LAYER) {
+        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) s += value(c);
+        mean = sums.one(s) / (float)a.cols;
+    }
+    s = 0.0f;
+    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+        const float d = value(c) - mean;
+        s = fmaf(d, d, s);
+    }
+    return make_float2(mean, 1.0f / sqrtf(sums.one(s) / (float)a.cols + a.eps));
+}
+
+__global__ __launch_bounds__(256) void norm_forward_any_kernel(NormArgs a) {
+    __shared__ float2 slots[2][16];
+    BlockSums sums(slots);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        Columns at{a, row, row / a.group_rows, make_float4(0.0f, 1.0f, 0.0f, 1.0f)};
+        if (a.y && a.after != VIOLA_NORM_NONE) {
+            const float2 s = statistics(a, a.after, sums, [&](int c) { return load_float(a.y, row * a.y_pitch + c, a.branch_dtype); });
+            at.stat.x = s.x;
+            at.stat.y = s.y;
+        }
+        if (a.h) {
+            const float2 s = statistics(a, a.before, sums, [&](int c) { return at.out(c); });
+            at.stat.z = s.x;
+            at.stat.w = s.y;
+        }
+        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+            const float x = at.out(c);
+            if (a.out) store_float(a.out, row * a.cols + c, a.x_dtype, x);
+            if (a.h) {
+                const float n = fmaf((x - at.stat.z) * at.stat.w, at.weight(c), at.vector(a.bias, 0, a.weight_dtype, c, 0.0f));
+                store_float(a.h, row * a.cols + c, a.branch_dtype, fmaf(n, at.scale(c), at.vector(a.shift.data, at.group * a.shift.pitch, a.vector_dtype, c, 0.0f)));
+            }
+        }
+        if (a.stats && threadIdx.x == 0) a.stats[row] = at.stat;
+    }
+}
+
+// One portion: up to ceil(group_rows / per_group) rows of one group.
+__global__ __launch_bounds__(256) void norm_backward_any_kernel(NormArgs a) {
+    __shared__ float2 slots[2][16];
+    BlockSums sums(slots);
+    const float inverse = 1.0f / (float)a.cols;
+    const int64_t length = (a.group_rows + a.per_group - 1) / a.per_group;
+    const int count = __popc(a.sums);
+    for (int64_t portion = blockIdx.x; portion < a.portions; portion += gridDim.x) {
+        const int64_t group = portion / a.per_group, group_end = (group + 1) * a.group_rows;
+        const int64_t begin = group * a.group_rows + portion % a.per_group * length;
+        const int64_t end = begin + length < group_end ? begin + length : group_end;
+        float* slot = a.parts + portion * count * a.cols;
+        for (int c = threadIdx.x; c < a.cols; c += blockDim.x)
+            for (int i = 0; i < count; ++i) slot[(int64_t)i * a.cols + c] = 0.0f;
+        for (int64_t row = begin; row < end; ++row) {
+            const Columns at{a, row, group, a.stats[row]};
+            auto x_hat = [&](int c) { return (at.out(c) - at.stat.z) * at.stat.w; };
+            auto dh = [&](int c) { return load_float(a.dh, row * a.cols + c, a.branch_dtype); };
+            auto q = [&](int c) { return dh(c) * at.weight(c) * at.scale(c); };
+            float m1 = 0.0f, m0 = 0.0f;
+            if (a.dh) {
+                float along = 0.0f, total = 0.0f;
+                for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+                    along = fmaf(q(c), x_hat(c), along);
+                    total += q(c);
+                }
+                const float2 both = sums.both(along, total);
+                m1 = both.x * inverse;
+                m0 = a.before == VIOLA_NORM_LAYER ? both.y * inverse : 0.0f;
+            }
+            auto d = [&](int c) {
+                const float from_out = a.dout ? load_float(a.dout, row * a.cols + c, a.x_dtype) : 0.0f;
+                return a.dh ? fmaf(at.stat.w, q(c) - fmaf(x_hat(c), m1, m0), from_out) : from_out;
+            };
+            float along = 0.0f, total = 0.0f;
+            for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+                const float grad = d(c);
+                if (a.dx) store_float(a.dx, row * a.cols + c, a.x_dtype, a.y ? a.rho * grad : grad);
+                float* to = slot + c;
+                if (a.y) {
+                    const float hat = at.y_hat(c), p = grad * at.gate(c) * at.after_weight(c);
+                    if (a.sums & SUM_A1) { *to = fmaf(grad, hat, *to); to += a.cols; }
+                    if (a.sums & SUM_A0) { *to += grad; to += a.cols; }
+                    along = fmaf(p, hat, along);
+                    total += p;
+                }
+                if (a.dh) {
+                    if (a.sums & SUM_S1) { *to = fmaf(dh(c), x_hat(c), *to); to += a.cols; }
+                    if (a.sums & SUM_S0) *to += dh(c);
+                }
+            }
+            if (!a.dy) continue;
+            float n1 = 0.0f, n0 = 0.0f;
+            if (a.after != VIOLA_NORM_NONE) {
+                const float2 both = sums.both(along, total);
+                n1 = both.x * inverse;
+                n0 = a.after == VIOLA_NORM_LAYER ? both.y * inverse : 0.0f;
+            }
+            for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+                const float p = d(c) * at.gate(c) * at.after_weight(c);
+                store_float(a.dy, row * a.cols + c, a.branch_dtype, a.after == VIOLA_NORM_NONE ? p : at.stat.y * (p - fmaf(at.y_hat(c), n1, n0)));
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- sums over rows
+struct ReduceArgs {
+    const float* parts;
+    int64_t portions, per_group;
+    int cols, sums, weight_dtype, vector_dtype;
+    float alpha;
+    const void *after_weight, *after_bias, *weight, *bias;
+    NormVector gate, scale;
+    // one for all rows (vectors with a pitch of 0 too), or one for each group
+    void *d_after_weight, *d_after_bias, *d_weight, *d_bias, *d_gate, *d_scale, *d_shift;
+    int gate_by_group, scale_by_group, shift_by_group;
+};
+
+constexpr int SLICES = 32;                                                   // of the portions, by 32 columns: 1024 threads
+
+// blockIdx.y 0: what is summed over all rows, 32 columns by 32 contiguous slices of the portions, the slices then added in order.
+// blockIdx.y > 0: what is summed group by group, 32 columns by 32 groups.
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(ReduceArgs a) {
+    __shared__ float piece[SLICES][8][33];
+    const int c = threadIdx.x % 32, slice = threadIdx.x / 32, col = blockIdx.x * 32 + c;
+    const int count = __popc(a.sums);
+    const int at_a0 = __popc(a.sums & SUM_A1), at_s1 = __popc(a.sums & (SUM_A1 | SUM_A0)), at_s0 = __popc(a.sums & (SUM_A1 | SUM_A0 | SUM_S1));
+    const bool in = col < a.cols;
+    auto vector = [&](const void* data, int64_t at, int dtype, float absent) { return data && in ? load_float(data, at + col, dtype) : absent; };
+    if (blockIdx.y) {
+        const int64_t group = (int64_t)(blockIdx.y - 1) * 32 + slice;
+        if (!in || group >= a.portions / a.per_group) return;
+        float a1 = 0.0f, a0 = 0.0f, s1 = 0.0f, s0 = 0.0f;
+        for (int64_t p = group * a.per_group; p < (group + 1) * a.per_group; ++p) {
+            const float* from = a.parts + p * count * a.cols + col;
+            if (a.sums & SUM_A1) a1 += from[0];
+            if (a.sums & SUM_A0) a0 += from[at_a0 * a.cols];
+            if (a.sums & SUM_S1) s1 += from[at_s1 * a.cols];
+            if (a.sums & SUM_S0) s0 += from[at_s0 * a.cols];
+        }
+        const int64_t to = group * a.cols + col;
+        const float w_a = vector(a.after_weight, 0, a.weight_dtype, 1.0f), b_a = vector(a.after_bias, 0, a.weight_dtype, 0.0f);
+        const float w_b = vector(a.weight, 0, a.weight_dtype, 1.0f), b_b = vector(a.bias, 0, a.weight_dtype, 0.0f);
+        if (a.d_gate && a.gate_by_group) store_float(a.d_gate, to, a.vector_dtype, a.alpha * fmaf(w_a, a1, a.after_bias ? b_a * a0 : 0.0f));
+        if (a.d_scale && a.scale_by_group) store_float(a.d_scale, to, a.vector_dtype, fmaf(w_b, s1, a.bias ? b_b * s0 : 0.0f));
+        if (a.d_shift && a.shift_by_group) store_float(a.d_shift, to, a.vector_dtype, s0);
+        return;
+    }
+    // the four sums, then the same under the gate and under one plus the scale
+    float sum[8] = {};
+    if (in) {
+        const int64_t per = (a.portions + SLICES - 1) / SLICES;
+        const int64_t begin = slice * per, end = begin + per < a.portions ? begin + per : a.portions;
+        for (int64_t p = begin; p < end; ++p) {
+            const float* from = a.parts + p * count * a.cols + col;
+            const int64_t group = p / a.per_group;
+            const float g = vector(a.gate.data, group * a.gate.pitch, a.vector_dtype, 1.0f), s = 1.0f + vector(a.scale.data, group * a.scale.pitch, a.vector_dtype, 0.0f);
+            const float a1 = a.sums & SUM_A1 ? from[0] : 0.0f, a0 = a.sums & SUM_A0 ? from[at_a0 * a.cols] : 0.0f;
+            const float s1 = a.sums & SUM_S1 ? from[at_s1 * a.cols] : 0.0f, s0 = a.sums & SUM_S0 ? from[at_s0 * a.cols] : 0.0f;
+            sum[0] += a1; sum[1] += a0; sum[2] += s1; sum[3] += s0;
+            sum[4] = fmaf(g, a1, sum[4]); sum[5] = fmaf(g, a0, sum[5]); sum[6] = fmaf(s, s1, sum[6]); sum[7] = fmaf(s, s0, sum[7]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) piece[slice][i][c] = sum[i];
+    __syncthreads();
+    if (slice < 8) {
+        float total = piece[0][slice][c];
+        for (int u = 1; u < SLICES; ++u) total += piece[u][slice][c];
+        piece[0][slice][c] = total;                                          // read by this thread only until the next barrier
+    }
+    __syncthreads();
+    if (slice || !in) return;
+    const float a1 = piece[0][0][c], a0 = piece[0][1][c], s1 = piece[0][2][c], s0 = piece[0][3][c];
+    if (a.d_after_weight) store_float(a.d_after_weight, col, a.weight_dtype, a.alpha * piece[0][4][c]);
+    if (a.d_after_bias) store_float(a.d_after_bias, col, a.weight_dtype, a.alpha * piece[0][5][c]);
+    if (a.d_weight) store_float(a.d_weight, col, a.weight_dtype, piece[0][6][c]);
+    if (a.d_bias) store_float(a.d_bias, col, a.weight_dtype, piece[0][7][c]);
+    if (a.d_gate && !a.gate_by_group) {
+        const float b_a = vector(a.after_bias, 0, a.weight_dtype, 0.0f);
+        store_float(a.d_gate, col, a.vector_dtype, a.alpha * fmaf(vector(a.after_weight, 0, a.weight_dtype, 1.0f), a1, a.after_bias ? b_a * a0 : 0.0f));
+    }
+    if (a.d_scale && !a.scale_by_group) {
+        const float b_b = vector(a.bias, 0, a.weight_dtype, 0.0f);
+        store_float(a.d_scale, col, a.vector_dtype, fmaf(vector(a.weight, 0, a.weight_dtype, 1.0f), s1, a.bias ? b_b * s0 : 0.0f));
+    }
+    if (a.d_shift && !a.shift_by_group) store_float(a.d_shift, col, a.vector_dtype, s0);
+}
+
+// A portion for every block that the chip holds at once, and no group's rows split finer than one by one.
+int64_t portions_per_group(int64_t rows, int64_t group_rows) {
+    const int64_t groups = rows / group_rows, wanted = (512 + groups - 1) / groups;
+    return wanted < group_rows ? wanted : group_rows;
+}
+
+bool valid_rows(const void* p, int64_t pitch, int64_t cols) { return p && pitch >= cols; }
+
+int set_common(NormArgs& a, const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols, int after,
+               const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype, const void* gate,
+               int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch, int vector_dtype, int64_t group_rows, float rho,
+               float alpha, float eps) {
+    VIOLA_CHECK_ARG(viola_is_float(x_dtype) && viola_is_float(branch_dtype) && viola_is_float(weight_dtype) && viola_is_float(vector_dtype));
+    VIOLA_CHECK_ARG(rows >= 0 && cols > 0 && group_rows > 0 && rows % group_rows == 0);
+    VIOLA_CHECK_ARG(after >= VIOLA_NORM_NONE && after <= VIOLA_NORM_LAYER && before >= VIOLA_NORM_NONE && before <= VIOLA_NORM_LAYER && eps >= 0.0f);
+    for (int64_t pitch : {gate_pitch, scale_pitch, shift_pitch}) VIOLA_CHECK_ARG(pitch == 0 || pitch >= cols);
+    VIOLA_CHECK_ARG(cols < (1LL << 31));
+    a.x = x; a.y = y; a.x_pitch = x_pitch; a.y_pitch = y_pitch; a.rows = rows; a.group_rows = group_rows;
+    a.cols = (int)cols; a.x_dtype = x_dtype; a.branch_dtype = branch_dtype; a.after = after; a.before = before;
+    a.weight_dtype = weight_dtype; a.vector_dtype = vector_dtype;
+    a.after_weight = after_weight; a.after_bias = after_bias; a.weight = weight; a.bias = bias;
+    a.gate = {gate, gate_pitch}; a.scale = {scale, scale_pitch}; a.shift = {shift, shift_pitch};
+    a.rho = rho; a.alpha = alpha; a.eps = eps;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols, int after,
+                                  const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
+                                  const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch, int vector_dtype,
+                                  int64_t group_rows, float residual_scale, float branch_scale, float eps, void* out, void* h, float* stats, viola_stream_t stream_) {
+    hipStream_t stream = viola_enter(stream_);
+    NormArgs a = {};
+    const int status = set_common(a, x, x_pitch, x_dtype, y, y_pitch, branch_dtype, rows, cols, after, after_weight, after_bias, before, weight, bias, weight_dtype, gate,
+                                  gate_pitch, scale, scale_pitch, shift, shift_pitch, vector_dtype, group_rows, residual_scale, branch_scale, eps);
+    if (status) return status;
+    if (rows == 0) return 0;
+    VIOLA_CHECK_ARG(valid_rows(x, x_pitch, cols) && (out || h) && (out != nullptr) == (y != nullptr) && (!y || y_pitch >= cols));
+    VIOLA_CHECK_ARG((h != nullptr) == (before != VIOLA_NORM_NONE) && (reinterpret_cast<uintptr_t>(stats) % 16) == 0);
+    a.out = out; a.h = h; a.stats = reinterpret_cast<float4*>(stats);
+    VIOLA_LAUNCH(norm_forward_any_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), 256, 0, stream, a);
+    return viola_launch_status();
+}
+
+extern "C" int64_t viola_norm_portions(int64_t rows, int64_t group_rows) {
+    if (rows <= 0 || group_rows <= 0 || rows % group_rows) return 0;
+    return rows / group_rows * portions_per_group(rows, group_rows);
+}
+
+extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols, int after,
+                                   const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
+                                   const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch, int vector_dtype,
+                                   int64_t group_rows, float residual_scale, float branch_scale, const float* stats, const void* dout, const void* dh, void* dx, void* dy,
+                                   float* parts, int64_t parts_floats, void* d_after_weight, void* d_after_bias, void* d_weight, void* d_bias, void* d_gate,
+                                   void* d_scale, void* d_shift, viola_stream_t stream_) {
+    hipStream_t stream = viola_enter(stream_);
+    NormArgs a = {};
+    const int status = set_common(a, x, x_pitch, x_dtype, y, y_pitch, branch_dtype, rows, cols, after, after_weight, after_bias, before, weight, bias, weight_dtype, gate,
+                                  gate_pitch, scale, scale_pitch, shift, shift_pitch, vector_dtype, group_rows, residual_scale, branch_scale, 0.0f);
+    if (status) return status;
+    const bool gate_sums = d_gate && y, scale_sums = d_scale && dh;
+    // rows of none: the sums over rows are still written, as zeros, by the reduction below
+    if (rows) {
+        VIOLA_CHECK_ARG(valid_rows(x, x_pitch, cols) && stats && (!y || y_pitch >= cols) && (dh || y) && (dh != nullptr) == (before != VIOLA_NORM_NONE) && (y || !dy));
+        VIOLA_CHECK_ARG(reinterpret_cast<uintptr_t>(stats) % 16 == 0);
+    }
+    a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
+    a.dout = dout; a.dh = dh; a.dx = dx; a.dy = dy; a.parts = parts;
+    a.sums = (d_after_weight || gate_sums ? SUM_A1 : 0) | (d_after_bias || (gate_sums && after_bias) ? SUM_A0 : 0) | (d_weight || scale_sums ? SUM_S1 : 0) |
+             (d_bias || d_shift || (scale_sums && bias) ? SUM_S0 : 0);
+    a.per_group = rows ? portions_per_group(rows, group_rows) : 1;
+    a.portions = rows ? rows / group_rows * a.per_group : 0;
+    if (a.sums && rows) VIOLA_CHECK_ARG(parts && parts_floats >= a.portions * __builtin_popcount((unsigned)a.sums) * cols);
+    const bool grouped = (d_gate && gate_pitch) || (d_scale && scale_pitch) || (d_shift && shift_pitch);
+    const int64_t sections = 1 + (grouped ? (rows / group_rows + 31) / 32 : 0);
+    if (sections > 65535) return VIOLA_EUNSUPPORTED;
+    if (rows) VIOLA_LAUNCH(norm_backward_any_kernel, dim3((unsigned)(a.portions < 65536 ? a.portions : 65536)), 256, 0, stream, a);
+    if (a.sums) {
+        ReduceArgs r = {};
+        r.parts = parts; r.portions = a.portions; r.per_group = a.per_group; r.cols = (int)cols; r.sums = a.sums;
+        r.weight_dtype = weight_dtype; r.vector_dtype = vector_dtype; r.alpha = branch_scale;
+        r.after_weight = after_weight; r.after_bias = after_bias; r.weight = weight; r.bias = bias; r.gate = a.gate; r.scale = a.scale;
+        r.d_after_weight = d_after_weight; r.d_after_bias = d_after_bias; r.d_weight = d_weight; r.d_bias = d_bias;
+        r.d_gate = d_gate; r.d_scale = d_scale; r.d_shift = d_shift;
+        r.gate_by_group = gate_pitch != 0; r.scale_by_group = scale_pitch != 0; r.shift_by_group = shift_pitch != 0;
+        VIOLA_LAUNCH(norm_reduce_kernel, dim3((unsigned)((cols + 31) / 32), (unsigned)sections), 1024, 0, stream, r);
+    }
+    return viola_launch_status();
+}
