@@ -78,10 +78,13 @@ struct NormPlan {
     at::ScalarType type_of(int i) const { return i < GATE ? weight_type : vector_type; }
     // A vector as the kernels read it: [cols], or [groups, cols] with whole rows.
     Tensor readable(int i, const Tensor& t, int64_t cols) const {
-        const Tensor v = t.to(type_of(i));
-        if (i < GATE || !by_group[i - GATE]) return v.reshape({cols}).contiguous();
-        const Tensor rows = v.reshape({groups, cols});
-        return (cols > 1 && rows.stride(1) != 1) || rows.stride(0) < cols ? rows.contiguous() : rows;
+        const bool grouped = i >= GATE && by_group[i - GATE];
+        Tensor v = t.to(type_of(i));
+        v = grouped ? v.reshape({groups, cols}) : v.reshape({cols}).contiguous();
+        if (grouped && ((cols > 1 && v.stride(1) != 1) || v.stride(0) < cols)) v = v.contiguous();
+        // whole pieces of 16 bytes, as the rows have them: a copy of a vector is little beside what it spares the rows
+        const bool whole = reinterpret_cast<uintptr_t>(ptr(v)) % 16 == 0 && (!grouped || v.stride(0) % 8 == 0);
+        return whole || cols % 8 ? v : v.clone(at::MemoryFormat::Contiguous);
     }
 };
 

@@ -1,7 +1,19 @@
 // Norms before and after a block with its gate and residual sum (norm.hpp), and the gradients of the vectors along the row.
-#include "norm.hpp"
+#include "norm_launch.hpp"
+
+#include <initializer_list>
 
 using namespace viola;
+
+// norm_rows_*.hip
+#define VIOLA_NORM_ROWS(TX, TY)                                                                             \
+    extern template void viola::norm_forward_rows<TX, TY>(const NormArgs&, int, dim3, hipStream_t);         \
+    extern template void viola::norm_backward_rows<TX, TY>(const NormArgs&, int, bool, bool, dim3, hipStream_t);
+VIOLA_NORM_ROWS(bf16_t, bf16_t)
+VIOLA_NORM_ROWS(f16_t, f16_t)
+VIOLA_NORM_ROWS(float, float)
+VIOLA_NORM_ROWS(float, bf16_t)
+VIOLA_NORM_ROWS(float, f16_t)
 
 namespace {
 
@@ -217,6 +229,26 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(ReduceArgs a) {
     if (a.d_shift && !a.shift_by_group) store_float(a.d_shift, col, a.vector_dtype, s0);
 }
 
+// Whether rows of these types, this width and these addresses are held in registers, in pieces of eight elements; then f(stream type, branch type).
+template <typename F> bool in_registers(const NormArgs& a, std::initializer_list<const void*> tensors, F&& f) {
+    if (a.cols % 8 || a.cols > ROW_COLUMNS || a.x_pitch % 8 || (a.y && a.y_pitch % 8)) return false;
+    for (const void* p : tensors)
+        if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+    for (const void* p : {a.after_weight, a.after_bias, a.weight, a.bias, a.gate.data, a.scale.data, a.shift.data})
+        if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+    for (const NormVector& v : {a.gate, a.scale, a.shift})
+        if (v.pitch % 8) return false;
+    const int x = a.x_dtype, y = a.branch_dtype;
+    if (x == VIOLA_BF16 && y == VIOLA_BF16) f(bf16_t(), bf16_t());
+    else if (x == VIOLA_F16 && y == VIOLA_F16) f(f16_t(), f16_t());
+    else if (x == VIOLA_F32 && y == VIOLA_F32) f(float(), float());
+    else if (x == VIOLA_F32 && y == VIOLA_BF16) f(float(), bf16_t());
+    else if (x == VIOLA_F32 && y == VIOLA_F16) f(float(), f16_t());
+    else return false;
+    return true;
+}
+int team_of(int cols) { return (cols + 511) / 512 * 64; }
+
 // A portion for every block that the chip holds at once, and no group's rows split finer than one by one.
 int64_t portions_per_group(int64_t rows, int64_t group_rows) {
     const int64_t groups = rows / group_rows, wanted = (512 + groups - 1) / groups;
@@ -257,7 +289,13 @@ extern "C" int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, c
     if (rows == 0) return 0;
     VIOLA_CHECK_ARG(valid_rows(x, x_pitch, cols) && (out || h) && (out != nullptr) == (y != nullptr) && (!y || y_pitch >= cols));
     VIOLA_CHECK_ARG((h != nullptr) == (before != VIOLA_NORM_NONE) && (reinterpret_cast<uintptr_t>(stats) % 16) == 0);
+    const int form = !y ? FORM_BEFORE : h ? FORM_BETWEEN : FORM_AFTER;
     a.out = out; a.h = h; a.stats = reinterpret_cast<float4*>(stats);
+    a.team = team_of((int)cols);
+    const int64_t blocks = 2048, teams = a.team >= 512 ? 1 : 512 / a.team;
+    a.chunk = ((rows + blocks - 1) / blocks + teams - 1) / teams * teams;
+    const dim3 grid((unsigned)((rows + a.chunk - 1) / a.chunk));
+    if (in_registers(a, {x, y, out, h}, [&](auto tx, auto ty) { norm_forward_rows<decltype(tx), decltype(ty)>(a, form, grid, stream); })) return viola_launch_status();
     VIOLA_LAUNCH(norm_forward_any_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), 256, 0, stream, a);
     return viola_launch_status();
 }
@@ -294,7 +332,14 @@ extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, 
     const bool grouped = (d_gate && gate_pitch) || (d_scale && scale_pitch) || (d_shift && shift_pitch);
     const int64_t sections = 1 + (grouped ? (rows / group_rows + 31) / 32 : 0);
     if (sections > 65535) return VIOLA_EUNSUPPORTED;
-    if (rows) VIOLA_LAUNCH(norm_backward_any_kernel, dim3((unsigned)(a.portions < 65536 ? a.portions : 65536)), 256, 0, stream, a);
+    if (rows) {
+        const dim3 grid((unsigned)(a.portions < 65536 ? a.portions : 65536));
+        const int form = !y ? FORM_BEFORE : dh ? FORM_BETWEEN : FORM_AFTER;
+        const bool with_bias = after_bias || (a.sums & SUM_A0), with_shift = (a.sums & SUM_S0) != 0;
+        a.team = team_of((int)cols);
+        if (!in_registers(a, {x, y, dout, dh, dx, dy, parts}, [&](auto tx, auto ty) { norm_backward_rows<decltype(tx), decltype(ty)>(a, form, with_bias, with_shift, grid, stream); }))
+            VIOLA_LAUNCH(norm_backward_any_kernel, grid, 256, 0, stream, a);
+    }
     if (a.sums) {
         ReduceArgs r = {};
         r.parts = parts; r.portions = a.portions; r.per_group = a.per_group; r.cols = (int)cols; r.sums = a.sums;

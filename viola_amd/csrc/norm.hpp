@@ -4,8 +4,8 @@
 //   after the block   x' = rho x + alpha g (n(y) w_a + b_a)         (or n(y) = y)
 //   before the next   h  = (n(x') w_b + b_b) (1 + s) + t
 //
-// Backward, from D_out = dL/dx' and dh, with x' computed again in 32 bits from x and y (as many bytes as reading x' would be, and
-// without its rounding):
+// Backward, from D_out = dL/dx' and dh, with x' computed again in 32 bits from x and y (as many bytes as reading x' would be, without its
+// rounding):
 //   q = dh w_b (1 + s),  D = D_out + r_x (q - x^ mean(q x^) - mean(q)),  dx = rho D,  p = D alpha g w_a,
 //   dy = r_y (p - y^ mean(p y^) - mean(p))
 // with x^ = (x' - mu_x) r_x and y^ alike (the means without a product only with mu). Sums over rows: A1 = sum D y^, A0 = sum D, S1 = sum dh x^, S0 = sum dh give every
@@ -37,6 +37,7 @@ struct NormArgs {
     void *out, *h;
     float4* stats;                                                           // mu_y, r_y, mu_x, r_x of a row
     int64_t chunk;                                                           // rows of a block
+    int team;                                                                // threads of a row, where rows are in registers
     // backward
     const void *dout, *dh;
     void *dx, *dy;
@@ -44,5 +45,327 @@ struct NormArgs {
     int64_t portions, per_group;                                             // portions in all, and of one group
     int sums;                                                                // which sums over rows are wanted (SUM_*)
 };
+
+// ---------------------------------------------------------------------------------------------------- rows in registers
+// A row belongs to a team of whole wavefronts, eight elements to a thread, from its loads to its stores: each tensor is read once and written
+// once whatever the norms in between need. A block has several teams where rows are narrow; they take its rows in turn. The vectors along
+// the row are kept folded for the rows of a group: x' = rho x + y^ GA + GB with GA = alpha g w_a, GB = alpha g b_a, and h = x^ W + B with
+// W = w_b (1 + s), B = b_b (1 + s) + t. BIAS: GB and A0 are there, SHIFT: S0 is; most norms
+// do without them and their registers.
+constexpr int ROW_THREADS = 1024, ROW_COLUMNS = 8 * ROW_THREADS;
+
+template <typename T> struct Piece { uint4 word[sizeof(T) / 2]; };           // eight elements as they lie in memory
+
+// `row` elements behind `base` for a whole wavefront, `col` more for a thread: the first is a scalar's work.
+template <typename T> __device__ __forceinline__ Piece<T> load_piece(const void* base, int64_t row, int col) {
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(base) + row + col);
+    Piece<T> p;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) p.word[i] = from[i];
+    return p;
+}
+template <typename T> __device__ __forceinline__ void widen_piece(const Piece<T>& p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            v[4 * i] = __uint_as_float(p.word[i].x); v[4 * i + 1] = __uint_as_float(p.word[i].y);
+            v[4 * i + 2] = __uint_as_float(p.word[i].z); v[4 * i + 3] = __uint_as_float(p.word[i].w);
+        }
+    } else {
+        const uint32_t w[4] = {p.word[0].x, p.word[0].y, p.word[0].z, p.word[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (__is_same(T, bf16_t)) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            } else {
+                v[2 * i] = widen16<f16_t>(w[i] & 0xffffu);
+                v[2 * i + 1] = widen16<f16_t>(w[i] >> 16);
+            }
+        }
+    }
+}
+template <typename T> __device__ __forceinline__ void store_piece(void* base, int64_t row, int col, const float (&v)[8]) {
+    uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(base) + row + col);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            to[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+    } else if constexpr (__is_same(T, bf16_t)) {
+        *to = make_uint4(f32_to_bf16x2_bits(v[0], v[1]), f32_to_bf16x2_bits(v[2], v[3]), f32_to_bf16x2_bits(v[4], v[5]), f32_to_bf16x2_bits(v[6], v[7]));
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = narrow16<f16_t>(v[2 * i]) | narrow16<f16_t>(v[2 * i + 1]) << 16;
+        *to = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Eight elements of a vector of any type; `absent` where there is none.
+__device__ __forceinline__ void load_vector(const void* base, int64_t row, int col, int dtype, bool in, float absent, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = absent;
+    if (base && in) {
+        if (dtype == VIOLA_F32) widen_piece(load_piece<float>(base, row, col), v);
+        else if (dtype == VIOLA_BF16) widen_piece(load_piece<bf16_t>(base, row, col), v);
+        else widen_piece(load_piece<f16_t>(base, row, col), v);
+    }
+    __builtin_amdgcn_sched_barrier(0);                                       // one vector after the other: together they would take every register
+}
+
+// Sums over the wavefronts of a team: those of BlockSums with the slots of the own team only. All teams of a block call it alike.
+struct TeamSums {
+    float2* slot;                                                            // two sets of 16 in LDS
+    int waves, first, wave, turn = 0;
+    __device__ __forceinline__ TeamSums(float2* slot, int waves) : slot(slot), waves(waves), first(threadIdx.x / 64 / waves * waves), wave(threadIdx.x / 64) {}
+    __device__ __forceinline__ float2 both(float a, float b) {
+        a = wave_total(a);
+        b = wave_total(b);
+        if (waves == 1) return make_float2(a, b);
+        if (threadIdx.x % 64 == 0) slot[turn * 16 + wave] = make_float2(a, b);
+        __syncthreads();
+        float2 sum = slot[turn * 16 + first];
+        for (int w = first + 1; w < first + waves; ++w) {
+            sum.x += slot[turn * 16 + w].x;
+            sum.y += slot[turn * 16 + w].y;
+        }
+        turn ^= 1;
+        return sum;
+    }
+    __device__ __forceinline__ float one(float a) {
+        a = wave_total(a);
+        if (waves == 1) return a;
+        if (threadIdx.x % 64 == 0) slot[turn * 16 + wave].x = a;
+        __syncthreads();
+        float sum = slot[turn * 16 + first].x;
+        for (int w = first + 1; w < first + waves; ++w) sum += slot[turn * 16 + w].x;
+        turn ^= 1;
+        return sum;
+    }
+};
+
+__device__ __forceinline__ float2 row_statistics(const float (&v)[8], bool in, int kind, float inverse, float eps, TeamSums& sums) {
+    float mean = 0.0f;
+    if (kind == VIOLA_NORM_LAYER) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
+        mean = sums.one(in ? s : 0.0f) * inverse;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float d = v[i] - mean;
+        q = fmaf(d, d, q);
+    }
+    return make_float2(mean, 1.0f / sqrtf(sums.one(in ? q : 0.0f) * inverse + eps));
+}
+
+template <int FORM> struct NormVectors {
+    float ga[8], gb[8], w[8], b[8];
+    __device__ __forceinline__ void load(const NormArgs& a, int64_t group, int col, bool in) {
+        float u[8];
+        if constexpr (FORM != FORM_BEFORE) {
+            load_vector(a.after_weight, 0, col, a.weight_dtype, in, 1.0f, ga);
+            load_vector(a.after_bias, 0, col, a.weight_dtype, in, 0.0f, gb);
+            load_vector(a.gate.data, group * a.gate.pitch, col, a.vector_dtype, in, 1.0f, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                ga[i] *= a.alpha * u[i];
+                gb[i] *= a.alpha * u[i];
+            }
+        }
+        if constexpr (FORM != FORM_AFTER) {
+            load_vector(a.weight, 0, col, a.weight_dtype, in, 1.0f, w);
+            load_vector(a.bias, 0, col, a.weight_dtype, in, 0.0f, b);
+            load_vector(a.scale.data, group * a.scale.pitch, col, a.vector_dtype, in, 0.0f, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i] = fmaf(w[i], u[i], w[i]);
+                b[i] = fmaf(b[i], u[i], b[i]);
+            }
+            load_vector(a.shift.data, group * a.shift.pitch, col, a.vector_dtype, in, 0.0f, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] += u[i];
+        }
+    }
+};
+
+// The rows [blockIdx.x chunk, + chunk), a team each in turn. Every team makes as many turns as the first, so that barriers meet.
+template <typename TX, typename TY, int FORM> __global__ __launch_bounds__(ROW_THREADS) void norm_forward_kernel(NormArgs a) {
+    __shared__ float2 slots[32];
+    const int threads = a.team, teams = blockDim.x / threads, team = __builtin_amdgcn_readfirstlane(threadIdx.x / threads), t = threadIdx.x - team * threads;
+    TeamSums sums(slots, threads / 64);
+    const int col = t * 8;
+    const bool in = col < a.cols;
+    const float inverse = 1.0f / (float)a.cols;
+    const int64_t begin = blockIdx.x * a.chunk, end = begin + a.chunk < a.rows ? begin + a.chunk : a.rows;
+    NormVectors<FORM> vectors;
+    int64_t group_end = -1;                                                  // of the rows that the vectors are those of
+    Piece<TX> raw_x = {};                                                    // zero beyond the row
+    Piece<TY> raw_y = {};
+    auto load = [&](int64_t row) {
+        if (!in || row >= end) return;                                       // beyond the end: the last row again, which nobody stores
+        raw_x = load_piece<TX>(a.x, row * a.x_pitch, col);
+        if constexpr (FORM != FORM_BEFORE) raw_y = load_piece<TY>(a.y, row * a.y_pitch, col);
+    };
+    load(begin + team);
+    for (int64_t base = begin; base < end; base += teams) {
+        const int64_t row = base + team;
+        const bool there = in && row < end;
+        if (row >= group_end && row < end) {
+            const int64_t group = row / a.group_rows;
+            group_end = (group + 1) * a.group_rows;
+            vectors.load(a, group, col, in);
+        }
+        float x[8], y[8];
+        widen_piece(raw_x, x);
+        if constexpr (FORM != FORM_BEFORE) widen_piece(raw_y, y);
+        load(row + teams);
+        float4 stat = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
+        if constexpr (FORM != FORM_BEFORE) {
+            if (a.after != VIOLA_NORM_NONE) {
+                const float2 s = row_statistics(y, in, a.after, inverse, a.eps, sums);
+                stat.x = s.x;
+                stat.y = s.y;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(a.rho, x[i], fmaf((y[i] - stat.x) * stat.y, vectors.ga[i], vectors.gb[i]));
+            if (there) store_piece<TX>(a.out, row * a.cols, col, x);
+        }
+        if constexpr (FORM != FORM_AFTER) {
+            const float2 s = row_statistics(x, in, a.before, inverse, a.eps, sums);
+            stat.z = s.x;
+            stat.w = s.y;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - s.x) * s.y, vectors.w[i], vectors.b[i]);
+            if (there) store_piece<TY>(a.h, row * a.cols, col, x);
+        }
+        if (a.stats && t == 0 && row < end) a.stats[row] = stat;
+    }
+}
+
+// One portion: rows of one group, a team each in turn. The teams' sums are joined in LDS at the end, team by team.
+template <typename TX, typename TY, int FORM, bool BIAS, bool SHIFT> __global__ __launch_bounds__(ROW_THREADS) void norm_backward_kernel(NormArgs a) {
+    __shared__ float2 slots[32];
+    extern __shared__ float joined[];                                        // [teams - 1][cols] where a block has several teams
+    const int threads = a.team, teams = blockDim.x / threads, team = __builtin_amdgcn_readfirstlane(threadIdx.x / threads), t = threadIdx.x - team * threads;
+    TeamSums sums(slots, threads / 64);
+    const int col = t * 8;
+    const bool in = col < a.cols;
+    const float inverse = 1.0f / (float)a.cols;
+    const int64_t length = (a.group_rows + a.per_group - 1) / a.per_group;
+    for (int64_t portion = blockIdx.x; portion < a.portions; portion += gridDim.x) {
+        const int64_t group = portion / a.per_group, group_end = (group + 1) * a.group_rows;
+        const int64_t begin = group * a.group_rows + portion % a.per_group * length;
+        const int64_t end = begin + length < group_end ? begin + length : group_end;
+        NormVectors<FORM> vectors;                                           // its b is not used, and neither is gb without BIAS
+        vectors.load(a, group, col, in);
+        float a1[8] = {}, a0[8] = {}, s1[8] = {}, s0[8] = {};
+        // Beyond the row and beyond the portion everything is zero, the row's statistics too, and stays zero: nothing below asks again.
+        Piece<TX> raw_x = {}, raw_dout = {};
+        Piece<TY> raw_y = {}, raw_dh = {};
+        auto load = [&](int64_t row) {
+            if (row < end) {
+                if (in) {
+                    if constexpr (FORM != FORM_AFTER) raw_x = load_piece<TX>(a.x, row * a.x_pitch, col);
+                    if constexpr (FORM != FORM_BEFORE) raw_y = load_piece<TY>(a.y, row * a.y_pitch, col);
+                    if constexpr (FORM != FORM_AFTER) raw_dh = load_piece<TY>(a.dh, row * a.cols, col);
+                    if constexpr (FORM != FORM_BEFORE) if (a.dout) raw_dout = load_piece<TX>(a.dout, row * a.cols, col);
+                }
+            } else {
+                raw_x = raw_dout = {};
+                raw_y = raw_dh = {};
+            }
+        };
+        load(begin + team);
+        for (int64_t base = begin; base < end; base += teams) {
+            const int64_t row = base + team;
+            const bool there = in && row < end;
+            float4 stat = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (there) stat = a.stats[row];
+            float x[8], y[8], d[8], q[8];                                    // x^, y^, D, dh W
+            if constexpr (FORM != FORM_BEFORE) {
+                widen_piece(raw_y, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = (y[i] - stat.x) * stat.y;
+            }
+            if constexpr (FORM != FORM_AFTER) {
+                widen_piece(raw_x, x);
+                widen_piece(raw_dh, q);
+            }
+            const Piece<TX> dout = raw_dout;
+            load(row + teams);
+            if constexpr (FORM != FORM_BEFORE) widen_piece(dout, d);
+            if constexpr (FORM != FORM_AFTER) {
+                float along = 0.0f, total = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if constexpr (FORM == FORM_BETWEEN) x[i] = fmaf(a.rho, x[i], BIAS ? fmaf(y[i], vectors.ga[i], vectors.gb[i]) : y[i] * vectors.ga[i]);
+                    x[i] = (x[i] - stat.z) * stat.w;
+                    s1[i] = fmaf(q[i], x[i], s1[i]);
+                    if constexpr (SHIFT) s0[i] += q[i];
+                    q[i] *= vectors.w[i];
+                    along = fmaf(q[i], x[i], along);
+                    total += q[i];
+                }
+                const float2 both = sums.both(along, total);
+                const float m1 = both.x * inverse, m0 = a.before == VIOLA_NORM_LAYER ? both.y * inverse : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float from_h = stat.w * (q[i] - fmaf(x[i], m1, m0));
+                    d[i] = FORM == FORM_BETWEEN ? d[i] + from_h : from_h;
+                }
+            }
+            if (a.dx && there) {
+                if constexpr (FORM == FORM_BEFORE) {
+                    store_piece<TX>(a.dx, row * a.cols, col, d);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = a.rho * d[i];
+                    store_piece<TX>(a.dx, row * a.cols, col, x);
+                }
+            }
+            if constexpr (FORM != FORM_BEFORE) {
+                float along = 0.0f, total = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    a1[i] = fmaf(d[i], y[i], a1[i]);
+                    if constexpr (BIAS) a0[i] += d[i];
+                    d[i] *= vectors.ga[i];
+                    along = fmaf(d[i], y[i], along);
+                    total += d[i];
+                }
+                if (!a.dy) continue;
+                if (a.after != VIOLA_NORM_NONE) {
+                    const float2 both = sums.both(along, total);
+                    const float m1 = both.x * inverse, m0 = a.after == VIOLA_NORM_LAYER ? both.y * inverse : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[i] = stat.y * (d[i] - fmaf(y[i], m1, m0));
+                }
+                if (there) store_piece<TY>(a.dy, row * a.cols, col, d);
+            }
+        }
+        float* to = a.parts + portion * __popc(a.sums) * a.cols;
+        auto write = [&](float (&v)[8]) {
+            if (teams > 1) {
+                __syncthreads();                                             // the sum before has been read
+                if (team && in) store_piece<float>(joined, (int64_t)(team - 1) * a.cols, col, v);
+                __syncthreads();
+                if (!team && in)
+                    for (int u = 1; u < teams; ++u) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] += joined[(u - 1) * a.cols + col + i];
+                    }
+            }
+            if (!team && in) store_piece<float>(to, 0, col, v);
+            to += a.cols;
+        };
+        if (a.sums & SUM_A1) write(a1);
+        if constexpr (BIAS) if (a.sums & SUM_A0) write(a0);
+        if (a.sums & SUM_S1) write(s1);
+        if constexpr (SHIFT) if (a.sums & SUM_S0) write(s0);
+    }
+}
 
 }  // namespace viola
