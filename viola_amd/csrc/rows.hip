@@ -25,8 +25,9 @@ struct RowsArgs {
     float* dots;
 };
 
+// ---------------------------------------------------------------------------------------------------- any width and address
 // one wavefront for each token; four tokens in a block
-template <typename T> __global__ __launch_bounds__(256) void gather_kernel(RowsArgs a) {
+template <typename T> __global__ __launch_bounds__(256) void gather_any_kernel(RowsArgs a) {
     const int lane = threadIdx.x % 64;
     for (int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; t < a.tokens; t += (int64_t)gridDim.x * 4) {
         const int* at = a.positions + t * a.top_k;
@@ -43,7 +44,7 @@ template <typename T> __global__ __launch_bounds__(256) void gather_kernel(RowsA
     }
 }
 
-template <typename T> __global__ __launch_bounds__(256) void scatter_kernel(RowsArgs a) {
+template <typename T> __global__ __launch_bounds__(256) void scatter_any_kernel(RowsArgs a) {
     const int lane = threadIdx.x % 64;
     T* out = static_cast<T*>(a.out);
     for (int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; t < a.tokens; t += (int64_t)gridDim.x * 4) {
@@ -72,13 +73,233 @@ template <typename T> __global__ __launch_bounds__(256) void scatter_kernel(Rows
     }
 }
 
+// ---------------------------------------------------------------------------------------------------- rows of whole 16-byte pieces
+// A wavefront takes PIECES pieces a lane of one token's row and the same ones of its experts' rows, CHOICES of them at a time. Which token and which
+// rows is the same for all lanes, so addresses are a scalar's work, and CHOICES * PIECES loads are in flight before the first is used.
+template <typename T> constexpr int WIDE = 16 / sizeof(T);                   // elements of a piece
+
+template <typename T> __device__ __forceinline__ void widen(const uint4& p, float (&v)[WIDE<T>]) {
+    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(w[i]);
+        } else {
+            v[2 * i] = widen16<T>(w[i] & 0xffffu);
+            v[2 * i + 1] = widen16<T>(w[i] >> 16);
+        }
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 narrow(const float (&v)[WIDE<T>]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+        else if constexpr (__is_same(T, bf16_t)) w[i] = f32_to_bf16x2_bits(v[2 * i], v[2 * i + 1]);
+        else w[i] = narrow16<T>(v[2 * i]) | narrow16<T>(v[2 * i + 1]) << 16;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A wavefront's pieces of work, `waves` in all: one, or beyond MOST_BLOCKS blocks several.
+constexpr int64_t MOST_BLOCKS = 1 << 22;
+template <typename F> __device__ __forceinline__ void each_wave(int64_t waves, F&& f) {
+    for (int64_t wave = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64); wave < waves; wave += (int64_t)gridDim.x * 4) f(wave);
+}
+unsigned blocks_for(int64_t waves) { return (unsigned)((waves + 3) / 4 < MOST_BLOCKS ? (waves + 3) / 4 : MOST_BLOCKS); }
+
+// The row of a choice, 0 with `there` false for none: the load of an absent row is that of row 0, and its values are not used.
+__device__ __forceinline__ int row_of(const RowsArgs& a, int64_t token, int j, bool& there) {
+    const int row = j < a.top_k ? a.positions[token * a.top_k + j] : -1;
+    there = row >= 0 && row < a.rows;
+    return there ? row : 0;
+}
+
+template <typename T, int CHOICES, int PIECES> __global__ __launch_bounds__(256) void gather_kernel(RowsArgs a) {
+    const int width = a.cols / WIDE<T>, cuts = (width + 64 * PIECES - 1) / (64 * PIECES);
+    each_wave(a.tokens * cuts, [&](int64_t wave) {
+        const int64_t token = wave / cuts;
+        const int first = (int)(wave % cuts) * 64 * PIECES + threadIdx.x % 64;
+        float sum[PIECES][WIDE<T>] = {};
+        for (int j0 = 0; j0 < a.top_k; j0 += CHOICES) {
+            uint4 piece[CHOICES][PIECES];
+            bool there[CHOICES];
+#pragma unroll
+            for (int j = 0; j < CHOICES; ++j) {
+                const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(a.in) + row_of(a, token, j0 + j, there[j]) * a.pitch);
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) piece[j][p] = from[first + 64 * p < width ? first + 64 * p : 0];
+            }
+#pragma unroll
+            for (int j = 0; j < CHOICES; ++j) {
+                if (!there[j]) continue;
+                const float gate = a.gates ? a.gates[token * a.top_k + j0 + j] : 1.0f;
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) {
+                    float v[WIDE<T>];
+                    widen<T>(piece[j][p], v);
+#pragma unroll
+                    for (int i = 0; i < WIDE<T>; ++i) sum[p][i] = fmaf(gate, v[i], sum[p][i]);
+                }
+            }
+        }
+        uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + token * a.cols);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+            if (first + 64 * p < width) to[first + 64 * p] = narrow<T>(sum[p]);
+    });
+}
+
+template <typename T, int PIECES> __global__ __launch_bounds__(256) void scatter_kernel(RowsArgs a) {
+    const int width = a.cols / WIDE<T>, cuts = (width + 64 * PIECES - 1) / (64 * PIECES);
+    each_wave(a.tokens * cuts, [&](int64_t wave) {
+        const int64_t token = wave / cuts;
+        const int first = (int)(wave % cuts) * 64 * PIECES + threadIdx.x % 64;
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(a.in) + token * a.pitch);
+        uint4 piece[PIECES];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) piece[p] = from[first + 64 * p < width ? first + 64 * p : 0];
+        for (int j = 0; j < a.top_k; ++j) {
+            bool there;
+            uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (int64_t)row_of(a, token, j, there) * a.cols);
+            if (!there) continue;
+            const float gate = a.gates ? a.gates[token * a.top_k + j] : 1.0f;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                uint4 word = piece[p];
+                if (a.gates) {
+                    float v[WIDE<T>];
+                    widen<T>(piece[p], v);
+#pragma unroll
+                    for (int i = 0; i < WIDE<T>; ++i) v[i] *= gate;
+                    word = narrow<T>(v);
+                }
+                if (first + 64 * p < width) to[first + 64 * p] = word;
+            }
+        }
+        // rows that no token has
+        if (a.total)
+            for (int64_t row = (*a.total > 0 ? *a.total : 0) + token; row < a.rows; row += a.tokens) {
+                uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.cols);
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p)
+                    if (first + 64 * p < width) to[first + 64 * p] = make_uint4(0, 0, 0, 0);
+            }
+    });
+}
+
+// scatter and the dots beside it: WAVES wavefronts to a token, which take its row in turn, so that a dot is summed in one place.
+template <typename T, int CHOICES, int WAVES> __global__ __launch_bounds__(256) void scatter_dots_kernel(RowsArgs a) {
+    __shared__ float parts[WAVES][CHOICES];
+    const int width = a.cols / WIDE<T>, lane = threadIdx.x % 64;
+    each_wave(a.tokens * WAVES, [&](int64_t wave) {                          // with several wavefronts a block is one token, and so all of it makes a turn
+        const int64_t token = wave / WAVES;
+        const int part = (int)(wave % WAVES);
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(a.in) + token * a.pitch);
+        for (int j0 = 0; j0 < a.top_k; j0 += CHOICES) {
+            const uint4* value[CHOICES];
+            uint4* to[CHOICES];
+            float gate[CHOICES], dot[CHOICES] = {};
+            bool there[CHOICES];
+#pragma unroll
+            for (int j = 0; j < CHOICES; ++j) {
+                const int64_t row = row_of(a, token, j0 + j, there[j]);
+                value[j] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.values) + row * a.values_pitch);
+                to[j] = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.cols);
+                gate[j] = a.gates && there[j] ? a.gates[token * a.top_k + j0 + j] : 1.0f;
+            }
+            for (int c = part * 64 + lane; c < width; c += WAVES * 64) {
+                const uint4 piece = from[c];
+                uint4 other[CHOICES];
+#pragma unroll
+                for (int j = 0; j < CHOICES; ++j) other[j] = value[j][c];
+                float v[WIDE<T>];
+                widen<T>(piece, v);
+#pragma unroll
+                for (int j = 0; j < CHOICES; ++j) {
+                    if (!there[j]) continue;
+                    float u[WIDE<T>];
+                    widen<T>(other[j], u);
+#pragma unroll
+                    for (int i = 0; i < WIDE<T>; ++i) {
+                        dot[j] = fmaf(v[i], u[i], dot[j]);
+                        u[i] = gate[j] * v[i];
+                    }
+                    if (a.out) to[j][c] = a.gates ? narrow<T>(u) : piece;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < CHOICES; ++j) {
+                dot[j] = wave_total(dot[j]);
+                if constexpr (WAVES == 1) {
+                    if (lane == 0 && j0 + j < a.top_k) a.dots[token * a.top_k + j0 + j] = dot[j];
+                } else if (lane == 0) {
+                    parts[part][j] = dot[j];
+                }
+            }
+            if constexpr (WAVES > 1) {
+                __syncthreads();
+                if ((int)threadIdx.x < CHOICES && j0 + (int)threadIdx.x < a.top_k) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w) sum += parts[w][threadIdx.x];
+                    a.dots[token * a.top_k + j0 + threadIdx.x] = sum;
+                }
+                __syncthreads();
+            }
+        }
+        if (a.out && a.total)
+            for (int64_t row = (*a.total > 0 ? *a.total : 0) + token; row < a.rows; row += a.tokens) {
+                uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.cols);
+                for (int c = part * 64 + lane; c < width; c += WAVES * 64) to[c] = make_uint4(0, 0, 0, 0);
+            }
+    });
+}
+
+// ---------------------------------------------------------------------------------------------------- launches
+bool whole_pieces(const RowsArgs& a, int dtype) {
+    const int size = viola_dtype_size(dtype);
+    for (const void* p : {a.in, a.values, (const void*)a.out})
+        if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+    return a.cols * (int64_t)size % 16 == 0 && a.pitch * size % 16 == 0 && (!a.dots || a.values_pitch * size % 16 == 0) && a.rows > 0;
+}
+
+template <typename T, int CHOICES, int PIECES> void launch_gather(const RowsArgs& a, hipStream_t stream) {
+    const int64_t cuts = (a.cols / WIDE<T> + 64 * PIECES - 1) / (64 * PIECES);
+    VIOLA_LAUNCH((gather_kernel<T, CHOICES, PIECES>), blocks_for(a.tokens * cuts), 256, 0, stream, a);
+}
+template <typename T, int PIECES> void launch_scatter(const RowsArgs& a, hipStream_t stream) {
+    const int64_t cuts = (a.cols / WIDE<T> + 64 * PIECES - 1) / (64 * PIECES);
+    VIOLA_LAUNCH((scatter_kernel<T, PIECES>), blocks_for(a.tokens * cuts), 256, 0, stream, a);
+}
+template <typename T, int CHOICES> void launch_dots(const RowsArgs& a, hipStream_t stream) {
+    if (a.tokens >= 4096 || a.cols / WIDE<T> <= 64) VIOLA_LAUNCH((scatter_dots_kernel<T, CHOICES, 1>), blocks_for(a.tokens), 256, 0, stream, a);
+    else VIOLA_LAUNCH((scatter_dots_kernel<T, CHOICES, 4>), blocks_for(a.tokens * 4), 256, 0, stream, a);
+}
+
+template <typename T> void run_gather(const RowsArgs& a, int dtype, hipStream_t stream) {
+    const bool narrow_rows = a.cols / WIDE<T> <= 64;
+    if (!whole_pieces(a, dtype)) VIOLA_LAUNCH(gather_any_kernel<T>, blocks_for(a.tokens), 256, 0, stream, a);
+    else if (a.top_k == 1) narrow_rows ? launch_gather<T, 1, 1>(a, stream) : launch_gather<T, 1, 4>(a, stream);
+    else if (a.top_k == 2) narrow_rows ? launch_gather<T, 2, 1>(a, stream) : launch_gather<T, 2, 2>(a, stream);
+    else if (a.top_k <= 4) launch_gather<T, 4, 1>(a, stream);
+    else launch_gather<T, 8, 1>(a, stream);
+}
+
+template <typename T> void run_scatter(const RowsArgs& a, int dtype, hipStream_t stream) {
+    if (!whole_pieces(a, dtype)) VIOLA_LAUNCH(scatter_any_kernel<T>, blocks_for(a.tokens), 256, 0, stream, a);
+    else if (!a.dots) a.cols / WIDE<T> <= 64 ? launch_scatter<T, 1>(a, stream) : launch_scatter<T, 2>(a, stream);
+    else if (a.top_k == 1) launch_dots<T, 1>(a, stream);
+    else if (a.top_k == 2) launch_dots<T, 2>(a, stream);
+    else if (a.top_k <= 4) launch_dots<T, 4>(a, stream);
+    else launch_dots<T, 8>(a, stream);
+}
+
 int check(const RowsArgs& a, int dtype) {
     VIOLA_CHECK_ARG(viola_is_float(dtype) && a.tokens >= 0 && a.rows >= 0 && a.top_k > 0 && a.cols > 0);
     VIOLA_CHECK_ARG(a.tokens < (1LL << 31) && a.tokens * a.top_k < (1LL << 31) && a.rows < (1LL << 31));
     return 0;
 }
-
-unsigned blocks_for(int64_t tokens) { return (unsigned)((tokens + 3) / 4 < 1 << 20 ? (tokens + 3) / 4 : 1 << 20); }
 
 }  // namespace
 
@@ -90,10 +311,9 @@ extern "C" int viola_rows_gather(const void* rows, int64_t pitch, int64_t row_co
     if (const int status = check(a, dtype)) return status;
     if (tokens == 0) return 0;
     VIOLA_CHECK_ARG(positions && out && (rows || row_count == 0) && pitch >= cols);
-    const unsigned grid = blocks_for(tokens);
-    if (dtype == VIOLA_BF16) VIOLA_LAUNCH(gather_kernel<bf16_t>, grid, 256, 0, stream, a);
-    else if (dtype == VIOLA_F16) VIOLA_LAUNCH(gather_kernel<f16_t>, grid, 256, 0, stream, a);
-    else VIOLA_LAUNCH(gather_kernel<float>, grid, 256, 0, stream, a);
+    if (dtype == VIOLA_BF16) run_gather<bf16_t>(a, dtype, stream);
+    else if (dtype == VIOLA_F16) run_gather<f16_t>(a, dtype, stream);
+    else run_gather<float>(a, dtype, stream);
     return viola_launch_status();
 }
 
@@ -105,9 +325,8 @@ extern "C" int viola_rows_scatter(const void* x, int64_t pitch, int dtype, int64
     if (const int status = check(a, dtype)) return status;
     if (tokens == 0) return 0;
     VIOLA_CHECK_ARG(positions && x && pitch >= cols && (rows || dots || row_count == 0) && (!dots || values || row_count == 0) && (!dots || values_pitch >= cols));
-    const unsigned grid = blocks_for(tokens);
-    if (dtype == VIOLA_BF16) VIOLA_LAUNCH(scatter_kernel<bf16_t>, grid, 256, 0, stream, a);
-    else if (dtype == VIOLA_F16) VIOLA_LAUNCH(scatter_kernel<f16_t>, grid, 256, 0, stream, a);
-    else VIOLA_LAUNCH(scatter_kernel<float>, grid, 256, 0, stream, a);
+    if (dtype == VIOLA_BF16) run_scatter<bf16_t>(a, dtype, stream);
+    else if (dtype == VIOLA_F16) run_scatter<f16_t>(a, dtype, stream);
+    else run_scatter<float>(a, dtype, stream);
     return viola_launch_status();
 }
