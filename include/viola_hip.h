@@ -533,7 +533,7 @@ int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, const void*
  * (where each expert's places begin), and the balance loss: the mean over sequences of `sequence` tokens of
  * experts * sum_e (choices of e / (tokens top_k)) (mean probability of e). chosen, positions, gates: [tokens, top_k]; a choice that is not there is
  * -1, -1 and a gate of 0. mask (null: all): 0 for a token that is left out, of choices, counts and loss. cost: float[tokens / sequence][experts],
- * stats: float[tokens][2] (8-byte aligned), both for the backward pass (stats null: not wanted). workspace: viola_route_workspace words of 4 bytes. experts <= 1024,
+ * 16-byte aligned, stats: float[tokens][2], 8-byte aligned, both for the backward pass (stats null: not wanted). workspace: viola_route_workspace words of 4 bytes, 16-byte aligned. experts <= 1024,
  * top_k <= 32 (VIOLA_EUNSUPPORTED beyond).
  * viola_balance_forward: loss and counts for choices made elsewhere (int32, or int64 with chosen_wide; indices out of range count nowhere).
  * viola_route_backward: dlogits [tokens, experts], contiguous, of the logits' type from the gates' and / or the loss's gradient (null: none). */
