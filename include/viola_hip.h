@@ -511,14 +511,14 @@ int viola_store_words(int64_t* dst, const int64_t* host_words, int64_t count, vi
  *
  * Backward: dout of x_dtype, dh and dy of branch_dtype, dx of x_dtype, all contiguous; a null dout is zeros, a null output is not wanted.
  * A call without dh (then before = VIOLA_NORM_NONE) is that of the form without h. Gradients of the vectors: [cols], or [groups][cols] where
- * the vector has a pitch, of the vector's type. parts: viola_norm_portions(rows, group_rows) * 4 * cols floats (fewer where fewer of the gradients are
+ * the vector has a pitch, of the vector's type. parts: viola_norm_portions(rows, cols, group_rows) * 4 * cols floats (fewer where fewer of the gradients are
  * wanted). Sums over rows are added in an order of their own that does not change from call to call. */
 int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols,
                        int after, const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
                        const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch,
                        int vector_dtype, int64_t group_rows, float residual_scale, float branch_scale, float eps, void* out, void* h, float* stats,
                        viola_stream_t stream);
-int64_t viola_norm_portions(int64_t rows, int64_t group_rows);
+int64_t viola_norm_portions(int64_t rows, int64_t cols, int64_t group_rows);
 int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols,
                         int after, const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
                         const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch,

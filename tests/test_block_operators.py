@@ -126,10 +126,11 @@ def test_norm_entry_points_refuse_what_no_kernel_takes():
 def test_norm_portions():
     from viola_amd import _lib
     portions = _lib.library().viola_norm_portions
-    assert portions(0, 1) == 0 and portions(10, 3) == 0 and portions(-1, 1) == 0
-    for rows, group in ((1, 1), (7, 7), (4096, 4096), (4096, 1), (9850, 197), (1 << 20, 1 << 10)):
-        count = portions(rows, group)
-        assert count % (rows // group) == 0 and rows // group <= count <= rows
+    assert portions(0, 8, 1) == 0 and portions(10, 8, 3) == 0 and portions(-1, 8, 1) == 0 and portions(4, 0, 4) == 0
+    for cols in (1, 64, 520, 1152, 4096, 5120, 8192, 8200, 20000):
+        for rows, group in ((1, 1), (7, 7), (4096, 4096), (4096, 1), (9850, 197), (1 << 20, 1 << 10)):
+            count = portions(rows, cols, group)
+            assert count % (rows // group) == 0 and rows // group <= count <= rows
 
 
 def _route(**changed):

@@ -116,7 +116,7 @@ def library():
         lib.viola_group_gemm_parts.argtypes, lib.viola_group_gemm_parts.restype = [_l, _l, _l], ctypes.c_int
         lib.viola_group_gemm_form.argtypes, lib.viola_group_gemm_form.restype = [_l, _l, _l, _i, _i, _i], ctypes.c_int
         lib.viola_scaled_gemm_form.argtypes, lib.viola_scaled_gemm_form.restype = [_l, _l, _l], ctypes.c_int
-        lib.viola_norm_portions.argtypes, lib.viola_norm_portions.restype = [_l, _l], ctypes.c_int64
+        lib.viola_norm_portions.argtypes, lib.viola_norm_portions.restype = [_l, _l, _l], ctypes.c_int64
         lib.viola_route_workspace.argtypes, lib.viola_route_workspace.restype = [_l, _l, _l], ctypes.c_int64
         lib.viola_ns_plan.argtypes, lib.viola_ns_plan.restype = [_l, _l, _l, _l, _i, _i, _i, ctypes.POINTER(ctypes.c_int)], ctypes.c_int
         lib.viola_ns_plan_many.argtypes, lib.viola_ns_plan_many.restype = [_p, _i, ctypes.POINTER(ctypes.c_int)], ctypes.c_int

@@ -254,7 +254,7 @@ variable_list NormBackward::apply(variable_list&& grads) {
         // the sums over rows that the wanted gradients are made of
         const int sums = (wanted[AFTER_WEIGHT] || wanted[GATE]) + (wanted[AFTER_BIAS] || (wanted[GATE] && has[AFTER_BIAS])) + (wanted[WEIGHT] || wanted[SCALE]) +
                          (wanted[BIAS] || wanted[SHIFT] || (wanted[SCALE] && has[BIAS]));
-        const int64_t floats = viola_norm_portions(rows, rows / plan.groups) * sums * cols;
+        const int64_t floats = viola_norm_portions(rows, cols, rows / plan.groups) * sums * cols;
         const Tensor parts = sums ? at::empty({floats}, options.dtype(at::kFloat)) : Tensor();
         for (int i = AFTER_WEIGHT; i < INPUTS; ++i)
             if (has[i]) t[i] = plan.readable(i, t[i], cols);

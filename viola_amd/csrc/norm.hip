@@ -156,29 +156,49 @@ struct ReduceArgs {
     // one for all rows (vectors with a pitch of 0 too), or one for each group
     void *d_after_weight, *d_after_bias, *d_weight, *d_bias, *d_gate, *d_scale, *d_shift;
     int gate_by_group, scale_by_group, shift_by_group;
+    int whole;                                                               // sections for gradients summed over all rows: 1 or 0
 };
 
+constexpr int BLOCKS_PER_SLOT = 1;
 constexpr int SLICES = 32;                                                   // of the portions, by 32 columns: 1024 threads
 
-// blockIdx.y 0: what is summed over all rows, 32 columns by 32 contiguous slices of the portions, the slices then added in order.
-// blockIdx.y > 0: what is summed group by group, 32 columns by 32 groups.
+struct Sums { float a1, a0, s1, s0; };
+
+// The wanted sums of one portion; `at`: where in the portion each lies.
+struct PortionLayout {
+    int sums, a0, s1, s0;
+    int64_t stride;
+    __device__ __forceinline__ PortionLayout(const ReduceArgs& a)
+        : sums(a.sums), a0(__popc(a.sums & SUM_A1) * a.cols), s1(__popc(a.sums & (SUM_A1 | SUM_A0)) * a.cols), s0(__popc(a.sums & (SUM_A1 | SUM_A0 | SUM_S1)) * a.cols),
+          stride((int64_t)__popc(a.sums) * a.cols) {}
+    __device__ __forceinline__ Sums load(const float* from) const {
+        Sums v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (sums & SUM_A1) v.a1 = from[0];
+        if (sums & SUM_A0) v.a0 = from[a0];
+        if (sums & SUM_S1) v.s1 = from[s1];
+        if (sums & SUM_S0) v.s0 = from[s0];
+        return v;
+    }
+};
+
+// Sections of blocks (blockIdx.y). `whole` of them, 1 or 0: what is summed over all rows, 32 columns by 32 contiguous slices of the portions,
+// the slices then added in order. The others: what is summed group by group, 32 columns by 32 groups.
 __global__ __launch_bounds__(1024) void norm_reduce_kernel(ReduceArgs a) {
     __shared__ float piece[SLICES][8][33];
+    constexpr int TOGETHER = 4;                                              // portions whose loads are under way together
     const int c = threadIdx.x % 32, slice = threadIdx.x / 32, col = blockIdx.x * 32 + c;
-    const int count = __popc(a.sums);
-    const int at_a0 = __popc(a.sums & SUM_A1), at_s1 = __popc(a.sums & (SUM_A1 | SUM_A0)), at_s0 = __popc(a.sums & (SUM_A1 | SUM_A0 | SUM_S1));
+    const PortionLayout layout(a);
     const bool in = col < a.cols;
     auto vector = [&](const void* data, int64_t at, int dtype, float absent) { return data && in ? load_float(data, at + col, dtype) : absent; };
-    if (blockIdx.y) {
-        const int64_t group = (int64_t)(blockIdx.y - 1) * 32 + slice;
+    if ((int)blockIdx.y >= a.whole) {
+        const int64_t group = (int64_t)(blockIdx.y - a.whole) * 32 + slice;
         if (!in || group >= a.portions / a.per_group) return;
         float a1 = 0.0f, a0 = 0.0f, s1 = 0.0f, s0 = 0.0f;
-        for (int64_t p = group * a.per_group; p < (group + 1) * a.per_group; ++p) {
-            const float* from = a.parts + p * count * a.cols + col;
-            if (a.sums & SUM_A1) a1 += from[0];
-            if (a.sums & SUM_A0) a0 += from[at_a0 * a.cols];
-            if (a.sums & SUM_S1) s1 += from[at_s1 * a.cols];
-            if (a.sums & SUM_S0) s0 += from[at_s0 * a.cols];
+        const float* from = a.parts + group * a.per_group * layout.stride + col;
+#pragma unroll 4
+        for (int64_t p = 0; p < a.per_group; ++p) {
+            const Sums v = layout.load(from + p * layout.stride);
+            a1 += v.a1; a0 += v.a0; s1 += v.s1; s0 += v.s0;
         }
         const int64_t to = group * a.cols + col;
         const float w_a = vector(a.after_weight, 0, a.weight_dtype, 1.0f), b_a = vector(a.after_bias, 0, a.weight_dtype, 0.0f);
@@ -193,21 +213,36 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(ReduceArgs a) {
     if (in) {
         const int64_t per = (a.portions + SLICES - 1) / SLICES;
         const int64_t begin = slice * per, end = begin + per < a.portions ? begin + per : a.portions;
-        for (int64_t p = begin; p < end; ++p) {
-            const float* from = a.parts + p * count * a.cols + col;
-            const int64_t group = p / a.per_group;
-            const float g = vector(a.gate.data, group * a.gate.pitch, a.vector_dtype, 1.0f), s = 1.0f + vector(a.scale.data, group * a.scale.pitch, a.vector_dtype, 0.0f);
-            const float a1 = a.sums & SUM_A1 ? from[0] : 0.0f, a0 = a.sums & SUM_A0 ? from[at_a0 * a.cols] : 0.0f;
-            const float s1 = a.sums & SUM_S1 ? from[at_s1 * a.cols] : 0.0f, s0 = a.sums & SUM_S0 ? from[at_s0 * a.cols] : 0.0f;
-            sum[0] += a1; sum[1] += a0; sum[2] += s1; sum[3] += s0;
-            sum[4] = fmaf(g, a1, sum[4]); sum[5] = fmaf(g, a0, sum[5]); sum[6] = fmaf(s, s1, sum[6]); sum[7] = fmaf(s, s0, sum[7]);
+        const bool gates = a.gate.pitch != 0, scales = a.scale.pitch != 0;   // one for each group: loaded with each portion
+        const float all_g = vector(a.gate.data, 0, a.vector_dtype, 1.0f), all_s = 1.0f + vector(a.scale.data, 0, a.vector_dtype, 0.0f);
+        auto gate_of = [&](int64_t p) { return gates ? vector(a.gate.data, (uint32_t)p / (uint32_t)a.per_group * a.gate.pitch, a.vector_dtype, 1.0f) : all_g; };
+        auto scale_of = [&](int64_t p) { return scales ? 1.0f + vector(a.scale.data, (uint32_t)p / (uint32_t)a.per_group * a.scale.pitch, a.vector_dtype, 0.0f) : all_s; };
+        auto add = [&](const Sums& v, float g, float s) {
+            sum[0] += v.a1; sum[1] += v.a0; sum[2] += v.s1; sum[3] += v.s0;
+            sum[4] = fmaf(g, v.a1, sum[4]); sum[5] = fmaf(g, v.a0, sum[5]); sum[6] = fmaf(s, v.s1, sum[6]); sum[7] = fmaf(s, v.s0, sum[7]);
+        };
+        const float* from = a.parts + begin * layout.stride + col;
+        int64_t p = begin;
+        for (; p + TOGETHER <= end; p += TOGETHER, from += TOGETHER * layout.stride) {
+            Sums v[TOGETHER];
+            float g[TOGETHER], s[TOGETHER];
+#pragma unroll
+            for (int u = 0; u < TOGETHER; ++u) {
+                v[u] = layout.load(from + u * layout.stride);
+                g[u] = gate_of(p + u);
+                s[u] = scale_of(p + u);
+            }
+#pragma unroll
+            for (int u = 0; u < TOGETHER; ++u) add(v[u], g[u], s[u]);
         }
+        for (; p < end; ++p, from += layout.stride) add(layout.load(from), gate_of(p), scale_of(p));
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) piece[slice][i][c] = sum[i];
     __syncthreads();
     if (slice < 8) {
         float total = piece[0][slice][c];
+#pragma unroll 8
         for (int u = 1; u < SLICES; ++u) total += piece[u][slice][c];
         piece[0][slice][c] = total;                                          // read by this thread only until the next barrier
     }
@@ -230,7 +265,7 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(ReduceArgs a) {
 }
 
 // Whether rows of these types, this width and these addresses are held in registers, in pieces of eight elements; then f(stream type, branch type).
-template <typename F> bool in_registers(const NormArgs& a, std::initializer_list<const void*> tensors, F&& f) {
+template <typename F> bool in_registers(NormArgs& a, std::initializer_list<const void*> tensors, F&& f) {
     if (a.cols % 8 || a.cols > ROW_COLUMNS || a.x_pitch % 8 || (a.y && a.y_pitch % 8)) return false;
     for (const void* p : tensors)
         if (reinterpret_cast<uintptr_t>(p) % 16) return false;
@@ -238,6 +273,7 @@ template <typename F> bool in_registers(const NormArgs& a, std::initializer_list
         if (reinterpret_cast<uintptr_t>(p) % 16) return false;
     for (const NormVector& v : {a.gate, a.scale, a.shift})
         if (v.pitch % 8) return false;
+    a.team = (a.cols + 511) / 512 * 64;
     const int x = a.x_dtype, y = a.branch_dtype;
     if (x == VIOLA_BF16 && y == VIOLA_BF16) f(bf16_t(), bf16_t());
     else if (x == VIOLA_F16 && y == VIOLA_F16) f(f16_t(), f16_t());
@@ -247,12 +283,20 @@ template <typename F> bool in_registers(const NormArgs& a, std::initializer_list
     else return false;
     return true;
 }
-int team_of(int cols) { return (cols + 511) / 512 * 64; }
+void stream(NormArgs& a, int64_t bytes_in, int64_t bytes_out) {
+    a.stream_in = bytes_in > STREAM_IN;
+    a.stream_out = bytes_out > STREAM_OUT;
+}
+bool plain(const NormArgs& a) { return a.after == VIOLA_NORM_NONE && !a.after_weight && !a.after_bias; }
 
-// A portion for every block that the chip holds at once, and no group's rows split finer than one by one.
-int64_t portions_per_group(int64_t rows, int64_t group_rows) {
-    const int64_t groups = rows / group_rows, wanted = (512 + groups - 1) / groups;
-    return wanted < group_rows ? wanted : group_rows;
+// A portion for every block that the chip holds at once (16 wavefronts a CU), of two rows for each of its teams at least, and of no more than one group.
+int64_t portions_per_group(int64_t rows, int64_t group_rows, int64_t cols) {
+    NormArgs a = {};
+    a.team = (int)((cols + 511) / 512 * 64);
+    const bool registers = cols <= ROW_COLUMNS;
+    const int64_t block = registers ? norm_block(a) : 1024, least = registers ? 2 * (block / a.team) : 1;
+    const int64_t groups = rows / group_rows, wanted = (256 * (1024 / block) + groups - 1) / groups, most = (group_rows + least - 1) / least;
+    return wanted < most ? wanted : most;
 }
 
 bool valid_rows(const void* p, int64_t pitch, int64_t cols) { return p && pitch >= cols; }
@@ -281,7 +325,7 @@ extern "C" int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, c
                                   const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
                                   const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch, int vector_dtype,
                                   int64_t group_rows, float residual_scale, float branch_scale, float eps, void* out, void* h, float* stats, viola_stream_t stream_) {
-    hipStream_t stream = viola_enter(stream_);
+    hipStream_t hip_stream = viola_enter(stream_);
     NormArgs a = {};
     const int status = set_common(a, x, x_pitch, x_dtype, y, y_pitch, branch_dtype, rows, cols, after, after_weight, after_bias, before, weight, bias, weight_dtype, gate,
                                   gate_pitch, scale, scale_pitch, shift, shift_pitch, vector_dtype, group_rows, residual_scale, branch_scale, eps);
@@ -289,20 +333,24 @@ extern "C" int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, c
     if (rows == 0) return 0;
     VIOLA_CHECK_ARG(valid_rows(x, x_pitch, cols) && (out || h) && (out != nullptr) == (y != nullptr) && (!y || y_pitch >= cols));
     VIOLA_CHECK_ARG((h != nullptr) == (before != VIOLA_NORM_NONE) && (reinterpret_cast<uintptr_t>(stats) % 16) == 0);
-    const int form = !y ? FORM_BEFORE : h ? FORM_BETWEEN : FORM_AFTER;
+    const int form = !y ? FORM_BEFORE : !h ? FORM_AFTER : plain(a) ? FORM_PLAIN : FORM_BETWEEN;
     a.out = out; a.h = h; a.stats = reinterpret_cast<float4*>(stats);
-    a.team = team_of((int)cols);
-    const int64_t blocks = 2048, teams = a.team >= 512 ? 1 : 512 / a.team;
-    a.chunk = ((rows + blocks - 1) / blocks + teams - 1) / teams * teams;
-    const dim3 grid((unsigned)((rows + a.chunk - 1) / a.chunk));
-    if (in_registers(a, {x, y, out, h}, [&](auto tx, auto ty) { norm_forward_rows<decltype(tx), decltype(ty)>(a, form, grid, stream); })) return viola_launch_status();
-    VIOLA_LAUNCH(norm_forward_any_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), 256, 0, stream, a);
+    if (in_registers(a, {x, y, out, h}, [&](auto tx, auto ty) {
+            // as many blocks as the chip holds at once by their registers, BLOCKS_PER_SLOT times: each loads the vectors along the row once
+            const int64_t block = norm_block(a), teams = block / a.team, waves = form == FORM_BETWEEN ? 16 : 20, held = waves * 64 / block;
+            const int64_t blocks = 256 * (held ? held : 1) * BLOCKS_PER_SLOT;
+            a.chunk = ((rows + blocks - 1) / blocks + teams - 1) / teams * teams;
+            stream(a, rows * cols * ((int)sizeof(tx) + (y ? (int)sizeof(ty) : 0)), rows * cols * ((out ? (int)sizeof(tx) : 0) + (h ? (int)sizeof(ty) : 0)));
+            norm_forward_rows<decltype(tx), decltype(ty)>(a, form, dim3((unsigned)((rows + a.chunk - 1) / a.chunk)), hip_stream);
+        }))
+        return viola_launch_status();
+    VIOLA_LAUNCH(norm_forward_any_kernel, dim3((unsigned)(rows < 65536 ? rows : 65536)), 256, 0, hip_stream, a);
     return viola_launch_status();
 }
 
-extern "C" int64_t viola_norm_portions(int64_t rows, int64_t group_rows) {
-    if (rows <= 0 || group_rows <= 0 || rows % group_rows) return 0;
-    return rows / group_rows * portions_per_group(rows, group_rows);
+extern "C" int64_t viola_norm_portions(int64_t rows, int64_t cols, int64_t group_rows) {
+    if (rows <= 0 || cols <= 0 || group_rows <= 0 || rows % group_rows) return 0;
+    return rows / group_rows * portions_per_group(rows, group_rows, cols);
 }
 
 extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols, int after,
@@ -311,7 +359,7 @@ extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, 
                                    int64_t group_rows, float residual_scale, float branch_scale, const float* stats, const void* dout, const void* dh, void* dx, void* dy,
                                    float* parts, int64_t parts_floats, void* d_after_weight, void* d_after_bias, void* d_weight, void* d_bias, void* d_gate,
                                    void* d_scale, void* d_shift, viola_stream_t stream_) {
-    hipStream_t stream = viola_enter(stream_);
+    hipStream_t hip_stream = viola_enter(stream_);
     NormArgs a = {};
     const int status = set_common(a, x, x_pitch, x_dtype, y, y_pitch, branch_dtype, rows, cols, after, after_weight, after_bias, before, weight, bias, weight_dtype, gate,
                                   gate_pitch, scale, scale_pitch, shift, shift_pitch, vector_dtype, group_rows, residual_scale, branch_scale, 0.0f);
@@ -326,29 +374,34 @@ extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, 
     a.dout = dout; a.dh = dh; a.dx = dx; a.dy = dy; a.parts = parts;
     a.sums = (d_after_weight || gate_sums ? SUM_A1 : 0) | (d_after_bias || (gate_sums && after_bias) ? SUM_A0 : 0) | (d_weight || scale_sums ? SUM_S1 : 0) |
              (d_bias || d_shift || (scale_sums && bias) ? SUM_S0 : 0);
-    a.per_group = rows ? portions_per_group(rows, group_rows) : 1;
+    a.per_group = rows ? portions_per_group(rows, group_rows, cols) : 1;
     a.portions = rows ? rows / group_rows * a.per_group : 0;
     if (a.sums && rows) VIOLA_CHECK_ARG(parts && parts_floats >= a.portions * __builtin_popcount((unsigned)a.sums) * cols);
     const bool grouped = (d_gate && gate_pitch) || (d_scale && scale_pitch) || (d_shift && shift_pitch);
-    const int64_t sections = 1 + (grouped ? (rows / group_rows + 31) / 32 : 0);
+    const bool whole = d_after_weight || d_after_bias || d_weight || d_bias || (d_gate && !gate_pitch) || (d_scale && !scale_pitch) || (d_shift && !shift_pitch);
+    const int64_t sections = whole + (grouped ? (rows / group_rows + 31) / 32 : 0);
     if (sections > 65535) return VIOLA_EUNSUPPORTED;
     if (rows) {
         const dim3 grid((unsigned)(a.portions < 65536 ? a.portions : 65536));
-        const int form = !y ? FORM_BEFORE : dh ? FORM_BETWEEN : FORM_AFTER;
+        const int form = !y ? FORM_BEFORE : !dh ? FORM_AFTER : plain(a) ? FORM_PLAIN : FORM_BETWEEN;
         const bool with_bias = after_bias || (a.sums & SUM_A0), with_shift = (a.sums & SUM_S0) != 0;
-        a.team = team_of((int)cols);
-        if (!in_registers(a, {x, y, dout, dh, dx, dy, parts}, [&](auto tx, auto ty) { norm_backward_rows<decltype(tx), decltype(ty)>(a, form, with_bias, with_shift, grid, stream); }))
-            VIOLA_LAUNCH(norm_backward_any_kernel, grid, 256, 0, stream, a);
+        if (!in_registers(a, {x, y, dout, dh, dx, dy, parts}, [&](auto tx, auto ty) {
+                const int64_t n = rows * cols, x_size = sizeof(tx), y_size = sizeof(ty);
+                stream(a, n * ((dh ? x_size + y_size : 0) + (y ? y_size : 0) + (dout ? x_size : 0)), n * ((dx ? x_size : 0) + (dy ? y_size : 0)));
+                norm_backward_rows<decltype(tx), decltype(ty)>(a, form, with_bias, with_shift, grid, hip_stream);
+            }))
+            VIOLA_LAUNCH(norm_backward_any_kernel, grid, 256, 0, hip_stream, a);
     }
-    if (a.sums) {
+    if (sections) {
         ReduceArgs r = {};
+        r.whole = whole;
         r.parts = parts; r.portions = a.portions; r.per_group = a.per_group; r.cols = (int)cols; r.sums = a.sums;
         r.weight_dtype = weight_dtype; r.vector_dtype = vector_dtype; r.alpha = branch_scale;
         r.after_weight = after_weight; r.after_bias = after_bias; r.weight = weight; r.bias = bias; r.gate = a.gate; r.scale = a.scale;
         r.d_after_weight = d_after_weight; r.d_after_bias = d_after_bias; r.d_weight = d_weight; r.d_bias = d_bias;
         r.d_gate = d_gate; r.d_scale = d_scale; r.d_shift = d_shift;
         r.gate_by_group = gate_pitch != 0; r.scale_by_group = scale_pitch != 0; r.shift_by_group = shift_pitch != 0;
-        VIOLA_LAUNCH(norm_reduce_kernel, dim3((unsigned)((cols + 31) / 32), (unsigned)sections), 1024, 0, stream, r);
+        VIOLA_LAUNCH(norm_reduce_kernel, dim3((unsigned)((cols + 31) / 32), (unsigned)sections), 1024, 0, hip_stream, r);
     }
     return viola_launch_status();
 }

@@ -15,9 +15,12 @@
 
 #include "block_ops.hpp"
 
+#include <type_traits>
+
 namespace viola {
 
-enum { FORM_BEFORE = 0, FORM_AFTER = 1, FORM_BETWEEN = 2 };
+// FORM_PLAIN: FORM_BETWEEN without a norm, weight or bias after the block: x' = rho x + alpha g y
+enum { FORM_BEFORE = 0, FORM_AFTER = 1, FORM_BETWEEN = 2, FORM_PLAIN = 3 };
 enum { SUM_A1 = 1, SUM_A0 = 2, SUM_S1 = 4, SUM_S0 = 8 };
 
 // A vector along the row: one for all rows (pitch 0), or one for each group of rows.
@@ -38,6 +41,7 @@ struct NormArgs {
     float4* stats;                                                           // mu_y, r_y, mu_x, r_x of a row
     int64_t chunk;                                                           // rows of a block
     int team;                                                                // threads of a row, where rows are in registers
+    bool stream_in, stream_out;                                              // rows are read, written past the caches' order
     // backward
     const void *dout, *dh;
     void *dx, *dy;
@@ -56,12 +60,15 @@ constexpr int ROW_THREADS = 1024, ROW_COLUMNS = 8 * ROW_THREADS;
 
 template <typename T> struct Piece { uint4 word[sizeof(T) / 2]; };           // eight elements as they lie in memory
 
-// `row` elements behind `base` for a whole wavefront, `col` more for a thread: the first is a scalar's work.
-template <typename T> __device__ __forceinline__ Piece<T> load_piece(const void* base, int64_t row, int col) {
-    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(base) + row + col);
+// Streamed or not (block_ops.hpp); 32-bit pieces never are: an access of a wavefront is every other 16 bytes of them, which streamed fill no line
+// (4 x 2048 rows of 2048 on a 32-bit stream: 56 instead of 45 us).
+// `row` elements behind `base` for a whole wavefront, `col` more for a thread: the first is a scalar's work, the second an offset of 32 bits.
+template <typename T, bool STREAM> __device__ __forceinline__ Piece<T> load_piece(const void* base, int64_t row, uint32_t col) {
+    const char* line = static_cast<const char*>(base) + row * (int64_t)sizeof(T);
+    const uint4* from = reinterpret_cast<const uint4*>(line + col * (uint32_t)sizeof(T));
     Piece<T> p;
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) p.word[i] = from[i];
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) p.word[i] = load16<STREAM && sizeof(T) == 2>(from + i);
     return p;
 }
 template <typename T> __device__ __forceinline__ void widen_piece(const Piece<T>& p, float (&v)[8]) {
@@ -85,90 +92,159 @@ template <typename T> __device__ __forceinline__ void widen_piece(const Piece<T>
         }
     }
 }
-template <typename T> __device__ __forceinline__ void store_piece(void* base, int64_t row, int col, const float (&v)[8]) {
-    uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(base) + row + col);
+template <typename T> __device__ __forceinline__ void store_piece(void* base, int64_t row, uint32_t col, const float (&v)[8], bool stream) {
+    char* line = static_cast<char*>(base) + row * (int64_t)sizeof(T);
+    uint4* to = reinterpret_cast<uint4*>(line + col * (uint32_t)sizeof(T));
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            to[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+            store16(to + i, make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])), false);
     } else if constexpr (__is_same(T, bf16_t)) {
-        *to = make_uint4(f32_to_bf16x2_bits(v[0], v[1]), f32_to_bf16x2_bits(v[2], v[3]), f32_to_bf16x2_bits(v[4], v[5]), f32_to_bf16x2_bits(v[6], v[7]));
+        store16(to, make_uint4(f32_to_bf16x2_bits(v[0], v[1]), f32_to_bf16x2_bits(v[2], v[3]), f32_to_bf16x2_bits(v[4], v[5]), f32_to_bf16x2_bits(v[6], v[7])), stream);
     } else {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = narrow16<f16_t>(v[2 * i]) | narrow16<f16_t>(v[2 * i + 1]) << 16;
-        *to = make_uint4(w[0], w[1], w[2], w[3]);
+        store16(to, make_uint4(w[0], w[1], w[2], w[3]), stream);
     }
 }
 
-// Eight elements of a vector of any type; `absent` where there is none.
-__device__ __forceinline__ void load_vector(const void* base, int64_t row, int col, int dtype, bool in, float absent, float (&v)[8]) {
+// Eight elements of a vector of any type, as they lie in memory: 32 bytes, or 16 and nothing.
+struct VectorPiece {
+    uint4 word[2] = {};
+    __device__ __forceinline__ void load(const void* base, int64_t row, uint32_t col, int dtype, bool in) {
+        if (!base || !in) return;
+        const char* line = static_cast<const char*>(base) + (dtype == VIOLA_F32 ? row * 4 : row * 2);
+        const uint4* from = reinterpret_cast<const uint4*>(line + (dtype == VIOLA_F32 ? col * 4 : col * 2));
+        word[0] = from[0];
+        if (dtype == VIOLA_F32) word[1] = from[1];
+    }
+    __device__ __forceinline__ void widen(const void* base, int dtype, bool in, float absent, float (&v)[8]) const {
+        if (!base || !in) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = absent;
-    if (base && in) {
-        if (dtype == VIOLA_F32) widen_piece(load_piece<float>(base, row, col), v);
-        else if (dtype == VIOLA_BF16) widen_piece(load_piece<bf16_t>(base, row, col), v);
-        else widen_piece(load_piece<f16_t>(base, row, col), v);
+            for (int i = 0; i < 8; ++i) v[i] = absent;
+        } else if (dtype == VIOLA_F32) {
+            widen_piece(Piece<float>{{word[0], word[1]}}, v);
+        } else if (dtype == VIOLA_BF16) {
+            widen_piece(Piece<bf16_t>{{word[0]}}, v);
+        } else {
+            widen_piece(Piece<f16_t>{{word[0]}}, v);
+        }
     }
-    __builtin_amdgcn_sched_barrier(0);                                       // one vector after the other: together they would take every register
-}
+};
 
-// Sums over the wavefronts of a team: those of BlockSums with the slots of the own team only. All teams of a block call it alike.
+// Sums over the wavefronts of a team of up to 16, in all of its threads: each wavefront's own in LDS, two sets of slots in turn (see
+// BlockSums), and from there in the 16 lanes of a row at once. All teams of a block call it alike.
 struct TeamSums {
     float2* slot;                                                            // two sets of 16 in LDS
-    int waves, first, wave, turn = 0;
-    __device__ __forceinline__ TeamSums(float2* slot, int waves) : slot(slot), waves(waves), first(threadIdx.x / 64 / waves * waves), wave(threadIdx.x / 64) {}
+    int waves, wave, mine, turn = 0;
+    __device__ __forceinline__ TeamSums(float2* slot, int waves) : slot(slot), waves(waves), wave(threadIdx.x / 64) {
+        const int other = threadIdx.x % 16;
+        mine = other < waves ? wave / waves * waves + other : -1;            // whose sum this lane fetches
+    }
+    static __device__ __forceinline__ float over_row(float v) {
+        v = dpp_add<0xB1>(v);
+        v = dpp_add<0x4E>(v);
+        v = dpp_add<0x141>(v);
+        return dpp_add<0x140>(v);
+    }
     __device__ __forceinline__ float2 both(float a, float b) {
         a = wave_total(a);
         b = wave_total(b);
         if (waves == 1) return make_float2(a, b);
         if (threadIdx.x % 64 == 0) slot[turn * 16 + wave] = make_float2(a, b);
         __syncthreads();
-        float2 sum = slot[turn * 16 + first];
-        for (int w = first + 1; w < first + waves; ++w) {
-            sum.x += slot[turn * 16 + w].x;
-            sum.y += slot[turn * 16 + w].y;
-        }
+        const float2 v = mine < 0 ? make_float2(0.0f, 0.0f) : slot[turn * 16 + mine];
         turn ^= 1;
-        return sum;
+        return make_float2(over_row(v.x), over_row(v.y));
     }
     __device__ __forceinline__ float one(float a) {
         a = wave_total(a);
         if (waves == 1) return a;
         if (threadIdx.x % 64 == 0) slot[turn * 16 + wave].x = a;
         __syncthreads();
-        float sum = slot[turn * 16 + first].x;
-        for (int w = first + 1; w < first + waves; ++w) sum += slot[turn * 16 + w].x;
+        const float v = mine < 0 ? 0.0f : slot[turn * 16 + mine].x;
         turn ^= 1;
-        return sum;
+        return over_row(v);
+    }
+    // s / n for inverse = 1 / n, but for the last place
+    static __device__ __forceinline__ float quotient(float s, float n, float inverse) {
+        const float near = s * inverse;
+        return fmaf(fmaf(-near, n, s), inverse, near);
+    }
+    // The mean of a row and the sum of squares around it: each wavefront around its own mean first, those then moved to the row's. A row far from
+    // zero keeps its digits, and the team meets once. columns: of the row, of which a wavefront has up to 512.
+    __device__ __forceinline__ float2 around_mean(const float (&v)[8], bool in, int columns, float inverse) {
+        const int here = columns - (wave % waves) * 512, other = columns - (threadIdx.x % 16) * 512;
+        float s = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
+        s = wave_total(in ? s : 0.0f);
+        const float mean = s * __builtin_amdgcn_rcpf((float)(here < 512 ? here : 512));      // any value near it serves
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q = fmaf(v[i] - mean, v[i] - mean, q);
+        q = wave_total(in ? q : 0.0f);
+        if (waves == 1) {
+            const float exact = quotient(s, (float)columns, inverse), off = exact - mean;
+            return make_float2(exact, q - (float)columns * off * off);
+        }
+        if (threadIdx.x % 64 == 0) slot[turn * 16 + wave] = make_float2(s, q);
+        __syncthreads();
+        float2 w = mine < 0 ? make_float2(0.0f, 0.0f) : slot[turn * 16 + mine];
+        turn ^= 1;
+        const float row_mean = quotient(over_row(w.x), (float)columns, inverse);
+        if (mine >= 0) {
+            const float n = (float)(other < 512 ? other : 512), near = w.x * __builtin_amdgcn_rcpf(n);
+            // around `near`, which is the wavefront's mean but for its last digits, and from there around the row's
+            const float off = near - row_mean;
+            w.y += n * off * off + 2.0f * off * fmaf(-n, near, w.x);
+        }
+        return make_float2(row_mean, over_row(w.y));
     }
 };
 
-__device__ __forceinline__ float2 row_statistics(const float (&v)[8], bool in, int kind, float inverse, float eps, TeamSums& sums) {
-    float mean = 0.0f;
-    if (kind == VIOLA_NORM_LAYER) {
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += v[i];
-        mean = sums.one(in ? s : 0.0f) * inverse;
+// v^-1/2 within an ulp; the hardware's root reads what is below the normal numbers as zero.
+__device__ __forceinline__ float inverse_root(float v) { return v < 1e-30f ? 1.0f / sqrtf(v) : __builtin_amdgcn_rsqf(v); }
+
+template <bool LAYER> __device__ __forceinline__ float2 row_statistics(const float (&v)[8], bool in, int kind, int columns, float inverse, float eps, TeamSums& sums) {
+    if (LAYER && kind == VIOLA_NORM_LAYER) {
+        const float2 around = sums.around_mean(v, in, columns, inverse);
+        return make_float2(around.x, inverse_root(around.y * inverse + eps));
     }
     float q = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float d = v[i] - mean;
-        q = fmaf(d, d, q);
-    }
-    return make_float2(mean, 1.0f / sqrtf(sums.one(in ? q : 0.0f) * inverse + eps));
+    for (int i = 0; i < 8; ++i) q = fmaf(v[i], v[i], q);
+    return make_float2(0.0f, inverse_root(sums.one(in ? q : 0.0f) * inverse + eps));
 }
 
+// All loads are under way before the first is used: a block waits for them once.
 template <int FORM> struct NormVectors {
     float ga[8], gb[8], w[8], b[8];
-    __device__ __forceinline__ void load(const NormArgs& a, int64_t group, int col, bool in) {
+    __device__ __forceinline__ void load(const NormArgs& a, int64_t group, uint32_t col, bool in) {
+        VectorPiece gate, after_weight, after_bias, weight, bias, scale, shift;
+        if constexpr (FORM == FORM_PLAIN) gate.load(a.gate.data, group * a.gate.pitch, col, a.vector_dtype, in);
+        if constexpr (FORM == FORM_AFTER || FORM == FORM_BETWEEN) {
+            after_weight.load(a.after_weight, 0, col, a.weight_dtype, in);
+            after_bias.load(a.after_bias, 0, col, a.weight_dtype, in);
+            gate.load(a.gate.data, group * a.gate.pitch, col, a.vector_dtype, in);
+        }
+        if constexpr (FORM != FORM_AFTER) {
+            weight.load(a.weight, 0, col, a.weight_dtype, in);
+            bias.load(a.bias, 0, col, a.weight_dtype, in);
+            scale.load(a.scale.data, group * a.scale.pitch, col, a.vector_dtype, in);
+            shift.load(a.shift.data, group * a.shift.pitch, col, a.vector_dtype, in);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         float u[8];
-        if constexpr (FORM != FORM_BEFORE) {
-            load_vector(a.after_weight, 0, col, a.weight_dtype, in, 1.0f, ga);
-            load_vector(a.after_bias, 0, col, a.weight_dtype, in, 0.0f, gb);
-            load_vector(a.gate.data, group * a.gate.pitch, col, a.vector_dtype, in, 1.0f, u);
+        if constexpr (FORM == FORM_PLAIN) {
+            gate.widen(a.gate.data, a.vector_dtype, in, 1.0f, ga);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ga[i] *= a.alpha;
+        }
+        if constexpr (FORM == FORM_AFTER || FORM == FORM_BETWEEN) {
+            after_weight.widen(a.after_weight, a.weight_dtype, in, 1.0f, ga);
+            after_bias.widen(a.after_bias, a.weight_dtype, in, 0.0f, gb);
+            gate.widen(a.gate.data, a.vector_dtype, in, 1.0f, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 ga[i] *= a.alpha * u[i];
@@ -176,15 +252,15 @@ template <int FORM> struct NormVectors {
             }
         }
         if constexpr (FORM != FORM_AFTER) {
-            load_vector(a.weight, 0, col, a.weight_dtype, in, 1.0f, w);
-            load_vector(a.bias, 0, col, a.weight_dtype, in, 0.0f, b);
-            load_vector(a.scale.data, group * a.scale.pitch, col, a.vector_dtype, in, 0.0f, u);
+            weight.widen(a.weight, a.weight_dtype, in, 1.0f, w);
+            bias.widen(a.bias, a.weight_dtype, in, 0.0f, b);
+            scale.widen(a.scale.data, a.vector_dtype, in, 0.0f, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 w[i] = fmaf(w[i], u[i], w[i]);
                 b[i] = fmaf(b[i], u[i], b[i]);
             }
-            load_vector(a.shift.data, group * a.shift.pitch, col, a.vector_dtype, in, 0.0f, u);
+            shift.widen(a.shift.data, a.vector_dtype, in, 0.0f, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) b[i] += u[i];
         }
@@ -192,24 +268,30 @@ template <int FORM> struct NormVectors {
 };
 
 // The rows [blockIdx.x chunk, + chunk), a team each in turn. Every team makes as many turns as the first, so that barriers meet.
-template <typename TX, typename TY, int FORM> __global__ __launch_bounds__(ROW_THREADS) void norm_forward_kernel(NormArgs a) {
+// LAYER: one of the norms subtracts a mean; without it the kinds are known to be the root mean square.
+template <typename TX, typename TY, int FORM, bool LAYER> __global__ __launch_bounds__(ROW_THREADS) void norm_forward_kernel(NormArgs a) {
     __shared__ float2 slots[32];
     const int threads = a.team, teams = blockDim.x / threads, team = __builtin_amdgcn_readfirstlane(threadIdx.x / threads), t = threadIdx.x - team * threads;
     TeamSums sums(slots, threads / 64);
-    const int col = t * 8;
-    const bool in = col < a.cols;
+    const uint32_t col = t * 8;
+    const bool in = (int)col < a.cols;
     const float inverse = 1.0f / (float)a.cols;
     const int64_t begin = blockIdx.x * a.chunk, end = begin + a.chunk < a.rows ? begin + a.chunk : a.rows;
     NormVectors<FORM> vectors;
     int64_t group_end = -1;                                                  // of the rows that the vectors are those of
-    Piece<TX> raw_x = {};                                                    // zero beyond the row
-    Piece<TY> raw_y = {};
-    auto load = [&](int64_t row) {
-        if (!in || row >= end) return;                                       // beyond the end: the last row again, which nobody stores
-        raw_x = load_piece<TX>(a.x, row * a.x_pitch, col);
-        if constexpr (FORM != FORM_BEFORE) raw_y = load_piece<TY>(a.y, row * a.y_pitch, col);
+    // Two rows are under way while one is worked on; zero beyond the row.
+    Piece<TX> raw_x = {}, next_x = {};
+    Piece<TY> raw_y = {}, next_y = {};
+    auto load = [&](int64_t row, Piece<TX>& to_x, Piece<TY>& to_y) {
+        if (!in || row >= end) return;                                       // beyond the end: some row before, which nobody stores
+        auto from = [&](auto stream) {
+            to_x = load_piece<TX, decltype(stream)::value>(a.x, row * a.x_pitch, col);
+            if constexpr (FORM != FORM_BEFORE) to_y = load_piece<TY, decltype(stream)::value>(a.y, row * a.y_pitch, col);
+        };
+        a.stream_in ? from(std::true_type()) : from(std::false_type());
     };
-    load(begin + team);
+    load(begin + team, raw_x, raw_y);
+    load(begin + team + teams, next_x, next_y);
     for (int64_t base = begin; base < end; base += teams) {
         const int64_t row = base + team;
         const bool there = in && row < end;
@@ -221,38 +303,44 @@ template <typename TX, typename TY, int FORM> __global__ __launch_bounds__(ROW_T
         float x[8], y[8];
         widen_piece(raw_x, x);
         if constexpr (FORM != FORM_BEFORE) widen_piece(raw_y, y);
-        load(row + teams);
+        raw_x = next_x;
+        raw_y = next_y;
+        load(row + 2 * teams, next_x, next_y);
         float4 stat = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
-        if constexpr (FORM != FORM_BEFORE) {
+        if constexpr (FORM == FORM_PLAIN) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(a.rho, x[i], y[i] * vectors.ga[i]);
+        } else if constexpr (FORM != FORM_BEFORE) {
             if (a.after != VIOLA_NORM_NONE) {
-                const float2 s = row_statistics(y, in, a.after, inverse, a.eps, sums);
+                const float2 s = row_statistics<LAYER>(y, in, a.after, a.cols, inverse, a.eps, sums);
                 stat.x = s.x;
                 stat.y = s.y;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = fmaf(a.rho, x[i], fmaf((y[i] - stat.x) * stat.y, vectors.ga[i], vectors.gb[i]));
-            if (there) store_piece<TX>(a.out, row * a.cols, col, x);
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(a.rho, x[i], fmaf((LAYER ? y[i] - stat.x : y[i]) * stat.y, vectors.ga[i], vectors.gb[i]));
         }
+        if constexpr (FORM != FORM_BEFORE)
+            if (there) store_piece<TX>(a.out, row * a.cols, col, x, a.stream_out);
         if constexpr (FORM != FORM_AFTER) {
-            const float2 s = row_statistics(x, in, a.before, inverse, a.eps, sums);
+            const float2 s = row_statistics<LAYER>(x, in, a.before, a.cols, inverse, a.eps, sums);
             stat.z = s.x;
             stat.w = s.y;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - s.x) * s.y, vectors.w[i], vectors.b[i]);
-            if (there) store_piece<TY>(a.h, row * a.cols, col, x);
+            for (int i = 0; i < 8; ++i) x[i] = fmaf((LAYER ? x[i] - s.x : x[i]) * s.y, vectors.w[i], vectors.b[i]);
+            if (there) store_piece<TY>(a.h, row * a.cols, col, x, a.stream_out);
         }
         if (a.stats && t == 0 && row < end) a.stats[row] = stat;
     }
 }
 
 // One portion: rows of one group, a team each in turn. The teams' sums are joined in LDS at the end, team by team.
-template <typename TX, typename TY, int FORM, bool BIAS, bool SHIFT> __global__ __launch_bounds__(ROW_THREADS) void norm_backward_kernel(NormArgs a) {
+template <typename TX, typename TY, int FORM, bool LAYER, bool BIAS, bool SHIFT> __global__ __launch_bounds__(ROW_THREADS) void norm_backward_kernel(NormArgs a) {
     __shared__ float2 slots[32];
     extern __shared__ float joined[];                                        // [teams - 1][cols] where a block has several teams
     const int threads = a.team, teams = blockDim.x / threads, team = __builtin_amdgcn_readfirstlane(threadIdx.x / threads), t = threadIdx.x - team * threads;
     TeamSums sums(slots, threads / 64);
-    const int col = t * 8;
-    const bool in = col < a.cols;
+    const uint32_t col = t * 8;
+    const bool in = (int)col < a.cols;
     const float inverse = 1.0f / (float)a.cols;
     const int64_t length = (a.group_rows + a.per_group - 1) / a.per_group;
     for (int64_t portion = blockIdx.x; portion < a.portions; portion += gridDim.x) {
@@ -267,12 +355,15 @@ template <typename TX, typename TY, int FORM, bool BIAS, bool SHIFT> __global__ 
         Piece<TY> raw_y = {}, raw_dh = {};
         auto load = [&](int64_t row) {
             if (row < end) {
-                if (in) {
-                    if constexpr (FORM != FORM_AFTER) raw_x = load_piece<TX>(a.x, row * a.x_pitch, col);
-                    if constexpr (FORM != FORM_BEFORE) raw_y = load_piece<TY>(a.y, row * a.y_pitch, col);
-                    if constexpr (FORM != FORM_AFTER) raw_dh = load_piece<TY>(a.dh, row * a.cols, col);
-                    if constexpr (FORM != FORM_BEFORE) if (a.dout) raw_dout = load_piece<TX>(a.dout, row * a.cols, col);
-                }
+                if (!in) return;
+                auto from = [&](auto stream) {
+                    constexpr bool STREAM = decltype(stream)::value;
+                    if constexpr (FORM != FORM_AFTER) raw_x = load_piece<TX, STREAM>(a.x, row * a.x_pitch, col);
+                    if constexpr (FORM != FORM_BEFORE) raw_y = load_piece<TY, STREAM>(a.y, row * a.y_pitch, col);
+                    if constexpr (FORM != FORM_AFTER) raw_dh = load_piece<TY, STREAM>(a.dh, row * a.cols, col);
+                    if constexpr (FORM != FORM_BEFORE) if (a.dout) raw_dout = load_piece<TX, STREAM>(a.dout, row * a.cols, col);
+                };
+                a.stream_in ? from(std::true_type()) : from(std::false_type());
             } else {
                 raw_x = raw_dout = {};
                 raw_y = raw_dh = {};
@@ -288,7 +379,8 @@ template <typename TX, typename TY, int FORM, bool BIAS, bool SHIFT> __global__ 
             if constexpr (FORM != FORM_BEFORE) {
                 widen_piece(raw_y, y);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = (y[i] - stat.x) * stat.y;
+                for (int i = 0; i < 8; ++i)
+                    if constexpr (FORM != FORM_PLAIN) y[i] = (LAYER ? y[i] - stat.x : y[i]) * stat.y;
             }
             if constexpr (FORM != FORM_AFTER) {
                 widen_piece(raw_x, x);
@@ -301,29 +393,35 @@ template <typename TX, typename TY, int FORM, bool BIAS, bool SHIFT> __global__ 
                 float along = 0.0f, total = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if constexpr (FORM == FORM_BETWEEN) x[i] = fmaf(a.rho, x[i], BIAS ? fmaf(y[i], vectors.ga[i], vectors.gb[i]) : y[i] * vectors.ga[i]);
-                    x[i] = (x[i] - stat.z) * stat.w;
+                    if constexpr (FORM == FORM_BETWEEN || FORM == FORM_PLAIN) x[i] = fmaf(a.rho, x[i], BIAS ? fmaf(y[i], vectors.ga[i], vectors.gb[i]) : y[i] * vectors.ga[i]);
+                    x[i] = (LAYER ? x[i] - stat.z : x[i]) * stat.w;
                     s1[i] = fmaf(q[i], x[i], s1[i]);
                     if constexpr (SHIFT) s0[i] += q[i];
                     q[i] *= vectors.w[i];
                     along = fmaf(q[i], x[i], along);
-                    total += q[i];
+                    if constexpr (LAYER) total += q[i];
                 }
-                const float2 both = sums.both(along, total);
-                const float m1 = both.x * inverse, m0 = a.before == VIOLA_NORM_LAYER ? both.y * inverse : 0.0f;
+                float m1, m0 = 0.0f;
+                if constexpr (LAYER) {
+                    const float2 both = sums.both(along, total);
+                    m1 = both.x * inverse;
+                    m0 = a.before == VIOLA_NORM_LAYER ? both.y * inverse : 0.0f;
+                } else {
+                    m1 = sums.one(along) * inverse;
+                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float from_h = stat.w * (q[i] - fmaf(x[i], m1, m0));
-                    d[i] = FORM == FORM_BETWEEN ? d[i] + from_h : from_h;
+                    const float from_h = q[i] - (LAYER ? fmaf(x[i], m1, m0) : x[i] * m1);
+                    d[i] = FORM == FORM_BEFORE ? stat.w * from_h : fmaf(stat.w, from_h, d[i]);
                 }
             }
             if (a.dx && there) {
                 if constexpr (FORM == FORM_BEFORE) {
-                    store_piece<TX>(a.dx, row * a.cols, col, d);
+                    store_piece<TX>(a.dx, row * a.cols, col, d, a.stream_out);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[i] = a.rho * d[i];
-                    store_piece<TX>(a.dx, row * a.cols, col, x);
+                    store_piece<TX>(a.dx, row * a.cols, col, x, a.stream_out);
                 }
             }
             if constexpr (FORM != FORM_BEFORE) {
@@ -333,24 +431,30 @@ template <typename TX, typename TY, int FORM, bool BIAS, bool SHIFT> __global__ 
                     a1[i] = fmaf(d[i], y[i], a1[i]);
                     if constexpr (BIAS) a0[i] += d[i];
                     d[i] *= vectors.ga[i];
-                    along = fmaf(d[i], y[i], along);
-                    total += d[i];
+                    if constexpr (FORM != FORM_PLAIN) along = fmaf(d[i], y[i], along);
+                    if constexpr (LAYER && FORM != FORM_PLAIN) total += d[i];
                 }
                 if (!a.dy) continue;
-                if (a.after != VIOLA_NORM_NONE) {
-                    const float2 both = sums.both(along, total);
-                    const float m1 = both.x * inverse, m0 = a.after == VIOLA_NORM_LAYER ? both.y * inverse : 0.0f;
+                if (FORM != FORM_PLAIN && a.after != VIOLA_NORM_NONE) {
+                    float m1, m0 = 0.0f;
+                    if constexpr (LAYER) {
+                        const float2 both = sums.both(along, total);
+                        m1 = both.x * inverse;
+                        m0 = a.after == VIOLA_NORM_LAYER ? both.y * inverse : 0.0f;
+                    } else {
+                        m1 = sums.one(along) * inverse;
+                    }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) d[i] = stat.y * (d[i] - fmaf(y[i], m1, m0));
+                    for (int i = 0; i < 8; ++i) d[i] = stat.y * (d[i] - (LAYER ? fmaf(y[i], m1, m0) : y[i] * m1));
                 }
-                if (there) store_piece<TY>(a.dy, row * a.cols, col, d);
+                if (there) store_piece<TY>(a.dy, row * a.cols, col, d, a.stream_out);
             }
         }
         float* to = a.parts + portion * __popc(a.sums) * a.cols;
         auto write = [&](float (&v)[8]) {
             if (teams > 1) {
                 __syncthreads();                                             // the sum before has been read
-                if (team && in) store_piece<float>(joined, (int64_t)(team - 1) * a.cols, col, v);
+                if (team && in) store_piece<float>(joined, (int64_t)(team - 1) * a.cols, col, v, false);
                 __syncthreads();
                 if (!team && in)
                     for (int u = 1; u < teams; ++u) {
@@ -358,7 +462,7 @@ template <typename TX, typename TY, int FORM, bool BIAS, bool SHIFT> __global__ 
                         for (int i = 0; i < 8; ++i) v[i] += joined[(u - 1) * a.cols + col + i];
                     }
             }
-            if (!team && in) store_piece<float>(to, 0, col, v);
+            if (!team && in) store_piece<float>(to, 0, col, v, false);
             to += a.cols;
         };
         if (a.sums & SUM_A1) write(a1);

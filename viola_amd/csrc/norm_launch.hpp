@@ -3,35 +3,38 @@
 
 #include "norm.hpp"
 
+#include <type_traits>
+
 namespace viola {
 
 // a.team threads for a row; as many teams as fit 512 threads
 inline int norm_block(const NormArgs& a) { return a.team >= 512 ? a.team : 512 / a.team * a.team; }
 
-template <typename TX, typename TY> void norm_forward_rows(const NormArgs& a, int form, dim3 grid, hipStream_t stream) {
-    const int block = norm_block(a);
-    if (form == FORM_BEFORE) VIOLA_LAUNCH((norm_forward_kernel<TX, TY, FORM_BEFORE>), grid, block, 0, stream, a);
-    else if (form == FORM_AFTER) VIOLA_LAUNCH((norm_forward_kernel<TX, TY, FORM_AFTER>), grid, block, 0, stream, a);
-    else VIOLA_LAUNCH((norm_forward_kernel<TX, TY, FORM_BETWEEN>), grid, block, 0, stream, a);
+// f(std::integral_constant of a form, std::bool_constant)
+template <typename F> void with_form(int form, bool flag, F&& f) {
+    auto second = [&](auto form_constant) { flag ? f(form_constant, std::true_type()) : f(form_constant, std::false_type()); };
+    if (form == FORM_BEFORE) second(std::integral_constant<int, FORM_BEFORE>());
+    else if (form == FORM_AFTER) second(std::integral_constant<int, FORM_AFTER>());
+    else if (form == FORM_BETWEEN) second(std::integral_constant<int, FORM_BETWEEN>());
+    else second(std::integral_constant<int, FORM_PLAIN>());
 }
 
+inline bool any_layer(const NormArgs& a) { return a.after == VIOLA_NORM_LAYER || a.before == VIOLA_NORM_LAYER; }
+
+template <typename TX, typename TY> void norm_forward_rows(const NormArgs& a, int form, dim3 grid, hipStream_t stream) {
+    with_form(form, any_layer(a), [&](auto f, auto layer) { VIOLA_LAUNCH((norm_forward_kernel<TX, TY, decltype(f)::value, decltype(layer)::value>), grid, norm_block(a), 0, stream, a); });
+}
+
+// A form has at most the sums of its own sides; between two blocks a bias after the one and a shift before the other share a kernel.
 template <typename TX, typename TY> void norm_backward_rows(const NormArgs& a, int form, bool bias, bool shift, dim3 grid, hipStream_t stream) {
     const int block = norm_block(a);
     const unsigned lds = (unsigned)((block / a.team - 1) * a.cols * 4);
-    if (form == FORM_BEFORE) {
-        if (shift) VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_BEFORE, false, true>), grid, block, lds, stream, a);
-        else VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_BEFORE, false, false>), grid, block, lds, stream, a);
-    } else if (form == FORM_AFTER) {
-        if (bias) VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_AFTER, true, false>), grid, block, lds, stream, a);
-        else VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_AFTER, false, false>), grid, block, lds, stream, a);
-    } else if (bias) {
-        if (shift) VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_BETWEEN, true, true>), grid, block, lds, stream, a);
-        else VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_BETWEEN, true, false>), grid, block, lds, stream, a);
-    } else if (shift) {
-        VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_BETWEEN, false, true>), grid, block, lds, stream, a);
-    } else {
-        VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_BETWEEN, false, false>), grid, block, lds, stream, a);
-    }
+    with_form(form, any_layer(a), [&](auto f, auto layer) {
+        constexpr int FORM = decltype(f)::value;
+        constexpr bool LAYER = decltype(layer)::value, WITH_BIAS = FORM == FORM_AFTER || FORM == FORM_BETWEEN, WITH_SHIFT = FORM != FORM_AFTER;
+        if ((WITH_BIAS && bias) || (WITH_SHIFT && shift)) VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM, LAYER, WITH_BIAS, WITH_SHIFT>), grid, block, lds, stream, a);
+        else VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM, LAYER, false, false>), grid, block, lds, stream, a);
+    });
 }
 
 }  // namespace viola

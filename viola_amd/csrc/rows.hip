@@ -8,6 +8,8 @@
 // Both are bound by memory: every row is read or written once, and a token's own row once for all of its experts.
 #include "block_ops.hpp"
 
+#include <type_traits>
+
 using namespace viola;
 
 namespace {
@@ -23,6 +25,7 @@ struct RowsArgs {
     int64_t values_pitch;
     void* out;
     float* dots;
+    bool stream_in, stream_out;                                              // rows are read, written past the caches' order
 };
 
 // ---------------------------------------------------------------------------------------------------- any width and address
@@ -123,13 +126,18 @@ template <typename T, int CHOICES, int PIECES> __global__ __launch_bounds__(256)
         float sum[PIECES][WIDE<T>] = {};
         for (int j0 = 0; j0 < a.top_k; j0 += CHOICES) {
             uint4 piece[CHOICES][PIECES];
+            const uint4* from[CHOICES];
             bool there[CHOICES];
 #pragma unroll
-            for (int j = 0; j < CHOICES; ++j) {
-                const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(a.in) + row_of(a, token, j0 + j, there[j]) * a.pitch);
+            for (int j = 0; j < CHOICES; ++j) from[j] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.in) + row_of(a, token, j0 + j, there[j]) * a.pitch);
+            auto load = [&](auto stream) {
 #pragma unroll
-                for (int p = 0; p < PIECES; ++p) piece[j][p] = from[first + 64 * p < width ? first + 64 * p : 0];
-            }
+                for (int j = 0; j < CHOICES; ++j) {
+#pragma unroll
+                    for (int p = 0; p < PIECES; ++p) piece[j][p] = load16<decltype(stream)::value>(from[j] + (first + 64 * p < width ? first + 64 * p : 0));
+                }
+            };
+            a.stream_in ? load(std::true_type()) : load(std::false_type());
 #pragma unroll
             for (int j = 0; j < CHOICES; ++j) {
                 if (!there[j]) continue;
@@ -146,7 +154,7 @@ template <typename T, int CHOICES, int PIECES> __global__ __launch_bounds__(256)
         uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + token * a.cols);
 #pragma unroll
         for (int p = 0; p < PIECES; ++p)
-            if (first + 64 * p < width) to[first + 64 * p] = narrow<T>(sum[p]);
+            if (first + 64 * p < width) store16(to + first + 64 * p, narrow<T>(sum[p]), a.stream_out);
     });
 }
 
@@ -174,7 +182,7 @@ template <typename T, int PIECES> __global__ __launch_bounds__(256) void scatter
                     for (int i = 0; i < WIDE<T>; ++i) v[i] *= gate;
                     word = narrow<T>(v);
                 }
-                if (first + 64 * p < width) to[first + 64 * p] = word;
+                if (first + 64 * p < width) store16(to + first + 64 * p, word, a.stream_out);
             }
         }
         // rows that no token has
@@ -188,8 +196,9 @@ template <typename T, int PIECES> __global__ __launch_bounds__(256) void scatter
     });
 }
 
-// scatter and the dots beside it: WAVES wavefronts to a token, which take its row in turn, so that a dot is summed in one place.
-template <typename T, int CHOICES, int WAVES> __global__ __launch_bounds__(256) void scatter_dots_kernel(RowsArgs a) {
+// scatter and the dots beside it: WAVES wavefronts to a token, which take its row in turn, PIECES pieces a lane at a time, so that a dot is summed in
+// one place.
+template <typename T, int CHOICES, int PIECES, int WAVES> __global__ __launch_bounds__(256) void scatter_dots_kernel(RowsArgs a) {
     __shared__ float parts[WAVES][CHOICES];
     const int width = a.cols / WIDE<T>, lane = threadIdx.x % 64;
     each_wave(a.tokens * WAVES, [&](int64_t wave) {                          // with several wavefronts a block is one token, and so all of it makes a turn
@@ -208,24 +217,38 @@ template <typename T, int CHOICES, int WAVES> __global__ __launch_bounds__(256) 
                 to[j] = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.cols);
                 gate[j] = a.gates && there[j] ? a.gates[token * a.top_k + j0 + j] : 1.0f;
             }
-            for (int c = part * 64 + lane; c < width; c += WAVES * 64) {
-                const uint4 piece = from[c];
-                uint4 other[CHOICES];
+            for (int first = part * 64 * PIECES + lane; first - lane < width; first += WAVES * 64 * PIECES) {
+                uint4 piece[PIECES], other[CHOICES][PIECES];
+                auto load = [&](auto stream) {
 #pragma unroll
-                for (int j = 0; j < CHOICES; ++j) other[j] = value[j][c];
-                float v[WIDE<T>];
-                widen<T>(piece, v);
+                    for (int p = 0; p < PIECES; ++p) {
+                        const int c = first + 64 * p < width ? first + 64 * p : 0;
+                        piece[p] = load16<decltype(stream)::value>(from + c);
 #pragma unroll
-                for (int j = 0; j < CHOICES; ++j) {
-                    if (!there[j]) continue;
-                    float u[WIDE<T>];
-                    widen<T>(other[j], u);
-#pragma unroll
-                    for (int i = 0; i < WIDE<T>; ++i) {
-                        dot[j] = fmaf(v[i], u[i], dot[j]);
-                        u[i] = gate[j] * v[i];
+                        for (int j = 0; j < CHOICES; ++j) other[j][p] = load16<decltype(stream)::value>(value[j] + c);
                     }
-                    if (a.out) to[j][c] = a.gates ? narrow<T>(u) : piece;
+                };
+                a.stream_in ? load(std::true_type()) : load(std::false_type());
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) {
+                    const bool in = first + 64 * p < width;
+                    float v[WIDE<T>];
+                    widen<T>(piece[p], v);
+#pragma unroll
+                    for (int j = 0; j < CHOICES; ++j) {
+                        if (!there[j]) continue;
+                        float u[WIDE<T>], sum = 0.0f;
+                        widen<T>(other[j][p], u);
+#pragma unroll
+                        for (int i = 0; i < WIDE<T>; ++i) {
+                            sum = fmaf(v[i], u[i], sum);
+                            u[i] = gate[j] * v[i];
+                        }
+                        if (in) {
+                            dot[j] += sum;
+                            if (a.out) store16(to[j] + first + 64 * p, a.gates ? narrow<T>(u) : piece[p], a.stream_out);
+                        }
+                    }
                 }
             }
 #pragma unroll
@@ -272,9 +295,13 @@ template <typename T, int PIECES> void launch_scatter(const RowsArgs& a, hipStre
     const int64_t cuts = (a.cols / WIDE<T> + 64 * PIECES - 1) / (64 * PIECES);
     VIOLA_LAUNCH((scatter_kernel<T, PIECES>), blocks_for(a.tokens * cuts), 256, 0, stream, a);
 }
-template <typename T, int CHOICES> void launch_dots(const RowsArgs& a, hipStream_t stream) {
-    if (a.tokens >= 4096 || a.cols / WIDE<T> <= 64) VIOLA_LAUNCH((scatter_dots_kernel<T, CHOICES, 1>), blocks_for(a.tokens), 256, 0, stream, a);
-    else VIOLA_LAUNCH((scatter_dots_kernel<T, CHOICES, 4>), blocks_for(a.tokens * 4), 256, 0, stream, a);
+template <typename T, int CHOICES, int PIECES> void launch_dots(const RowsArgs& a, hipStream_t stream) {
+    // Four wavefronts to a token where its row has a piece for every lane of them (16384 tokens of 4096 in BF16, two choices: 130 against 155 us with one
+    // wavefront), one below (1024, eight choices: 112 against 125 us).
+    const int64_t width = a.cols / WIDE<T>;
+    if (width <= 64) VIOLA_LAUNCH((scatter_dots_kernel<T, CHOICES, 1, 1>), blocks_for(a.tokens), 256, 0, stream, a);
+    else if (width < 256) VIOLA_LAUNCH((scatter_dots_kernel<T, CHOICES, PIECES, 1>), blocks_for(a.tokens), 256, 0, stream, a);
+    else VIOLA_LAUNCH((scatter_dots_kernel<T, CHOICES, 1, 4>), blocks_for(a.tokens * 4), 256, 0, stream, a);
 }
 
 template <typename T> void run_gather(const RowsArgs& a, int dtype, hipStream_t stream) {
@@ -289,10 +316,10 @@ template <typename T> void run_gather(const RowsArgs& a, int dtype, hipStream_t 
 template <typename T> void run_scatter(const RowsArgs& a, int dtype, hipStream_t stream) {
     if (!whole_pieces(a, dtype)) VIOLA_LAUNCH(scatter_any_kernel<T>, blocks_for(a.tokens), 256, 0, stream, a);
     else if (!a.dots) a.cols / WIDE<T> <= 64 ? launch_scatter<T, 1>(a, stream) : launch_scatter<T, 2>(a, stream);
-    else if (a.top_k == 1) launch_dots<T, 1>(a, stream);
-    else if (a.top_k == 2) launch_dots<T, 2>(a, stream);
-    else if (a.top_k <= 4) launch_dots<T, 4>(a, stream);
-    else launch_dots<T, 8>(a, stream);
+    else if (a.top_k == 1) launch_dots<T, 1, 4>(a, stream);
+    else if (a.top_k == 2) launch_dots<T, 2, 4>(a, stream);
+    else if (a.top_k <= 4) launch_dots<T, 4, 2>(a, stream);
+    else launch_dots<T, 8, 1>(a, stream);
 }
 
 int check(const RowsArgs& a, int dtype) {
@@ -310,6 +337,8 @@ extern "C" int viola_rows_gather(const void* rows, int64_t pitch, int64_t row_co
     RowsArgs a = {positions, gates, nullptr, tokens, row_count, pitch, top_k, (int)cols, rows, nullptr, 0, out, nullptr};
     if (const int status = check(a, dtype)) return status;
     if (tokens == 0) return 0;
+    a.stream_in = tokens * top_k * cols * viola_dtype_size(dtype) > STREAM_IN;
+    a.stream_out = tokens * cols * viola_dtype_size(dtype) > STREAM_OUT;
     VIOLA_CHECK_ARG(positions && out && (rows || row_count == 0) && pitch >= cols);
     if (dtype == VIOLA_BF16) run_gather<bf16_t>(a, dtype, stream);
     else if (dtype == VIOLA_F16) run_gather<f16_t>(a, dtype, stream);
@@ -324,6 +353,8 @@ extern "C" int viola_rows_scatter(const void* x, int64_t pitch, int dtype, int64
     RowsArgs a = {positions, gates, total, tokens, row_count, pitch, top_k, (int)cols, x, values, values_pitch, rows, dots};
     if (const int status = check(a, dtype)) return status;
     if (tokens == 0) return 0;
+    a.stream_in = dots && tokens * top_k * cols * viola_dtype_size(dtype) > STREAM_IN;
+    a.stream_out = rows && row_count * cols * viola_dtype_size(dtype) > STREAM_OUT;
     VIOLA_CHECK_ARG(positions && x && pitch >= cols && (rows || dots || row_count == 0) && (!dots || values || row_count == 0) && (!dots || values_pitch >= cols));
     if (dtype == VIOLA_BF16) run_scatter<bf16_t>(a, dtype, stream);
     else if (dtype == VIOLA_F16) run_scatter<f16_t>(a, dtype, stream);
