@@ -107,6 +107,23 @@ def test_types_and_ties(dtype, experts):
     _check_route((torch.randn(200, experts) * 2).round().div(2).to(dtype), 6)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_an_only_choice_has_no_gradient_from_its_gate(score):
+    """Its share of itself is one whatever its logit: the balance loss's gradient is all there is, however small beside the gate's."""
+    from viola_amd import nn
+    torch.manual_seed(12)
+    logits = torch.randn(300, 16)
+    logits[:100, 1:] = -math.inf                                             # one open expert of two choices
+    for part, top_k in ((logits[:100], 2), (logits[100:], 1)):
+        l = part.cuda().requires_grad_()
+        r = nn.route(l, top_k, score=score)
+        grad, = torch.autograd.grad(r.gates, l, torch.randn(r.gates.shape, device="cuda"), retain_graph=True)
+        assert (grad == 0).all()
+        both, = torch.autograd.grad([r.gates, r.balance], l, [torch.randn(r.gates.shape, device="cuda"), torch.tensor(1e-6, device="cuda")])
+        chosen = routing.choose(part, top_k)
+        _close("dlogits", both, routing.gradient(part, chosen, score, dloss=1e-6), _pull(part, chosen, score, None, False, 1e-6, None, True, 1.0))
+
+
 def test_all_equal_and_signed_zeros():
     logits = torch.zeros(40, 24)
     logits[::2, ::3] = -0.0

@@ -582,23 +582,33 @@ template <int LANES, int VALUES, bool SIGMOID> __global__ __launch_bounds__(256)
             __builtin_amdgcn_wave_barrier();
         }
         auto part = [&](int i) { return word[i] == NOT_CHOSEN ? 0.0f : __uint_as_float(word[i]); };
-        float p[VALUES], towards = 0.0f, picked = 0.0f, along = 0.0f;        // sum of p pull; over the chosen, of p and of p dgate
+        float p[VALUES], from_gates[VALUES], towards = 0.0f, picked = 0.0f, along = 0.0f;    // sum of p pull; over the chosen, of p and of p dgate
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) {
             p[i] = score<SIGMOID>(l[i], stat.x) * stat.y;
             towards = fmaf(p[i], pull[i], towards);
             picked += word[i] == NOT_CHOSEN ? 0.0f : p[i];
             along = fmaf(p[i], part(i), along);
+            from_gates[i] = 0.0f;
         }
         towards = lanes_sum<LANES>(towards);
         if (g.dgates && (a.normalize || !SIGMOID)) {
-            along = lanes_sum<LANES>(along);
-            if (a.normalize) {                                               // gate_i = scale p_i / picked; its part of `towards` is zero
+            if (a.normalize) {                                               // gate_i = scale q_i, q = p / picked: q_i (dgate_i - sum q dgate)
                 picked = lanes_sum<LANES>(picked);
-                const float inverse = 1.0f / picked, mean = along * inverse;
+                const float inverse = 1.0f / picked;
+                along = 0.0f;
 #pragma unroll
-                for (int i = 0; i < VALUES; ++i) pull[i] += word[i] == NOT_CHOSEN ? 0.0f : (__uint_as_float(word[i]) - mean) * inverse;
+                for (int i = 0; i < VALUES; ++i) {
+                    // the quotient to its last place: of a row's only choice it is 1, whose gradient is 0 and not what rounding leaves of it
+                    const float near = p[i] * inverse, q = fmaf(fmaf(-near, picked, p[i]), inverse, near);
+                    from_gates[i] = word[i] == NOT_CHOSEN ? 0.0f : q;
+                    along = fmaf(from_gates[i], part(i), along);
+                }
+                const float mean = lanes_sum<LANES>(along);
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) from_gates[i] = word[i] == NOT_CHOSEN ? 0.0f : from_gates[i] * (__uint_as_float(word[i]) - mean);
             } else {                                                         // gate_i = scale p_i
+                along = lanes_sum<LANES>(along);
 #pragma unroll
                 for (int i = 0; i < VALUES; ++i) pull[i] += part(i);
                 towards += along;
@@ -607,7 +617,7 @@ template <int LANES, int VALUES, bool SIGMOID> __global__ __launch_bounds__(256)
         float d[VALUES];
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) {
-            d[i] = p[i] * (pull[i] - towards);
+            d[i] = fmaf(p[i], pull[i] - towards, from_gates[i]);
             if constexpr (SIGMOID) {
                 if (!a.normalize) d[i] = fmaf(part(i), sigmoid_of(l[i]), d[i]);                                // gate_i = scale sigmoid(l_i)
                 d[i] *= sigmoid_of(-l[i]);
