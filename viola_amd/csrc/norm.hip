@@ -289,12 +289,13 @@ void stream(NormArgs& a, int64_t bytes_in, int64_t bytes_out) {
 }
 bool plain(const NormArgs& a) { return a.after == VIOLA_NORM_NONE && !a.after_weight && !a.after_bias; }
 
-// A portion for every block that the chip holds at once (16 wavefronts a CU), of two rows for each of its teams at least, and of no more than one group.
+// A portion for every block that the chip holds at once (16 wavefronts a CU), of two rows for each of its teams at least
+// (2000 rows of 256: 14.7 us, with four 16.4) and of four (1024 rows of 4096: 20.3 us, with two 21.8), and of no more than one group.
 int64_t portions_per_group(int64_t rows, int64_t group_rows, int64_t cols) {
     NormArgs a = {};
     a.team = (int)((cols + 511) / 512 * 64);
     const bool registers = cols <= ROW_COLUMNS;
-    const int64_t block = registers ? norm_block(a) : 1024, least = registers ? 2 * (block / a.team) : 1;
+    const int64_t block = registers ? norm_block(a, false) : 1024, teams = block / a.team, least = !registers ? 1 : teams > 1 ? 2 * teams : 4;
     const int64_t groups = rows / group_rows, wanted = (256 * (1024 / block) + groups - 1) / groups, most = (group_rows + least - 1) / least;
     return wanted < most ? wanted : most;
 }
@@ -337,7 +338,7 @@ extern "C" int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, c
     a.out = out; a.h = h; a.stats = reinterpret_cast<float4*>(stats);
     if (in_registers(a, {x, y, out, h}, [&](auto tx, auto ty) {
             // as many blocks as the chip holds at once by their registers, BLOCKS_PER_SLOT times: each loads the vectors along the row once
-            const int64_t block = norm_block(a), teams = block / a.team, waves = form == FORM_BETWEEN ? 16 : 20, held = waves * 64 / block;
+            const int64_t block = norm_block(a, true), teams = block / a.team, waves = form == FORM_BETWEEN ? 16 : 20, held = waves * 64 / block;
             const int64_t blocks = 256 * (held ? held : 1) * BLOCKS_PER_SLOT;
             a.chunk = ((rows + blocks - 1) / blocks + teams - 1) / teams * teams;
             stream(a, rows * cols * ((int)sizeof(tx) + (y ? (int)sizeof(ty) : 0)), rows * cols * ((out ? (int)sizeof(tx) : 0) + (h ? (int)sizeof(ty) : 0)));

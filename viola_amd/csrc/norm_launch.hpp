@@ -7,8 +7,14 @@
 
 namespace viola {
 
-// a.team threads for a row; as many teams as fit 512 threads
-inline int norm_block(const NormArgs& a) { return a.team >= 512 ? a.team : 512 / a.team * a.team; }
+// Threads of a block, of a.team for a row. Backward: as many teams as fit 512 threads (1024: 182 against 168 us for 16384 rows of 4096). Forward: of three
+// wavefronts and more as many as fit 1024 (102 against 107 us there, 29 against 34 us for 16384 rows of 1152; rows of 512 and 1024 the other way, 31
+// against 29 us), and a row to a block where there are few.
+inline int norm_block(const NormArgs& a, bool forward) {
+    if (forward && a.rows < 1024) return a.team;
+    const int most = a.team >= 512 || (forward && a.team >= 192) ? 1024 : 512;
+    return !forward && a.team >= 512 ? a.team : most / a.team * a.team;
+}
 
 // f(std::integral_constant of a form, std::bool_constant)
 template <typename F> void with_form(int form, bool flag, F&& f) {
@@ -22,12 +28,12 @@ template <typename F> void with_form(int form, bool flag, F&& f) {
 inline bool any_layer(const NormArgs& a) { return a.after == VIOLA_NORM_LAYER || a.before == VIOLA_NORM_LAYER; }
 
 template <typename TX, typename TY> void norm_forward_rows(const NormArgs& a, int form, dim3 grid, hipStream_t stream) {
-    with_form(form, any_layer(a), [&](auto f, auto layer) { VIOLA_LAUNCH((norm_forward_kernel<TX, TY, decltype(f)::value, decltype(layer)::value>), grid, norm_block(a), 0, stream, a); });
+    with_form(form, any_layer(a), [&](auto f, auto layer) { VIOLA_LAUNCH((norm_forward_kernel<TX, TY, decltype(f)::value, decltype(layer)::value>), grid, norm_block(a, true), 0, stream, a); });
 }
 
 // A form has at most the sums of its own sides; between two blocks a bias after the one and a shift before the other share a kernel.
 template <typename TX, typename TY> void norm_backward_rows(const NormArgs& a, int form, bool bias, bool shift, dim3 grid, hipStream_t stream) {
-    const int block = norm_block(a);
+    const int block = norm_block(a, false);
     const unsigned lds = (unsigned)((block / a.team - 1) * a.cols * 4);
     with_form(form, any_layer(a), [&](auto f, auto layer) {
         constexpr int FORM = decltype(f)::value;
