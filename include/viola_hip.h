@@ -512,7 +512,8 @@ int viola_store_words(int64_t* dst, const int64_t* host_words, int64_t count, vi
  * Backward: dout of x_dtype, dh and dy of branch_dtype, dx of x_dtype, all contiguous; a null dout is zeros, a null output is not wanted.
  * A call without dh (then before = VIOLA_NORM_NONE) is that of the form without h. Gradients of the vectors: [cols], or [groups][cols] where
  * the vector has a pitch, of the vector's type. parts: viola_norm_portions(rows, cols, group_rows) * 4 * cols floats (fewer where fewer of the gradients are
- * wanted). Sums over rows are added in an order of their own that does not change from call to call. */
+ * wanted). Sums over rows are added in an order of their own that does not change from call to call. cols <= 2^28; rows <= 2^32 and groups <= 2^21 where vectors
+ * have a pitch (VIOLA_EUNSUPPORTED beyond). */
 int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols,
                        int after, const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
                        const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch,
@@ -552,7 +553,7 @@ int viola_route_backward(const void* logits, int64_t pitch, int dtype, int64_t t
  * viola_rows_gather: out[t] = sum_j gates[t, j] rows[positions[t, j]] (gates null: ones), out [tokens, cols] contiguous.
  * viola_rows_scatter: rows[positions[t, j]] = gates[t, j] x[t], rows [row_count, cols] contiguous, and zeros in the rows from *total (on the device) on;
  * dots (null: not wanted): dots[t, j] = sum_c x[t, c] values[positions[t, j], c]. rows may be null when only dots are wanted.
- * Positions of row_count and beyond are read as none. */
+ * Positions of row_count and beyond are read as none. cols <= 2^28. */
 int viola_rows_gather(const void* rows, int64_t pitch, int64_t row_count, int dtype, int64_t cols, const int32_t* positions, const float* gates, int64_t tokens,
                       int top_k, void* out, viola_stream_t stream);
 int viola_rows_scatter(const void* x, int64_t pitch, int dtype, int64_t cols, const int32_t* positions, const float* gates, int64_t tokens, int top_k,

@@ -20,7 +20,7 @@ ARCH = "gfx950"
 COMMON = ["-O3", f"--offload-arch={ARCH}", "-fPIC", "-std=c++17", "-ffp-contract=off", "-fno-fast-math",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-command-line-argument"]
 SOURCES = ["gemm_generic.hip", "gemm_fast.hip", "gemm_fast_mx.hip", "gemm_fast_tensor.hip", "gemm_pingpong_grouped.hip", "gemm_pingpong_mx.hip", "gemm_pingpong_tensor.hip", "gemm.hip", "gemm_skinny.hip", "quantize.hip", "ns.hip", "ns_fast.hip", "optim.hip", "misc.hip", "tensor.hip",
-           "norm.hip", "norm_rows_bf16.hip", "norm_rows_f16.hip", "norm_rows_f32.hip", "norm_rows_f32_bf16.hip", "norm_rows_f32_f16.hip", "route.hip", "rows.hip"]
+           "norm.hip", "norm_rows_bf16.hip", "norm_rows_f16.hip", "norm_rows_f32.hip", "norm_rows_f32_bf16.hip", "norm_rows_f32_f16.hip", "norm_rows_loose.hip", "route.hip", "rows.hip"]
 
 
 def hipcc():

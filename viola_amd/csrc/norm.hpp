@@ -58,21 +58,58 @@ struct NormArgs {
 // do without them and their registers.
 constexpr int ROW_THREADS = 1024, ROW_COLUMNS = 8 * ROW_THREADS;
 
+// The type of rows that are no whole aligned pieces: any of the three, known when they are read. A thread then has the elements `step` apart from its
+// first on, so that a wavefront's access is of neighbours.
+struct loose_t {};
+
 template <typename T> struct Piece { uint4 word[sizeof(T) / 2]; };           // eight elements as they lie in memory
+template <> struct Piece<loose_t> { float value[8]; };
+
+// A thread's elements of a row: eight from `col` on, or `count` of them `step` apart.
+struct Place {
+    uint32_t col, step;
+    int count;
+    __device__ __forceinline__ Place(const NormArgs& a, int t, int threads, bool loose) : col(loose ? t : 8 * t), step(loose ? threads : 1) {
+        const int left = a.cols - (int)col;
+        count = left <= 0 ? 0 : loose ? min((left + threads - 1) / threads, 8) : 8;
+    }
+    __device__ __forceinline__ bool any() const { return count > 0; }
+    __device__ __forceinline__ uint32_t column(int i) const { return col + i * step; }
+};
 
 // Streamed or not (block_ops.hpp); 32-bit pieces never are: an access of a wavefront is every other 16 bytes of them, which streamed fill no line
 // (4 x 2048 rows of 2048 on a 32-bit stream: 56 instead of 45 us).
 // `row` elements behind `base` for a whole wavefront, `col` more for a thread: the first is a scalar's work, the second an offset of 32 bits.
-template <typename T, bool STREAM> __device__ __forceinline__ Piece<T> load_piece(const void* base, int64_t row, uint32_t col) {
-    const char* line = static_cast<const char*>(base) + row * (int64_t)sizeof(T);
-    const uint4* from = reinterpret_cast<const uint4*>(line + col * (uint32_t)sizeof(T));
-    Piece<T> p;
+template <typename T, bool STREAM> __device__ __forceinline__ Piece<T> load_piece(const void* base, int64_t row, const Place& at, int dtype) {
+    if constexpr (__is_same(T, loose_t)) {
+        Piece<T> p = {};
+        auto from = [&](auto type) {
+            using U = decltype(type);
+            const char* line = static_cast<const char*>(base) + row * (int64_t)sizeof(U);
+            uint32_t offset = at.col * (uint32_t)sizeof(U);
+            asm volatile("" : "+v"(offset));                                 // or eight of them for each tensor stay in registers from row to row
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) p.word[i] = load16<STREAM && sizeof(T) == 2>(from + i);
-    return p;
+            for (int i = 0; i < 8; ++i)
+                if (i < at.count) p.value[i] = to_f32(*reinterpret_cast<const U*>(line + (offset + i * at.step * (uint32_t)sizeof(U))));
+        };
+        if (dtype == VIOLA_F32) from(float());
+        else if (dtype == VIOLA_BF16) from(bf16_t());
+        else from(f16_t());
+        return p;
+    } else {
+        const char* line = static_cast<const char*>(base) + row * (int64_t)sizeof(T);
+        const uint4* from = reinterpret_cast<const uint4*>(line + at.col * (uint32_t)sizeof(T));
+        Piece<T> p;
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) p.word[i] = load16<STREAM && sizeof(T) == 2>(from + i);
+        return p;
+    }
 }
 template <typename T> __device__ __forceinline__ void widen_piece(const Piece<T>& p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (__is_same(T, loose_t)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p.value[i];
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             v[4 * i] = __uint_as_float(p.word[i].x); v[4 * i + 1] = __uint_as_float(p.word[i].y);
@@ -92,10 +129,23 @@ template <typename T> __device__ __forceinline__ void widen_piece(const Piece<T>
         }
     }
 }
-template <typename T> __device__ __forceinline__ void store_piece(void* base, int64_t row, uint32_t col, const float (&v)[8], bool stream) {
+template <typename T> __device__ __forceinline__ void store_piece(void* base, int64_t row, const Place& at, int dtype, const float (&v)[8], bool stream) {
     char* line = static_cast<char*>(base) + row * (int64_t)sizeof(T);
-    uint4* to = reinterpret_cast<uint4*>(line + col * (uint32_t)sizeof(T));
-    if constexpr (sizeof(T) == 4) {
+    uint4* to = reinterpret_cast<uint4*>(line + at.col * (uint32_t)sizeof(T));
+    if constexpr (__is_same(T, loose_t)) {
+        auto to_line = [&](auto type) {
+            using U = decltype(type);
+            char* out = static_cast<char*>(base) + row * (int64_t)sizeof(U);
+            uint32_t offset = at.col * (uint32_t)sizeof(U);
+            asm volatile("" : "+v"(offset));
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < at.count) *reinterpret_cast<U*>(out + (offset + i * at.step * (uint32_t)sizeof(U))) = from_f32<U>(v[i]);
+        };
+        if (dtype == VIOLA_F32) to_line(float());
+        else if (dtype == VIOLA_BF16) to_line(bf16_t());
+        else to_line(f16_t());
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             store16(to + i, make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])), false);
@@ -109,20 +159,26 @@ template <typename T> __device__ __forceinline__ void store_piece(void* base, in
     }
 }
 
-// Eight elements of a vector of any type, as they lie in memory: 32 bytes, or 16 and nothing.
-struct VectorPiece {
+// A thread's elements of a vector of any type, as they lie in memory: 32 bytes, or 16 and nothing. Loose ones are loaded when they are widened, one vector after
+// the other: together they would take every register.
+template <bool LOOSE> struct VectorPiece {
     uint4 word[2] = {};
-    __device__ __forceinline__ void load(const void* base, int64_t row, uint32_t col, int dtype, bool in) {
-        if (!base || !in) return;
+    int64_t row = 0;
+    __device__ __forceinline__ void load(const void* base, int64_t begin, const Place& at, int dtype) {
+        row = begin;
+        if (LOOSE || !base || !at.any()) return;
         const char* line = static_cast<const char*>(base) + (dtype == VIOLA_F32 ? row * 4 : row * 2);
-        const uint4* from = reinterpret_cast<const uint4*>(line + (dtype == VIOLA_F32 ? col * 4 : col * 2));
+        const uint4* from = reinterpret_cast<const uint4*>(line + (dtype == VIOLA_F32 ? at.col * 4 : at.col * 2));
         word[0] = from[0];
         if (dtype == VIOLA_F32) word[1] = from[1];
     }
-    __device__ __forceinline__ void widen(const void* base, int dtype, bool in, float absent, float (&v)[8]) const {
-        if (!base || !in) {
+    __device__ __forceinline__ void widen(const void* base, const Place& at, int dtype, float absent, float (&v)[8]) const {
+        if (!base || !at.any()) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = absent;
+        } else if constexpr (LOOSE) {
+            widen_piece(load_piece<loose_t, false>(base, row, at, dtype), v);
+            __builtin_amdgcn_sched_barrier(0);
         } else if (dtype == VIOLA_F32) {
             widen_piece(Piece<float>{{word[0], word[1]}}, v);
         } else if (dtype == VIOLA_BF16) {
@@ -206,45 +262,55 @@ struct TeamSums {
 // v^-1/2 within an ulp; the hardware's root reads what is below the normal numbers as zero.
 __device__ __forceinline__ float inverse_root(float v) { return v < 1e-30f ? 1.0f / sqrtf(v) : __builtin_amdgcn_rsqf(v); }
 
-template <bool LAYER> __device__ __forceinline__ float2 row_statistics(const float (&v)[8], bool in, int kind, int columns, float inverse, float eps, TeamSums& sums) {
+template <bool LAYER, bool LOOSE>
+__device__ __forceinline__ float2 row_statistics(const float (&v)[8], const Place& at, int kind, int columns, float inverse, float eps, TeamSums& sums) {
+    float mean = 0.0f, q = 0.0f;                                             // columns beyond the row are zero, or their thread has none
     if (LAYER && kind == VIOLA_NORM_LAYER) {
-        const float2 around = sums.around_mean(v, in, columns, inverse);
-        return make_float2(around.x, inverse_root(around.y * inverse + eps));
-    }
-    float q = 0.0f;
+        if constexpr (!LOOSE) {
+            const float2 around = sums.around_mean(v, at.any(), columns, inverse);
+            return make_float2(around.x, inverse_root(around.y * inverse + eps));
+        }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q = fmaf(v[i], v[i], q);
-    return make_float2(0.0f, inverse_root(sums.one(in ? q : 0.0f) * inverse + eps));
+        for (int i = 0; i < 8; ++i) mean += v[i];
+        mean = TeamSums::quotient(sums.one(mean), (float)columns, inverse);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float d = LOOSE ? (i < at.count ? v[i] - mean : 0.0f) : v[i];
+        q = fmaf(d, d, q);
+    }
+    return make_float2(mean, inverse_root(sums.one(at.any() ? q : 0.0f) * inverse + eps));
 }
 
 // All loads are under way before the first is used: a block waits for them once.
-template <int FORM> struct NormVectors {
+template <int FORM, bool LOOSE> struct NormVectors {
     float ga[8], gb[8], w[8], b[8];
-    __device__ __forceinline__ void load(const NormArgs& a, int64_t group, uint32_t col, bool in) {
-        VectorPiece gate, after_weight, after_bias, weight, bias, scale, shift;
-        if constexpr (FORM == FORM_PLAIN) gate.load(a.gate.data, group * a.gate.pitch, col, a.vector_dtype, in);
+    __device__ __forceinline__ void load(const NormArgs& a, int64_t group, Place at) {
+        asm volatile("" : "+v"(at.col));                                     // or the addresses are kept in registers from group to group
+        VectorPiece<LOOSE> gate, after_weight, after_bias, weight, bias, scale, shift;
+        if constexpr (FORM == FORM_PLAIN) gate.load(a.gate.data, group * a.gate.pitch, at, a.vector_dtype);
         if constexpr (FORM == FORM_AFTER || FORM == FORM_BETWEEN) {
-            after_weight.load(a.after_weight, 0, col, a.weight_dtype, in);
-            after_bias.load(a.after_bias, 0, col, a.weight_dtype, in);
-            gate.load(a.gate.data, group * a.gate.pitch, col, a.vector_dtype, in);
+            after_weight.load(a.after_weight, 0, at, a.weight_dtype);
+            after_bias.load(a.after_bias, 0, at, a.weight_dtype);
+            gate.load(a.gate.data, group * a.gate.pitch, at, a.vector_dtype);
         }
         if constexpr (FORM != FORM_AFTER) {
-            weight.load(a.weight, 0, col, a.weight_dtype, in);
-            bias.load(a.bias, 0, col, a.weight_dtype, in);
-            scale.load(a.scale.data, group * a.scale.pitch, col, a.vector_dtype, in);
-            shift.load(a.shift.data, group * a.shift.pitch, col, a.vector_dtype, in);
+            weight.load(a.weight, 0, at, a.weight_dtype);
+            bias.load(a.bias, 0, at, a.weight_dtype);
+            scale.load(a.scale.data, group * a.scale.pitch, at, a.vector_dtype);
+            shift.load(a.shift.data, group * a.shift.pitch, at, a.vector_dtype);
         }
         __builtin_amdgcn_sched_barrier(0);
         float u[8];
         if constexpr (FORM == FORM_PLAIN) {
-            gate.widen(a.gate.data, a.vector_dtype, in, 1.0f, ga);
+            gate.widen(a.gate.data, at, a.vector_dtype, 1.0f, ga);
 #pragma unroll
             for (int i = 0; i < 8; ++i) ga[i] *= a.alpha;
         }
         if constexpr (FORM == FORM_AFTER || FORM == FORM_BETWEEN) {
-            after_weight.widen(a.after_weight, a.weight_dtype, in, 1.0f, ga);
-            after_bias.widen(a.after_bias, a.weight_dtype, in, 0.0f, gb);
-            gate.widen(a.gate.data, a.vector_dtype, in, 1.0f, u);
+            after_weight.widen(a.after_weight, at, a.weight_dtype, 1.0f, ga);
+            after_bias.widen(a.after_bias, at, a.weight_dtype, 0.0f, gb);
+            gate.widen(a.gate.data, at, a.vector_dtype, 1.0f, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 ga[i] *= a.alpha * u[i];
@@ -252,17 +318,25 @@ template <int FORM> struct NormVectors {
             }
         }
         if constexpr (FORM != FORM_AFTER) {
-            weight.widen(a.weight, a.weight_dtype, in, 1.0f, w);
-            bias.widen(a.bias, a.weight_dtype, in, 0.0f, b);
-            scale.widen(a.scale.data, a.vector_dtype, in, 0.0f, u);
+            weight.widen(a.weight, at, a.weight_dtype, 1.0f, w);
+            bias.widen(a.bias, at, a.weight_dtype, 0.0f, b);
+            scale.widen(a.scale.data, at, a.vector_dtype, 0.0f, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 w[i] = fmaf(w[i], u[i], w[i]);
                 b[i] = fmaf(b[i], u[i], b[i]);
             }
-            shift.widen(a.shift.data, a.vector_dtype, in, 0.0f, u);
+            shift.widen(a.shift.data, at, a.vector_dtype, 0.0f, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) b[i] += u[i];
+        }
+        if constexpr (LOOSE) {                                               // columns beyond the row weigh nothing
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i < at.count) continue;
+                if constexpr (FORM != FORM_BEFORE) ga[i] = gb[i] = 0.0f;
+                if constexpr (FORM != FORM_AFTER) w[i] = b[i] = 0.0f;
+            }
         }
     }
 };
@@ -273,11 +347,12 @@ template <typename TX, typename TY, int FORM, bool LAYER> __global__ __launch_bo
     __shared__ float2 slots[32];
     const int threads = a.team, teams = blockDim.x / threads, team = __builtin_amdgcn_readfirstlane(threadIdx.x / threads), t = threadIdx.x - team * threads;
     TeamSums sums(slots, threads / 64);
-    const uint32_t col = t * 8;
-    const bool in = (int)col < a.cols;
+    constexpr bool LOOSE = __is_same(TX, loose_t);
+    const Place at(a, t, threads, LOOSE);
+    const bool in = at.any();
     const float inverse = 1.0f / (float)a.cols;
     const int64_t begin = blockIdx.x * a.chunk, end = begin + a.chunk < a.rows ? begin + a.chunk : a.rows;
-    NormVectors<FORM> vectors;
+    NormVectors<FORM, LOOSE> vectors;
     int64_t group_end = -1;                                                  // of the rows that the vectors are those of
     // Two rows are under way while one is worked on; zero beyond the row.
     Piece<TX> raw_x = {}, next_x = {};
@@ -285,49 +360,58 @@ template <typename TX, typename TY, int FORM, bool LAYER> __global__ __launch_bo
     auto load = [&](int64_t row, Piece<TX>& to_x, Piece<TY>& to_y) {
         if (!in || row >= end) return;                                       // beyond the end: some row before, which nobody stores
         auto from = [&](auto stream) {
-            to_x = load_piece<TX, decltype(stream)::value>(a.x, row * a.x_pitch, col);
-            if constexpr (FORM != FORM_BEFORE) to_y = load_piece<TY, decltype(stream)::value>(a.y, row * a.y_pitch, col);
+            to_x = load_piece<TX, decltype(stream)::value>(a.x, row * a.x_pitch, at, a.x_dtype);
+            if constexpr (FORM != FORM_BEFORE) to_y = load_piece<TY, decltype(stream)::value>(a.y, row * a.y_pitch, at, a.branch_dtype);
         };
         a.stream_in ? from(std::true_type()) : from(std::false_type());
     };
-    load(begin + team, raw_x, raw_y);
-    load(begin + team + teams, next_x, next_y);
+    if constexpr (!LOOSE) {
+        load(begin + team, raw_x, raw_y);
+        load(begin + team + teams, next_x, next_y);
+    }
     for (int64_t base = begin; base < end; base += teams) {
         const int64_t row = base + team;
         const bool there = in && row < end;
         if (row >= group_end && row < end) {
             const int64_t group = row / a.group_rows;
             group_end = (group + 1) * a.group_rows;
-            vectors.load(a, group, col, in);
+            vectors.load(a, group, at);
         }
         float x[8], y[8];
+        if constexpr (LOOSE) load(row, raw_x, raw_y);                        // eight loads for each of them: no registers for more
         widen_piece(raw_x, x);
         if constexpr (FORM != FORM_BEFORE) widen_piece(raw_y, y);
-        raw_x = next_x;
-        raw_y = next_y;
-        load(row + 2 * teams, next_x, next_y);
+        if constexpr (!LOOSE) {
+            raw_x = next_x;
+            raw_y = next_y;
+            load(row + 2 * teams, next_x, next_y);
+        }
         float4 stat = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
         if constexpr (FORM == FORM_PLAIN) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(a.rho, x[i], y[i] * vectors.ga[i]);
         } else if constexpr (FORM != FORM_BEFORE) {
             if (a.after != VIOLA_NORM_NONE) {
-                const float2 s = row_statistics<LAYER>(y, in, a.after, a.cols, inverse, a.eps, sums);
+                const float2 s = row_statistics<LAYER, LOOSE>(y, at, a.after, a.cols, inverse, a.eps, sums);
                 stat.x = s.x;
                 stat.y = s.y;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(a.rho, x[i], fmaf((LAYER ? y[i] - stat.x : y[i]) * stat.y, vectors.ga[i], vectors.gb[i]));
         }
+        if constexpr (FORM != FORM_BEFORE && LOOSE) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = i < at.count ? x[i] : 0.0f;
+        }
         if constexpr (FORM != FORM_BEFORE)
-            if (there) store_piece<TX>(a.out, row * a.cols, col, x, a.stream_out);
+            if (there) store_piece<TX>(a.out, row * a.cols, at, a.x_dtype, x, a.stream_out);
         if constexpr (FORM != FORM_AFTER) {
-            const float2 s = row_statistics<LAYER>(x, in, a.before, a.cols, inverse, a.eps, sums);
+            const float2 s = row_statistics<LAYER, LOOSE>(x, at, a.before, a.cols, inverse, a.eps, sums);
             stat.z = s.x;
             stat.w = s.y;
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf((LAYER ? x[i] - s.x : x[i]) * s.y, vectors.w[i], vectors.b[i]);
-            if (there) store_piece<TY>(a.h, row * a.cols, col, x, a.stream_out);
+            if (there) store_piece<TY>(a.h, row * a.cols, at, a.branch_dtype, x, a.stream_out);
         }
         if (a.stats && t == 0 && row < end) a.stats[row] = stat;
     }
@@ -336,19 +420,21 @@ template <typename TX, typename TY, int FORM, bool LAYER> __global__ __launch_bo
 // One portion: rows of one group, a team each in turn. The teams' sums are joined in LDS at the end, team by team.
 template <typename TX, typename TY, int FORM, bool LAYER, bool BIAS, bool SHIFT> __global__ __launch_bounds__(ROW_THREADS) void norm_backward_kernel(NormArgs a) {
     __shared__ float2 slots[32];
+    using Sum = std::conditional_t<__is_same(TX, loose_t), loose_t, float>;
     extern __shared__ float joined[];                                        // [teams - 1][cols] where a block has several teams
     const int threads = a.team, teams = blockDim.x / threads, team = __builtin_amdgcn_readfirstlane(threadIdx.x / threads), t = threadIdx.x - team * threads;
     TeamSums sums(slots, threads / 64);
-    const uint32_t col = t * 8;
-    const bool in = (int)col < a.cols;
+    constexpr bool LOOSE = __is_same(TX, loose_t);
+    const Place at(a, t, threads, LOOSE);
+    const bool in = at.any();
     const float inverse = 1.0f / (float)a.cols;
     const int64_t length = (a.group_rows + a.per_group - 1) / a.per_group;
     for (int64_t portion = blockIdx.x; portion < a.portions; portion += gridDim.x) {
         const int64_t group = portion / a.per_group, group_end = (group + 1) * a.group_rows;
         const int64_t begin = group * a.group_rows + portion % a.per_group * length;
         const int64_t end = begin + length < group_end ? begin + length : group_end;
-        NormVectors<FORM> vectors;                                           // its b is not used, and neither is gb without BIAS
-        vectors.load(a, group, col, in);
+        NormVectors<FORM, LOOSE> vectors;                                           // its b is not used, and neither is gb without BIAS
+        vectors.load(a, group, at);
         float a1[8] = {}, a0[8] = {}, s1[8] = {}, s0[8] = {};
         // Beyond the row and beyond the portion everything is zero, the row's statistics too, and stays zero: nothing below asks again.
         Piece<TX> raw_x = {}, raw_dout = {};
@@ -358,10 +444,10 @@ template <typename TX, typename TY, int FORM, bool LAYER, bool BIAS, bool SHIFT>
                 if (!in) return;
                 auto from = [&](auto stream) {
                     constexpr bool STREAM = decltype(stream)::value;
-                    if constexpr (FORM != FORM_AFTER) raw_x = load_piece<TX, STREAM>(a.x, row * a.x_pitch, col);
-                    if constexpr (FORM != FORM_BEFORE) raw_y = load_piece<TY, STREAM>(a.y, row * a.y_pitch, col);
-                    if constexpr (FORM != FORM_AFTER) raw_dh = load_piece<TY, STREAM>(a.dh, row * a.cols, col);
-                    if constexpr (FORM != FORM_BEFORE) if (a.dout) raw_dout = load_piece<TX, STREAM>(a.dout, row * a.cols, col);
+                    if constexpr (FORM != FORM_AFTER) raw_x = load_piece<TX, STREAM>(a.x, row * a.x_pitch, at, a.x_dtype);
+                    if constexpr (FORM != FORM_BEFORE) raw_y = load_piece<TY, STREAM>(a.y, row * a.y_pitch, at, a.branch_dtype);
+                    if constexpr (FORM != FORM_AFTER) raw_dh = load_piece<TY, STREAM>(a.dh, row * a.cols, at, a.branch_dtype);
+                    if constexpr (FORM != FORM_BEFORE) if (a.dout) raw_dout = load_piece<TX, STREAM>(a.dout, row * a.cols, at, a.x_dtype);
                 };
                 a.stream_in ? from(std::true_type()) : from(std::false_type());
             } else {
@@ -369,25 +455,28 @@ template <typename TX, typename TY, int FORM, bool LAYER, bool BIAS, bool SHIFT>
                 raw_y = raw_dh = {};
             }
         };
-        load(begin + team);
+        if constexpr (!LOOSE) load(begin + team);
         for (int64_t base = begin; base < end; base += teams) {
             const int64_t row = base + team;
             const bool there = in && row < end;
+            if constexpr (LOOSE) load(row);
             float4 stat = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (there) stat = a.stats[row];
             float x[8], y[8], d[8], q[8];                                    // x^, y^, D, dh W
             if constexpr (FORM != FORM_BEFORE) {
                 widen_piece(raw_y, y);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < 8; ++i) {
                     if constexpr (FORM != FORM_PLAIN) y[i] = (LAYER ? y[i] - stat.x : y[i]) * stat.y;
+                    if constexpr (LOOSE) y[i] = i < at.count ? y[i] : 0.0f;
+                }
             }
             if constexpr (FORM != FORM_AFTER) {
                 widen_piece(raw_x, x);
                 widen_piece(raw_dh, q);
             }
             const Piece<TX> dout = raw_dout;
-            load(row + teams);
+            if constexpr (!LOOSE) load(row + teams);
             if constexpr (FORM != FORM_BEFORE) widen_piece(dout, d);
             if constexpr (FORM != FORM_AFTER) {
                 float along = 0.0f, total = 0.0f;
@@ -395,6 +484,7 @@ template <typename TX, typename TY, int FORM, bool LAYER, bool BIAS, bool SHIFT>
                 for (int i = 0; i < 8; ++i) {
                     if constexpr (FORM == FORM_BETWEEN || FORM == FORM_PLAIN) x[i] = fmaf(a.rho, x[i], BIAS ? fmaf(y[i], vectors.ga[i], vectors.gb[i]) : y[i] * vectors.ga[i]);
                     x[i] = (LAYER ? x[i] - stat.z : x[i]) * stat.w;
+                    if constexpr (LOOSE) x[i] = i < at.count ? x[i] : 0.0f;
                     s1[i] = fmaf(q[i], x[i], s1[i]);
                     if constexpr (SHIFT) s0[i] += q[i];
                     q[i] *= vectors.w[i];
@@ -417,11 +507,11 @@ template <typename TX, typename TY, int FORM, bool LAYER, bool BIAS, bool SHIFT>
             }
             if (a.dx && there) {
                 if constexpr (FORM == FORM_BEFORE) {
-                    store_piece<TX>(a.dx, row * a.cols, col, d, a.stream_out);
+                    store_piece<TX>(a.dx, row * a.cols, at, a.x_dtype, d, a.stream_out);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[i] = a.rho * d[i];
-                    store_piece<TX>(a.dx, row * a.cols, col, x, a.stream_out);
+                    store_piece<TX>(a.dx, row * a.cols, at, a.x_dtype, x, a.stream_out);
                 }
             }
             if constexpr (FORM != FORM_BEFORE) {
@@ -447,22 +537,23 @@ template <typename TX, typename TY, int FORM, bool LAYER, bool BIAS, bool SHIFT>
 #pragma unroll
                     for (int i = 0; i < 8; ++i) d[i] = stat.y * (d[i] - (LAYER ? fmaf(y[i], m1, m0) : y[i] * m1));
                 }
-                if (there) store_piece<TY>(a.dy, row * a.cols, col, d, a.stream_out);
+                if (there) store_piece<TY>(a.dy, row * a.cols, at, a.branch_dtype, d, a.stream_out);
             }
         }
         float* to = a.parts + portion * __popc(a.sums) * a.cols;
         auto write = [&](float (&v)[8]) {
             if (teams > 1) {
                 __syncthreads();                                             // the sum before has been read
-                if (team && in) store_piece<float>(joined, (int64_t)(team - 1) * a.cols, col, v, false);
+                if (team && in) store_piece<Sum>(joined, (int64_t)(team - 1) * a.cols, at, VIOLA_F32, v, false);
                 __syncthreads();
                 if (!team && in)
                     for (int u = 1; u < teams; ++u) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] += joined[(u - 1) * a.cols + col + i];
+                        for (int i = 0; i < 8; ++i)
+                            if (i < at.count) v[i] += joined[(u - 1) * a.cols + at.column(i)];
                     }
             }
-            if (!team && in) store_piece<float>(to, 0, col, v, false);
+            if (!team && in) store_piece<Sum>(to, 0, at, VIOLA_F32, v, false);
             to += a.cols;
         };
         if (a.sums & SUM_A1) write(a1);

@@ -28,19 +28,31 @@ template <typename F> void with_form(int form, bool flag, F&& f) {
 inline bool any_layer(const NormArgs& a) { return a.after == VIOLA_NORM_LAYER || a.before == VIOLA_NORM_LAYER; }
 
 template <typename TX, typename TY> void norm_forward_rows(const NormArgs& a, int form, dim3 grid, hipStream_t stream) {
-    with_form(form, any_layer(a), [&](auto f, auto layer) { VIOLA_LAUNCH((norm_forward_kernel<TX, TY, decltype(f)::value, decltype(layer)::value>), grid, norm_block(a, true), 0, stream, a); });
+    if constexpr (__is_same(TX, loose_t)) {                                  // one kernel for each form
+        if (form == FORM_BEFORE) VIOLA_LAUNCH((norm_forward_kernel<TX, TY, FORM_BEFORE, true>), grid, norm_block(a, true), 0, stream, a);
+        else if (form == FORM_AFTER) VIOLA_LAUNCH((norm_forward_kernel<TX, TY, FORM_AFTER, true>), grid, norm_block(a, true), 0, stream, a);
+        else VIOLA_LAUNCH((norm_forward_kernel<TX, TY, FORM_BETWEEN, true>), grid, norm_block(a, true), 0, stream, a);
+    } else {
+        with_form(form, any_layer(a), [&](auto f, auto layer) { VIOLA_LAUNCH((norm_forward_kernel<TX, TY, decltype(f)::value, decltype(layer)::value>), grid, norm_block(a, true), 0, stream, a); });
+    }
 }
 
 // A form has at most the sums of its own sides; between two blocks a bias after the one and a shift before the other share a kernel.
 template <typename TX, typename TY> void norm_backward_rows(const NormArgs& a, int form, bool bias, bool shift, dim3 grid, hipStream_t stream) {
     const int block = norm_block(a, false);
     const unsigned lds = (unsigned)((block / a.team - 1) * a.cols * 4);
-    with_form(form, any_layer(a), [&](auto f, auto layer) {
-        constexpr int FORM = decltype(f)::value;
-        constexpr bool LAYER = decltype(layer)::value, WITH_BIAS = FORM == FORM_AFTER || FORM == FORM_BETWEEN, WITH_SHIFT = FORM != FORM_AFTER;
-        if ((WITH_BIAS && bias) || (WITH_SHIFT && shift)) VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM, LAYER, WITH_BIAS, WITH_SHIFT>), grid, block, lds, stream, a);
-        else VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM, LAYER, false, false>), grid, block, lds, stream, a);
-    });
+    if constexpr (__is_same(TX, loose_t)) {
+        if (form == FORM_BEFORE) VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_BEFORE, true, false, true>), grid, block, lds, stream, a);
+        else if (form == FORM_AFTER) VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_AFTER, true, true, false>), grid, block, lds, stream, a);
+        else VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM_BETWEEN, true, true, true>), grid, block, lds, stream, a);
+    } else {
+        with_form(form, any_layer(a), [&](auto f, auto layer) {
+            constexpr int FORM = decltype(f)::value;
+            constexpr bool LAYER = decltype(layer)::value, WITH_BIAS = FORM == FORM_AFTER || FORM == FORM_BETWEEN, WITH_SHIFT = FORM != FORM_AFTER;
+            if ((WITH_BIAS && bias) || (WITH_SHIFT && shift)) VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM, LAYER, WITH_BIAS, WITH_SHIFT>), grid, block, lds, stream, a);
+            else VIOLA_LAUNCH((norm_backward_kernel<TX, TY, FORM, LAYER, false, false>), grid, block, lds, stream, a);
+        });
+    }
 }
 
 }  // namespace viola
