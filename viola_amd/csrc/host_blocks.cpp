@@ -3,6 +3,7 @@
 // of another type) and make what a kernel cannot read contiguous first.
 #include "host.hpp"
 
+#include <ATen/hip/EmptyTensor.h>
 #include <torch/csrc/autograd/functions/utils.h>
 
 using namespace viola_host;
@@ -27,6 +28,10 @@ void check_float(const char* name, const char* what, const Tensor& t, const at::
 
 // The gradients of these nodes are computed by kernels that autograd does not see.
 void check_once(const char* name) { TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), name, " can be differentiated once only (create_graph is not supported)"); }
+
+// Memory for a result: the allocator at once, without the dispatcher's two rounds (a router has up to eight results and workspaces, and a
+// decoding step's call of it takes as long on the host as on the GPU).
+Tensor room(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) { return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt)); }
 
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
@@ -181,9 +186,9 @@ std::vector<Tensor> norm(const char* name, const Tensor (&input)[INPUTS], NormPl
         for (int i = AFTER_WEIGHT; i < INPUTS; ++i)
             if (t[i].defined()) value[i] = plan.readable(i, t[i], cols);
         const std::optional<Rows> yr = t[Y].defined() ? std::optional<Rows>(t[Y]) : std::nullopt;
-        if (want_out) out = at::empty(x.sizes(), x.options());
-        if (want_h) h = at::empty(x.sizes(), x.options().dtype(plan.branch));
-        if (need) stats = at::empty({xr.count, 4}, x.options().dtype(at::kFloat));
+        if (want_out) out = room(x.sizes(), x.scalar_type(), device);
+        if (want_h) h = room(x.sizes(), plan.branch, device);
+        if (need) stats = room({xr.count, 4}, at::kFloat, device);
         if (xr.count) {
             Vectors v;
             v.set(plan, value);
@@ -225,7 +230,6 @@ variable_list NormBackward::apply(variable_list&& grads) {
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Device device = (d_out.defined() ? d_out : d_h).device();
     const c10::DeviceGuard guard(device);
-    const auto options = at::TensorOptions().device(device);
     Tensor t[INPUTS];
     for (int i = 0; i < INPUTS; ++i) {
         if (!has[i]) continue;
@@ -243,8 +247,8 @@ variable_list NormBackward::apply(variable_list&& grads) {
     Tensor grad[INPUTS];
     for (int i = 0; i < INPUTS; ++i) {
         if (!wanted[i]) continue;
-        const auto to = options.dtype(i < AFTER_WEIGHT ? type[i] : plan.type_of(i));
-        grad[i] = rows ? at::empty(shape[i], to) : at::zeros(shape[i], to);
+        const at::ScalarType to = i < AFTER_WEIGHT ? type[i] : plan.type_of(i);
+        grad[i] = rows ? room(shape[i], to, device) : at::zeros(shape[i], at::TensorOptions().device(device).dtype(to));
     }
     if (rows) {
         const Tensor dout = d_out.defined() ? d_out.contiguous() : Tensor(), dh = d_h.defined() ? d_h.contiguous() : Tensor();
@@ -255,7 +259,7 @@ variable_list NormBackward::apply(variable_list&& grads) {
         const int sums = (wanted[AFTER_WEIGHT] || wanted[GATE]) + (wanted[AFTER_BIAS] || (wanted[GATE] && has[AFTER_BIAS])) + (wanted[WEIGHT] || wanted[SCALE]) +
                          (wanted[BIAS] || wanted[SHIFT] || (wanted[SCALE] && has[BIAS]));
         const int64_t floats = viola_norm_portions(rows, cols, rows / plan.groups) * sums * cols;
-        const Tensor parts = sums ? at::empty({floats}, options.dtype(at::kFloat)) : Tensor();
+        const Tensor parts = sums ? room({floats}, at::kFloat, device) : Tensor();
         for (int i = AFTER_WEIGHT; i < INPUTS; ++i)
             if (has[i]) t[i] = plan.readable(i, t[i], cols);
         Vectors v;
@@ -339,14 +343,14 @@ Routed router(const char* name, const Tensor& logits, const Tensor& given, const
             r.counts = at::zeros({plan.experts}, ints);
             r.balance = at::zeros({}, floats);
         } else {
-            r.counts = at::empty({plan.experts}, ints);
-            r.balance = at::empty({}, floats);
+            r.counts = room({plan.experts}, at::kInt, device);
+            r.balance = room({}, at::kFloat, device);
         }
         if (!plan.given) {
-            r.chosen = at::empty(choices, ints);
-            r.gates = at::empty(choices, floats);
-            r.positions = at::empty(choices, ints);
-            r.offsets = plan.tokens ? at::empty({plan.experts + 1}, ints) : at::zeros({plan.experts + 1}, ints);
+            r.chosen = room(choices, at::kInt, device);
+            r.gates = room(choices, at::kFloat, device);
+            r.positions = room(choices, at::kInt, device);
+            r.offsets = plan.tokens ? room({plan.experts + 1}, at::kInt, device) : at::zeros({plan.experts + 1}, ints);
         }
         if (plan.tokens) {
             const Tensor counted = mask.defined() ? mask.contiguous() : Tensor();
@@ -354,10 +358,10 @@ Routed router(const char* name, const Tensor& logits, const Tensor& given, const
             const int64_t cost_at = kept.take(sequences * plan.experts * 4);
             stats_at = need ? kept.take(plan.tokens * 8) : 0;
             const int64_t words = viola_route_workspace(plan.tokens, plan.experts, plan.sequence);
-            Arena temp;
-            temp.take(words * 4);
+            Arena freed, &temp = need ? freed : kept;                        // nothing is kept without a gradient
+            const int64_t temp_at = temp.take(words * 4);
             kept.make(device);
-            temp.make(device);
+            if (need) freed.make(device);
             float* stats = need ? kept.as<float>(stats_at) : nullptr;
             const viola_stream_t stream = stream_of(logits);
             const int type = code_of(logits.scalar_type());
@@ -366,12 +370,12 @@ Routed router(const char* name, const Tensor& logits, const Tensor& given, const
             if (plan.given) {
                 const Tensor choice = given.contiguous();
                 VIOLA_CALL(viola_balance_forward, rows.data(), rows.pitch, type, plan.tokens, plan.experts, (int)plan.top_k, plan.score, mask_p, plan.sequence,
-                           choice.const_data_ptr(), choice.scalar_type() == at::kLong, counts, loss, kept.as<float>(cost_at), stats, temp.as<int32_t>(0), words, stream);
+                           choice.const_data_ptr(), choice.scalar_type() == at::kLong, counts, loss, kept.as<float>(cost_at), stats, temp.as<int32_t>(temp_at), words, stream);
             } else {
                 VIOLA_CALL(viola_route_forward, rows.data(), rows.pitch, type, plan.tokens, plan.experts, (int)plan.top_k, plan.score, plan.normalize, (float)plan.scale, mask_p,
                            plan.sequence, static_cast<int*>(r.chosen.mutable_data_ptr()), static_cast<float*>(r.gates.mutable_data_ptr()),
                            static_cast<int*>(r.positions.mutable_data_ptr()), counts, static_cast<int*>(r.offsets.mutable_data_ptr()), loss, kept.as<float>(cost_at), stats,
-                           temp.as<int32_t>(0), words, stream);
+                           temp.as<int32_t>(temp_at), words, stream);
             }
         }
     }
@@ -401,7 +405,7 @@ variable_list RouterBackward::apply(variable_list&& grads) {
     const c10::DeviceGuard guard(device);
     const Tensor l = logits.unpack();
     TORCH_CHECK(l.device() == device && l.scalar_type() == type && l.sizes() == at::IntArrayRef(shape), "the logits of a router were moved or replaced between forward and backward");
-    result[0] = at::empty(shape, at::TensorOptions().device(device).dtype(type));
+    result[0] = room(shape, type, device);
     if (!plan.tokens) return result;
     const Tensor arena = restored(kept, device, at::kByte, {kept_bytes});
     const float* base = static_cast<const float*>(arena.const_data_ptr());
@@ -456,7 +460,7 @@ struct DispatchBackward : public Node {
         at::AutoDispatchBelowADInplaceOrView below;
         const c10::DeviceGuard guard(grads[0].device());
         const Tensor p = restored(positions, grads[0].device(), at::kInt, places);
-        result[0] = at::empty(shape, grads[0].options().dtype(type));
+        result[0] = room(shape, type, grads[0].device());
         if (result[0].numel()) gather(grads[0], p, Tensor(), result[0]);
         return result;
     }
@@ -481,7 +485,7 @@ Tensor dispatch(const Tensor& x, const Tensor& positions_, const Tensor& offsets
     {
         at::AutoDispatchBelowADInplaceOrView below;
         positions = positions_.contiguous();
-        out = tokens ? at::empty({rows, cols}, x.options()) : at::zeros({rows, cols}, x.options());
+        out = tokens ? room({rows, cols}, x.scalar_type(), device) : at::zeros({rows, cols}, x.options());
         if (tokens && rows) scatter(x, positions, offsets_.contiguous(), Tensor(), out, rows, Tensor(), Tensor());
     }
     if (need) {
@@ -519,8 +523,8 @@ struct CombineBackward : public Node {
         }
         const auto options = at::TensorOptions().device(device);
         const bool any = p.numel() && shape[0];
-        if (needs_y) result[0] = any ? at::empty(shape, options.dtype(type)) : at::zeros(shape, options.dtype(type));
-        Tensor dots = needs_gates ? any ? at::empty(places, options.dtype(at::kFloat)) : at::zeros(places, options.dtype(at::kFloat)) : Tensor();
+        if (needs_y) result[0] = any ? room(shape, type, device) : at::zeros(shape, options.dtype(type));
+        Tensor dots = needs_gates ? any ? room(places, at::kFloat, device) : at::zeros(places, options.dtype(at::kFloat)) : Tensor();
         if (any && (needs_y || needs_gates)) scatter(grads[0], p, o, g, result[0], shape[0], rows, dots);
         if (needs_gates) result[1] = gates_type == at::kFloat ? dots : dots.to(gates_type);
         return result;
@@ -552,7 +556,7 @@ Tensor combine(const Tensor& y, const Tensor& positions_, const Tensor& offsets_
         if (gates_.defined()) gates = gates_.to(at::kFloat).contiguous();
         std::vector<int64_t> shape(positions.sizes().begin(), positions.sizes().end() - 1);
         shape.push_back(y.size(1));
-        out = at::empty(shape, y.options());
+        out = room(shape, y.scalar_type(), device);
         if (out.numel()) gather(y, positions, gates, out);
     }
     if (need) {
