@@ -31,6 +31,8 @@ Pinning status (what fixes each function besides its own formula):
                      fall (2048 + 1 -> 2048 across steps, exact within a step, cleared per period). Where an
                      NVIDIA mma rounds inside a 32-k step is not in the reference's text   -> the model's own
                      arithmetic is pinned, its agreement with the reference's hardware is parity unpinned
+  norms around a block, expert routing (oracle.norms, oracle.routing) : NOT in the reference; central differences
+                     of every gradient, hand cases of choices and places                   -> parity unpinned
   NaN/Inf inside a quantize group: the reference's GPU and CPU branches disagree
                      (GPU reduce_absmax ignores NaN); the GPU behaviour is restated
                                                                    -> parity unpinned

@@ -3,7 +3,8 @@
 What is here, by sub-package:
 
   nn           `Linear` (grouped FP32 scales, per-tensor `current` / `delayed` scaling, MXFP8), `MLP` (gated, the
-               activation fused into the GEMM epilogues), `grouped_linear` for variable-sized expert groups
+               activation fused into the GEMM epilogues), `grouped_linear` for variable-sized expert groups; around a block
+               `norm_before`, `norm_after`, `norm_between`, `route`, `balance_loss`, `dispatch`, `combine`
   optim        `FP8Muon` (FP8 momentum state, Newton-Schulz orthogonalisation in bf16 or fp16), `bind_optimizer`
                (master weights behind FP8 / 16-bit parameters)
   distributed  `FP8Communication`, the FP8 wire codec for gradient buckets, and `packet_bytes`
