@@ -313,10 +313,6 @@ template <int LANES, int VALUES, bool GIVEN, bool SIGMOID> __global__ __launch_b
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) sum[i] = 0.0f;
         int here = 0;                                                        // tokens that the wavefront has counted
-        if (threadIdx.x == 0) counted_tokens = 0;
-        if (!GIVEN)
-            for (int i = threadIdx.x; i < a.experts * WORDS; i += threads) bits[i] = 0;
-        __syncthreads();
         float next[VALUES];
         bool next_taken;
         auto load = [&](int64_t token) {
@@ -329,6 +325,10 @@ template <int LANES, int VALUES, bool GIVEN, bool SIGMOID> __global__ __launch_b
             }
         };
         load(begin + slot);
+        if (threadIdx.x == 0) counted_tokens = 0;
+        if (!GIVEN)
+            for (int i = threadIdx.x; i < a.experts * WORDS; i += threads) bits[i] = 0;
+        __syncthreads();
         for (int64_t base = begin; base < end; base += STAGED) {
             for (int row = slot; row - slot < STAGED && base + row - slot < end; row += rows) {
                 const int64_t token = base + row;
