@@ -35,22 +35,23 @@ Tensor room(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device
 
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
-// A tensor as rows of its last dimension with one distance between them; copied where it has none.
+// A tensor as rows of its last dimension with one distance between them; copied where it has none, and where rows overlap: those of a
+// broadcast dimension, whose distance is 0, too (autograd hands out such gradients: that of a sum over tokens repeats every row).
 struct Rows {
     Tensor holder;
     int64_t count, cols, pitch;
-    explicit Rows(const Tensor& t) : holder(t), count(1), cols(t.size(-1)) {
+    explicit Rows(const Tensor& t) : holder(t), count(1), cols(t.size(-1)), pitch(cols) {
         for (int64_t i = 0; i + 1 < t.dim(); ++i) count *= t.size(i);
-        bool whole = cols <= 1 || t.stride(-1) == 1;
-        int64_t expected = 0;                                    // 0: no dimension of more than one yet
-        pitch = cols;
+        bool whole = cols <= 1 || t.stride(-1) == 1, first = true;
+        int64_t expected = 0;                                    // distance of a dimension's rows where all inside of it lie `pitch` apart
         for (int64_t i = t.dim() - 2; i >= 0 && whole; --i) {
             if (t.size(i) == 1) continue;
-            if (!expected) pitch = t.stride(i);
-            else whole = t.stride(i) == expected;
+            if (first) pitch = t.stride(i);
+            whole = pitch >= cols && (first || t.stride(i) == expected);
             expected = t.stride(i) * t.size(i);
+            first = false;
         }
-        if (!whole || pitch < cols) {
+        if (!whole) {
             holder = t.contiguous();
             pitch = cols;
         }
@@ -583,6 +584,11 @@ Tensor or_none(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
 }  // namespace
 
 void viola_host::register_blocks(py::module_& m) {
+    // How the operators below read a tensor: (rows, distance between them in elements, whether they are a copy's). Stride arithmetic only, for tests on the host.
+    m.def("row_layout", torch::wrap_pybind_function([](const Tensor& t) {
+        const Rows r(t);
+        return std::make_tuple(r.count, r.pitch, !r.holder.is_same(t));
+    }));
     // (name, x, y, after_weight, after_bias, weight, bias, gate, scale, shift, kind after, kind before, residual scale, branch scale, eps, type of h, with out,
     // with h) -> [out], [h] or [out, h]
     m.def("norm", torch::wrap_pybind_function([](const std::string& name, const Tensor& x, const std::optional<Tensor>& y, const std::optional<Tensor>& after_weight,
