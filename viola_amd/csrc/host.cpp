@@ -1072,8 +1072,7 @@ PYBIND11_MODULE(_host, m) {
     }));
     m.def("experts", torch::wrap_pybind_function([](const Tensor& x, const Tensor& weight, const Tensor& scale, const std::vector<int64_t>& counts,
                                                     const std::shared_ptr<Recipe>& recipe, const py::object& weight_grad) {
-        TORCH_CHECK_NOT_IMPLEMENTED(plain(x) && plain(weight) && plain(scale) && !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode),
-                                    "the grouped linear has neither forward-mode derivatives nor rules for functorch transforms");
+        check_seen("the grouped linear", {x, weight, scale});
         const at::ScalarType grad = torch::python::detail::py_object_to_dtype(weight_grad);
         py::gil_scoped_release release;
         return experts(x, weight, scale, counts, recipe, grad);

@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <atomic>
@@ -89,6 +90,22 @@ inline bool holds(const Tensor& t, const at::Device& device, at::ScalarType type
 
 // A tensor subclass with its own dispatch, or a dual number of forward-mode differentiation, whose tangent would be lost here.
 inline bool plain(const Tensor& t) { return !t.defined() || (!t.unsafeGetTensorImpl()->is_python_dispatch() && !t._fw_grad(0).defined()); }
+
+// Raises where what runs here would not be seen by who has to see it: derivatives and transforms that have no rule for it, and whatever records a graph of
+// operators (torch.jit.trace, make_fx, fake tensors), in which this call's result would stand as a constant for every input. Modes of a program's own that only
+// watch (a counter of operations, selective checkpointing) are no obstacle: to them these kernels are as any code below the dispatcher.
+inline void check_seen(const char* name, at::ArrayRef<Tensor> tensors) {
+    using c10::DispatchKey;
+    using c10::impl::TorchDispatchModeKey;
+    bool transformed = c10::impl::tls_is_dispatch_key_included(DispatchKey::FuncTorchDynamicLayerFrontMode);
+    for (const Tensor& t : tensors) transformed = transformed || !plain(t);
+    TORCH_CHECK_NOT_IMPLEMENTED(!transformed, name, " has neither forward-mode derivatives nor rules for functorch transforms");
+    bool recorded = c10::impl::tls_is_dispatch_key_included(DispatchKey::Tracer) || c10::impl::tls_is_dispatch_key_included(DispatchKey::PreDispatch);
+    if (c10::impl::dispatch_mode_enabled())
+        for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+            recorded = recorded || c10::impl::TorchDispatchModeTLS::get_mode(mode).has_value();
+    TORCH_CHECK_NOT_IMPLEMENTED(!recorded, name, " cannot be recorded into a graph of operators: its result would be a constant there");
+}
 
 // A tensor that was saved for backward, as it comes back: a saved-tensor hook may have moved it or made another of it.
 inline Tensor restored(const torch::autograd::SavedVariable& saved, const at::Device& device, at::ScalarType type, at::IntArrayRef sizes) {

@@ -13,12 +13,6 @@ using torch::autograd::variable_list;
 
 namespace {
 
-void check_plain(const char* name, at::ArrayRef<Tensor> tensors) {
-    for (const Tensor& t : tensors)
-        TORCH_CHECK_NOT_IMPLEMENTED(plain(t) && !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode), name,
-                                    " has neither forward-mode derivatives nor rules for functorch transforms");
-}
-
 void check_float(const char* name, const char* what, const Tensor& t, const at::Device& device) {
     TORCH_CHECK(t.is_cuda(), "viola_amd kernels run on the GPU only");
     TORCH_CHECK(t.device() == device, name, ": ", what, " is on ", t.device(), ", not on ", device);
@@ -125,7 +119,7 @@ std::vector<Tensor> norm(const char* name, const Tensor (&input)[INPUTS], NormPl
     Tensor t[INPUTS];
     for (int i = 0; i < INPUTS; ++i) t[i] = input[i];
     const Tensor& x = t[X];
-    check_plain(name, input);
+    check_seen(name, input);
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, name, ": x needs a last dimension of features, got ", x.sizes());
     const at::Device device = x.device();
     for (int i = 0; i < INPUTS; ++i)
@@ -306,7 +300,7 @@ struct Routed {
 
 // given: choices made elsewhere; only counts and balance come back then
 Routed router(const char* name, const Tensor& logits, const Tensor& given, const Tensor& mask, RouterPlan plan, bool per_sequence) {
-    check_plain(name, {logits, given, mask});
+    check_seen(name, {logits, given, mask});
     TORCH_CHECK(logits.dim() >= 2 && logits.size(-1) > 0, name, ": logits have to be [..., tokens, experts], got ", logits.sizes());
     const at::Device device = logits.device();
     check_float(name, "logits", logits, device);
@@ -470,7 +464,7 @@ struct DispatchBackward : public Node {
 };
 
 Tensor dispatch(const Tensor& x, const Tensor& positions_, const Tensor& offsets_, int64_t rows) {
-    check_plain("dispatch", {x, positions_, offsets_});
+    check_seen("dispatch", {x, positions_, offsets_});
     const at::Device device = x.device();
     check_float("dispatch", "x", x, device);
     check_places("dispatch", positions_, offsets_, device);
@@ -537,7 +531,7 @@ struct CombineBackward : public Node {
 };
 
 Tensor combine(const Tensor& y, const Tensor& positions_, const Tensor& offsets_, const Tensor& gates_) {
-    check_plain("combine", {y, positions_, offsets_, gates_});
+    check_seen("combine", {y, positions_, offsets_, gates_});
     const at::Device device = y.device();
     check_float("combine", "y", y, device);
     check_places("combine", positions_, offsets_, device);
