@@ -510,7 +510,8 @@ int viola_store_words(int64_t* dst, const int64_t* host_words, int64_t count, vi
  * float[rows][4] for the backward pass.
  *
  * Backward: dout of x_dtype, dh and dy of branch_dtype, dx of x_dtype, all contiguous; a null dout is zeros, a null output is not wanted.
- * A call without dh (then before = VIOLA_NORM_NONE) is that of the form without h. Gradients of the vectors: [cols], or [groups][cols] where
+ * A call without dh (then before = VIOLA_NORM_NONE) is that of the form without h, and does not read x (null then, or not). shift is not read, after_bias only
+ * with dh or d_gate, bias only with d_scale: null where they are not at hand. Gradients of the vectors: [cols], or [groups][cols] where
  * the vector has a pitch, of the vector's type. parts: viola_norm_portions(rows, cols, group_rows) * 4 * cols floats (fewer where fewer of the gradients are
  * wanted). Sums over rows are added in an order of their own that does not change from call to call. cols <= 2^28; rows <= 2^32 and groups <= 2^21 where vectors
  * have a pitch (VIOLA_EUNSUPPORTED beyond). */

@@ -117,3 +117,86 @@ def test_recording_the_grouped_linear_is_refused():
         with pytest.raises(NotImplementedError):
             make_fx(lambda t: experts(t, [16, 32]))(x)
         assert experts(x, [16, 32]).shape == (48, 32)
+
+
+def test_what_no_gradient_reads_may_change_and_go():
+    """The residual stream that norm_after adds to, shifts and biases whose values no gradient needs, gates where the rows have none: changed in place, the gradients
+    stay those of the call, and nothing holds their memory."""
+    from viola_amd import nn
+    torch.manual_seed(4)
+    cuda = lambda *shape: torch.randn(*shape, device="cuda")  # noqa: E731
+    y, w, gate, d = cuda(64, 256, 512), cuda(512), cuda(512), cuda(64, 256, 512)
+    for change in (False, True):
+        x, bias, out_bias, shift = cuda(64, 256, 512).requires_grad_(), torch.ones(512, device="cuda"), torch.ones(512, device="cuda"), cuda(64, 1, 512).requires_grad_()
+        leaf = [t.detach().requires_grad_() for t in (y, w, gate)]
+        before = torch.cuda.memory_allocated()
+        stream = x * 1.0
+        out = nn.norm_after(stream, leaf[0], leaf[1], gate=leaf[2])
+        held = torch.cuda.memory_allocated() - before
+        if change:
+            stream.data_ptr()
+            with torch.no_grad():
+                stream.add_(1.0)
+        del stream
+        # out and the statistics are left
+        assert torch.cuda.memory_allocated() - before <= held - x.numel() * 4
+        grads = torch.autograd.grad(out, [x, *leaf], d)
+        h = nn.norm_before(y, leaf[1], bias, shift=shift)
+        plain = nn.norm_after(y, leaf[0], leaf[1], out_bias)
+        if change:
+            with torch.no_grad():
+                for t in (bias, out_bias, shift):
+                    t.add_(1.0)
+        grads = (*grads, *torch.autograd.grad(h, [leaf[1], shift], d), *torch.autograd.grad(plain, leaf[:2], d))
+        if not change:
+            first = grads
+    assert torch.equal(first[0], d) and all(torch.equal(a, b) for a, b in zip(first[1:], grads[1:]))
+    r = nn.route(cuda(50, 8), 2)
+    rows, gates = cuda(100, 64), r.gates.clone().requires_grad_()
+    out = nn.combine(rows, r._replace(gates=gates))
+    expected, = torch.autograd.grad(out, gates, torch.ones_like(out), retain_graph=True)
+    with torch.no_grad():
+        gates.add_(1.0)
+    again, = torch.autograd.grad(out, gates, torch.ones_like(out))
+    assert torch.equal(expected, again)
+
+
+def test_what_a_gradient_reads_may_not_change():
+    from viola_amd import nn
+    torch.manual_seed(5)
+    cuda = lambda *shape: torch.randn(*shape, device="cuda")  # noqa: E731
+    given = dict(x=cuda(4, 6, 64), y=cuda(4, 6, 64), after_weight=cuda(64), after_bias=cuda(64), weight=cuda(64), bias=cuda(64), gate=cuda(64), scale=cuda(64))
+    for name in given:
+        on = {k: t.clone().requires_grad_() for k, t in given.items()}
+        out, h = nn.norm_between(**on)
+        with torch.no_grad():
+            on[name].add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            (out.sum() + h.sum()).backward()
+    on = {k: t.clone().requires_grad_() for k, t in given.items()}
+    out = nn.norm_after(on["x"], on["y"], on["after_weight"], on["after_bias"], gate=on["gate"])
+    with torch.no_grad():
+        on["after_bias"].add_(1.0)                                           # the gate's gradient reads it
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("c", [64, 250, 1152, 8200])
+@pytest.mark.parametrize("after", ["layer", None])
+def test_norm_after_without_its_stream(c, after):
+    """The gradients without x's values, in each of the kernels (rows in registers, odd widths, rows beyond them), to the last bit those of a call that kept them:
+    the same pass with a gradient of zeros for the h of norm_between."""
+    from viola_amd import nn
+    torch.manual_seed(6)
+    cuda = lambda *shape: torch.randn(*shape, device="cuda")  # noqa: E731
+    given = dict(x=cuda(3, 5, c), y=cuda(3, 5, c), after_weight=cuda(c), after_bias=cuda(c), gate=cuda(3, 1, c))
+    d = cuda(3, 5, c)
+    on = {k: t.clone().requires_grad_() for k, t in given.items()}
+    out = nn.norm_after(on["x"], on["y"], on["after_weight"], on["after_bias"], gate=on["gate"], kind=after, residual_scale=0.7)
+    with torch.no_grad():
+        on["x"].fill_(float("nan"))
+    grads = torch.autograd.grad(out, list(on.values()), d)
+    on = {k: t.clone().requires_grad_() for k, t in given.items()}
+    out, h = nn.norm_between(**on, after=after, residual_scale=0.7)
+    expected = torch.autograd.grad([out, h], list(on.values()), [d, torch.zeros_like(h)])
+    assert all(torch.equal(a, b) for a, b in zip(grads, expected))

@@ -91,7 +91,7 @@ struct NormPlan {
 struct NormBackward : public Node {
     NormPlan plan;
     SavedVariable saved[INPUTS], stats;
-    bool has[INPUTS] = {};
+    bool has[INPUTS] = {}, kept[INPUTS] = {};                    // given; its values are read by a gradient
     std::vector<int64_t> shape[INPUTS];
     at::ScalarType type[INPUTS];
     int64_t rows = 0;
@@ -109,9 +109,10 @@ struct NormBackward : public Node {
 struct Vectors {
     const void* data[INPUTS] = {};
     int64_t pitch[3] = {};
-    void set(const NormPlan& plan, const Tensor (&t)[INPUTS]) {
+    void set(const NormPlan& plan, const Tensor (&t)[INPUTS], int64_t cols) {
         for (int i = AFTER_WEIGHT; i < INPUTS; ++i) data[i] = ptr(t[i]);
-        for (int i = 0; i < 3; ++i) pitch[i] = t[GATE + i].defined() && plan.by_group[i] ? t[GATE + i].stride(0) : 0;
+        // of one whose values are not kept (a shift's in backward): as its gradient has it
+        for (int i = 0; i < 3; ++i) pitch[i] = !plan.by_group[i] ? 0 : t[GATE + i].defined() ? t[GATE + i].stride(0) : cols;
     }
 };
 
@@ -186,7 +187,7 @@ std::vector<Tensor> norm(const char* name, const Tensor (&input)[INPUTS], NormPl
         if (need) stats = room({xr.count, 4}, at::kFloat, device);
         if (xr.count) {
             Vectors v;
-            v.set(plan, value);
+            v.set(plan, value, cols);
             VIOLA_CALL(viola_norm_forward, xr.data(), xr.pitch, code_of(x.scalar_type()), yr ? yr->data() : nullptr, yr ? yr->pitch : cols, code_of(plan.branch), xr.count,
                        cols, plan.after, v.data[AFTER_WEIGHT], v.data[AFTER_BIAS], plan.before, v.data[WEIGHT], v.data[BIAS], code_of(plan.weight_type), v.data[GATE],
                        v.pitch[0], v.data[SCALE], v.pitch[1], v.data[SHIFT], v.pitch[2], code_of(plan.vector_type), xr.count / plan.groups, (float)plan.residual_scale,
@@ -204,7 +205,9 @@ std::vector<Tensor> norm(const char* name, const Tensor (&input)[INPUTS], NormPl
             node->has[i] = true;
             node->shape[i] = t[i].sizes().vec();
             node->type[i] = t[i].scalar_type();
-            node->saved[i] = SavedVariable(t[i], false);
+            // The rest may change and go: x where it is only added to, a shift always, biases where only a gate's or a scale's gradient would read them.
+            node->kept[i] = i == X ? want_h : i == AFTER_BIAS ? want_h || wants(t[GATE]) : i == BIAS ? wants(t[SCALE]) : i != SHIFT;
+            if (node->kept[i]) node->saved[i] = SavedVariable(t[i], false);
         }
         node->stats = SavedVariable(stats, false);
         node->set_next_edges(torch::autograd::collect_next_edges(t[X], t[Y], t[AFTER_WEIGHT], t[AFTER_BIAS], t[WEIGHT], t[BIAS], t[GATE], t[SCALE], t[SHIFT]));
@@ -227,12 +230,12 @@ variable_list NormBackward::apply(variable_list&& grads) {
     const c10::DeviceGuard guard(device);
     Tensor t[INPUTS];
     for (int i = 0; i < INPUTS; ++i) {
-        if (!has[i]) continue;
+        if (!kept[i] || (i == X && !d_h.defined())) continue;
         t[i] = saved[i].unpack();
         TORCH_CHECK(t[i].device() == device && t[i].scalar_type() == type[i] && t[i].sizes() == at::IntArrayRef(shape[i]),
                     "a tensor saved by a norm around a block came back changed");
     }
-    const int64_t cols = t[X].size(-1);
+    const int64_t cols = shape[X].back();
     // without dh the part before the next block has no gradient at all
     const bool wanted[INPUTS] = {task_should_compute_output(X), has[Y] && task_should_compute_output(Y),
                                  has[AFTER_WEIGHT] && task_should_compute_output(AFTER_WEIGHT), has[AFTER_BIAS] && task_should_compute_output(AFTER_BIAS),
@@ -248,7 +251,7 @@ variable_list NormBackward::apply(variable_list&& grads) {
     if (rows) {
         const Tensor dout = d_out.defined() ? d_out.contiguous() : Tensor(), dh = d_h.defined() ? d_h.contiguous() : Tensor();
         const Tensor state = restored(stats, device, at::kFloat, {rows, 4});
-        const Rows xr(t[X]);
+        const std::optional<Rows> xr = t[X].defined() ? std::optional<Rows>(t[X]) : std::nullopt;
         const std::optional<Rows> yr = has[Y] ? std::optional<Rows>(t[Y]) : std::nullopt;
         // the sums over rows that the wanted gradients are made of
         const int sums = (wanted[AFTER_WEIGHT] || wanted[GATE]) + (wanted[AFTER_BIAS] || (wanted[GATE] && has[AFTER_BIAS])) + (wanted[WEIGHT] || wanted[SCALE]) +
@@ -256,16 +259,16 @@ variable_list NormBackward::apply(variable_list&& grads) {
         const int64_t floats = viola_norm_portions(rows, cols, rows / plan.groups) * sums * cols;
         const Tensor parts = sums ? room({floats}, at::kFloat, device) : Tensor();
         for (int i = AFTER_WEIGHT; i < INPUTS; ++i)
-            if (has[i]) t[i] = plan.readable(i, t[i], cols);
+            if (t[i].defined()) t[i] = plan.readable(i, t[i], cols);
         Vectors v;
-        v.set(plan, t);
+        v.set(plan, t, cols);
         auto to = [&](int i) { return grad[i].defined() ? grad[i].mutable_data_ptr() : nullptr; };
-        VIOLA_CALL(viola_norm_backward, xr.data(), xr.pitch, code_of(t[X].scalar_type()), yr ? yr->data() : nullptr, yr ? yr->pitch : cols, code_of(plan.branch), rows, cols,
+        VIOLA_CALL(viola_norm_backward, xr ? xr->data() : nullptr, xr ? xr->pitch : cols, code_of(type[X]), yr ? yr->data() : nullptr, yr ? yr->pitch : cols, code_of(plan.branch), rows, cols,
                    plan.after, v.data[AFTER_WEIGHT], v.data[AFTER_BIAS], dh.defined() ? plan.before : VIOLA_NORM_NONE, v.data[WEIGHT], v.data[BIAS],
                    code_of(plan.weight_type), v.data[GATE], v.pitch[0], v.data[SCALE], v.pitch[1], v.data[SHIFT], v.pitch[2], code_of(plan.vector_type), rows / plan.groups,
                    (float)plan.residual_scale, (float)plan.branch_scale, static_cast<const float*>(state.const_data_ptr()), ptr(dout), ptr(dh), to(X), to(Y),
                    parts.defined() ? static_cast<float*>(parts.mutable_data_ptr()) : nullptr, floats, to(AFTER_WEIGHT), to(AFTER_BIAS), to(WEIGHT), to(BIAS), to(GATE),
-                   to(SCALE), to(SHIFT), stream_of(t[X]));
+                   to(SCALE), to(SHIFT), stream_of(state));
     }
     for (int i = 0; i < INPUTS; ++i)
         if (grad[i].defined()) result[i] = grad[i].scalar_type() == type[i] ? grad[i] : grad[i].to(type[i]);
@@ -510,7 +513,7 @@ struct CombineBackward : public Node {
         const c10::DeviceGuard guard(device);
         const bool needs_y = task_should_compute_output(0), needs_gates = has_gates && task_should_compute_output(1);
         const Tensor p = restored(positions, device, at::kInt, places), o = restored(offsets, device, at::kInt, {experts});
-        const Tensor g = has_gates ? restored(gates, device, at::kFloat, places) : Tensor();
+        const Tensor g = has_gates && needs_y ? restored(gates, device, at::kFloat, places) : Tensor();
         Tensor rows;
         if (needs_gates) {
             rows = y.unpack();
@@ -562,7 +565,7 @@ Tensor combine(const Tensor& y, const Tensor& positions_, const Tensor& offsets_
         node->has_gates = gates.defined();
         if (gates.defined()) {
             node->gates_type = gates_.scalar_type();
-            node->gates = SavedVariable(gates, false);
+            if (y.requires_grad()) node->gates = SavedVariable(gates, false);            // their own gradient is made of the rows
         }
         if (wants(gates_)) node->y = SavedVariable(y, false);
         node->positions = SavedVariable(positions, false);

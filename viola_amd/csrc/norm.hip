@@ -367,7 +367,7 @@ extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, 
     const bool gate_sums = d_gate && y, scale_sums = d_scale && dh;
     // rows of none: the sums over rows are still written, as zeros, by the reduction below
     if (rows) {
-        VIOLA_CHECK_ARG(valid_rows(x, x_pitch, cols) && stats && (!y || y_pitch >= cols) && (dh || y) && (dh != nullptr) == (before != VIOLA_NORM_NONE) && (y || !dy));
+        VIOLA_CHECK_ARG((!dh || valid_rows(x, x_pitch, cols)) && stats && (!y || y_pitch >= cols) && (dh || y) && (dh != nullptr) == (before != VIOLA_NORM_NONE) && (y || !dy));
         VIOLA_CHECK_ARG(reinterpret_cast<uintptr_t>(stats) % 16 == 0);
     }
     a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
