@@ -74,3 +74,12 @@ def test_modes_that_watch_are_no_obstacle(name):
     f, x = _calls()[name]
     with FlopCounterMode(display=False), pytest.raises(RuntimeError, match="GPU only"):
         f(x)
+
+
+def test_a_negative_number_of_rows_is_refused():
+    """-1 is no way to ask for the default: a count that went wrong would lay out rows of none."""
+    from viola_amd import nn
+    places = nn.Routing(torch.zeros(4, 2, dtype=I32), torch.zeros(7, dtype=I32))
+    for rows in (-1, -8):
+        with pytest.raises(RuntimeError, match="rows is negative"):
+            nn.dispatch(torch.randn(4, 8), places, rows)

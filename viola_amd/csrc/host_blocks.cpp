@@ -466,15 +466,16 @@ struct DispatchBackward : public Node {
     void release_variables() override { positions.reset_data(); }
 };
 
-Tensor dispatch(const Tensor& x, const Tensor& positions_, const Tensor& offsets_, int64_t rows) {
+Tensor dispatch(const Tensor& x, const Tensor& positions_, const Tensor& offsets_, std::optional<int64_t> wanted) {
     check_seen("dispatch", {x, positions_, offsets_});
+    TORCH_CHECK(!wanted || *wanted >= 0, "dispatch: rows is negative");
     const at::Device device = x.device();
     check_float("dispatch", "x", x, device);
     check_places("dispatch", positions_, offsets_, device);
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "dispatch: x needs a last dimension of features, got ", x.sizes());
     const int64_t cols = x.size(-1), tokens = x.numel() / cols, top_k = positions_.size(-1);
     TORCH_CHECK(positions_.numel() == tokens * top_k, "dispatch: positions of ", positions_.sizes(), " do not belong to x of ", x.sizes());
-    if (rows < 0) rows = tokens * top_k;
+    const int64_t rows = wanted.value_or(tokens * top_k);
     TORCH_CHECK(rows < (int64_t{1} << 31), "dispatch lays out fewer than 2^31 rows");
     const c10::DeviceGuard guard(device);
     const bool need = at::GradMode::is_enabled() && x.requires_grad();
@@ -627,7 +628,7 @@ void viola_host::register_blocks(py::module_& m) {
         }
         return std::make_tuple(r.balance, r.counts);
     }));
-    m.def("dispatch", torch::wrap_pybind_function([](const Tensor& x, const Tensor& positions, const Tensor& offsets, int64_t rows) {
+    m.def("dispatch", torch::wrap_pybind_function([](const Tensor& x, const Tensor& positions, const Tensor& offsets, std::optional<int64_t> rows) {
         py::gil_scoped_release release;
         return dispatch(x, positions, offsets, rows);
     }));

@@ -66,7 +66,7 @@ def dispatch(x, routing, rows=None):
     """The rows of x [..., features] in the order of the experts: [rows, features], each token's once for each expert it goes to. rows: how many to
     lay out, tokens * chosen by default; the sum of the counts where tokens are masked and the experts should not see the rest. Rows that no token
     has are zero; positions from `rows` on are left out (and in `combine` too)."""
-    return _lib.host().dispatch(x, routing.positions, routing.offsets, -1 if rows is None else rows)
+    return _lib.host().dispatch(x, routing.positions, routing.offsets, rows)
 
 
 def combine(y, routing):
