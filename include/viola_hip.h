@@ -513,8 +513,8 @@ int viola_store_words(int64_t* dst, const int64_t* host_words, int64_t count, vi
  * A call without dh (then before = VIOLA_NORM_NONE) is that of the form without h, and does not read x (null then, or not). shift is not read, after_bias only
  * with dh or d_gate, bias only with d_scale: null where they are not at hand. Gradients of the vectors: [cols], or [groups][cols] where
  * the vector has a pitch, of the vector's type. parts: viola_norm_portions(rows, cols, group_rows) * 4 * cols floats (fewer where fewer of the gradients are
- * wanted). Sums over rows are added in an order of their own that does not change from call to call. cols <= 2^28; rows <= 2^32 and groups <= 2^21 where vectors
- * have a pitch (VIOLA_EUNSUPPORTED beyond). */
+ * wanted). Sums over rows are added in an order of their own that does not change from call to call. cols <= 2^28; fewer than 2^32 rows
+ * where vectors have a pitch (VIOLA_EUNSUPPORTED beyond). */
 int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols,
                        int after, const void* after_weight, const void* after_bias, int before, const void* weight, const void* bias, int weight_dtype,
                        const void* gate, int64_t gate_pitch, const void* scale, int64_t scale_pitch, const void* shift, int64_t shift_pitch,

@@ -116,3 +116,22 @@ def test_rows_of_broadcast_tokens_and_gradients(cols, dtype):
     expected, expected_gates = routing.combine_gradient(d.repeat_interleave(s, 0), y, positions, gates.detach().cpu().view(b * s, k))
     _close("dy", dy, expected)
     _close("dgates", dg.view(b * s, k), expected_gates, torch.full_like(expected_gates, cols ** 0.5))
+
+
+# ---------------------------------------------------------------------------------------------------------- many groups
+@pytest.mark.parametrize("with_weight", [False, True])
+def test_vectors_for_more_than_two_million_tokens(with_weight):
+    """More groups than one launch has slices for: a scale and a shift for each token. 64-bit formulas on the device; each gradient is one product, and the weight's a
+    sum of 64 slices of 2^16 terms, whose partial sums and rounding errors both go as their root: 2^-24 2^8 of them, 2^-16 of the sum of all magnitudes."""
+    from viola_amd import nn
+    torch.manual_seed(5)
+    n, c = (1 << 22) + 100, 8
+    x, d = torch.randn(n, c, device="cuda"), torch.randn(n, c, device="cuda")
+    scale, shift, weight = torch.randn(n, c, device="cuda"), torch.randn(n, c, device="cuda"), torch.rand(c, device="cuda")
+    wanted = [t.requires_grad_() for t in ((scale, shift, weight) if with_weight else (scale, shift))]
+    grads = torch.autograd.grad(nn.norm_before(x, weight, scale=scale, shift=shift), wanted, d)
+    hat = x.double() / (x.double().square().mean(-1, keepdim=True) + 1e-6).sqrt()
+    expected = [d * hat * weight.detach(), d.double(), (d * hat * (1 + scale.detach())).sum(0)]
+    measures = [expected[0], expected[1], (d * hat * (1 + scale.detach())).abs().sum(0)]
+    for name, g, e, m in zip(("scale", "shift", "weight"), grads, expected, measures):
+        assert (g.double() - e).norm() <= SUMS * m.norm(), name

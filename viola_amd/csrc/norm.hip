@@ -163,6 +163,8 @@ struct ReduceArgs {
 
 struct Sums { float a1, a0, s1, s0; };
 
+constexpr int64_t MOST_SECTIONS = 32768;                                     // of groups: a grid has up to 65535 in y
+
 // The wanted sums of one portion; `at`: where in the portion each lies.
 struct PortionLayout {
     int sums, a0, s1, s0;
@@ -181,7 +183,8 @@ struct PortionLayout {
 };
 
 // Sections of blocks (blockIdx.y). `whole` of them, 1 or 0: what is summed over all rows, WIDTH columns by as many contiguous slices of the portions as 1024
-// threads have, the slices then added in order. The others: what is summed group by group, WIDTH columns by a group for each slice.
+// threads have, the slices then added in order. The others: what is summed group by group, WIDTH columns by a group for each slice,
+// in turns where there are more groups than sections have slices.
 template <int WIDTH> __global__ __launch_bounds__(1024) void norm_reduce_kernel(ReduceArgs a) {
     constexpr int SLICES = 1024 / WIDTH;
     __shared__ float piece[SLICES][8][WIDTH + 1];
@@ -191,21 +194,23 @@ template <int WIDTH> __global__ __launch_bounds__(1024) void norm_reduce_kernel(
     const bool in = col < a.cols;
     auto vector = [&](const void* data, int64_t at, int dtype, float absent) { return data && in ? load_float(data, at + col, dtype) : absent; };
     if ((int)blockIdx.y >= a.whole) {
-        const int64_t group = (int64_t)(blockIdx.y - a.whole) * SLICES + slice;
-        if (!in || group >= a.portions / a.per_group) return;
-        float a1 = 0.0f, a0 = 0.0f, s1 = 0.0f, s0 = 0.0f;
-        const float* from = a.parts + group * a.per_group * layout.stride + col;
-#pragma unroll 4
-        for (int64_t p = 0; p < a.per_group; ++p) {
-            const Sums v = layout.load(from + p * layout.stride);
-            a1 += v.a1; a0 += v.a0; s1 += v.s1; s0 += v.s0;
-        }
-        const int64_t to = group * a.cols + col;
+        if (!in) return;
+        const int64_t groups = a.portions / a.per_group, step = (int64_t)(gridDim.y - a.whole) * SLICES;
         const float w_a = vector(a.after_weight, 0, a.weight_dtype, 1.0f), b_a = vector(a.after_bias, 0, a.weight_dtype, 0.0f);
         const float w_b = vector(a.weight, 0, a.weight_dtype, 1.0f), b_b = vector(a.bias, 0, a.weight_dtype, 0.0f);
-        if (a.d_gate && a.gate_by_group) store_float(a.d_gate, to, a.vector_dtype, a.alpha * fmaf(w_a, a1, a.after_bias ? b_a * a0 : 0.0f));
-        if (a.d_scale && a.scale_by_group) store_float(a.d_scale, to, a.vector_dtype, fmaf(w_b, s1, a.bias ? b_b * s0 : 0.0f));
-        if (a.d_shift && a.shift_by_group) store_float(a.d_shift, to, a.vector_dtype, s0);
+        for (int64_t group = (int64_t)(blockIdx.y - a.whole) * SLICES + slice; group < groups; group += step) {
+            float a1 = 0.0f, a0 = 0.0f, s1 = 0.0f, s0 = 0.0f;
+            const float* from = a.parts + group * a.per_group * layout.stride + col;
+#pragma unroll 4
+            for (int64_t p = 0; p < a.per_group; ++p) {
+                const Sums v = layout.load(from + p * layout.stride);
+                a1 += v.a1; a0 += v.a0; s1 += v.s1; s0 += v.s0;
+            }
+            const int64_t to = group * a.cols + col;
+            if (a.d_gate && a.gate_by_group) store_float(a.d_gate, to, a.vector_dtype, a.alpha * fmaf(w_a, a1, a.after_bias ? b_a * a0 : 0.0f));
+            if (a.d_scale && a.scale_by_group) store_float(a.d_scale, to, a.vector_dtype, fmaf(w_b, s1, a.bias ? b_b * s0 : 0.0f));
+            if (a.d_shift && a.shift_by_group) store_float(a.d_shift, to, a.vector_dtype, s0);
+        }
         return;
     }
     // the four sums, then the same under the gate and under one plus the scale
@@ -382,8 +387,8 @@ extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, 
     // Sums over all rows of few columns: 16 to a block, or there are too few blocks (50 x 197 rows of 768: 5.3 us, with 32 columns 6.6; 4096 columns 8.4 and 7.3).
     const bool narrow = whole && cols <= 1024;
     const int64_t width = narrow ? 16 : 32, slices = 1024 / width;
-    const int64_t sections = whole + (grouped ? (rows / group_rows + slices - 1) / slices : 0);
-    if (sections > 65535 || a.portions > UINT32_MAX) return VIOLA_EUNSUPPORTED;
+    const int64_t by_groups = grouped ? (rows / group_rows + slices - 1) / slices : 0, sections = whole + (by_groups < MOST_SECTIONS ? by_groups : MOST_SECTIONS);
+    if (a.portions > UINT32_MAX) return VIOLA_EUNSUPPORTED;
     if (rows) {
         const dim3 grid((unsigned)(a.portions < 65536 ? a.portions : 65536));
         const int form = !y ? FORM_BEFORE : !dh ? FORM_AFTER : plain(a) ? FORM_PLAIN : FORM_BETWEEN;
