@@ -135,3 +135,117 @@ def test_vectors_for_more_than_two_million_tokens(with_weight):
     measures = [expected[0], expected[1], (d * hat * (1 + scale.detach())).abs().sum(0)]
     for name, g, e, m in zip(("scale", "shift", "weight"), grads, expected, measures):
         assert (g.double() - e).norm() <= SUMS * m.norm(), name
+
+
+# ---------------------------------------------------------------------------------------------------------- rows cut out of wider ones
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("width,at_x,at_y,pieces", [(768, 0, 512, True), (768, 8, 264, True), (768, 257, 511, False), (768, 1, 512, False), (768, 0, 3, False), (771, 0, 0, False)])
+def test_norms_of_rows_cut_out_of_wider_ones(dtype, width, at_x, at_y, pieces):
+    """Rows of another distance than their width, from whole pieces of 16 bytes on or not, in a 3-D tensor whose rows still have one distance."""
+    from viola_amd import _lib
+    torch.manual_seed(6)
+    wide = torch.randn(2, 4, 9, width, device="cuda").to(dtype)
+    x, y = wide[0, ..., at_x:at_x + 256], wide[1, ..., at_y:at_y + 256]
+    for t in (x, y):
+        assert not t.is_contiguous() and _lib.host().row_layout(t) == (36, width, False)
+    assert pieces == (x.data_ptr() % 16 == 0 and y.data_ptr() % 16 == 0 and width % 8 == 0)
+    _between(dict(x=x, y=y, **_vectors(4, 256)), after="layer", before="rms")
+    _between(dict(x=x, y=y, **_vectors(4, 256)), after="rms", before="layer")
+
+
+def test_norms_of_rows_without_a_common_distance():
+    torch.manual_seed(7)
+    x, y = torch.randn(9, 4, 256, device="cuda").bfloat16().transpose(0, 1), torch.randn(4, 18, 256, device="cuda").bfloat16()[:, ::2]
+    _between(dict(x=x, y=y, **_vectors(4, 256)))
+    y = torch.randn(4, 12, 256, device="cuda").bfloat16()[:, :9]              # sequences further apart than their rows
+    _between(dict(x=x, y=y, **_vectors(4, 256)))
+
+
+def test_vectors_cut_out_of_wider_ones():
+    """Gate, scale and shift as parts of one projection, aligned or not."""
+    torch.manual_seed(8)
+    for c, first in ((256, 0), (256, 3), (250, 1)):
+        parts = (0.3 * torch.randn(4, 6 * 256 + 8, device="cuda")).bfloat16()
+        cut = [parts[:, None, first + i * c:first + (i + 1) * c] for i in range(3)]
+        x, y = torch.randn(4, 9, c, device="cuda").bfloat16(), torch.randn(4, 9, c, device="cuda").bfloat16()
+        _between(dict(x=x, y=y, gate=cut[0], scale=cut[1], shift=cut[2]), after="rms", before="layer")
+
+
+# ---------------------------------------------------------------------------------------------------------- many rows to a block
+@pytest.mark.parametrize("c", [384, 1001, 1152, 4096])
+@pytest.mark.parametrize("stream,branch", [(BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("options", [dict(after="rms", before="layer"), dict(after=None, before="rms")], ids=["normed", "plain"])
+def test_blocks_of_many_rows(c, stream, branch, options):
+    """Twelve to twenty rows to a block, in groups of 37 that begin and end inside one: teams of one to eight wavefronts make several turns, with the rows of the next ones
+    under way and another group's vectors on the way."""
+    torch.manual_seed(c)
+    b, s = 136, 37
+    given = dict(x=torch.randn(b, s, c, device="cuda").to(stream), y=torch.randn(b, s, c, device="cuda").to(branch))
+    vectors = _vectors(b, c)
+    if options["after"] is None:                                             # the kernel of its own: neither norm, weight nor bias after the block
+        vectors = {k: v for k, v in vectors.items() if not k.startswith("after")}
+    _between({**given, **vectors}, **options)
+
+
+@pytest.mark.parametrize("form", ["before", "after"])
+@pytest.mark.parametrize("c", [384, 1001, 1152])
+def test_one_side_of_a_block_of_many_rows(form, c):
+    from viola_amd import nn
+    torch.manual_seed(c)
+    b, s = 136, 37
+    v = _vectors(b, c)
+    if form == "before":
+        on = dict(x=torch.randn(b, s, c, device="cuda"), weight=v["weight"], bias=v["bias"], scale=v["scale"], shift=v["shift"])
+        call = lambda t: nn.norm_before(**t, kind="layer", dtype=BF16)  # noqa: E731
+        options = dict(before="layer")
+    else:
+        on = dict(x=torch.randn(b, s, c, device="cuda"), y=torch.randn(b, s, c, device="cuda").bfloat16(), after_weight=v["after_weight"], after_bias=v["after_bias"], gate=v["gate"])
+        call = lambda t: nn.norm_after(t["x"], t["y"], t["after_weight"], t["after_bias"], gate=t["gate"], kind="layer")  # noqa: E731
+        options = dict(after="layer", before=None)
+    on = {k: _leaf(t) for k, t in on.items()}
+    result = call(on)
+    d = torch.randn(b, s, c).to(result.dtype)
+    grads = torch.autograd.grad(result, list(on.values()), d.cuda())
+    expected = norms.norm(**{k: t.detach().cpu() for k, t in on.items()}, **options, **{"dh" if form == "before" else "dout": d})
+    _close(form, result, expected["h" if form == "before" else "out"])
+    for k, g in zip(on, grads):
+        _close("d" + k, g, expected["d" + k], expected["m" + k] if k not in ("x", "y") else None)
+
+
+def test_more_rows_than_the_caches_hold():
+    """Inputs beyond 128 MB are read past the caches' order."""
+    torch.manual_seed(9)
+    x, y = torch.randn(8, 1026, 4096, device="cuda").bfloat16(), torch.randn(8, 1026, 4096, device="cuda").bfloat16()
+    assert 2 * x.numel() * x.element_size() > 128 << 20
+    _between(dict(x=x, y=y, **{k: v for k, v in _vectors(8, 4096).items() if k in ("after_weight", "weight", "gate")}))
+
+
+@pytest.mark.parametrize("top_k", [1, 8])
+def test_more_rows_of_experts_than_the_caches_hold(top_k):
+    """The same on the way to the experts and back; a sample of the tokens against the formulas, every row against the rows of its token."""
+    from viola_amd import nn
+    torch.manual_seed(10)
+    cols = 4096
+    tokens = (128 << 20) // (2 * cols * top_k) + 5
+    chosen = torch.randint(0, 16, (tokens, top_k))
+    flat = chosen.flatten()
+    positions = torch.empty_like(flat)
+    positions[torch.argsort(flat, stable=True)] = torch.arange(flat.numel())
+    positions = positions.view(tokens, top_k)
+    offsets = torch.nn.functional.pad(torch.bincount(flat, minlength=16).cumsum(0), (1, 0))
+    gates = torch.rand(tokens, top_k).cuda().requires_grad_()
+    r = nn.Routing(positions.int().cuda(), offsets.int().cuda(), gates)
+    x = torch.randn(tokens, cols, device="cuda").bfloat16()
+    rows = nn.dispatch(x, r)
+    assert torch.equal(rows[positions.cuda()], x[:, None].expand(-1, top_k, -1))
+    y = torch.randn(tokens * top_k, cols, device="cuda").bfloat16().requires_grad_()
+    d = torch.randn(tokens, cols, device="cuda").bfloat16()
+    out = nn.combine(y, r)
+    dy, dg = torch.autograd.grad(out, [y, gates], d)
+    some = torch.randperm(tokens)[:200]
+    at = positions[some].cuda()
+    y64, d64, g64 = y.detach()[at].double(), d[some.cuda()].double(), gates.detach()[some.cuda()].double()
+    _close("out", out[some.cuda()], (g64[..., None] * y64).sum(1))
+    _close("dy", dy[at], g64[..., None] * d64[:, None])
+    dots = (d64[:, None] * y64).sum(-1)
+    _close("dgates", dg[some.cuda()], dots, torch.full_like(dots, cols ** 0.5))
