@@ -183,8 +183,7 @@ struct PortionLayout {
 };
 
 // Sections of blocks (blockIdx.y). `whole` of them, 1 or 0: what is summed over all rows, WIDTH columns by as many contiguous slices of the portions as 1024
-// threads have, the slices then added in order. The others: what is summed group by group, WIDTH columns by a group for each slice,
-// in turns where there are more groups than sections have slices.
+// threads have, the slices then added in order. The others: what is summed group by group, WIDTH columns by a group for each slice.
 template <int WIDTH> __global__ __launch_bounds__(1024) void norm_reduce_kernel(ReduceArgs a) {
     constexpr int SLICES = 1024 / WIDTH;
     __shared__ float piece[SLICES][8][WIDTH + 1];
@@ -194,23 +193,21 @@ template <int WIDTH> __global__ __launch_bounds__(1024) void norm_reduce_kernel(
     const bool in = col < a.cols;
     auto vector = [&](const void* data, int64_t at, int dtype, float absent) { return data && in ? load_float(data, at + col, dtype) : absent; };
     if ((int)blockIdx.y >= a.whole) {
-        if (!in) return;
-        const int64_t groups = a.portions / a.per_group, step = (int64_t)(gridDim.y - a.whole) * SLICES;
+        const int64_t group = (int64_t)(blockIdx.y - a.whole) * SLICES + slice;
+        if (!in || group >= a.portions / a.per_group) return;
+        float a1 = 0.0f, a0 = 0.0f, s1 = 0.0f, s0 = 0.0f;
+        const float* from = a.parts + group * a.per_group * layout.stride + col;
+#pragma unroll 4
+        for (int64_t p = 0; p < a.per_group; ++p) {
+            const Sums v = layout.load(from + p * layout.stride);
+            a1 += v.a1; a0 += v.a0; s1 += v.s1; s0 += v.s0;
+        }
+        const int64_t to = group * a.cols + col;
         const float w_a = vector(a.after_weight, 0, a.weight_dtype, 1.0f), b_a = vector(a.after_bias, 0, a.weight_dtype, 0.0f);
         const float w_b = vector(a.weight, 0, a.weight_dtype, 1.0f), b_b = vector(a.bias, 0, a.weight_dtype, 0.0f);
-        for (int64_t group = (int64_t)(blockIdx.y - a.whole) * SLICES + slice; group < groups; group += step) {
-            float a1 = 0.0f, a0 = 0.0f, s1 = 0.0f, s0 = 0.0f;
-            const float* from = a.parts + group * a.per_group * layout.stride + col;
-#pragma unroll 4
-            for (int64_t p = 0; p < a.per_group; ++p) {
-                const Sums v = layout.load(from + p * layout.stride);
-                a1 += v.a1; a0 += v.a0; s1 += v.s1; s0 += v.s0;
-            }
-            const int64_t to = group * a.cols + col;
-            if (a.d_gate && a.gate_by_group) store_float(a.d_gate, to, a.vector_dtype, a.alpha * fmaf(w_a, a1, a.after_bias ? b_a * a0 : 0.0f));
-            if (a.d_scale && a.scale_by_group) store_float(a.d_scale, to, a.vector_dtype, fmaf(w_b, s1, a.bias ? b_b * s0 : 0.0f));
-            if (a.d_shift && a.shift_by_group) store_float(a.d_shift, to, a.vector_dtype, s0);
-        }
+        if (a.d_gate && a.gate_by_group) store_float(a.d_gate, to, a.vector_dtype, a.alpha * fmaf(w_a, a1, a.after_bias ? b_a * a0 : 0.0f));
+        if (a.d_scale && a.scale_by_group) store_float(a.d_scale, to, a.vector_dtype, fmaf(w_b, s1, a.bias ? b_b * s0 : 0.0f));
+        if (a.d_shift && a.shift_by_group) store_float(a.d_shift, to, a.vector_dtype, s0);
         return;
     }
     // the four sums, then the same under the gate and under one plus the scale
@@ -387,7 +384,7 @@ extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, 
     // Sums over all rows of few columns: 16 to a block, or there are too few blocks (50 x 197 rows of 768: 5.3 us, with 32 columns 6.6; 4096 columns 8.4 and 7.3).
     const bool narrow = whole && cols <= 1024;
     const int64_t width = narrow ? 16 : 32, slices = 1024 / width;
-    const int64_t by_groups = grouped ? (rows / group_rows + slices - 1) / slices : 0, sections = whole + (by_groups < MOST_SECTIONS ? by_groups : MOST_SECTIONS);
+    const int64_t by_groups = grouped ? (rows / group_rows + slices - 1) / slices : 0;
     if (a.portions > UINT32_MAX) return VIOLA_EUNSUPPORTED;
     if (rows) {
         const dim3 grid((unsigned)(a.portions < 65536 ? a.portions : 65536));
@@ -400,7 +397,7 @@ extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, 
             }))
             VIOLA_LAUNCH(norm_backward_any_kernel, grid, 256, 0, hip_stream, a);
     }
-    if (sections) {
+    if (whole || by_groups) {
         ReduceArgs r = {};
         r.whole = whole;
         r.parts = parts; r.portions = a.portions; r.per_group = a.per_group; r.cols = (int)cols; r.sums = a.sums;
@@ -409,9 +406,25 @@ extern "C" int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, 
         r.d_after_weight = d_after_weight; r.d_after_bias = d_after_bias; r.d_weight = d_weight; r.d_bias = d_bias;
         r.d_gate = d_gate; r.d_scale = d_scale; r.d_shift = d_shift;
         r.gate_by_group = gate_pitch != 0; r.scale_by_group = scale_pitch != 0; r.shift_by_group = shift_pitch != 0;
-        const dim3 grid((unsigned)((cols + width - 1) / width), (unsigned)sections);
-        if (narrow) VIOLA_LAUNCH(norm_reduce_kernel<16>, grid, 1024, 0, hip_stream, r);
-        else VIOLA_LAUNCH(norm_reduce_kernel<32>, grid, 1024, 0, hip_stream, r);
+        // A launch for every MOST_SECTIONS of groups: the next one's begin where this one's end.
+        for (int64_t left = by_groups;;) {
+            const int64_t sections = left < MOST_SECTIONS ? left : MOST_SECTIONS;
+            const dim3 grid((unsigned)((cols + width - 1) / width), (unsigned)(r.whole + sections));
+            if (narrow) VIOLA_LAUNCH(norm_reduce_kernel<16>, grid, 1024, 0, hip_stream, r);
+            else VIOLA_LAUNCH(norm_reduce_kernel<32>, grid, 1024, 0, hip_stream, r);
+            left -= sections;
+            if (left <= 0) break;
+            const int64_t groups = sections * slices;
+            auto advance = [&](void*& p, int by_group) {
+                if (p && by_group) p = static_cast<char*>(p) + groups * cols * viola_dtype_size(vector_dtype);
+            };
+            r.whole = 0;
+            r.portions -= groups * a.per_group;
+            r.parts += groups * a.per_group * __builtin_popcount((unsigned)a.sums) * cols;
+            advance(r.d_gate, r.gate_by_group);
+            advance(r.d_scale, r.scale_by_group);
+            advance(r.d_shift, r.shift_by_group);
+        }
     }
     return viola_launch_status();
 }
