@@ -415,3 +415,17 @@ def test_refusals():
     l = logits.clone().requires_grad_()
     with pytest.raises(NotImplementedError, match="once only"):
         torch.autograd.grad(nn.route(l, 2).balance, l, create_graph=True)
+
+
+def test_gates_near_the_end_of_the_normal_numbers():
+    """sigmoid(l) itself, element by element: to 2^-21 where it is a normal number, 0 or as good as that below (an exponential is within 2^-22, its reciprocal
+    and the product within 2^-24 each)."""
+    from viola_amd import nn
+    logits = torch.full((2001, 4), -math.inf)
+    logits[:, 1] = torch.linspace(-110.0, -75.0, 2001)
+    r = nn.route(logits.cuda(), 1, score="sigmoid", normalize=False)
+    expected = torch.sigmoid(logits[:, 1].double())
+    assert ((r.gates[:, 0].cpu().double() - expected).abs() <= 2.0 ** -21 * expected + 2.0 ** -126).all()
+    assert (r.gates[:, 0].cpu()[expected > 2.0 ** -125] > 0).all() and (r.gates >= 0).all()
+    again = nn.route(logits.cuda(), 1, score="sigmoid")                       # its share of itself
+    assert (again.gates == 1).all()

@@ -59,7 +59,7 @@ struct NormArgs {
 //
 // Bound by memory: two or three reads and two writes an element against some 40 operations. Forward and backward between two blocks, cold caches: 16384 rows
 // of 4096 in bf16 104 and 161 us (5.2 and 5.0 TB/s, what a large copy reaches here), 16384 rows of 1152 with a gate, a scale and a shift for each of 64 images 35
-// and 49 us (4.2 and 4.6: 18 of 64 lanes of a row's third wavefront have work, and 128 registers leave the backward pass four wavefronts a SIMD).
+// and 49 us (4.2 and 4.6: 16 of 64 lanes of a row's third wavefront have work, and 128 registers leave the backward pass four wavefronts a SIMD).
 // Eight elements a thread are one load of 16 bytes from a 16-bit tensor, and leave registers for the next rows' loads under way.
 // x' is computed twice and not stored in 32 bits between the passes: its reading would cost what x and y cost.
 constexpr int ROW_THREADS = 1024, ROW_COLUMNS = 8 * ROW_THREADS;

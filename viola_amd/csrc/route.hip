@@ -14,8 +14,8 @@
 //
 // A row belongs to `LANES` lanes of VALUES logits each; a block takes a run of tokens (a portion) of one sequence. Counts are integers
 // and probabilities are added in one order, so results do not change from run to run: places of equal experts come from a bit for
-// each token in LDS, blocks leave their counts and sums behind, and a second kernel adds those of the blocks before. Up to STAGE tokens
-// are one block's, which finishes by itself.
+// each token in LDS, blocks leave their counts and sums behind, and a second kernel adds those of the blocks before. Tokens of one stage (128;
+// 256 of up to 16 experts, 512 of up to 8) in one sequence are one block's, which finishes by itself.
 //
 // Bound by instructions, not by memory: a wavefront spends some 860 of them on four rows of 128 logits, 55 on each choice (largest, its lowest index, taking it
 // out), and the vector units are busy 70 % of the time. 32768 tokens to eight of 128 experts: choosing 18 us (its logits and results are 4 us of traffic), places and
@@ -86,7 +86,8 @@ __device__ __forceinline__ uint32_t key_of(float l) {
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
-// exp(x) within 2 ulp for x <= 0 (0 below -150): exp2 of the product's two halves, the low one multiplied in afterwards.
+// exp(x) for x <= 0, within 2 ulp where that is a normal number, x >= -87.3: exp2 of the product's two halves, the low one multiplied in afterwards. What is smaller
+// than 2^-126 comes out as 0, as the hardware's exp2 has no subnormal results; the last line is for -inf, whose halves are no numbers.
 __device__ __forceinline__ float exp_of(float x) {
     const float t = x * 1.44269502f;                                         // log2(e) = 1.44269502 + 1.92596e-8
     const float low = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -t));

@@ -46,7 +46,7 @@ def route(logits, top_k, *, score="softmax", normalize=True, scale=1.0, mask=Non
     """The `top_k` experts of each token with the largest logits [..., tokens, experts] (ties to the lowest index), as a `Routing`.
 
     Probabilities are softmax(logits), or with score="sigmoid" sigmoid(logits) over their sum. gates: with `normalize` the chosen ones' share of
-    their own sum, otherwise the probability (softmax) or sigmoid(logit) itself; times `scale`. An expert with a logit of -inf is never chosen. mask
+    their own sum, otherwise the probability (softmax) or sigmoid(logit) itself, 0 below 2^-126; times `scale`. An expert with a logit of -inf is never chosen. mask
     (bool, [..., tokens]): False for tokens that go nowhere and are not counted. A token whose logits are all -inf is treated like that.
 
     balance: experts * sum_e (share of the choices that fall on e) * (mean probability of e) over the counted tokens, of the whole batch or
@@ -65,7 +65,11 @@ def balance_loss(logits, experts, *, score="softmax", mask=None, per_sequence=Fa
 def dispatch(x, routing, rows=None):
     """The rows of x [..., features] in the order of the experts: [rows, features], each token's once for each expert it goes to. rows: how many to
     lay out, tokens * chosen by default; the sum of the counts where tokens are masked and the experts should not see the rest. Rows that no token
-    has are zero; positions from `rows` on are left out (and in `combine` too)."""
+    has are zero; positions from `rows` on are left out (and in `combine` too).
+
+    Places made by hand are taken as they are, since looking at them would wait for the GPU. They stay within the rows whatever they hold, but where they break what
+    `Routing` says, values are undefined: of a row that two choices name or that lies at or beyond offsets[-1] (there zeros and tokens are written by one launch), and
+    of rows below offsets[-1] that none names (nothing is written there)."""
     return _lib.host().dispatch(x, routing.positions, routing.offsets, rows)
 
 
