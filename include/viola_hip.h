@@ -512,7 +512,7 @@ int viola_store_words(int64_t* dst, const int64_t* host_words, int64_t count, vi
  * Backward: dout of x_dtype, dh and dy of branch_dtype, dx of x_dtype, all contiguous; a null dout is zeros, a null output is not wanted.
  * A call without dh (then before = VIOLA_NORM_NONE) is that of the form without h, and does not read x (null then, or not). shift is not read, after_bias only
  * with dh or d_gate, bias only with d_scale: null where they are not at hand. Gradients of the vectors: [cols], or [groups][cols] where
- * the vector has a pitch, of the vector's type. parts: viola_norm_portions(rows, cols, group_rows) * 4 * cols floats (fewer where fewer of the gradients are
+ * the vector has a pitch, of the vector's type. parts: viola_norm_portions(rows, cols, group_rows) * 4 * cols floats (0 portions for what is refused; fewer floats where fewer of the gradients are
  * wanted). Sums over rows are added in an order of their own that does not change from call to call. cols <= 2^28; fewer than 2^32 rows
  * where vectors have a pitch (VIOLA_EUNSUPPORTED beyond). */
 int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols,
@@ -535,8 +535,8 @@ int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, const void*
  * (where each expert's places begin), and the balance loss: the mean over sequences of `sequence` tokens of
  * experts * sum_e (choices of e / (tokens top_k)) (mean probability of e). chosen, positions, gates: [tokens, top_k]; a choice that is not there is
  * -1, -1 and a gate of 0. mask (null: all): 0 for a token that is left out, of choices, counts and loss. cost: float[tokens / sequence][experts],
- * 16-byte aligned, stats: float[tokens][2], 8-byte aligned, both for the backward pass (stats null: not wanted). workspace: viola_route_workspace words of 4 bytes, 16-byte aligned. experts <= 1024,
- * top_k <= 32 (VIOLA_EUNSUPPORTED beyond).
+ * 16-byte aligned, stats: float[tokens][2], 8-byte aligned, both for the backward pass (stats null: not wanted). workspace: viola_route_workspace words of 4 bytes (0 for what is refused), 16-byte aligned. experts <= 1024,
+ * top_k <= 32 (VIOLA_EUNSUPPORTED beyond); tokens < 2^26.
  * viola_balance_forward: loss and counts for choices made elsewhere (int32, or int64 with chosen_wide; indices out of range count nowhere).
  * viola_route_backward: dlogits [tokens, experts], contiguous, of the logits' type from the gates' and / or the loss's gradient (null: none). */
 int64_t viola_route_workspace(int64_t tokens, int64_t experts, int64_t sequence);

@@ -3,6 +3,7 @@ places by brute force), and what the entry points and the Python operators refus
 
 import itertools
 import math
+from pathlib import Path
 
 import pytest
 import torch
@@ -189,3 +190,20 @@ def test_operators_refuse_on_the_host():
         nn.dispatch(x, places)
     with pytest.raises(RuntimeError, match="GPU only"):
         nn.combine(x, places)
+
+
+def test_sizes_beyond_the_limits_have_no_workspace():
+    """Asked beyond what the entry points take, the two sizes are 0: no division by what an overflow left, which ends the process."""
+    import subprocess
+    import sys
+    program = """if True:
+        from viola_amd import _lib
+        words, portions = _lib.library().viola_route_workspace, _lib.library().viola_norm_portions
+        assert words((1 << 26) - 1, 16, (1 << 26) - 1) > 0 and portions(8, 1 << 28, 8) == 8
+        for experts in (4, 16, 128, 1024):
+            for bits in range(26, 63):
+                assert words(1 << bits, experts, 1 << bits) == 0 and words(1 << bits, experts, 1) == 0, (experts, bits)
+        for bits in range(29, 63):
+            assert portions(8, 1 << bits, 8) == 0 and portions(8, (1 << bits) + 1, 1) == 0, bits"""
+    done = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True)
+    assert done.returncode == 0, (done.returncode, done.stderr[-500:])

@@ -301,6 +301,8 @@ int64_t portions_per_group(int64_t rows, int64_t group_rows, int64_t cols) {
     return wanted < most ? wanted : most;
 }
 
+constexpr int64_t MOST_COLUMNS = 1 << 28;
+
 bool valid_rows(const void* p, int64_t pitch, int64_t cols) { return p && pitch >= cols; }
 
 int set_common(NormArgs& a, const void* x, int64_t x_pitch, int x_dtype, const void* y, int64_t y_pitch, int branch_dtype, int64_t rows, int64_t cols, int after,
@@ -311,7 +313,7 @@ int set_common(NormArgs& a, const void* x, int64_t x_pitch, int x_dtype, const v
     VIOLA_CHECK_ARG(rows >= 0 && cols > 0 && group_rows > 0 && rows % group_rows == 0);
     VIOLA_CHECK_ARG(after >= VIOLA_NORM_NONE && after <= VIOLA_NORM_LAYER && before >= VIOLA_NORM_NONE && before <= VIOLA_NORM_LAYER && eps >= 0.0f);
     for (int64_t pitch : {gate_pitch, scale_pitch, shift_pitch}) VIOLA_CHECK_ARG(pitch == 0 || pitch >= cols);
-    VIOLA_CHECK_ARG(cols <= 1 << 28);
+    VIOLA_CHECK_ARG(cols <= MOST_COLUMNS);
     a.x = x; a.y = y; a.x_pitch = x_pitch; a.y_pitch = y_pitch; a.rows = rows; a.group_rows = group_rows;
     a.cols = (int)cols; a.x_dtype = x_dtype; a.branch_dtype = branch_dtype; a.after = after; a.before = before;
     a.weight_dtype = weight_dtype; a.vector_dtype = vector_dtype;
@@ -351,7 +353,7 @@ extern "C" int viola_norm_forward(const void* x, int64_t x_pitch, int x_dtype, c
 }
 
 extern "C" int64_t viola_norm_portions(int64_t rows, int64_t cols, int64_t group_rows) {
-    if (rows <= 0 || cols <= 0 || group_rows <= 0 || rows % group_rows) return 0;
+    if (rows <= 0 || cols <= 0 || cols > MOST_COLUMNS || group_rows <= 0 || rows % group_rows) return 0;
     return rows / group_rows * portions_per_group(rows, group_rows, cols);
 }
 

@@ -31,6 +31,7 @@ using namespace viola;
 namespace {
 
 constexpr int STAGE = 128, PLACE_THREADS = 512, MOST_EXPERTS = 1024, MOST_CHOSEN = 32, MOST_BLOCKS = 256;
+constexpr int64_t MOST_TOKENS = (int64_t{1} << 31) / MOST_CHOSEN;            // so that choices are counted in 32 bits
 
 struct RouteArgs {
     const void* logits;
@@ -696,7 +697,7 @@ int set_common(RouteArgs& a, const void* logits, int64_t pitch, int dtype, int64
     VIOLA_CHECK_ARG(viola_is_float(dtype) && tokens >= 0 && experts > 0 && top_k > 0 && sequence > 0 && tokens % sequence == 0);
     VIOLA_CHECK_ARG((score == VIOLA_SOFTMAX || score == VIOLA_SIGMOID) && pitch >= experts);
     if (experts > MOST_EXPERTS || top_k > MOST_CHOSEN) return VIOLA_EUNSUPPORTED;
-    VIOLA_CHECK_ARG(tokens < (1LL << 31) / MOST_CHOSEN);
+    VIOLA_CHECK_ARG(tokens < MOST_TOKENS);
     const size_t unit = dtype == VIOLA_F32 ? 16 : 8;
     a.logits = logits; a.pitch = pitch; a.dtype = dtype; a.tokens = tokens; a.experts = (int)experts; a.top_k = top_k;
     a.sigmoid = score == VIOLA_SIGMOID; a.normalize = normalize; a.scale = scale; a.mask = mask;
@@ -735,7 +736,7 @@ int forward(RouteArgs& a, int32_t* workspace, int64_t words, hipStream_t stream)
 }  // namespace
 
 extern "C" int64_t viola_route_workspace(int64_t tokens, int64_t experts, int64_t sequence) {
-    if (tokens <= 0 || experts <= 0 || experts > MOST_EXPERTS || sequence <= 0 || tokens % sequence) return 0;
+    if (tokens <= 0 || tokens >= MOST_TOKENS || experts <= 0 || experts > MOST_EXPERTS || sequence <= 0 || tokens % sequence) return 0;
     RouteArgs a = {};
     a.tokens = tokens; a.experts = (int)experts; a.sequence = sequence; a.sequences = tokens / sequence;
     plan(a);
