@@ -247,9 +247,6 @@ def _codes(v):
     return torch.where(scale > 0, v.double() / scale.double(), 0.0).round().float(), scale
 
 
-_ERF = math.sqrt(0.5)
-
-
 def _plain_gate(g, activation):
     """(act(g), act'(g)) in 32 bits"""
     if activation == "relu":
@@ -257,8 +254,9 @@ def _plain_gate(g, activation):
     if activation == "silu":
         s = 1 / (1 + torch.exp(-g))
         return g * s, s * (1 + g * (1 - s))
-    cdf = 0.5 * (1 + torch.erf(g * _ERF))
-    return g * cdf, cdf + g * torch.exp(-0.5 * g * g) * (1 / math.sqrt(2 * math.pi))
+    c = 2 * math.sqrt(2 / math.pi)                                           # gelu as this framework has it: g (1 + tanh y) / 2 = g sigmoid(2 y)
+    s = 1 / (1 + torch.exp(-c * g * (1 + 0.044715 * g * g)))
+    return g * s, s + g * s * (1 - s) * c * (1 + 3 * 0.044715 * g * g)
 
 
 def _plain_input(state):
@@ -420,8 +418,9 @@ def _exact_gate(g, kind):
     if kind == "silu":
         s = torch.sigmoid(g)
         return g * s, s + g * s * torch.sigmoid(-g)
-    cdf = torch.special.ndtr(g)
-    return g * cdf, cdf + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    y = math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)
+    half = (1 + torch.tanh(y)) / 2
+    return g * half, half + g / 2 / torch.cosh(y) ** 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * g ** 2)
 
 
 def _exact_rows(x, dy, weight, scale, bias, activation):
