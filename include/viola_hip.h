@@ -560,6 +560,25 @@ int viola_rows_gather(const void* rows, int64_t pitch, int64_t row_count, int dt
 int viola_rows_scatter(const void* x, int64_t pitch, int dtype, int64_t cols, const int32_t* positions, const float* gates, int64_t tokens, int top_k,
                        const int32_t* total, void* rows, int64_t row_count, const void* values, int64_t values_pitch, float* dots, viola_stream_t stream);
 
+/* ---------------------------------------------------------------- products of 8-bit integers
+ * No counterpart in the reference. A scale for each row of either operand (tokens and channels).
+ * viola_int8_quantize: of the rows of x (f32 / bf16 / f16, `pitch` values apart) codes [rows, code_pitch] int8 (code_pitch: cols rounded up to 16, zeros behind
+ * them; 16-byte aligned) and scales [rows]: s = max|v| / 127, code = v / s to the nearest integer, a half to the even one; s = 0 for a row of zeros, NaN with zero codes for
+ * one that holds an Inf or a NaN. v = x; with activation >= 0 (VIOLA_SILU ..) act(g) u of rows [g | u] of 2 cols; with factors (float [groups][cols], 16-byte
+ * aligned) x * factors, those of the group whose rows offsets (int32 [groups + 1], null: one group) has the row among. partial (with factors only; null: not wanted): float
+ * [viola_int8_sum_parts(rows, cols)][cols] sums of x over rows, for viola_column_reduce.
+ * viola_int8_gemm: out[r, c] = (sum_k a[r, k] b[c, k]) sa[r] sb[c] + bias[c], a [m, k] and b [n, k] with rows lda and ldb bytes apart (16-byte aligned, multiples of
+ * 16, columns of a beyond k up to the next 16 zero), out [m, n] contiguous. With offsets (int32 [groups + 1] on the device; no bias) rows offsets[g] to offsets[g + 1] take b +
+ * g b_stride and sb + g n, and rows from offsets[groups] on are zero. k <= 2^17, ldb <= 2^22 (VIOLA_EUNSUPPORTED beyond).
+ * viola_int8_gated_backward: dz [rows, 2 cols] = [dh u act'(g) | dh act(g)], contiguous, of z = [g | u] and dh float [rows, cols]; rows from *total (null: none) on are zero. */
+int64_t viola_int8_sum_parts(int64_t rows, int64_t cols);
+int viola_int8_quantize(const void* x, int64_t pitch, int dtype, int64_t rows, int64_t cols, int activation, const float* factors, const int32_t* offsets,
+                        int64_t groups, int8_t* codes, int64_t code_pitch, float* scales, float* partial, viola_stream_t stream);
+int viola_int8_gemm(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, int64_t b_stride, const float* sb, const int32_t* offsets,
+                    int64_t groups, int64_t m, int64_t n, int64_t k, const void* bias, int bias_dtype, void* out, int out_dtype, viola_stream_t stream);
+int viola_int8_gated_backward(const void* z, int64_t pitch, int dtype, int64_t rows, int64_t cols, int activation, const float* dh, const int32_t* total,
+                              void* dz, viola_stream_t stream);
+
 /* ---------------------------------------------------------------- self checks (test support)
  * Compare the hardware FP8 conversion instructions with the software codecs over every fp32 bit
  * pattern of magnitude <= the format's clamp range (encode) and all 256 codes (decode); writes

@@ -33,6 +33,8 @@ Pinning status (what fixes each function besides its own formula):
                      arithmetic is pinned, its agreement with the reference's hardware is parity unpinned
   norms around a block, expert routing (oracle.norms, oracle.routing) : NOT in the reference; central differences
                      of every gradient, hand cases of choices and places                   -> parity unpinned
+  products of 8-bit integers (oracle.int8) : NOT in the reference; brute force over all codes, hand cases,
+                     differences of the layer without rounding within half a step           -> parity unpinned
   NaN/Inf inside a quantize group: the reference's GPU and CPU branches disagree
                      (GPU reduce_absmax ignores NaN); the GPU behaviour is restated
                                                                    -> parity unpinned

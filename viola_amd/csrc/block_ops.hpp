@@ -1,5 +1,5 @@
-// Helpers shared by the kernels around a block (norm.hip, rows.hip, route.hip): sums over a wavefront on the vector ALU, and sums
-// over the wavefronts of a block.
+// Helpers shared by the kernels around a block (norm.hip, rows.hip, route.hip) and of 8-bit integers (int8.hip): sums and largest values
+// over a wavefront on the vector ALU, and sums over the wavefronts of a block.
 #pragma once
 
 #include "common.hpp"
@@ -21,6 +21,30 @@ __device__ __forceinline__ float wave_total(float v) {
     v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x142, 0xa, 0xf, true));   // row_bcast:15 into rows 1 and 3
     v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x143, 0xc, 0xf, true));   // row_bcast:31 into rows 2 and 3
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// Over aligned runs of LANES lanes, in every one of them
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+
+template <int LANES, typename F> __device__ __forceinline__ uint32_t over_lanes(uint32_t v, F&& f) {
+    if constexpr (LANES >= 2) v = f(v, dpp<0xB1>(v));
+    if constexpr (LANES >= 4) v = f(v, dpp<0x4E>(v));
+    if constexpr (LANES >= 8) v = f(v, dpp<0x141>(v));                       // halves of eight hold one value each: a mirror swaps them
+    if constexpr (LANES >= 16) v = f(v, dpp<0x140>(v));
+    if constexpr (LANES >= 32) {                                             // of a value and itself: rows 0 0 2 2 and rows 1 1 3 3 of 16 lanes
+        const auto pair = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = f(pair[0], pair[1]);
+    }
+    if constexpr (LANES >= 64) {                                             // the lower half twice and the upper half twice
+        const auto pair = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = f(pair[0], pair[1]);
+    }
+    return v;
+}
+template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) { return over_lanes<LANES>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
+template <int LANES> __device__ __forceinline__ uint32_t lanes_min(uint32_t v) { return over_lanes<LANES>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; }); }
+template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
+    return __uint_as_float(over_lanes<LANES>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 
 // Sums over all threads of a block of at most 16 wavefronts, in every thread. Two sets of slots are used in turn, so one barrier a

@@ -1047,6 +1047,7 @@ PYBIND11_MODULE(_host, m) {
     });
     register_optimizer(m);
     register_blocks(m);
+    register_int8(m);
     m.def("segment_offsets", torch::wrap_pybind_function([](const std::vector<int64_t>& counts, const at::Device& device) {
         Groups g;
         make_groups(g, counts, device, c10::hip::getCurrentHIPStream(device.index()).stream());

@@ -1,14 +1,18 @@
-// Shared by the native host files (host.cpp: modules, host_blocks.cpp: norms around a block and routing, host_optim.cpp: optimizer and
-// wire codec): calling the library's entry points, tensor helpers, arenas.
+// Shared by the native host files (host.cpp: modules, host_blocks.cpp: norms around a block and routing, host_int8.cpp: products of 8-bit
+// integers, host_optim.cpp: optimizer and wire codec): calling the library's entry points, tensor helpers, arenas.
 #pragma once
 #include <torch/extension.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/saved_variable.h>
+
+#include <ATen/hip/EmptyTensor.h>
 
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <atomic>
 #include <memory>
+#include <optional>
 #include <string>
 #include <vector>
 
@@ -114,7 +118,50 @@ inline Tensor restored(const torch::autograd::SavedVariable& saved, const at::De
     return t.contiguous();
 }
 
+inline void check_float(const char* name, const char* what, const Tensor& t, const at::Device& device) {
+    TORCH_CHECK(t.is_cuda(), "viola_amd kernels run on the GPU only");
+    TORCH_CHECK(t.device() == device, name, ": ", what, " is on ", t.device(), ", not on ", device);
+    const at::ScalarType type = t.scalar_type();
+    TORCH_CHECK(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf, name, ": ", what, " has to be float32, bfloat16 or float16, not ", type);
+}
+
+// The gradients of these nodes are computed by kernels that autograd does not see.
+inline void check_once(const char* name) { TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), name, " can be differentiated once only (create_graph is not supported)"); }
+
+// Memory for a result: the allocator at once, without the dispatcher's two rounds (a router has up to eight results and workspaces, and a
+// decoding step's call of it takes as long on the host as on the GPU).
+inline Tensor room(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) { return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt)); }
+
+inline bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// A tensor as rows of its last dimension with one distance between them; copied where it has none, and where rows overlap: those of a
+// broadcast dimension, whose distance is 0, too (autograd hands out such gradients: that of a sum over tokens repeats every row).
+struct Rows {
+    Tensor holder;
+    int64_t count, cols, pitch;
+    explicit Rows(const Tensor& t) : holder(t), count(1), cols(t.size(-1)), pitch(cols) {
+        for (int64_t i = 0; i + 1 < t.dim(); ++i) count *= t.size(i);
+        bool whole = cols <= 1 || t.stride(-1) == 1, first = true;
+        int64_t expected = 0;                                    // distance of a dimension's rows where all inside of it lie `pitch` apart
+        for (int64_t i = t.dim() - 2; i >= 0 && whole; --i) {
+            if (t.size(i) == 1) continue;
+            if (first) pitch = t.stride(i);
+            whole = pitch >= cols && (first || t.stride(i) == expected);
+            expected = t.stride(i) * t.size(i);
+            first = false;
+        }
+        if (!whole) {
+            holder = t.contiguous();
+            pitch = cols;
+        }
+    }
+    const void* data() const { return ptr(holder); }
+};
+
+inline Tensor or_none(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
+
 void register_optimizer(py::module_& m);                         // host_optim.cpp
 void register_blocks(py::module_& m);                            // host_blocks.cpp
+void register_int8(py::module_& m);                              // host_int8.cpp
 
 }  // namespace viola_host

@@ -3,7 +3,6 @@
 // of another type) and make what a kernel cannot read contiguous first.
 #include "host.hpp"
 
-#include <ATen/hip/EmptyTensor.h>
 #include <torch/csrc/autograd/functions/utils.h>
 
 using namespace viola_host;
@@ -12,46 +11,6 @@ using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 namespace {
-
-void check_float(const char* name, const char* what, const Tensor& t, const at::Device& device) {
-    TORCH_CHECK(t.is_cuda(), "viola_amd kernels run on the GPU only");
-    TORCH_CHECK(t.device() == device, name, ": ", what, " is on ", t.device(), ", not on ", device);
-    const at::ScalarType type = t.scalar_type();
-    TORCH_CHECK(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf, name, ": ", what, " has to be float32, bfloat16 or float16, not ", type);
-}
-
-// The gradients of these nodes are computed by kernels that autograd does not see.
-void check_once(const char* name) { TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), name, " can be differentiated once only (create_graph is not supported)"); }
-
-// Memory for a result: the allocator at once, without the dispatcher's two rounds (a router has up to eight results and workspaces, and a
-// decoding step's call of it takes as long on the host as on the GPU).
-Tensor room(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) { return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt)); }
-
-bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
-
-// A tensor as rows of its last dimension with one distance between them; copied where it has none, and where rows overlap: those of a
-// broadcast dimension, whose distance is 0, too (autograd hands out such gradients: that of a sum over tokens repeats every row).
-struct Rows {
-    Tensor holder;
-    int64_t count, cols, pitch;
-    explicit Rows(const Tensor& t) : holder(t), count(1), cols(t.size(-1)), pitch(cols) {
-        for (int64_t i = 0; i + 1 < t.dim(); ++i) count *= t.size(i);
-        bool whole = cols <= 1 || t.stride(-1) == 1, first = true;
-        int64_t expected = 0;                                    // distance of a dimension's rows where all inside of it lie `pitch` apart
-        for (int64_t i = t.dim() - 2; i >= 0 && whole; --i) {
-            if (t.size(i) == 1) continue;
-            if (first) pitch = t.stride(i);
-            whole = pitch >= cols && (first || t.stride(i) == expected);
-            expected = t.stride(i) * t.size(i);
-            first = false;
-        }
-        if (!whole) {
-            holder = t.contiguous();
-            pitch = cols;
-        }
-    }
-    const void* data() const { return ptr(holder); }
-};
 
 // ---------------------------------------------------------------------------------------------------- norms
 enum { X, Y, AFTER_WEIGHT, AFTER_BIAS, WEIGHT, BIAS, GATE, SCALE, SHIFT, INPUTS };
@@ -576,8 +535,6 @@ Tensor combine(const Tensor& y, const Tensor& positions_, const Tensor& offsets_
     }
     return out;
 }
-
-Tensor or_none(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
 
 }  // namespace
 

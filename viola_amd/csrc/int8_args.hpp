@@ -1,0 +1,64 @@
+// Shared by the products of 8-bit integers.
+#pragma once
+#include "common.hpp"
+
+namespace viola {
+
+// out[r, c] = (sum_k a[r, k] b[c, k]) sa[r] sb[c] + bias[c]; with offsets rows offsets[g] to offsets[g + 1] have the g-th b and sb, and rows from offsets[groups]
+// on are zero. The sum is exact: |a| <= 127, |b| <= 128, k <= 2^17.
+struct Int8Args {
+    const int8_t* a; const int8_t* b;
+    const float* sa; const float* sb;
+    const void* bias; void* out;
+    int64_t m, n, k;                                                         // k: a's columns, whole 16-byte pieces (zeros past the end)
+    int64_t lda, ldb, ldo;                                                   // lda, ldb: bytes, multiples of 16
+    const int* offsets; int groups; int64_t b_stride;                        // bytes from one b to the next
+    int bias_dtype, out_dtype;
+    int tiles_m, tiles_n;
+};
+
+constexpr int64_t INT8_MOST_K = 1 << 17;
+
+// Row tile `index` of `rows` rows, counted over the groups (each has whole tiles of its own) and then over the rows behind them: its group (groups: rows that are zero),
+// and its rows [begin, end). False: there are not so many. Every lane of a wavefront has to call it.
+__device__ __forceinline__ bool int8_row_tile(const Int8Args& p, int64_t index, int rows, int& group, int64_t& begin, int64_t& end) {
+    if (!p.offsets) {
+        group = 0;
+        begin = index * rows;
+        end = begin + rows < p.m ? begin + rows : p.m;
+        return begin < p.m;
+    }
+    const int lane = threadIdx.x % WAVE;
+    int64_t before = 0;                                                      // tiles of the groups so far
+    for (int base = 0; base <= p.groups; base += WAVE) {
+        const int g = base + lane;
+        // offsets that a program made by hand are taken within the rows and in order: a product must stay inside its buffers whatever they hold
+        int64_t from = g <= p.groups ? p.offsets[g] : p.m, to = g < p.groups ? p.offsets[g + 1] : p.m;
+        from = from < 0 ? 0 : from < p.m ? from : p.m;
+        to = to < from ? from : to < p.m ? to : p.m;
+        const int tiles = g <= p.groups ? (int)((to - from + rows - 1) / rows) : 0;
+        int upto = tiles;
+#pragma unroll
+        for (int d = 1; d < WAVE; d *= 2) {
+            const int other = __shfl_up(upto, d, WAVE);
+            upto += lane >= d ? other : 0;
+        }
+        const int64_t want = index - before;
+        const uint64_t past = __ballot((int64_t)upto > want);
+        if (past) {
+            const int at = __ffsll((long long)past) - 1;
+            group = __builtin_amdgcn_readfirstlane(base + at);
+            const int skipped = __builtin_amdgcn_readfirstlane(__shfl(upto - tiles, at, WAVE));
+            const int first = __builtin_amdgcn_readfirstlane(__shfl((int)from, at, WAVE)), last = __builtin_amdgcn_readfirstlane(__shfl((int)to, at, WAVE));
+            begin = first + (want - skipped) * rows;
+            end = begin + rows < last ? begin + rows : last;
+            return true;
+        }
+        before += __builtin_amdgcn_readfirstlane(__shfl(upto, WAVE - 1, WAVE));
+    }
+    return false;
+}
+// (tiles of rows that a launch has to provide for: each group can leave one unfilled)
+inline int64_t int8_row_tiles(const Int8Args& p, int rows) { return (p.m + rows - 1) / rows + (p.offsets ? p.groups + 1 : 0); }
+
+}  // namespace viola

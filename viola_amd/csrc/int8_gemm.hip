@@ -1,0 +1,277 @@
+// Products of 8-bit integers with a scale for each row of either operand (tokens and channels), whole or by groups of rows.
+//
+// The integers are multiplied by v_mfma_i32_32x32x32_i8, whose 32-bit sums are exact; the scales are applied to the finished sums in registers:
+// out = (sum * sa) * sb + bias, one rounding each. Bound by the matrix pipes (as many operations a cycle as FP8) and, on large products, by the power limit.
+//
+// The tiles are those of gemm_pingpong.hpp: eight wavefronts, two on each SIMD, whose memory work and math alternate; a chunk of 128 k is two pairs of
+// instructions for each 32 x 32 sub-tile where FP8 has one of 64 k, and an operand's 16-byte pieces are in the instruction's own order.
+#include <type_traits>
+
+#include "gemm_pingpong.hpp"
+#include "int8_args.hpp"
+
+namespace viola {
+
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// The finished sums of a wave times their scales plus bias, through its own part of the ring (which every wave has left), out in 16-byte pieces.
+template <typename S, typename TO>
+__device__ __forceinline__ void store_int8_tile(const i32x16 (&total)[S::TN][S::TM], const Int8Args& p, TO* out, int64_t m_begin, int64_t m_end, int64_t n_begin,
+                                                uint8_t* ring, const float* columns) {
+    const int lane = threadIdx.x % WAVE, l32 = lane % 32, lhi = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE), wm = wave / S::WN, wn = wave % S::WN;
+    const bool pieces_out = (p.ldo * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    constexpr int PER = 16 / (int)sizeof(TO), COLS_W = 32 * S::TN, PLD = COLS_W + PER, PIECES = COLS_W / PER;
+    static_assert(8 * 32 * PLD * (int)sizeof(TO) <= S::STAGES * S::STAGE);
+    TO* park = reinterpret_cast<TO*>(ring) + wave * 32 * PLD;
+    const int64_t ncol0 = n_begin + wn * COLS_W;
+#pragma unroll
+    for (int j = 0; j < S::TM; ++j) {
+        const int64_t row0 = m_begin + (wm * S::TM + j) * 32;
+        const float sa = row0 + l32 < m_end ? p.sa[row0 + l32] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int col = (wn * S::TN + i) * 32 + q * 8 + lhi * 4;
+                const float4 sb = *reinterpret_cast<const float4*>(&columns[col]), bias = *reinterpret_cast<const float4*>(&columns[S::COLS + col]);
+                const float v[4] = {(float)total[i][j][4 * q] * sa * sb.x + bias.x, (float)total[i][j][4 * q + 1] * sa * sb.y + bias.y,
+                                    (float)total[i][j][4 * q + 2] * sa * sb.z + bias.z, (float)total[i][j][4 * q + 3] * sa * sb.w + bias.w};
+                Quad<TO>::store(&park[l32 * PLD + i * 32 + q * 8 + lhi * 4], v);
+            }
+#pragma unroll
+        for (int it = 0; it < 32 * PIECES / WAVE; ++it) {
+            const int id = it * WAVE + lane, pr = id / PIECES, pc = id % PIECES;
+            const int64_t mrow = row0 + pr, ncol = ncol0 + pc * PER;
+            const uint4 value = *reinterpret_cast<const uint4*>(&park[pr * PLD + pc * PER]);
+            if (mrow >= m_end || ncol >= p.n) continue;
+            if (pieces_out && ncol + PER <= p.n) {
+                store_streaming(out + mrow * p.ldo + ncol, value);
+            } else {
+                const TO* values = reinterpret_cast<const TO*>(&value);
+                for (int e = 0; e < PER; ++e)
+                    if (ncol + e < p.n) out[mrow * p.ldo + ncol + e] = values[e];
+            }
+        }
+    }
+}
+
+template <typename S> constexpr int int8_lds() { return S::STAGES * S::STAGE + 2 * S::COLS * 4; }
+
+// Rows [m_begin, m_end) of one group and the columns from n_begin on.
+template <typename S>
+__device__ __forceinline__ void int8_tile(const Int8Args& p, int group, int64_t m_begin, int64_t m_end, int64_t n_begin, uint8_t* lds) {
+    constexpr int TM = S::TM, TN = S::TN, STAGES = S::STAGES, RING = STAGES * S::STAGE, HALVES = S::HALVES;
+    static_assert(S::TEAMS == 1);
+    const int tid = threadIdx.x, lane = tid % WAVE, l32 = lane % 32, lhi = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const int wm = wave / S::WN, wn = wave % S::WN;
+    float* columns = reinterpret_cast<float*>(lds + RING);                   // the channels' scales, then the bias
+    if (tid < S::COLS) {
+        const int64_t col = n_begin + tid;
+        columns[tid] = col < p.n ? p.sb[(int64_t)group * p.n + col] : 0.0f;
+        columns[S::COLS + tid] = p.bias && col < p.n ? load_float(p.bias, col, p.bias_dtype) : -0.0f;   // adding -0 changes nothing
+    }
+
+    // ---- load plan: instruction `it` brings LOAD_ROWS rows of an operand, unit U = PIECES row + slot holds piece slot ^ swizzle(row)
+    const i32x4 res_a = raw_resource(p.a + m_begin * p.lda), res_b = raw_resource(p.b + (int64_t)group * p.b_stride + n_begin * p.ldb);
+    constexpr uint32_t OUTSIDE = 0x80000000u;
+    const int chunks = (int)((p.k + S::CHUNK - 1) / S::CHUNK), full_chunks = (int)(p.k / S::CHUNK);
+    auto swizzle = [](int row) -> int { return S::PIECES == 4 ? (row >> 2) & 3 : (row >> 1) & 7; };
+    const int piece = tid % S::PIECES ^ swizzle(tid / S::PIECES);
+    const bool inside_tail = (int64_t)full_chunks * S::CHUNK + piece * 16 < p.k;
+    uint32_t cur[S::LOADS];
+#pragma unroll
+    for (int it = 0; it < S::LOADS; ++it) {
+        const int r = (it < S::A_LOADS ? it : it - S::A_LOADS) * S::LOAD_ROWS + tid / S::PIECES;
+        const int64_t rows = it < S::A_LOADS ? m_end - m_begin : p.n - n_begin;
+        cur[it] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)(it < S::A_LOADS ? p.lda : p.ldb) + piece * 16;
+    }
+    const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    auto issue = [&](int c, int stage) {
+        if (__builtin_expect(c >= full_chunks, 0)) {                         // the chunk that straddles the end of k, and those past it
+            asm volatile("; end of the k range");
+            const bool here = c == full_chunks && inside_tail;
+#pragma unroll
+            for (int it = 0; it < S::LOADS; ++it) {
+                const uint32_t at = here ? cur[it] : OUTSIDE;
+                load16_to_lds(it < S::A_LOADS ? res_a : res_b, lds_base + (uint32_t)stage * S::STAGE + it * 8192 + (uint32_t)wave * 1024, at, (uint32_t)c * S::CHUNK);
+            }
+            return;
+        }
+#pragma unroll
+        for (int it = 0; it < S::LOADS; ++it)
+            load16_to_lds(it < S::A_LOADS ? res_a : res_b, lds_base + (uint32_t)stage * S::STAGE + it * 8192 + (uint32_t)wave * 1024, cur[it], (uint32_t)c * S::CHUNK);
+    };
+
+    // ---- operand reads
+    const int sw = swizzle(l32);
+    const int rd_a0 = (wm * TM * 32 + l32) * S::CHUNK + ((lhi ^ sw) * 16), rd_b0 = S::A_BYTES + (wn * TN * 32 + l32) * S::CHUNK + ((lhi ^ sw) * 16);
+    i32x16 total[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) total[i][j][r] = 0;
+    i32x4 oa[HALVES][TM][2], ob[HALVES][TN][2];                              // 32 k each
+    auto read = [&](int stage) {
+        const uint8_t* base = lds + stage * S::STAGE;
+        int rd_a = rd_a0, rd_b = rd_b0;
+        asm volatile("" : "+v"(rd_a), "+v"(rd_b));                           // the addresses below: formed anew, 256 x 256 has no registers to keep them
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int i = 0; i < TN; ++i) ob[h][i][e] = *reinterpret_cast<const i32x4*>(base + ((rd_b + i * 32 * S::CHUNK) ^ (h * 64 + e * 32)));
+#pragma unroll
+                for (int j = 0; j < TM; ++j) oa[h][j][e] = *reinterpret_cast<const i32x4*>(base + ((rd_a + j * 32 * S::CHUNK) ^ (h * 64 + e * 32)));
+            }
+    };
+    auto math = [&] {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < TN; ++i)
+#pragma unroll
+                    for (int j = 0; j < TM; ++j) total[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(ob[h][i][e], oa[h][j][e], total[i][j], 0, 0, 0);
+        // (the compiler sinks MFMAs into the following read phase otherwise: intrinsics without side effects cross a barrier)
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(total[i][j]));
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto pin_operands = [&] {                                                // in registers before the barrier
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(oa[h][j][e]));
+#pragma unroll
+                for (int i = 0; i < TN; ++i) asm volatile("" : "+v"(ob[h][i][e]));
+            }
+    };
+    auto barrier = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    // Phases as in pingpong_tile (gemm_pingpong.hpp): waves 0-3 read chunk c in phase 2c and multiply in phase 2c + 1, waves 4-7 one phase later; the loads of
+    // chunk c + STAGES - 1 go into the stage of chunk c - 1, whose last readers had their operands in registers before the barrier that ended
+    // their phase; every wave ends its read phase of chunk c with its own loads of chunk c + 1 landed. Two stages: chunk c + 1 goes out once
+    // waves 4-7 have read chunk c - 1, and every wave waits for its part before the barrier that ends phase 2c + 1.
+    constexpr bool TWO = STAGES == 2;
+    constexpr int AHEAD = TWO ? 0 : (STAGES - 2) * S::LOADS;
+    static_assert((STAGES - 1) * S::LOADS < 16);
+#pragma unroll
+    for (int s = 0; s < (TWO ? 2 : STAGES - 1); ++s) issue(s, s);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (TWO ? S::LOADS : AHEAD));           // chunk 0
+    barrier();
+    const bool late = wave >= 4;
+    if (late) barrier();
+    int stage = 0, fill = TWO && late ? 0 : STAGES - 1;
+    for (int c = 0; c < chunks; ++c) {
+        read(stage);
+        auto issue_next = [&](int next) {
+            if (!TWO || next > 1) issue(next, fill);                         // (two stages: chunk 1 went out with chunk 0)
+            fill = fill == STAGES - 1 ? 0 : fill + 1;
+        };
+        if (!TWO || !late) issue_next(c + STAGES - 1);
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        __builtin_amdgcn_sched_barrier(0);
+        if (!TWO || late) __builtin_amdgcn_s_waitcnt(0x0070 | AHEAD);
+        else __builtin_amdgcn_s_waitcnt(0xC07F);                             // the LDS reads alone
+        pin_operands();
+        barrier();
+        if (TWO && late) issue_next(c + 2);
+        math();
+        if (TWO && !late) __builtin_amdgcn_s_waitcnt(0x0F70);
+        barrier();
+    }
+    if (!late) barrier();
+    __builtin_amdgcn_s_waitcnt(0x0F70);                                      // the trailing loads must not land in what follows
+    __syncthreads();                                                         // every wave has left the ring, and the columns' scales are there
+    if (p.out_dtype == VIOLA_F32) store_int8_tile<S>(total, p, static_cast<float*>(p.out), m_begin, m_end, n_begin, lds, columns);
+    else if (p.out_dtype == VIOLA_BF16) store_int8_tile<S>(total, p, static_cast<bf16_t*>(p.out), m_begin, m_end, n_begin, lds, columns);
+    else store_int8_tile<S>(total, p, static_cast<f16_t*>(p.out), m_begin, m_end, n_begin, lds, columns);
+}
+
+// Rows that no group has.
+__device__ __forceinline__ void int8_zeros(const Int8Args& p, int64_t m_begin, int64_t m_end, int64_t n_begin, int cols) {
+    const int64_t left = p.n - n_begin;
+    const int here = left < cols ? (int)left : cols;
+    for (int64_t row = m_begin; row < m_end; ++row)
+        for (int c = threadIdx.x; c < here; c += blockDim.x) store_float(p.out, row * p.ldo + n_begin + c, p.out_dtype, 0.0f);
+}
+
+template <typename S> __device__ __forceinline__ void int8_place(const Int8Args& p, int t, uint8_t* lds) {
+    // groups of 8 row tiles, as in pingpong_place
+    const int across = 8 * p.tiles_n, first_m = t / across * 8;
+    const int rows_here = p.tiles_m - first_m < 8 ? p.tiles_m - first_m : 8;
+    const int64_t n_begin = (int64_t)(t % across / rows_here) * S::COLS;
+    int group;
+    int64_t m_begin, m_end;
+    if (!int8_row_tile(p, first_m + t % across % rows_here, S::ROWS, group, m_begin, m_end)) return;
+    if (p.offsets && group == p.groups) int8_zeros(p, m_begin, m_end, n_begin, S::COLS);
+    else int8_tile<S>(p, group, m_begin, m_end, n_begin, lds);
+}
+
+template <typename S, int WAVES_PER_SIMD> __global__ __launch_bounds__(512, WAVES_PER_SIMD) void int8_gemm(Int8Args p) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[int8_lds<S>()];
+    const int t = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;       // contiguous ranges per XCD
+    if (t >= p.tiles_m * p.tiles_n) return;
+    int8_place<S>(p, t, lds);
+}
+
+using Int8L = PingPongShape<2, 4, 4, 2, 2, 128>;                             // 256 x 256
+using Int8M = PingPongShape<4, 2, 2, 2, 3, 128>;                             // 256 x 128
+using Int8S = PingPongShape<2, 4, 2, 1, 3, 128>;                             // 128 x 128
+using Int8Pairs = PingPongShape<2, 4, 2, 1, 4>;                              // 128 x 128, two blocks on a CU
+
+template <typename S, int WAVES_PER_SIMD> static int launch_tiles(const Int8Args& args, hipStream_t stream) {
+    Int8Args p = args;
+    const int64_t tiles_m = int8_row_tiles(p, S::ROWS), tiles_n = (p.n + S::COLS - 1) / S::COLS;
+    if (tiles_m * tiles_n >= (int64_t{1} << 30)) return VIOLA_ETOOLARGE;
+    p.tiles_m = (int)tiles_m;
+    p.tiles_n = (int)tiles_n;
+    VIOLA_LAUNCH((int8_gemm<S, WAVES_PER_SIMD>), dim3((unsigned)((tiles_m * tiles_n + 7) / 8 * 8)), 512, 0, stream, p);
+    return viola_launch_status();
+}
+
+static int launch_int8(const Int8Args& p, hipStream_t stream) {
+    ScaledTile tile = choose_scaled_tile(p.m, p.n, p.k, false);
+    switch (tile) {
+        case SCALED_TILE_L: return launch_tiles<Int8L, 2>(p, stream);
+        case SCALED_TILE_M: return launch_tiles<Int8M, 2>(p, stream);
+        default: break;
+    }
+    if ((p.m + 127) / 128 * ((p.n + 127) / 128) <= 256) return launch_tiles<Int8S, 2>(p, stream);
+    return launch_tiles<Int8Pairs, 4>(p, stream);
+}
+
+}  // namespace viola
+
+using namespace viola;
+
+extern "C" int viola_int8_gemm(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, int64_t b_stride, const float* sb, const int32_t* offsets,
+                               int64_t groups, int64_t m, int64_t n, int64_t k, const void* bias, int bias_dtype, void* out, int out_dtype, viola_stream_t stream_) {
+    hipStream_t stream = viola_enter(stream_);
+    VIOLA_CHECK_ARG(m >= 0 && n > 0 && k > 0 && m < (int64_t{1} << 31) && n < (int64_t{1} << 31) && groups >= 0 && groups < (int64_t{1} << 16) && viola_is_float(out_dtype) &&
+                    (!bias || viola_is_float(bias_dtype)) && (!offsets || (groups > 0 && !bias)));
+    if (k > INT8_MOST_K) return VIOLA_EUNSUPPORTED;
+    if (m == 0) return 0;
+    VIOLA_CHECK_ARG(a && sa && b && sb && out && lda >= k && ldb >= k && lda % 16 == 0 && ldb % 16 == 0 && lda <= 2 * INT8_MOST_K && b_stride % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(b) % 16 == 0);
+    if (ldb > (int64_t{1} << 22)) return VIOLA_EUNSUPPORTED;                  // rows of one tile within 32 bits
+    Int8Args p = {};
+    p.a = a; p.b = b; p.sa = sa; p.sb = sb; p.bias = bias; p.out = out; p.m = m; p.n = n; p.k = (k + 15) / 16 * 16;
+    p.lda = lda; p.ldb = ldb; p.ldo = n; p.offsets = offsets; p.groups = (int)groups; p.b_stride = b_stride; p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
+    return launch_int8(p, stream);
+}

@@ -53,30 +53,6 @@ struct RouteArgs {
     float* portion_sums;
 };
 
-// ---------------------------------------------------------------------------------------------------- over the lanes of a row
-template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
-
-template <int LANES, typename F> __device__ __forceinline__ uint32_t over_lanes(uint32_t v, F&& f) {
-    if constexpr (LANES >= 2) v = f(v, dpp<0xB1>(v));
-    if constexpr (LANES >= 4) v = f(v, dpp<0x4E>(v));
-    if constexpr (LANES >= 8) v = f(v, dpp<0x141>(v));                       // halves of eight hold one value each: a mirror swaps them
-    if constexpr (LANES >= 16) v = f(v, dpp<0x140>(v));
-    if constexpr (LANES >= 32) {                                             // of a value and itself: rows 0 0 2 2 and rows 1 1 3 3 of 16 lanes
-        const auto pair = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-        v = f(pair[0], pair[1]);
-    }
-    if constexpr (LANES >= 64) {                                             // the lower half twice and the upper half twice
-        const auto pair = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-        v = f(pair[0], pair[1]);
-    }
-    return v;
-}
-template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) { return over_lanes<LANES>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
-template <int LANES> __device__ __forceinline__ uint32_t lanes_min(uint32_t v) { return over_lanes<LANES>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; }); }
-template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
-    return __uint_as_float(over_lanes<LANES>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
-}
-
 // ---------------------------------------------------------------------------------------------------- values
 // Order of logits as that of unsigned integers: NaN above all, -0 equal to 0, 0 for -inf, which is never chosen.
 __device__ __forceinline__ uint32_t key_of(float l) {
