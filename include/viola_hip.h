@@ -537,12 +537,21 @@ int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, const void*
  * -1, -1 and a gate of 0. mask (null: all): 0 for a token that is left out, of choices, counts and loss. cost: float[tokens / sequence][experts],
  * 16-byte aligned, stats: float[tokens][2], 8-byte aligned, both for the backward pass (stats null: not wanted). workspace: viola_route_workspace words of 4 bytes (0 for what is refused), 16-byte aligned. experts <= 1024,
  * top_k <= 32 (VIOLA_EUNSUPPORTED beyond); tokens < 2^26.
+ * viola_route_steered_forward: the same with a choice by c = s + bias (bias float[experts], null: none; s = p, or sigmoid(logit) for VIOLA_SIGMOID) among the experts of the
+ * top_groups of `groups` equal runs of experts (at most 64) whose ranks are largest (ties to the lower run), a rank being the sum of the group_top (1 or 2) largest c of a run;
+ * without a bias the choice among them is by the logits. Scores are compared as in 64 bits. An expert whose logit is -inf, or whose c is -inf or NaN, is not chosen; a row with a NaN
+ * among its logits (or, for VIOLA_SOFTMAX, +inf) is chosen by the logits alone. Gates and loss are of s. workspace: viola_route_steered_workspace words; backward: viola_route_backward.
  * viola_balance_forward: loss and counts for choices made elsewhere (int32, or int64 with chosen_wide; indices out of range count nowhere).
  * viola_route_backward: dlogits [tokens, experts], contiguous, of the logits' type from the gates' and / or the loss's gradient (null: none). */
 int64_t viola_route_workspace(int64_t tokens, int64_t experts, int64_t sequence);
+int64_t viola_route_steered_workspace(int64_t tokens, int64_t experts, int64_t sequence);
 int viola_route_forward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
                         const uint8_t* mask, int64_t sequence, int32_t* chosen, float* gates, int32_t* positions, int32_t* counts, int32_t* offsets,
                         float* loss, float* cost, float* stats, int32_t* workspace, int64_t workspace_words, viola_stream_t stream);
+int viola_route_steered_forward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
+                                const float* bias, int groups, int top_groups, int group_top, const uint8_t* mask, int64_t sequence, int32_t* chosen, float* gates,
+                                int32_t* positions, int32_t* counts, int32_t* offsets, float* loss, float* cost, float* stats, int32_t* workspace,
+                                int64_t workspace_words, viola_stream_t stream);
 int viola_balance_forward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, const uint8_t* mask,
                           int64_t sequence, const void* chosen, int chosen_wide, int32_t* counts, float* loss, float* cost, float* stats,
                           int32_t* workspace, int64_t workspace_words, viola_stream_t stream);

@@ -138,3 +138,42 @@ def combine_gradient(dout, y, positions, gates=None):
                 dy[r] = g[t, j].double() * d[t]
                 dg[t, j] = (d[t] * y[r]).sum()
     return dy, dg.reshape(positions.shape)
+
+
+def steered_scores(logits, score, bias=None):
+    """c = s + bias in 64 bits, -inf where an expert is never chosen; None for a row whose choice is by the logits alone"""
+    l = logits.detach().double().cpu().reshape(-1, logits.shape[-1])
+    rows = []
+    for row in l:
+        if bool(torch.isnan(row).any()) or (score == "softmax" and bool((row == math.inf).any())):
+            rows.append(None)
+            continue
+        s = torch.sigmoid(row) if score == "sigmoid" else torch.softmax(row, -1)
+        c = s if bias is None else s + bias.detach().double().cpu()
+        rows.append([-math.inf if row[e] == -math.inf or c[e] != c[e] else c[e].item() for e in range(len(row))])
+    return rows
+
+
+def choose_steered(logits, top_k, score, mask=None, bias=None, groups=1, top_groups=1, group_top=1):
+    """`choose` by s + bias among the experts of the top_groups runs whose group_top largest add up to most. Row by row."""
+    by_logits = choose(logits, top_k, mask).reshape(-1, top_k)
+    counted = (torch.ones(by_logits.shape[0], dtype=torch.bool) if mask is None else mask.cpu().reshape(-1))
+    flat = logits.detach().double().cpu().reshape(-1, logits.shape[-1]).tolist()
+    size = logits.shape[-1] // groups
+    chosen = torch.full_like(by_logits, -1)
+    for t, c in enumerate(steered_scores(logits, score, bias)):
+        if not counted[t]:
+            continue
+        if c is None:
+            chosen[t] = by_logits[t]
+            continue
+        ranks = []
+        for g in range(groups):
+            best = sorted((v for v in c[g * size:(g + 1) * size] if v > -math.inf), reverse=True)[:group_top]
+            ranks.append(sum(best) if best else -math.inf)
+        kept = sorted(range(groups), key=lambda g: (-ranks[g], g))[:top_groups]
+        value = c if bias is not None else flat[t]
+        order = sorted((e for e in range(len(c)) if e // size in kept and c[e] > -math.inf), key=lambda e: (-value[e], e))
+        for j, e in enumerate(order[:top_k]):
+            chosen[t, j] = e
+    return chosen.reshape(*logits.shape[:-1], top_k)

@@ -86,6 +86,7 @@ _SIGNATURES = {
     "viola_norm_forward": [_p, _l, _i, _p, _l, _i, _l, _l, _i, _p, _p, _i, _p, _p, _i, _p, _l, _p, _l, _p, _l, _i, _l, _f, _f, _f, _p, _p, _p, _p],
     "viola_norm_backward": [_p, _l, _i, _p, _l, _i, _l, _l, _i, _p, _p, _i, _p, _p, _i, _p, _l, _p, _l, _p, _l, _i, _l, _f, _f, _p, _p, _p, _p, _p, _p, _l, _p, _p, _p, _p, _p, _p, _p, _p],
     "viola_route_forward": [_p, _l, _i, _l, _l, _i, _i, _i, _f, _p, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p, _l, _p],
+    "viola_route_steered_forward": [_p, _l, _i, _l, _l, _i, _i, _i, _f, _p, _i, _i, _i, _p, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p, _l, _p],
     "viola_balance_forward": [_p, _l, _i, _l, _l, _i, _i, _p, _l, _p, _i, _p, _p, _p, _p, _p, _l, _p],
     "viola_route_backward": [_p, _l, _i, _l, _l, _i, _i, _i, _f, _l, _p, _p, _p, _p, _p, _p, _p],
     "viola_rows_gather": [_p, _l, _l, _i, _l, _p, _p, _l, _i, _p, _p],
@@ -97,7 +98,7 @@ _SIGNATURES = {
     "viola_selftest_philox": [_p, _p, _l, _p],
 }
 EXPORTS = tuple(_SIGNATURES) + ("viola_abi_version", "viola_error_string", "viola_ns_plan", "viola_ns_plan_many", "viola_tensor_encode_slices", "viola_group_gemm_parts",
-                                "viola_group_gemm_form", "viola_scaled_gemm_form", "viola_norm_portions", "viola_route_workspace", "viola_int8_sum_parts")
+                                "viola_group_gemm_form", "viola_scaled_gemm_form", "viola_norm_portions", "viola_route_workspace", "viola_route_steered_workspace", "viola_int8_sum_parts")
 
 _lib = None
 
@@ -121,6 +122,7 @@ def library():
         lib.viola_scaled_gemm_form.argtypes, lib.viola_scaled_gemm_form.restype = [_l, _l, _l], ctypes.c_int
         lib.viola_norm_portions.argtypes, lib.viola_norm_portions.restype = [_l, _l, _l], ctypes.c_int64
         lib.viola_route_workspace.argtypes, lib.viola_route_workspace.restype = [_l, _l, _l], ctypes.c_int64
+        lib.viola_route_steered_workspace.argtypes, lib.viola_route_steered_workspace.restype = [_l, _l, _l], ctypes.c_int64
         lib.viola_int8_sum_parts.argtypes, lib.viola_int8_sum_parts.restype = [_l, _l], ctypes.c_int64
         lib.viola_ns_plan.argtypes, lib.viola_ns_plan.restype = [_l, _l, _l, _l, _i, _i, _i, ctypes.POINTER(ctypes.c_int)], ctypes.c_int
         lib.viola_ns_plan_many.argtypes, lib.viola_ns_plan_many.restype = [_p, _i, ctypes.POINTER(ctypes.c_int)], ctypes.c_int

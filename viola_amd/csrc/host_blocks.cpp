@@ -240,6 +240,7 @@ struct RouterPlan {
     int score = VIOLA_SOFTMAX;
     bool normalize = true, given = false;
     double scale = 1.0;
+    int64_t groups = 0, top_groups = 1, group_top = 1;           // groups 0: the choice is by the logits alone
 };
 
 struct RouterBackward : public Node {
@@ -261,8 +262,8 @@ struct Routed {
 };
 
 // given: choices made elsewhere; only counts and balance come back then
-Routed router(const char* name, const Tensor& logits, const Tensor& given, const Tensor& mask, RouterPlan plan, bool per_sequence) {
-    check_seen(name, {logits, given, mask});
+Routed router(const char* name, const Tensor& logits, const Tensor& given, const Tensor& mask, RouterPlan plan, bool per_sequence, const Tensor& bias = Tensor()) {
+    check_seen(name, {logits, given, mask, bias});
     TORCH_CHECK(logits.dim() >= 2 && logits.size(-1) > 0, name, ": logits have to be [..., tokens, experts], got ", logits.sizes());
     const at::Device device = logits.device();
     check_float(name, "logits", logits, device);
@@ -280,6 +281,20 @@ Routed router(const char* name, const Tensor& logits, const Tensor& given, const
                 " experts (1 to 32, and no more than there are)");
     TORCH_CHECK(!mask.defined() || (mask.device() == device && mask.scalar_type() == at::kBool && mask.sizes() == lead), name, ": mask has to be bool of shape ", lead, " on ",
                 device);
+    if (bias.defined()) {
+        check_float(name, "bias", bias, device);
+        TORCH_CHECK(bias.sizes() == at::IntArrayRef({plan.experts}), name, ": bias has to be of shape [", plan.experts, "], got ", bias.sizes());
+        TORCH_CHECK(!bias.requires_grad(), name, ": bias steers a choice, which has no gradient: it cannot require one");
+    }
+    if (plan.groups) {
+        TORCH_CHECK(plan.groups > 0 && plan.groups <= 64 && plan.experts % plan.groups == 0, name, ": ", plan.groups, " groups of ", plan.experts, " experts (1 to 64, of one size)");
+        const int64_t size = plan.experts / plan.groups;
+        TORCH_CHECK(plan.top_groups >= 1 && plan.top_groups <= plan.groups && (plan.group_top == 1 || plan.group_top == 2) && plan.group_top <= size, name, ": top_groups has to be 1 to ",
+                    plan.groups, " and group_top 1 or 2 and no more than the ", size, " experts of a group, got ", plan.top_groups, " and ", plan.group_top);
+        TORCH_CHECK(plan.top_k <= plan.top_groups * size, name, ": ", plan.top_k, " choices of ", plan.top_groups, " groups of ", size, " experts");
+        if (plan.top_groups == plan.groups) plan.groups = plan.top_groups = plan.group_top = 1;      // all are open
+        if (plan.groups == 1 && !bias.defined()) plan.groups = 0;
+    }
     const c10::DeviceGuard guard(device);
     const bool need = at::GradMode::is_enabled() && logits.requires_grad();
     auto node = need ? std::shared_ptr<RouterBackward>(new RouterBackward(), torch::autograd::deleteNode) : nullptr;
@@ -314,7 +329,7 @@ Routed router(const char* name, const Tensor& logits, const Tensor& given, const
             const uint8_t* mask_p = counted.defined() ? static_cast<const uint8_t*>(counted.const_data_ptr()) : nullptr;
             const int64_t cost_at = kept.take(sequences * plan.experts * 4);
             stats_at = need ? kept.take(plan.tokens * 8) : 0;
-            const int64_t words = viola_route_workspace(plan.tokens, plan.experts, plan.sequence);
+            const int64_t words = (plan.groups ? viola_route_steered_workspace : viola_route_workspace)(plan.tokens, plan.experts, plan.sequence);
             Arena freed, &temp = need ? freed : kept;                        // nothing is kept without a gradient
             const int64_t temp_at = temp.take(words * 4);
             kept.make(device);
@@ -328,6 +343,12 @@ Routed router(const char* name, const Tensor& logits, const Tensor& given, const
                 const Tensor choice = given.contiguous();
                 VIOLA_CALL(viola_balance_forward, rows.data(), rows.pitch, type, plan.tokens, plan.experts, (int)plan.top_k, plan.score, mask_p, plan.sequence,
                            choice.const_data_ptr(), choice.scalar_type() == at::kLong, counts, loss, kept.as<float>(cost_at), stats, temp.as<int32_t>(temp_at), words, stream);
+            } else if (plan.groups) {
+                const Tensor steer = bias.defined() ? bias.to(at::kFloat).contiguous() : Tensor();
+                VIOLA_CALL(viola_route_steered_forward, rows.data(), rows.pitch, type, plan.tokens, plan.experts, (int)plan.top_k, plan.score, plan.normalize, (float)plan.scale,
+                           static_cast<const float*>(ptr(steer)), (int)plan.groups, (int)plan.top_groups, (int)plan.group_top, mask_p, plan.sequence,
+                           static_cast<int*>(r.chosen.mutable_data_ptr()), static_cast<float*>(r.gates.mutable_data_ptr()), static_cast<int*>(r.positions.mutable_data_ptr()),
+                           counts, static_cast<int*>(r.offsets.mutable_data_ptr()), loss, kept.as<float>(cost_at), stats, temp.as<int32_t>(temp_at), words, stream);
             } else {
                 VIOLA_CALL(viola_route_forward, rows.data(), rows.pitch, type, plan.tokens, plan.experts, (int)plan.top_k, plan.score, plan.normalize, (float)plan.scale, mask_p,
                            plan.sequence, static_cast<int*>(r.chosen.mutable_data_ptr()), static_cast<float*>(r.gates.mutable_data_ptr()),
@@ -562,16 +583,19 @@ void viola_host::register_blocks(py::module_& m) {
         return norm(name.c_str(), input, plan, want_out, want_h);
     }));
     m.def("route", torch::wrap_pybind_function([](const Tensor& logits, int64_t top_k, int score, bool normalize, double scale, const std::optional<Tensor>& mask,
-                                                  bool per_sequence) {
+                                                  bool per_sequence, const std::optional<Tensor>& bias, int64_t groups, int64_t top_groups, int64_t group_top) {
         RouterPlan plan;
         plan.top_k = top_k;
         plan.score = score;
         plan.normalize = normalize;
         plan.scale = scale;
+        plan.groups = groups;
+        plan.top_groups = top_groups;
+        plan.group_top = group_top;
         Routed r;
         {
             py::gil_scoped_release release;
-            r = router("route", logits, Tensor(), or_none(mask), plan, per_sequence);
+            r = router("route", logits, Tensor(), or_none(mask), plan, per_sequence, or_none(bias));
         }
         return std::make_tuple(r.chosen, r.gates, r.positions, r.counts, r.offsets, r.balance);
     }));

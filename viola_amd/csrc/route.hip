@@ -4,6 +4,8 @@
 // logit, so a row far from zero neither overflows nor vanishes. p = u / sum u.
 //
 //   choice    the top_k largest logits, NaN above all numbers, ties to the lowest index, -inf never
+//             steered: the top_k largest c = s + bias (s = p for softmax, sigmoid(l) for sigmoid) in the top_groups runs of experts of largest rank, a
+//             rank being the sum of the group_top largest c of a run
 //   gates     scale u_i / (sum over the chosen), or scale p_i (softmax) / scale sigmoid(l_i)
 //   balance   mean over sequences of E sum_e (c_e / (n k)) (sum_t p_te / n), with c_e choices of e in its n counted tokens
 //   position  (choices of experts before e) + (choices of e by tokens before t): rows sorted by expert, then by token
@@ -41,6 +43,9 @@ struct RouteArgs {
     const uint8_t* mask;
     int64_t sequence, sequences, per_sequence, chunk, portions, per_block, blocks;
     int threads;                                                             // of a block that chooses
+    // a steered choice
+    const float* bias;                                                       // null: none
+    int groups, top_groups, group_top;
     // choices made elsewhere (balance alone)
     const void* given;
     int given_wide;
@@ -114,6 +119,179 @@ template <int LANES, int VALUES> __device__ __forceinline__ void load_logits(con
     if (a.dtype == VIOLA_F32) load_logits_as<LANES, VALUES, float>(a, token, lane, l);
     else if (a.dtype == VIOLA_BF16) load_logits_as<LANES, VALUES, bf16_t>(a, token, lane, l);
     else load_logits_as<LANES, VALUES, f16_t>(a, token, lane, l);
+}
+
+// ---------------------------------------------------------------------------------------------------- a steered choice
+// A choice is a whole number, so the order of two scores next to each other has to be the exact one. In 32 bits a score is off by at most
+//   sigmoid  5 2^-24 s (exp_of 2 ulp, sum and quotient half an ulp each)
+//   softmax  24 2^-24 of the row's largest (besides, l - m is rounded: |l - m| 2^-24 p, at most a third of 2^-24 of the largest; the sum of at most 16 values of 64 lanes)
+// and the sum with its bias by 2^-24 of itself. Where two that are told apart lie nearer than NEAR times their magnitudes and the row's largest score,
+// the row is chosen again in 64 bits by the whole wavefront: one row in 400 of 256 experts with sigmoid scores and a bias. Without a bias the choice itself is by
+// logits, as ever, and exact; ranks of single experts are too.
+template <bool SIGMOID> constexpr float NEAR = SIGMOID ? 0x1p-21f : 0x1p-19f;
+constexpr int MOST_GROUPS = 64;
+
+__device__ __forceinline__ float logit_at(const RouteArgs& a, int64_t token, int e) { return load_float(a.logits, token * a.pitch + e, a.dtype); }
+
+__device__ __forceinline__ double over_wave(double v, int step) {
+    const uint64_t b = __double_as_longlong(v);
+    const uint32_t low = __shfl_xor((int)(uint32_t)b, step, WAVE), high = __shfl_xor((int)(uint32_t)(b >> 32), step, WAVE);
+    return __longlong_as_double((long long)((uint64_t)high << 32 | low));
+}
+
+// The choice of one row in 64 bits, by a whole wavefront that has experts lane, lane + 64, ..; into chosen and values (logits), top_k each.
+template <int EACH, bool SIGMOID> __device__ __forceinline__ void choose_exactly(const RouteArgs& a, int64_t token, float m, int* chosen, float* values) {
+    const int lane = threadIdx.x % WAVE, size = a.experts / a.groups;
+    double c[EACH];
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int e = lane + i * WAVE;
+        const float l = e < a.experts ? logit_at(a, token, e) : -__builtin_inff();
+        c[i] = SIGMOID ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)l - (double)m);
+        sum += c[i];
+        if (l == -__builtin_inff()) c[i] = -__builtin_inf();                 // never chosen
+    }
+    if (!SIGMOID)
+        for (int d = 1; d < WAVE; d *= 2) sum += over_wave(sum, d);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        if (!SIGMOID) c[i] /= sum;
+        const int e = lane + i * WAVE;
+        if (a.bias && e < a.experts) c[i] += (double)a.bias[e];
+        if (!(c[i] > -__builtin_inf())) c[i] = -__builtin_inf();
+    }
+    if (a.groups > 1) {
+        double rank = -__builtin_inf();                                      // of group `lane`
+        for (int g = 0; g < a.groups; ++g) {
+            double first = -__builtin_inf(), second = first;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int e = lane + i * WAVE;
+                const double v = e / size == g && e < a.experts ? c[i] : -__builtin_inf();
+                second = fmax(second, fmin(first, v));
+                first = fmax(first, v);
+            }
+            for (int d = 1; d < WAVE; d *= 2) {
+                const double other = over_wave(first, d), behind = over_wave(second, d);
+                second = fmax(fmax(second, behind), fmin(first, other));
+                first = fmax(first, other);
+            }
+            if (lane == g) rank = a.group_top > 1 && second > -__builtin_inf() ? first + second : first;
+        }
+        int before = 0;
+        for (int g = 0; g < a.groups; ++g) {
+            const uint64_t b = __double_as_longlong(rank);
+            const double other = __longlong_as_double((long long)((uint64_t)(uint32_t)__shfl((int)(uint32_t)(b >> 32), g, WAVE) << 32 | (uint32_t)__shfl((int)(uint32_t)b, g, WAVE)));
+            before += other > rank || (other == rank && g < lane);
+        }
+        const uint64_t kept = __ballot(lane < a.groups && before < a.top_groups);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int e = lane + i * WAVE;
+            if (e < a.experts && !(kept >> (e / size) & 1)) c[i] = -__builtin_inf();
+        }
+    }
+    if (!a.bias) {                                                           // the choice is by logits
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int e = lane + i * WAVE;
+            if (e < a.experts && c[i] > -__builtin_inf()) c[i] = logit_at(a, token, e);
+        }
+    }
+    for (int j = 0; j < a.top_k; ++j) {
+        double best = -__builtin_inf();
+        int at = MOST_EXPERTS;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (c[i] > best) {
+                best = c[i];
+                at = lane + i * WAVE;
+            }
+        for (int d = 1; d < WAVE; d *= 2) {
+            const double other = over_wave(best, d);
+            const int there = __shfl_xor(at, d, WAVE);
+            if (other > best || (other == best && there < at)) {
+                best = other;
+                at = there;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (lane + i * WAVE == at) c[i] = -__builtin_inf();
+        if (lane == 0) {
+            chosen[j] = at < MOST_EXPERTS ? at : -1;
+            values[j] = at < MOST_EXPERTS ? logit_at(a, token, at) : 0.0f;
+        }
+    }
+}
+
+// The runs of experts that a row's choice is open to, of values v (-inf: not there) in the row's part of `keys`; `ranks`: [2 groups]. In each lane whether that of value i is;
+// near: two runs' ranks could be the other way round.
+template <int LANES, int VALUES> __device__ __forceinline__ void open_groups(const RouteArgs& a, const float (&v)[VALUES], int lane, float* keys, float* ranks, float slack,
+                                                                             float near_by, bool (&open)[VALUES], bool& near) {
+    const int size = a.experts / a.groups;
+#pragma unroll
+    for (int i = 0; i < VALUES; i += 4) *reinterpret_cast<float4*>(&keys[expert_of<LANES>(i, lane)]) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    int parts = 1;                                                           // lanes that share a run
+    while (2 * parts * a.groups <= LANES) parts *= 2;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");                   // a row's lanes are of one wavefront, whose LDS accesses stay in order
+    __builtin_amdgcn_wave_barrier();
+    for (int g0 = 0; g0 < a.groups; g0 += LANES) {
+        const int g = g0 + lane / parts;
+        float first = -__builtin_inff(), second = first;
+        if (g < a.groups)
+            for (int e = g * size + lane % parts; e < (g + 1) * size; e += parts) {
+                const float x = keys[e];
+                second = fmaxf(second, fminf(first, x));
+                first = fmaxf(first, x);
+            }
+        for (int d = 1; d < parts; d *= 2) {
+            const float other = __shfl_xor(first, d, WAVE), behind = __shfl_xor(second, d, WAVE);
+            second = fmaxf(fmaxf(second, behind), fminf(first, other));
+            first = fmaxf(first, other);
+        }
+        if (g < a.groups && lane % parts == 0) {
+            const bool both = a.group_top > 1 && second > -__builtin_inff();
+            ranks[2 * g] = both ? first + second : first;
+            ranks[2 * g + 1] = both ? fabsf(first) + fabsf(second) : fabsf(first);
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    bool close = false;
+    constexpr int TURNS = (LANES * VALUES < MOST_GROUPS ? LANES * VALUES : MOST_GROUPS) / LANES > 1 ? (LANES * VALUES < MOST_GROUPS ? LANES * VALUES : MOST_GROUPS) / LANES : 1;
+    float kept[TURNS];
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+        const int g = t * LANES + lane;
+        kept[t] = 0.0f;
+        if (g >= a.groups) continue;
+        const float2 mine = *reinterpret_cast<const float2*>(&ranks[2 * g]);
+        int before = 0;
+        for (int h = 0; h < a.groups; ++h) {
+            const float2 other = *reinterpret_cast<const float2*>(&ranks[2 * h]);
+            before += other.x > mine.x || (other.x == mine.x && h < g);
+            close = close || (h != g && fabsf(other.x - mine.x) <= near_by * (other.y + mine.y + slack));    // of two without experts: a NaN
+        }
+        kept[t] = before < a.top_groups ? 1.0f : 0.0f;
+    }
+    near = lanes_max<LANES>(close ? 1u : 0u) != 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t)
+        if (t * LANES + lane < a.groups) ranks[2 * (t * LANES + lane)] = kept[t];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const float each = 1.0f / (float)size;
+#pragma unroll
+    for (int i = 0; i < VALUES; ++i) {                                       // e / size by its reciprocal: e below 1024, half a run from a border
+        const int e = expert_of<LANES>(i, lane);
+        open[i] = e < a.experts && ranks[2 * (int)(((float)e + 0.5f) * each)] != 0.0f;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // ---------------------------------------------------------------------------------------------------- after the blocks
@@ -259,14 +437,22 @@ template <int VALUES> __host__ __device__ constexpr int threads_of() { return VA
 // Tokens of a stage: as many as that at once, STAGE at least
 template <int LANES, int VALUES> __host__ __device__ constexpr int stage_of() { return threads_of<VALUES>() / LANES > STAGE ? threads_of<VALUES>() / LANES : STAGE; }
 
-template <int LANES, int VALUES> size_t choose_lds(int experts, int top_k, bool given) {
+// A steered choice has besides, for each wavefront, the values of its rows and the ranks of their runs of experts.
+constexpr int STEERED_THREADS = 512;
+template <int LANES, int VALUES> __host__ __device__ constexpr int ranks_of() { return 2 * (64 / LANES) * (LANES * VALUES < MOST_GROUPS ? LANES * VALUES : MOST_GROUPS); }
+__host__ __device__ constexpr size_t up_to_16(size_t words) { return (words + 3) / 4 * 4; }
+
+template <int LANES, int VALUES> size_t choose_lds(int experts, int top_k, bool given, bool steered) {
     const size_t rows = stage_of<LANES, VALUES>();
-    const size_t choice = given ? 0 : (size_t)experts * (rows / 32) + 2 * rows * top_k + rows;
+    size_t choice = given ? 0 : (size_t)experts * (rows / 32) + 2 * rows * top_k + rows;
+    if (steered) choice = up_to_16(choice) + STEERED_THREADS / 64 * (64 * VALUES + ranks_of<LANES, VALUES>());
     const size_t sums = (size_t)(threads_of<VALUES>() / 64) * experts;
     return 4 * (8 * (size_t)quads_of(experts) + (choice > sums ? choice : sums));
 }
 
-template <int LANES, int VALUES, bool GIVEN, bool SIGMOID> __global__ __launch_bounds__(threads_of<VALUES>()) void choose_kernel(RouteArgs a) {
+enum { CHOOSE = 0, GIVEN_CHOICE = 1, STEERED_CHOICE = 2 };
+template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bounds__(MODE == STEERED_CHOICE ? STEERED_THREADS : threads_of<VALUES>()) void choose_kernel(RouteArgs a) {
+    constexpr bool GIVEN = MODE == GIVEN_CHOICE, STEERED = MODE == STEERED_CHOICE;
     extern __shared__ int lds[];
     __shared__ int counted_tokens;
     __shared__ float2 slots[2][16];
@@ -281,6 +467,14 @@ template <int LANES, int VALUES, bool GIVEN, bool SIGMOID> __global__ __launch_b
     float* sums = reinterpret_cast<float*>(rest);
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
     const bool alone = a.blocks == 1;                                        // then there is one portion of one stage, and nothing to leave behind
+    float *keys = nullptr, *ranks = nullptr;                                 // of the wavefront
+    float bias[STEERED ? VALUES : 1];
+    if constexpr (STEERED) {
+        keys = reinterpret_cast<float*>(rest) + up_to_16(a.experts * WORDS + 2 * STAGED * a.top_k + STAGED) + threadIdx.x / 64 * (64 * VALUES + ranks_of<LANES, VALUES>());
+        ranks = keys + 64 * VALUES;
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) bias[i] = a.bias && expert_of<LANES>(i, lane) < a.experts ? a.bias[expert_of<LANES>(i, lane)] : 0.0f;
+    }
     for (int e = threadIdx.x; e < 4 * quads; e += threads) counts[e] = start[e] = 0;
     const int64_t last = (blockIdx.x + 1) * a.per_block < a.portions ? (blockIdx.x + 1) * a.per_block : a.portions;
     for (int64_t portion = blockIdx.x * a.per_block; portion < last; ++portion) {
@@ -344,6 +538,83 @@ template <int LANES, int VALUES, bool GIVEN, bool SIGMOID> __global__ __launch_b
                             const int64_t e = a.given_wide ? static_cast<const int64_t*>(a.given)[at] : static_cast<const int*>(a.given)[at];
                             if (e >= 0 && e < a.experts) atomicAdd(&counts[e], 1);
                         }
+                } else if constexpr (STEERED) {
+                    const int in_wave = slot % (64 / LANES);
+                    // a row whose scores are no numbers is chosen by its logits alone
+                    const bool odd = best == 0xffffffffu || (!SIGMOID && m == __builtin_inff());
+                    const float largest = SIGMOID ? sigmoid_of(m) : inverse;
+                    float c[VALUES];
+#pragma unroll
+                    for (int i = 0; i < VALUES; ++i) {
+                        c[i] = (SIGMOID ? sigmoid_of(l[i]) : u[i] * inverse) + bias[i];
+                        c[i] = key[i] && c[i] > -__builtin_inff() ? c[i] : -__builtin_inff();
+                        if (!odd && a.bias) key[i] = c[i] > -__builtin_inff() ? key_of(c[i]) : 0;
+                    }
+                    bool near = false;
+                    if (a.groups > 1) {
+                        const bool inexact = a.bias || a.group_top > 1;
+                        if (!inexact) {
+#pragma unroll
+                            for (int i = 0; i < VALUES; ++i) c[i] = l[i];
+                        }
+                        bool open[VALUES];
+                        open_groups<LANES, VALUES>(a, c, lane, keys + in_wave * LANES * VALUES, ranks + in_wave * (ranks_of<LANES, VALUES>() / (64 / LANES)), 4.0f * largest,
+                                                   NEAR<SIGMOID>, open, near);
+                        near = near && inexact;
+#pragma unroll
+                        for (int i = 0; i < VALUES; ++i) key[i] = odd || open[i] ? key[i] : 0;
+                    }
+                    float before = 0.0f;
+                    const int picks = a.bias && a.top_k < a.experts ? a.top_k + 1 : a.top_k;    // with a bias the next one is compared too
+                    for (int j = 0; j < picks; ++j) {
+                        best = 0;
+#pragma unroll
+                        for (int i = 0; i < VALUES; ++i) best = key[i] > best ? key[i] : best;
+                        best = lanes_max<LANES>(best);
+                        if (a.bias && j && best) {
+                            const float v = value_of(best);
+                            near = near || before - v <= NEAR<SIGMOID> * (fabsf(before) + fabsf(v) + 2.0f * largest);
+                        }
+                        before = value_of(best);
+                        if (j == a.top_k) break;
+                        uint32_t first = 0xffffffffu;
+#pragma unroll
+                        for (int i = VALUES - 1; i >= 0; --i) first = key[i] == best ? (uint32_t)expert_of<LANES>(i, lane) : first;
+                        first = lanes_min<LANES>(first);
+                        float logit = 0.0f;
+                        bool mine = false;
+#pragma unroll
+                        for (int i = 0; i < VALUES; ++i)
+                            if (first == (uint32_t)expert_of<LANES>(i, lane)) {
+                                key[i] = 0;
+                                logit = l[i];
+                                mine = true;
+                            }
+                        if (mine) {                                          // (of a row without any left: some lane's expert, with a key of 0)
+                            chosen[row * a.top_k + j] = best ? (int)first : -1;
+                            values[row * a.top_k + j] = logit;
+                        }
+                    }
+                    near = near && counted && !odd;
+                    for (uint64_t again = __ballot(near && lane == 0); again; again &= again - 1) {
+                        const int at = __ffsll((long long)again) - 1, there = __shfl(row, at, WAVE);
+                        choose_exactly<(LANES * VALUES + 63) / 64, SIGMOID>(a, base + there, __shfl(m, at, WAVE), chosen + there * a.top_k, values + there * a.top_k);
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    float picked = 0.0f;
+                    if (token < end)
+                        for (int j = lane; j < a.top_k; j += LANES) {
+                            const int at = row * a.top_k + j, e = chosen[at];
+                            const float v = values[at], value = !a.normalize && SIGMOID ? sigmoid_of(v) : score<SIGMOID>(v, m);
+                            values[at] = value;
+                            if (e >= 0) {
+                                picked += value;
+                                atomicOr(&bits[e * WORDS + row / 32], 1u << (row % 32));
+                            }
+                        }
+                    picked = lanes_sum<LANES>(picked);
+                    if (lane == 0) factors[row] = a.scale * (a.normalize ? (counted ? 1.0f / picked : 0.0f) : SIGMOID ? 1.0f : inverse);
                 } else {
                     // LANES choices at a time, one left with each lane: its score and its bit are that lane's work
                     float picked = 0.0f;
@@ -651,6 +922,7 @@ void plan(RouteArgs& a) {
     with_shape(a.experts, [&](auto lanes, auto values) {
         lanes_of_row = decltype(lanes)::value;
         a.threads = threads_of<decltype(values)::value>();
+        if (a.groups && a.threads > STEERED_THREADS) a.threads = STEERED_THREADS;
         staged = stage_of<decltype(lanes)::value, decltype(values)::value>();
     });
     // half the threads where blocks of them are fewer than CUs; no more than a sequence's tokens have lanes, two wavefronts at least
@@ -698,12 +970,15 @@ int forward(RouteArgs& a, int32_t* workspace, int64_t words, hipStream_t stream)
     a.portion_tokens = a.portion_counts + (a.portions + (a.per_block > 1 ? a.blocks : 0)) * row;
     with_shape(a.experts, [&](auto lanes, auto values) {
         constexpr int LANES = decltype(lanes)::value, VALUES = decltype(values)::value;
-        const unsigned lds = (unsigned)choose_lds<LANES, VALUES>(a.experts, a.top_k, a.given != nullptr);
-        auto launch = [&](auto given, auto sigmoid) {
-            VIOLA_LAUNCH((choose_kernel<LANES, VALUES, decltype(given)::value, decltype(sigmoid)::value>), dim3((unsigned)a.blocks), a.threads, lds, stream, a);
+        const unsigned lds = (unsigned)choose_lds<LANES, VALUES>(a.experts, a.top_k, a.given != nullptr, a.groups != 0);
+        auto launch = [&](auto mode) {
+            constexpr int MODE = decltype(mode)::value;
+            if (a.sigmoid) VIOLA_LAUNCH((choose_kernel<LANES, VALUES, MODE, true>), dim3((unsigned)a.blocks), a.threads, lds, stream, a);
+            else VIOLA_LAUNCH((choose_kernel<LANES, VALUES, MODE, false>), dim3((unsigned)a.blocks), a.threads, lds, stream, a);
         };
-        if (a.given) a.sigmoid ? launch(std::true_type(), std::true_type()) : launch(std::true_type(), std::false_type());
-        else a.sigmoid ? launch(std::false_type(), std::true_type()) : launch(std::false_type(), std::false_type());
+        if (a.given) launch(std::integral_constant<int, GIVEN_CHOICE>());
+        else if (a.groups) launch(std::integral_constant<int, STEERED_CHOICE>());
+        else launch(std::integral_constant<int, CHOOSE>());
     });
     if (a.blocks > 1) VIOLA_LAUNCH(place_kernel, dim3(a.given ? 2 : (unsigned)a.blocks + 1), PLACE_THREADS, 0, stream, a);
     return viola_launch_status();
@@ -711,13 +986,15 @@ int forward(RouteArgs& a, int32_t* workspace, int64_t words, hipStream_t stream)
 
 }  // namespace
 
-extern "C" int64_t viola_route_workspace(int64_t tokens, int64_t experts, int64_t sequence) {
+static int64_t workspace_for(int64_t tokens, int64_t experts, int64_t sequence, bool steered) {
     if (tokens <= 0 || tokens >= MOST_TOKENS || experts <= 0 || experts > MOST_EXPERTS || sequence <= 0 || tokens % sequence) return 0;
     RouteArgs a = {};
-    a.tokens = tokens; a.experts = (int)experts; a.sequence = sequence; a.sequences = tokens / sequence;
+    a.tokens = tokens; a.experts = (int)experts; a.sequence = sequence; a.sequences = tokens / sequence; a.groups = steered;
     plan(a);
     return workspace_words(a);
 }
+extern "C" int64_t viola_route_workspace(int64_t tokens, int64_t experts, int64_t sequence) { return workspace_for(tokens, experts, sequence, false); }
+extern "C" int64_t viola_route_steered_workspace(int64_t tokens, int64_t experts, int64_t sequence) { return workspace_for(tokens, experts, sequence, true); }
 
 extern "C" int viola_route_forward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
                                    const uint8_t* mask, int64_t sequence, int32_t* chosen, float* gates, int32_t* positions, int32_t* counts, int32_t* offsets,
@@ -728,6 +1005,24 @@ extern "C" int viola_route_forward(const void* logits, int64_t pitch, int dtype,
     VIOLA_CHECK_ARG(top_k <= experts);
     if (tokens == 0) return 0;
     VIOLA_CHECK_ARG(logits && chosen && gates && positions && counts && offsets && loss && cost && reinterpret_cast<uintptr_t>(stats) % 8 == 0);
+    a.chosen = chosen; a.gates = gates; a.positions = positions; a.counts = counts; a.offsets = offsets; a.loss = loss; a.cost = cost;
+    a.stats = reinterpret_cast<float2*>(stats);
+    return forward(a, workspace, workspace_words, stream);
+}
+
+extern "C" int viola_route_steered_forward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
+                                           const float* bias, int groups, int top_groups, int group_top, const uint8_t* mask, int64_t sequence, int32_t* chosen, float* gates,
+                                           int32_t* positions, int32_t* counts, int32_t* offsets, float* loss, float* cost, float* stats, int32_t* workspace,
+                                           int64_t workspace_words, viola_stream_t stream_) {
+    hipStream_t stream = viola_enter(stream_);
+    RouteArgs a = {};
+    if (const int status = set_common(a, logits, pitch, dtype, tokens, experts, top_k, score, normalize, scale, mask, sequence)) return status;
+    VIOLA_CHECK_ARG(groups > 0 && experts % groups == 0 && top_groups > 0 && top_groups <= groups && (group_top == 1 || group_top == 2) && group_top <= experts / groups &&
+                    top_k <= top_groups * (experts / groups));
+    if (groups > MOST_GROUPS) return VIOLA_EUNSUPPORTED;
+    if (tokens == 0) return 0;
+    VIOLA_CHECK_ARG(logits && chosen && gates && positions && counts && offsets && loss && cost && reinterpret_cast<uintptr_t>(stats) % 8 == 0);
+    a.bias = bias; a.groups = groups; a.top_groups = top_groups; a.group_top = group_top;
     a.chosen = chosen; a.gates = gates; a.positions = positions; a.counts = counts; a.offsets = offsets; a.loss = loss; a.cost = cost;
     a.stats = reinterpret_cast<float2*>(stats);
     return forward(a, workspace, workspace_words, stream);

@@ -42,7 +42,13 @@ def _score(score):
     return _lib.SCORE[score]
 
 
-def route(logits, top_k, *, score="softmax", normalize=True, scale=1.0, mask=None, per_sequence=False):
+def _groups(groups):
+    if groups < 1:
+        raise AssertionError(f"groups must be 1 or more, got {groups!r}")
+    return groups
+
+
+def route(logits, top_k, *, score="softmax", normalize=True, scale=1.0, mask=None, per_sequence=False, bias=None, groups=1, top_groups=None, group_top=1):
     """The `top_k` experts of each token with the largest logits [..., tokens, experts] (ties to the lowest index), as a `Routing`.
 
     Probabilities are softmax(logits), or with score="sigmoid" sigmoid(logits) over their sum. gates: with `normalize` the chosen ones' share of
@@ -51,8 +57,16 @@ def route(logits, top_k, *, score="softmax", normalize=True, scale=1.0, mask=Non
 
     balance: experts * sum_e (share of the choices that fall on e) * (mean probability of e) over the counted tokens, of the whole batch or
     with `per_sequence` of each sequence (the last but one dimension), then the mean over sequences; 1 where all experts are used alike. Gradients
-    flow to the logits from gates and balance. Up to 1024 experts and 32 choices."""
-    experts, gates, positions, counts, offsets, balance = _lib.host().route(logits, top_k, _score(score), normalize, scale, mask, per_sequence)
+    flow to the logits from gates and balance. Up to 1024 experts and 32 choices.
+
+    bias [experts]: the choice is by s + bias instead, s being the softmax's probability or sigmoid(logit); gates and balance remain those of s. A program that balances the load
+    moves it after each step, for instance by bias += rate * torch.sign(counts.float().mean() - counts); it has no gradient. An expert whose bias is -inf or NaN is never chosen.
+    groups: equal runs of experts (up to 64), of which a token's choice is open to the top_groups (all by default) of largest rank, ties to the lower run; a rank is the sum of the
+    group_top (1 or 2) largest s + bias of a run. Scores are compared as in 64 bits, ties to the lowest index. A row with a NaN logit (with softmax, +inf too) is
+    chosen by its logits alone, as without bias and groups."""
+    top_groups = groups if top_groups is None else top_groups
+    experts, gates, positions, counts, offsets, balance = _lib.host().route(logits, top_k, _score(score), normalize, scale, mask, per_sequence, bias, _groups(groups), top_groups,
+                                                                            group_top)
     return Routing(positions, offsets, gates, experts, counts, balance)
 
 
