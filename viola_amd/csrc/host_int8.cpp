@@ -133,15 +133,23 @@ Tensor run(const char* name, const Tensor& x, const Tensor& weight, const Tensor
         if (grouped) places = offsets.contiguous();
         if (plan.rows) {
             const Codes w(weight, stream);
-            const int64_t pitch = ceil_to(plan.k, 16);
-            Arena temp;
-            const int64_t scales_at = temp.take(plan.rows * 4), codes_at = temp.take(plan.rows * pitch);
-            temp.make(device);
-            VIOLA_CALL(viola_int8_quantize, rows.data(), rows.pitch, code_of(plan.x_type), plan.rows, plan.k, activation, nullptr, nullptr, 0, temp.as<int8_t>(codes_at), pitch,
-                       temp.as<float>(scales_at), nullptr, stream);
             const Tensor channels = scale.contiguous(), b = bias.defined() ? bias.contiguous() : Tensor();
-            product(plan, temp.as<int8_t>(codes_at), pitch, temp.as<float>(scales_at), w, static_cast<const float*>(channels.const_data_ptr()), places, b, plan.n, plan.k,
-                    out.mutable_data_ptr(), plan.out_type, stream);
+            const float* channel_data = static_cast<const float*>(channels.const_data_ptr());
+            int status = VIOLA_EUNSUPPORTED;
+            if (!grouped && plan.rows <= 16) {                               // few rows: quantized on the way into the product
+                status = VIOLA_TRY(viola_int8_rows_linear, rows.data(), rows.pitch, code_of(plan.x_type), plan.rows, plan.k, activation, w.data(), w.pitch, channel_data, plan.n,
+                                   ptr(b), b.defined() ? code_of(b.scalar_type()) : VIOLA_F32, out.mutable_data_ptr(), code_of(plan.out_type), stream);
+                if (status != VIOLA_EUNSUPPORTED) check("viola_int8_rows_linear", status);
+            }
+            if (status == VIOLA_EUNSUPPORTED) {
+                const int64_t pitch = ceil_to(plan.k, 16);
+                Arena temp;
+                const int64_t scales_at = temp.take(plan.rows * 4), codes_at = temp.take(plan.rows * pitch);
+                temp.make(device);
+                VIOLA_CALL(viola_int8_quantize, rows.data(), rows.pitch, code_of(plan.x_type), plan.rows, plan.k, activation, nullptr, nullptr, 0, temp.as<int8_t>(codes_at), pitch,
+                           temp.as<float>(scales_at), nullptr, stream);
+                product(plan, temp.as<int8_t>(codes_at), pitch, temp.as<float>(scales_at), w, channel_data, places, b, plan.n, plan.k, out.mutable_data_ptr(), plan.out_type, stream);
+            }
         }
     }
     if (need) {
@@ -204,9 +212,8 @@ variable_list ProductBackward::apply(variable_list&& grads) {
     TORCH_CHECK(w.defined() && w.device() == device && w.scalar_type() == at::kChar && w.size(-2) == turned[0] && w.size(-1) == turned[1] &&
                     (plan.groups ? w.dim() == 3 && w.size(0) == plan.groups : w.dim() == 2), "a tensor saved by ", label, " came back changed");
     const Codes back = has_turned ? Codes(w, stream) : Codes::turned(w, stream);
-    const Tensor ones = at::ones({std::max<int64_t>(plan.groups, 1) * plan.k}, options.dtype(at::kFloat));
     result[0] = room(shape, plan.x_type, device);
-    product(plan, temp.as<int8_t>(codes_at), pitch, temp.as<float>(scales_at), back, static_cast<const float*>(ones.const_data_ptr()), places, Tensor(), plan.k, plan.n,
+    product(plan, temp.as<int8_t>(codes_at), pitch, temp.as<float>(scales_at), back, nullptr, places, Tensor(), plan.k, plan.n,
             gated ? temp.at(dh_at) : result[0].mutable_data_ptr(), gated ? at::kFloat : plan.x_type, stream);
     if (gated) {
         const Tensor z = x.unpack();

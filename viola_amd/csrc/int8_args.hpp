@@ -1,4 +1,4 @@
-// Shared by the products of 8-bit integers.
+// Shared by the products of 8-bit integers: int8_gemm.hip (tiles from LDS) and int8_rows.hip (few rows).
 #pragma once
 #include "common.hpp"
 
@@ -8,7 +8,7 @@ namespace viola {
 // on are zero. The sum is exact: |a| <= 127, |b| <= 128, k <= 2^17.
 struct Int8Args {
     const int8_t* a; const int8_t* b;
-    const float* sa; const float* sb;
+    const float* sa; const float* sb;                                        // sb null: ones
     const void* bias; void* out;
     int64_t m, n, k;                                                         // k: a's columns, whole 16-byte pieces (zeros past the end)
     int64_t lda, ldb, ldo;                                                   // lda, ldb: bytes, multiples of 16
@@ -60,5 +60,8 @@ __device__ __forceinline__ bool int8_row_tile(const Int8Args& p, int64_t index, 
 }
 // (tiles of rows that a launch has to provide for: each group can leave one unfilled)
 inline int64_t int8_row_tiles(const Int8Args& p, int rows) { return (p.m + rows - 1) / rows + (p.offsets ? p.groups + 1 : 0); }
+
+// VIOLA_EUNSUPPORTED: too many rows. int8_rows.hip
+int launch_int8_rows(const Int8Args& p, hipStream_t stream);
 
 }  // namespace viola

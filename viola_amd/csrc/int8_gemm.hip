@@ -69,7 +69,7 @@ __device__ __forceinline__ void int8_tile(const Int8Args& p, int group, int64_t 
     float* columns = reinterpret_cast<float*>(lds + RING);                   // the channels' scales, then the bias
     if (tid < S::COLS) {
         const int64_t col = n_begin + tid;
-        columns[tid] = col < p.n ? p.sb[(int64_t)group * p.n + col] : 0.0f;
+        columns[tid] = !p.sb ? 1.0f : col < p.n ? p.sb[(int64_t)group * p.n + col] : 0.0f;
         columns[S::COLS + tid] = p.bias && col < p.n ? load_float(p.bias, col, p.bias_dtype) : -0.0f;   // adding -0 changes nothing
     }
 
@@ -246,6 +246,8 @@ template <typename S, int WAVES_PER_SIMD> static int launch_tiles(const Int8Args
 }
 
 static int launch_int8(const Int8Args& p, hipStream_t stream) {
+    const int status = launch_int8_rows(p, stream);
+    if (status != VIOLA_EUNSUPPORTED) return status;
     ScaledTile tile = choose_scaled_tile(p.m, p.n, p.k, false);
     switch (tile) {
         case SCALED_TILE_L: return launch_tiles<Int8L, 2>(p, stream);
@@ -267,7 +269,7 @@ extern "C" int viola_int8_gemm(const int8_t* a, int64_t lda, const float* sa, co
                     (!bias || viola_is_float(bias_dtype)) && (!offsets || (groups > 0 && !bias)));
     if (k > INT8_MOST_K) return VIOLA_EUNSUPPORTED;
     if (m == 0) return 0;
-    VIOLA_CHECK_ARG(a && sa && b && sb && out && lda >= k && ldb >= k && lda % 16 == 0 && ldb % 16 == 0 && lda <= 2 * INT8_MOST_K && b_stride % 16 == 0 &&
+    VIOLA_CHECK_ARG(a && sa && b && out && lda >= k && ldb >= k && lda % 16 == 0 && ldb % 16 == 0 && lda <= 2 * INT8_MOST_K && b_stride % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(b) % 16 == 0);
     if (ldb > (int64_t{1} << 22)) return VIOLA_EUNSUPPORTED;                  // rows of one tile within 32 bits
     Int8Args p = {};
