@@ -123,15 +123,14 @@ template <int LANES, int VALUES> __device__ __forceinline__ void load_logits(con
 
 // ---------------------------------------------------------------------------------------------------- a steered choice
 // A choice is a whole number, so the order of two scores next to each other has to be the exact one. In 32 bits a score is off by at most
-//   sigmoid  5 2^-24 s (exp_of 2 ulp, sum and quotient half an ulp each)
-//   softmax  24 2^-24 of the row's largest (besides, l - m is rounded: |l - m| 2^-24 p, at most a third of 2^-24 of the largest; the sum of at most 16 values of 64 lanes)
+//   sigmoid  14 2^-24 of the row's largest (u within 8 2^-24: exp_of 2 ulp, sum and quotient half an ulp each, and the rounding of l - m, which is |l - m| 2^-24 u or at
+//            most a third of 2^-24 of the largest; the factor exp(min(m, 0)) 4 2^-24 where it is not one; their product)
+//   softmax  24 2^-24 of the row's largest (the sum of at most 16 values of 64 lanes besides)
 // and the sum with its bias by 2^-24 of itself. Where two that are told apart lie nearer than NEAR times their magnitudes and the row's largest score,
-// the row is chosen again in 64 bits by the whole wavefront: one row in 400 of 256 experts with sigmoid scores and a bias. Without a bias the choice itself is by
+// the row is chosen again in 64 bits by the whole wavefront: one row in 150 of 256 experts with sigmoid scores and a bias. Without a bias the choice itself is by
 // logits, as ever, and exact; ranks of single experts are too.
-template <bool SIGMOID> constexpr float NEAR = SIGMOID ? 0x1p-21f : 0x1p-19f;
+template <bool SIGMOID> constexpr float NEAR = SIGMOID ? 0x1p-20f : 0x1p-19f;
 constexpr int MOST_GROUPS = 64;
-
-__device__ __forceinline__ float logit_at(const RouteArgs& a, int64_t token, int e) { return load_float(a.logits, token * a.pitch + e, a.dtype); }
 
 __device__ __forceinline__ double over_wave(double v, int step) {
     const uint64_t b = __double_as_longlong(v);
@@ -139,91 +138,123 @@ __device__ __forceinline__ double over_wave(double v, int step) {
     return __longlong_as_double((long long)((uint64_t)high << 32 | low));
 }
 
-// The choice of one row in 64 bits, by a whole wavefront that has experts lane, lane + 64, ..; into chosen and values (logits), top_k each.
-template <int EACH, bool SIGMOID> __device__ __forceinline__ void choose_exactly(const RouteArgs& a, int64_t token, float m, int* chosen, float* values) {
-    const int lane = threadIdx.x % WAVE, size = a.experts / a.groups;
-    double c[EACH];
+// The choice of one row in 64 bits, by a whole wavefront that has experts lane, lane + 64, ..; into chosen and values (logits), top_k each. c: [experts] in the
+// wavefront's own LDS. A function of its own, as inlined the exponential's constants stay in registers all through the kernel, which has none to spare.
+struct ExactChoice {
+    const void* row;
+    const float* bias;
+    int dtype, experts, top_k, groups, top_groups, group_top;
+    float largest;
+    bool by_logits;                                                          // a row whose scores are no numbers: NaN above all, then +inf
+    double* c;
+    int* chosen;
+    float* values;
+};
+template <bool SIGMOID> __device__ __forceinline__ void choose_exactly(const ExactChoice a) {
+    int lane = threadIdx.x % WAVE;
+    asm volatile("" : "+v"(lane));                                           // nothing of this rare path is kept ready for it
+    const int size = a.experts / a.groups;
+    double* const c = a.c;
+    auto logit_at = [&](int e) { return load_float(a.row, e, a.dtype); };
+    const double none = -__builtin_inf();
     double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const int e = lane + i * WAVE;
-        const float l = e < a.experts ? logit_at(a, token, e) : -__builtin_inff();
-        c[i] = SIGMOID ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)l - (double)m);
-        sum += c[i];
-        if (l == -__builtin_inff()) c[i] = -__builtin_inf();                 // never chosen
+#pragma unroll 1
+    for (int e = lane; e < a.experts; e += WAVE) {
+        const double l = logit_at(e), u = exp(SIGMOID ? -l : l - (double)a.largest);
+        sum += u;
+        c[e] = l == none ? none : SIGMOID ? 1.0 / (1.0 + u) : u;             // -inf is never chosen
+        if (a.by_logits) c[e] = l != l ? 2e300 : fmin(l, 1e300);
     }
-    if (!SIGMOID)
+    if (!SIGMOID && !a.by_logits)
         for (int d = 1; d < WAVE; d *= 2) sum += over_wave(sum, d);
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        if (!SIGMOID) c[i] /= sum;
-        const int e = lane + i * WAVE;
-        if (a.bias && e < a.experts) c[i] += (double)a.bias[e];
-        if (!(c[i] > -__builtin_inf())) c[i] = -__builtin_inf();
+#pragma unroll 1
+    for (int e = lane; e < a.experts; e += WAVE) {                           // a lane's own experts: no other lane has seen them yet
+        double v = c[e];
+        if (!SIGMOID && !a.by_logits) v /= sum;
+        if (a.bias) v += (double)a.bias[e];
+        c[e] = v > none ? v : none;
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");                   // LDS accesses of a wavefront stay in order
+    __builtin_amdgcn_wave_barrier();
     if (a.groups > 1) {
-        double rank = -__builtin_inf();                                      // of group `lane`
-        for (int g = 0; g < a.groups; ++g) {
-            double first = -__builtin_inf(), second = first;
-#pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                const int e = lane + i * WAVE;
-                const double v = e / size == g && e < a.experts ? c[i] : -__builtin_inf();
-                second = fmax(second, fmin(first, v));
-                first = fmax(first, v);
+        double rank = none;                                                  // of group `lane`
+        if (lane < a.groups) {
+            double second = none;
+#pragma unroll 1
+            for (int e = lane * size; e < (lane + 1) * size; ++e) {
+                const double v = c[e];
+                second = fmax(second, fmin(rank, v));
+                rank = fmax(rank, v);
             }
-            for (int d = 1; d < WAVE; d *= 2) {
-                const double other = over_wave(first, d), behind = over_wave(second, d);
-                second = fmax(fmax(second, behind), fmin(first, other));
-                first = fmax(first, other);
-            }
-            if (lane == g) rank = a.group_top > 1 && second > -__builtin_inf() ? first + second : first;
+            if (a.group_top > 1 && second > none) rank += second;
         }
         int before = 0;
+#pragma unroll 1
         for (int g = 0; g < a.groups; ++g) {
             const uint64_t b = __double_as_longlong(rank);
             const double other = __longlong_as_double((long long)((uint64_t)(uint32_t)__shfl((int)(uint32_t)(b >> 32), g, WAVE) << 32 | (uint32_t)__shfl((int)(uint32_t)b, g, WAVE)));
             before += other > rank || (other == rank && g < lane);
         }
         const uint64_t kept = __ballot(lane < a.groups && before < a.top_groups);
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int e = lane + i * WAVE;
-            if (e < a.experts && !(kept >> (e / size) & 1)) c[i] = -__builtin_inf();
-        }
+#pragma unroll 1
+        for (int e = lane; e < a.experts; e += WAVE)
+            if (!(kept >> (e / size) & 1)) c[e] = none;
     }
-    if (!a.bias) {                                                           // the choice is by logits
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int e = lane + i * WAVE;
-            if (e < a.experts && c[i] > -__builtin_inf()) c[i] = logit_at(a, token, e);
-        }
+    if (!a.bias && !a.by_logits) {                                           // the choice is by logits
+#pragma unroll 1
+        for (int e = lane; e < a.experts; e += WAVE)
+            if (c[e] > none) c[e] = logit_at(e);
     }
+#pragma unroll 1
     for (int j = 0; j < a.top_k; ++j) {
-        double best = -__builtin_inf();
+        double best = none;
         int at = MOST_EXPERTS;
-#pragma unroll
-        for (int i = 0; i < EACH; ++i)
-            if (c[i] > best) {
-                best = c[i];
-                at = lane + i * WAVE;
-            }
+#pragma unroll 1
+        for (int e = lane; e < a.experts; e += WAVE) {
+            const double v = c[e];
+            at = v > best ? e : at;
+            best = fmax(best, v);
+        }
+#pragma unroll 1
         for (int d = 1; d < WAVE; d *= 2) {
             const double other = over_wave(best, d);
             const int there = __shfl_xor(at, d, WAVE);
-            if (other > best || (other == best && there < at)) {
-                best = other;
-                at = there;
-            }
+            at = other > best || (other == best && there < at) ? there : at;
+            best = fmax(best, other);
         }
-#pragma unroll
-        for (int i = 0; i < EACH; ++i)
-            if (lane + i * WAVE == at) c[i] = -__builtin_inf();
         if (lane == 0) {
-            chosen[j] = at < MOST_EXPERTS ? at : -1;
-            values[j] = at < MOST_EXPERTS ? logit_at(a, token, at) : 0.0f;
+            if (at < MOST_EXPERTS) c[at] = none;
+            a.chosen[j] = at < MOST_EXPERTS ? at : -1;
+            a.values[j] = at < MOST_EXPERTS ? logit_at(at) : 0.0f;
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
+}
+
+// Batcher's network of comparisons, largest first
+template <int N> __device__ __forceinline__ void sort_down(uint32_t (&v)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const uint32_t a = v[i + j], b = v[i + j + k];
+                        v[i + j] = a > b ? a : b;
+                        v[i + j + k] = a > b ? b : a;
+                    }
+}
+// Of a wavefront's votes the first lane, counted within its row, that said yes in the row of this lane
+template <int LANES> __device__ __forceinline__ int first_lane(uint64_t votes) {
+    if constexpr (LANES == 64) return __ffsll((long long)votes) - 1;
+    const int shift = (int)(threadIdx.x % 64) / LANES * LANES;
+    uint32_t half = shift >= 32 ? (uint32_t)(votes >> 32) : (uint32_t)votes;
+    if constexpr (LANES < 32) half = half >> (shift % 32) & ((1u << (LANES % 32)) - 1u);
+    return __ffs((int)half) - 1;
 }
 
 // The runs of experts that a row's choice is open to, of values v (-inf: not there) in the row's part of `keys`; `ranks`: [2 groups]. In each lane whether that of value i is;
@@ -284,11 +315,14 @@ template <int LANES, int VALUES> __device__ __forceinline__ void open_groups(con
         if (t * LANES + lane < a.groups) ranks[2 * (t * LANES + lane)] = kept[t];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const float each = 1.0f / (float)size;
+    const float each = 1.0f / (float)size;                                   // e / size by its reciprocal: e below 1024, half an expert from a border
+    auto kept_at = [&](int e) { return e < a.experts && ranks[2 * (int)(((float)e + 0.5f) * each)] != 0.0f; };
+    if (size % 4 == 0) {                                                     // four experts that follow each other are of one run
 #pragma unroll
-    for (int i = 0; i < VALUES; ++i) {                                       // e / size by its reciprocal: e below 1024, half a run from a border
-        const int e = expert_of<LANES>(i, lane);
-        open[i] = e < a.experts && ranks[2 * (int)(((float)e + 0.5f) * each)] != 0.0f;
+        for (int i = 0; i < VALUES; i += 4) open[i] = open[i + 1] = open[i + 2] = open[i + 3] = kept_at(expert_of<LANES>(i, lane));
+    } else {
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) open[i] = kept_at(expert_of<LANES>(i, lane));
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -438,21 +472,22 @@ template <int VALUES> __host__ __device__ constexpr int threads_of() { return VA
 template <int LANES, int VALUES> __host__ __device__ constexpr int stage_of() { return threads_of<VALUES>() / LANES > STAGE ? threads_of<VALUES>() / LANES : STAGE; }
 
 // A steered choice has besides, for each wavefront, the values of its rows and the ranks of their runs of experts.
-constexpr int STEERED_THREADS = 512;
 template <int LANES, int VALUES> __host__ __device__ constexpr int ranks_of() { return 2 * (64 / LANES) * (LANES * VALUES < MOST_GROUPS ? LANES * VALUES : MOST_GROUPS); }
+// Values of a wavefront's rows: a float for each expert of each; room for a row of doubles at least
+template <int LANES, int VALUES> __host__ __device__ constexpr int keys_of() { return 64 * VALUES > 2 * LANES * VALUES ? 64 * VALUES : 2 * LANES * VALUES; }
 __host__ __device__ constexpr size_t up_to_16(size_t words) { return (words + 3) / 4 * 4; }
 
 template <int LANES, int VALUES> size_t choose_lds(int experts, int top_k, bool given, bool steered) {
     const size_t rows = stage_of<LANES, VALUES>();
     size_t choice = given ? 0 : (size_t)experts * (rows / 32) + 2 * rows * top_k + rows;
-    if (steered) choice = up_to_16(choice) + STEERED_THREADS / 64 * (64 * VALUES + ranks_of<LANES, VALUES>());
+    if (steered) choice = up_to_16(choice) + threads_of<VALUES>() / 64 * (keys_of<LANES, VALUES>() + ranks_of<LANES, VALUES>());
     const size_t sums = (size_t)(threads_of<VALUES>() / 64) * experts;
     return 4 * (8 * (size_t)quads_of(experts) + (choice > sums ? choice : sums));
 }
 
-enum { CHOOSE = 0, GIVEN_CHOICE = 1, STEERED_CHOICE = 2 };
-template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bounds__(MODE == STEERED_CHOICE ? STEERED_THREADS : threads_of<VALUES>()) void choose_kernel(RouteArgs a) {
-    constexpr bool GIVEN = MODE == GIVEN_CHOICE, STEERED = MODE == STEERED_CHOICE;
+enum { CHOOSE = 0, GIVEN_CHOICE = 1, GROUPED_CHOICE = 2, BIASED_CHOICE = 3 };
+template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bounds__(threads_of<VALUES>()) void choose_kernel(RouteArgs a) {
+    constexpr bool GIVEN = MODE == GIVEN_CHOICE, BIASED = MODE == BIASED_CHOICE, STEERED = BIASED || MODE == GROUPED_CHOICE;
     extern __shared__ int lds[];
     __shared__ int counted_tokens;
     __shared__ float2 slots[2][16];
@@ -468,12 +503,16 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
     const bool alone = a.blocks == 1;                                        // then there is one portion of one stage, and nothing to leave behind
     float *keys = nullptr, *ranks = nullptr;                                 // of the wavefront
-    float bias[STEERED ? VALUES : 1];
+    __shared__ __attribute__((aligned(16))) float bias[BIASED ? LANES * VALUES : 4];
+    constexpr int AGAIN = STEERED ? STAGED : 1;
+    __shared__ int again, again_row[AGAIN];
+    __shared__ float2 again_stat[AGAIN];
     if constexpr (STEERED) {
-        keys = reinterpret_cast<float*>(rest) + up_to_16(a.experts * WORDS + 2 * STAGED * a.top_k + STAGED) + threadIdx.x / 64 * (64 * VALUES + ranks_of<LANES, VALUES>());
-        ranks = keys + 64 * VALUES;
-#pragma unroll
-        for (int i = 0; i < VALUES; ++i) bias[i] = a.bias && expert_of<LANES>(i, lane) < a.experts ? a.bias[expert_of<LANES>(i, lane)] : 0.0f;
+        keys = reinterpret_cast<float*>(rest) + up_to_16(a.experts * WORDS + 2 * STAGED * a.top_k + STAGED) + threadIdx.x / 64 * (keys_of<LANES, VALUES>() + ranks_of<LANES, VALUES>());
+        ranks = keys + keys_of<LANES, VALUES>();
+        if (threadIdx.x == 0) again = 0;
+        if constexpr (BIASED)
+            for (int e = threadIdx.x; e < LANES * VALUES; e += threads) bias[e] = e < a.experts ? a.bias[e] : 0.0f;
     }
     for (int e = threadIdx.x; e < 4 * quads; e += threads) counts[e] = start[e] = 0;
     const int64_t last = (blockIdx.x + 1) * a.per_block < a.portions ? (blockIdx.x + 1) * a.per_block : a.portions;
@@ -539,74 +578,90 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                             if (e >= 0 && e < a.experts) atomicAdd(&counts[e], 1);
                         }
                 } else if constexpr (STEERED) {
-                    const int in_wave = slot % (64 / LANES);
+                    // (addresses are formed anew for each row: kept from row to row they take the registers that the kernel has not)
+                    int lane = (int)threadIdx.x % LANES, in_wave = slot % (64 / LANES);
+                    asm volatile("" : "+v"(lane), "+v"(in_wave));
                     // a row whose scores are no numbers is chosen by its logits alone
                     const bool odd = best == 0xffffffffu || (!SIGMOID && m == __builtin_inff());
-                    const float largest = SIGMOID ? sigmoid_of(m) : inverse;
+                    const float largest = SIGMOID ? exp_of(fminf(m, 0.0f)) : inverse;    // s = u times this, which is at least the row's largest s
+                    float* mine = keys + in_wave * LANES * VALUES;
                     float c[VALUES];
+                    bool near = false, open[VALUES];
 #pragma unroll
                     for (int i = 0; i < VALUES; ++i) {
-                        c[i] = (SIGMOID ? sigmoid_of(l[i]) : u[i] * inverse) + bias[i];
+                        c[i] = u[i] * largest + (BIASED ? bias[expert_of<LANES>(i, lane)] : 0.0f);
                         c[i] = key[i] && c[i] > -__builtin_inff() ? c[i] : -__builtin_inff();
-                        if (!odd && a.bias) key[i] = c[i] > -__builtin_inff() ? key_of(c[i]) : 0;
+                        if (!BIASED && a.group_top == 1) c[i] = l[i];        // ranks of single experts, exactly
+                        open[i] = true;
                     }
-                    bool near = false;
-                    if (a.groups > 1) {
-                        const bool inexact = a.bias || a.group_top > 1;
-                        if (!inexact) {
+                    if (!BIASED || a.groups > 1) {
+                        open_groups<LANES, VALUES>(a, c, lane, mine, ranks + in_wave * (ranks_of<LANES, VALUES>() / (64 / LANES)), 4.0f * largest, NEAR<SIGMOID>, open, near);
+                        near = near && (BIASED || a.group_top > 1);
+                    }
+                    if constexpr (BIASED) {
+                        // Keys give their last bits to say which of the lane's values they are of, are sorted within the lane, and each choice is the largest head, which its
+                        // lane takes off its list. (Of 256 experts 38 operations to sort and some 35 for a choice, which otherwise takes 80.)
+                        constexpr uint32_t LAST = VALUES - 1;
+                        constexpr float CUT = VALUES * 0x1p-23f;             // of a key without its last bits
 #pragma unroll
-                            for (int i = 0; i < VALUES; ++i) c[i] = l[i];
+                        for (int i = 0; i < VALUES; ++i) key[i] = open[i] && c[i] > -__builtin_inff() ? (key_of(c[i]) & ~LAST) | (LAST - i) : 0;
+                        sort_down(key);
+                        float before = 0.0f;
+                        const int picks = a.top_k < a.experts ? a.top_k + 1 : a.top_k;       // the next one is compared too
+                        for (int j = 0; j < picks; ++j) {
+                            const uint32_t head = lanes_max<LANES>(key[0]);
+                            const float v = value_of(head);
+                            // (infinite biases tie: their order is the exact one's too)
+                            near = near || head >= 0xff800000u || (j && head && before - v <= (NEAR<SIGMOID> + CUT) * (fabsf(before) + fabsf(v)) + 2.0f * NEAR<SIGMOID> * largest);
+                            before = v;
+                            if (j == a.top_k) break;
+                            const int owner = first_lane<LANES>(__ballot(key[0] == head));       // of equal heads the row is near
+                            if (lane == owner) {
+                                chosen[row * a.top_k + j] = head ? expert_of<LANES>((int)(LAST - (head & LAST)), lane) : -1;
+#pragma unroll
+                                for (int n = 0; n + 1 < VALUES; ++n) key[n] = key[n + 1];
+                                key[VALUES - 1] = 0;
+                            }
                         }
-                        bool open[VALUES];
-                        open_groups<LANES, VALUES>(a, c, lane, keys + in_wave * LANES * VALUES, ranks + in_wave * (ranks_of<LANES, VALUES>() / (64 / LANES)), 4.0f * largest,
-                                                   NEAR<SIGMOID>, open, near);
-                        near = near && inexact;
+                        near = near || odd;
+#pragma unroll
+                        for (int i = 0; i < VALUES; i += 4) *reinterpret_cast<float4*>(&mine[expert_of<LANES>(i, lane)]) = make_float4(l[i], l[i + 1], l[i + 2], l[i + 3]);
+                    } else {
 #pragma unroll
                         for (int i = 0; i < VALUES; ++i) key[i] = odd || open[i] ? key[i] : 0;
-                    }
-                    float before = 0.0f;
-                    const int picks = a.bias && a.top_k < a.experts ? a.top_k + 1 : a.top_k;    // with a bias the next one is compared too
-                    for (int j = 0; j < picks; ++j) {
-                        best = 0;
+                        near = near && !odd;
+                        for (int j = 0; j < a.top_k; ++j) {
+                            best = 0;
 #pragma unroll
-                        for (int i = 0; i < VALUES; ++i) best = key[i] > best ? key[i] : best;
-                        best = lanes_max<LANES>(best);
-                        if (a.bias && j && best) {
-                            const float v = value_of(best);
-                            near = near || before - v <= NEAR<SIGMOID> * (fabsf(before) + fabsf(v) + 2.0f * largest);
-                        }
-                        before = value_of(best);
-                        if (j == a.top_k) break;
-                        uint32_t first = 0xffffffffu;
+                            for (int i = 0; i < VALUES; ++i) best = key[i] > best ? key[i] : best;
+                            best = lanes_max<LANES>(best);
+                            uint32_t first = 0xffffffffu;
 #pragma unroll
-                        for (int i = VALUES - 1; i >= 0; --i) first = key[i] == best ? (uint32_t)expert_of<LANES>(i, lane) : first;
-                        first = lanes_min<LANES>(first);
-                        float logit = 0.0f;
-                        bool mine = false;
+                            for (int i = VALUES - 1; i >= 0; --i) first = key[i] == best ? (uint32_t)expert_of<LANES>(i, lane) : first;
+                            first = lanes_min<LANES>(first);
 #pragma unroll
-                        for (int i = 0; i < VALUES; ++i)
-                            if (first == (uint32_t)expert_of<LANES>(i, lane)) {
-                                key[i] = 0;
-                                logit = l[i];
-                                mine = true;
+                            for (int i = 0; i < VALUES; ++i) key[i] = first == (uint32_t)expert_of<LANES>(i, lane) ? 0 : key[i];
+                            if (lane == 0) {
+                                chosen[row * a.top_k + j] = best ? (int)first : -1;
+                                values[row * a.top_k + j] = value_of(best);
                             }
-                        if (mine) {                                          // (of a row without any left: some lane's expert, with a key of 0)
-                            chosen[row * a.top_k + j] = best ? (int)first : -1;
-                            values[row * a.top_k + j] = logit;
                         }
                     }
-                    near = near && counted && !odd;
-                    for (uint64_t again = __ballot(near && lane == 0); again; again &= again - 1) {
-                        const int at = __ffsll((long long)again) - 1, there = __shfl(row, at, WAVE);
-                        choose_exactly<(LANES * VALUES + 63) / 64, SIGMOID>(a, base + there, __shfl(m, at, WAVE), chosen + there * a.top_k, values + there * a.top_k);
+                    near = near && counted;
+                    if (near && lane == 0) {
+                        const int at = atomicAdd(&again, 1);
+                        again_row[at] = row;
+                        again_stat[at] = make_float2(m, odd ? -inverse : inverse);
                     }
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     __builtin_amdgcn_wave_barrier();
                     float picked = 0.0f;
-                    if (token < end)
+                    if (token < end && !near)
                         for (int j = lane; j < a.top_k; j += LANES) {
                             const int at = row * a.top_k + j, e = chosen[at];
-                            const float v = values[at], value = !a.normalize && SIGMOID ? sigmoid_of(v) : score<SIGMOID>(v, m);
+                            float v = values[at];
+                            if constexpr (BIASED) v = e >= 0 ? mine[e] : 0.0f;
+                            const float value = !a.normalize && SIGMOID ? sigmoid_of(v) : score<SIGMOID>(v, m);
                             values[at] = value;
                             if (e >= 0) {
                                 picked += value;
@@ -615,6 +670,8 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                         }
                     picked = lanes_sum<LANES>(picked);
                     if (lane == 0) factors[row] = a.scale * (a.normalize ? (counted ? 1.0f / picked : 0.0f) : SIGMOID ? 1.0f : inverse);
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
                 } else {
                     // LANES choices at a time, one left with each lane: its score and its bit are that lane's work
                     float picked = 0.0f;
@@ -652,6 +709,32 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                     picked = lanes_sum<LANES>(picked);
                     if (lane == 0) factors[row] = a.scale * (a.normalize ? (counted ? 1.0f / picked : 0.0f) : SIGMOID ? 1.0f : inverse);
                 }
+            }
+            if constexpr (STEERED) {                                         // rows that 32 bits do not settle, one for a wavefront
+                __syncthreads();
+                for (int n = threadIdx.x / 64; n < again; n += threads / 64) {
+                    const int row = again_row[n], of = threadIdx.x % 64;
+                    const float2 stat = again_stat[n];
+                    const float m = stat.x, inverse = fabsf(stat.y);
+                    const bool odd = stat.y < 0.0f || stat.y != stat.y;
+                    const char* logits = static_cast<const char*>(a.logits) + (base + row) * a.pitch * (a.dtype == VIOLA_F32 ? 4 : 2);
+                    choose_exactly<SIGMOID>({logits, odd ? nullptr : a.bias, a.dtype, a.experts, a.top_k, odd ? 1 : a.groups, a.top_groups, a.group_top, m, odd,
+                                             reinterpret_cast<double*>(keys), chosen + row * a.top_k, values + row * a.top_k});
+                    float picked = 0.0f;
+                    if (of < a.top_k) {
+                        const int at = row * a.top_k + of, e = chosen[at];
+                        const float v = values[at], value = !a.normalize && SIGMOID ? sigmoid_of(v) : score<SIGMOID>(v, m);
+                        values[at] = value;
+                        if (e >= 0) {
+                            picked = value;
+                            atomicOr(&bits[e * WORDS + row / 32], 1u << (row % 32));
+                        }
+                    }
+                    picked = lanes_sum<64>(picked);
+                    if (of == 0) factors[row] = a.scale * (a.normalize ? 1.0f / picked : SIGMOID ? 1.0f : inverse);
+                }
+                __syncthreads();
+                if (threadIdx.x == 0) again = 0;
             }
             if constexpr (!GIVEN) {
                 __syncthreads();
@@ -922,16 +1005,18 @@ void plan(RouteArgs& a) {
     with_shape(a.experts, [&](auto lanes, auto values) {
         lanes_of_row = decltype(lanes)::value;
         a.threads = threads_of<decltype(values)::value>();
-        if (a.groups && a.threads > STEERED_THREADS) a.threads = STEERED_THREADS;
         staged = stage_of<decltype(lanes)::value, decltype(values)::value>();
     });
     // half the threads where blocks of them are fewer than CUs; no more than a sequence's tokens have lanes, two wavefronts at least
     const int64_t used = (a.sequence * lanes_of_row + 127) / 128 * 128;
     if (a.threads == 1024 && a.tokens * lanes_of_row < 1024 * MOST_BLOCKS) a.threads = 512;
+    // a steered choice is some 1500 operations for a wavefront: a few tokens go to as many CUs as two wavefronts each give, though that takes a second launch
+    if (a.groups)
+        while (a.threads > 128 && a.tokens * lanes_of_row <= (int64_t)a.threads / 2 * MOST_BLOCKS) a.threads /= 2;
     if (used < a.threads) a.threads = (int)used;
     rows = a.threads / lanes_of_row;
     const int64_t most = (MOST_BLOCKS + a.sequences - 1) / a.sequences, needed = (a.sequence + rows - 1) / rows;
-    const bool stage = a.sequences == 1 && a.tokens <= staged;                      // one block, one launch
+    const bool stage = a.sequences == 1 && a.tokens <= (a.groups ? rows : staged);  // one block, one launch
     const int64_t cuts = stage || a.sequences >= MOST_BLOCKS ? 1 : most < needed ? most : needed;
     a.chunk = ((a.sequence + cuts - 1) / cuts + rows - 1) / rows * rows;
     a.per_sequence = (a.sequence + a.chunk - 1) / a.chunk;
@@ -977,7 +1062,8 @@ int forward(RouteArgs& a, int32_t* workspace, int64_t words, hipStream_t stream)
             else VIOLA_LAUNCH((choose_kernel<LANES, VALUES, MODE, false>), dim3((unsigned)a.blocks), a.threads, lds, stream, a);
         };
         if (a.given) launch(std::integral_constant<int, GIVEN_CHOICE>());
-        else if (a.groups) launch(std::integral_constant<int, STEERED_CHOICE>());
+        else if (a.bias) launch(std::integral_constant<int, BIASED_CHOICE>());
+        else if (a.groups) launch(std::integral_constant<int, GROUPED_CHOICE>());
         else launch(std::integral_constant<int, CHOOSE>());
     });
     if (a.blocks > 1) VIOLA_LAUNCH(place_kernel, dim3(a.given ? 2 : (unsigned)a.blocks + 1), PLACE_THREADS, 0, stream, a);
