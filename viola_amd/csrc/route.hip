@@ -88,6 +88,14 @@ __device__ __forceinline__ float sigmoid_of(float l) {
     return (l < 0.0f ? t : 1.0f) / (1.0f + t);
 }
 
+// sigmoid(l) within 8 2^-24, without the steps that make a quotient the nearest one
+__device__ __forceinline__ float near_sigmoid(float l) {
+    const float t = exp_of(-fabsf(l)), d = 1.0f + t;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    return (l < 0.0f ? t : 1.0f) * r;
+}
+
 // VALUES logits of a lane: runs of four, LANES runs apart; -inf beyond the experts
 template <int LANES> __device__ __forceinline__ int expert_of(int i, int lane) { return ((i / 4) * LANES + lane) * 4 + i % 4; }
 
@@ -123,11 +131,11 @@ template <int LANES, int VALUES> __device__ __forceinline__ void load_logits(con
 
 // ---------------------------------------------------------------------------------------------------- a steered choice
 // A choice is a whole number, so the order of two scores next to each other has to be the exact one. In 32 bits a score is off by at most
-//   sigmoid  14 2^-24 of the row's largest (u within 8 2^-24: exp_of 2 ulp, sum and quotient half an ulp each, and the rounding of l - m, which is |l - m| 2^-24 u or at
-//            most a third of 2^-24 of the largest; the factor exp(min(m, 0)) 4 2^-24 where it is not one; their product)
+//   sigmoid  14 2^-24 of the row's largest (u within 8 2^-24: exp_of 2 ulp, sum and quotient or reciprocal; where l - m is in it, the rounding of that, which is
+//            |l - m| 2^-24 u or at most a third of 2^-24 of the largest; the factor exp(min(m, 0)) 4 2^-24 where it is not one; their product)
 //   softmax  24 2^-24 of the row's largest (the sum of at most 16 values of 64 lanes besides)
 // and the sum with its bias by 2^-24 of itself. Where two that are told apart lie nearer than NEAR times their magnitudes and the row's largest score,
-// the row is chosen again in 64 bits by the whole wavefront: one row in 150 of 256 experts with sigmoid scores and a bias. Without a bias the choice itself is by
+// the row is chosen again in 64 bits by the whole wavefront: about one row in 150 of 256 experts with sigmoid scores and a bias. Without a bias the choice itself is by
 // logits, as ever, and exact; ranks of single experts are too.
 template <bool SIGMOID> constexpr float NEAR = SIGMOID ? 0x1p-20f : 0x1p-19f;
 constexpr int MOST_GROUPS = 64;
@@ -146,7 +154,7 @@ struct ExactChoice {
     int dtype, experts, top_k, groups, top_groups, group_top;
     float largest;
     bool by_logits;                                                          // a row whose scores are no numbers: NaN above all, then +inf
-    double* c;
+    double *c, *ranks;
     int* chosen;
     float* values;
 };
@@ -155,7 +163,12 @@ template <bool SIGMOID> __device__ __forceinline__ void choose_exactly(const Exa
     asm volatile("" : "+v"(lane));                                           // nothing of this rare path is kept ready for it
     const int size = a.experts / a.groups;
     double* const c = a.c;
+    uint64_t* const key = reinterpret_cast<uint64_t*>(a.c);                  // in the same places: the order of doubles as that of integers, 0 for what is not chosen
     auto logit_at = [&](int e) { return load_float(a.row, e, a.dtype); };
+    auto in_order = [] {                                                     // LDS accesses of a wavefront stay in order
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
     const double none = -__builtin_inf();
     double sum = 0.0;
 #pragma unroll 1
@@ -174,62 +187,57 @@ template <bool SIGMOID> __device__ __forceinline__ void choose_exactly(const Exa
         if (a.bias) v += (double)a.bias[e];
         c[e] = v > none ? v : none;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");                   // LDS accesses of a wavefront stay in order
-    __builtin_amdgcn_wave_barrier();
+    in_order();
+    uint64_t kept = ~uint64_t{0};
     if (a.groups > 1) {
         double rank = none;                                                  // of group `lane`
         if (lane < a.groups) {
             double second = none;
-#pragma unroll 1
+#pragma unroll 4
             for (int e = lane * size; e < (lane + 1) * size; ++e) {
                 const double v = c[e];
                 second = fmax(second, fmin(rank, v));
                 rank = fmax(rank, v);
             }
             if (a.group_top > 1 && second > none) rank += second;
+            a.ranks[lane] = rank;
         }
+        in_order();
         int before = 0;
-#pragma unroll 1
+#pragma unroll 4
         for (int g = 0; g < a.groups; ++g) {
-            const uint64_t b = __double_as_longlong(rank);
-            const double other = __longlong_as_double((long long)((uint64_t)(uint32_t)__shfl((int)(uint32_t)(b >> 32), g, WAVE) << 32 | (uint32_t)__shfl((int)(uint32_t)b, g, WAVE)));
+            const double other = a.ranks[g];
             before += other > rank || (other == rank && g < lane);
         }
-        const uint64_t kept = __ballot(lane < a.groups && before < a.top_groups);
-#pragma unroll 1
-        for (int e = lane; e < a.experts; e += WAVE)
-            if (!(kept >> (e / size) & 1)) c[e] = none;
+        kept = __ballot(lane < a.groups && before < a.top_groups);
     }
-    if (!a.bias && !a.by_logits) {                                           // the choice is by logits
 #pragma unroll 1
-        for (int e = lane; e < a.experts; e += WAVE)
-            if (c[e] > none) c[e] = logit_at(e);
+    for (int e = lane; e < a.experts; e += WAVE) {
+        double v = c[e];
+        const bool there = v > none && (a.groups == 1 || (kept >> (e / size) & 1));
+        if (!a.bias && !a.by_logits) v = logit_at(e);                        // the choice among them is by logits
+        const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+        key[e] = !there ? 0 : b >> 63 ? ~b : b | uint64_t{1} << 63;
     }
 #pragma unroll 1
     for (int j = 0; j < a.top_k; ++j) {
-        double best = none;
+        uint64_t best = 0;
         int at = MOST_EXPERTS;
-#pragma unroll 1
+#pragma unroll 4
         for (int e = lane; e < a.experts; e += WAVE) {
-            const double v = c[e];
+            const uint64_t v = key[e];
             at = v > best ? e : at;
-            best = fmax(best, v);
+            best = v > best ? v : best;
         }
-#pragma unroll 1
-        for (int d = 1; d < WAVE; d *= 2) {
-            const double other = over_wave(best, d);
-            const int there = __shfl_xor(at, d, WAVE);
-            at = other > best || (other == best && there < at) ? there : at;
-            best = fmax(best, other);
+        const uint32_t high = lanes_max<64>((uint32_t)(best >> 32)), low = lanes_max<64>((uint32_t)(best >> 32) == high ? (uint32_t)best : 0);
+        const int first = (int)lanes_min<64>(best && best == ((uint64_t)high << 32 | low) ? at : MOST_EXPERTS);
+        if (lane == first % WAVE) {                                          // its own lane, or of none lane 0
+            if (first < MOST_EXPERTS) key[first] = 0;
+            a.chosen[j] = first < MOST_EXPERTS ? first : -1;
+            a.values[j] = first < MOST_EXPERTS ? logit_at(first) : 0.0f;
         }
-        if (lane == 0) {
-            if (at < MOST_EXPERTS) c[at] = none;
-            a.chosen[j] = at < MOST_EXPERTS ? at : -1;
-            a.values[j] = at < MOST_EXPERTS ? logit_at(at) : 0.0f;
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     }
+    in_order();
 }
 
 // Batcher's network of comparisons, largest first
@@ -556,18 +564,31 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                 const bool counted = best != 0;
                 const float m = value_of(best);
                 float u[VALUES], all = 0.0f;
+                // A steered choice needs sigmoids themselves: unless a row of the wavefront lies so far below zero that they vanish, u is those, unit what s is u times
+                const bool near_zero = STEERED && SIGMOID && !__any(counted && !(m > -60.0f));
+                float unit = 1.0f;
+                if (near_zero) {
 #pragma unroll
-                for (int i = 0; i < VALUES; ++i) {
-                    u[i] = score<SIGMOID>(l[i], m);
-                    u[i] = counted ? u[i] : 0.0f;
-                    all += u[i];
+                    for (int i = 0; i < VALUES; ++i) {
+                        u[i] = near_sigmoid(l[i]);
+                        u[i] = counted ? u[i] : 0.0f;
+                        all += u[i];
+                    }
+                } else {
+                    if constexpr (STEERED) unit = exp_of(fminf(m, 0.0f));
+#pragma unroll
+                    for (int i = 0; i < VALUES; ++i) {
+                        u[i] = score<SIGMOID>(l[i], m);
+                        u[i] = counted ? u[i] : 0.0f;
+                        all += u[i];
+                    }
                 }
                 all = lanes_sum<LANES>(all);
                 const float inverse = counted ? 1.0f / all : 0.0f;
 #pragma unroll
                 for (int i = 0; i < VALUES; ++i) sum[i] = fmaf(u[i], inverse, sum[i]);
                 if (lane == 0 && token < end) {
-                    if (a.stats) a.stats[token] = make_float2(counted ? m : 0.0f, inverse);
+                    if (a.stats) a.stats[token] = make_float2(counted ? m : 0.0f, near_zero ? inverse * exp_of(fminf(m, 0.0f)) : inverse);
                 }
                 here += __popcll(__ballot(lane == 0 && counted));
                 if constexpr (GIVEN) {
@@ -583,13 +604,14 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                     asm volatile("" : "+v"(lane), "+v"(in_wave));
                     // a row whose scores are no numbers is chosen by its logits alone
                     const bool odd = best == 0xffffffffu || (!SIGMOID && m == __builtin_inff());
-                    const float largest = SIGMOID ? exp_of(fminf(m, 0.0f)) : inverse;    // s = u times this, which is at least the row's largest s
+                    if constexpr (!SIGMOID) unit = inverse;
+                    const float largest = SIGMOID ? exp_of(fminf(m, 0.0f)) : inverse;    // at least the row's largest s
                     float* mine = keys + in_wave * LANES * VALUES;
                     float c[VALUES];
                     bool near = false, open[VALUES];
 #pragma unroll
                     for (int i = 0; i < VALUES; ++i) {
-                        c[i] = u[i] * largest + (BIASED ? bias[expert_of<LANES>(i, lane)] : 0.0f);
+                        c[i] = u[i] * unit + (BIASED ? bias[expert_of<LANES>(i, lane)] : 0.0f);
                         c[i] = key[i] && c[i] > -__builtin_inff() ? c[i] : -__builtin_inff();
                         if (!BIASED && a.group_top == 1) c[i] = l[i];        // ranks of single experts, exactly
                         open[i] = true;
@@ -612,7 +634,7 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                             const uint32_t head = lanes_max<LANES>(key[0]);
                             const float v = value_of(head);
                             // (infinite biases tie: their order is the exact one's too)
-                            near = near || head >= 0xff800000u || (j && head && before - v <= (NEAR<SIGMOID> + CUT) * (fabsf(before) + fabsf(v)) + 2.0f * NEAR<SIGMOID> * largest);
+                            near = near || head >= 0xff800000u || (j && head && before - v <= (0x1p-24f + CUT) * (fabsf(before) + fabsf(v)) + 2.0f * NEAR<SIGMOID> * largest);
                             before = v;
                             if (j == a.top_k) break;
                             const int owner = first_lane<LANES>(__ballot(key[0] == head));       // of equal heads the row is near
@@ -719,7 +741,7 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                     const bool odd = stat.y < 0.0f || stat.y != stat.y;
                     const char* logits = static_cast<const char*>(a.logits) + (base + row) * a.pitch * (a.dtype == VIOLA_F32 ? 4 : 2);
                     choose_exactly<SIGMOID>({logits, odd ? nullptr : a.bias, a.dtype, a.experts, a.top_k, odd ? 1 : a.groups, a.top_groups, a.group_top, m, odd,
-                                             reinterpret_cast<double*>(keys), chosen + row * a.top_k, values + row * a.top_k});
+                                             reinterpret_cast<double*>(keys), reinterpret_cast<double*>(ranks), chosen + row * a.top_k, values + row * a.top_k});
                     float picked = 0.0f;
                     if (of < a.top_k) {
                         const int at = row * a.top_k + of, e = chosen[at];
