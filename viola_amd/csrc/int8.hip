@@ -7,7 +7,7 @@
 // A row of zeros has s = 0 and zeros; a row that holds an Inf or a NaN has s = NaN and zeros, so a product makes all of it NaN and no other row. Where s is
 // subnormal the quotient may pass 127 and is cut off there.
 //
-// The integer is that of the exact quotient: v times the reciprocal is within 2^-14 of it, which settles all but the neighbourhood of a half; there the
+// The integer is that of the exact quotient: v times the reciprocal is within 2^-17 of it (127 times half a last place), which settles all but 2 10^-5 around a half; there the
 // residual v - q s, one fused operation without error where it is near s / 2 (s and v are multiples of the smaller one's last place, which the result has
 // 24 bits of), is compared with s / 2.
 //
@@ -26,7 +26,7 @@ enum { PLAIN = 0, GATED = 1, SCALED = 2 };                                   // 
 struct QuantizeArgs {
     const void* x;
     int64_t pitch, rows;                                                     // pitch in values
-    int cols, activation, groups, whole;                                     // whole: x can be read eight values at a time
+    int cols, activation, groups;
     const float* factors;                                                    // SCALED: [groups][cols]
     const int* offsets;                                                      // SCALED: where the rows of each group begin; null: one group
     int8_t* codes;
@@ -34,7 +34,6 @@ struct QuantizeArgs {
     float* scales;
     float* partial;                                                          // SCALED: [parts][cols] sums of x, null: not wanted
     int64_t per_block;                                                       // rows
-    bool stream_in;
 };
 
 // The group whose rows `row` is among (the last one for rows behind all of them, which no product reads).
@@ -48,77 +47,128 @@ __device__ __forceinline__ int group_of(const int* offsets, int groups, int64_t 
     return low;
 }
 
-// What is quantized of a piece, of columns c to c + 7; raw: x itself
-template <typename T, int MODE>
-__device__ __forceinline__ void value8(const QuantizeArgs& a, const T* row, const float* factors, int c, float (&v)[8], float (&raw)[8]) {
-    load8<T>(row, c, a.cols, a.whole, a.stream_in, v);
+// What is quantized of columns c to c + 7
+template <typename T, int MODE> __device__ __forceinline__ void value8(const QuantizeArgs& a, const T* row, int c, float (&v)[8]) {
+    load8<T>(row, c, a.cols, v);
     if constexpr (MODE == GATED) {
         float u[8];
-        load8<T>(row + a.cols, c, a.cols, a.whole, a.stream_in, u);
+        load8<T>(row + a.cols, c, a.cols, u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float act, derivative;
             gate_math(a.activation, v[i], act, derivative);
             v[i] = act * u[i];
         }
-    } else if constexpr (MODE == SCALED) {
-        float f[8];
-        load8<float>(factors, c, a.cols, a.cols % 4 == 0, false, f);         // rows of whole 16 bytes
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            raw[i] = v[i];
-            v[i] *= f[i];
-        }
     }
 }
 
 constexpr int threads_of(int waves) { return waves <= 4 ? 256 : 64 * waves; }
 
-// A row of WAVES wavefronts, PIECES pieces of eight values a thread. SCALED: a block goes through per_block rows and leaves the sums of x
-// over those of each of its rows of threads.
+// The largest magnitude of a row of WAVES wavefronts, in all of them: two sets of slots in turn, so one barrier a row is enough
+template <int WAVES> __device__ __forceinline__ uint32_t over_row(uint32_t most, uint32_t (*slots)[threads_of(WAVES) / 64], int& turn) {
+    most = lanes_max<64>(most);
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x % 64 == 0) slots[turn][threadIdx.x / 64] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const uint32_t other = slots[turn][threadIdx.x / 64 / WAVES * WAVES + w];
+            most = other > most ? other : most;
+        }
+        turn ^= 1;
+    }
+    return most;
+}
+
+// A row of WAVES wavefronts, PIECES pieces of eight values a thread.
 template <typename T, int MODE, int WAVES, int PIECES> __global__ __launch_bounds__(threads_of(WAVES)) void quantize_rows(QuantizeArgs a) {
     constexpr int THREADS = 64 * WAVES, TOGETHER = threads_of(WAVES) / THREADS;
-    __shared__ uint32_t most_of[2][threads_of(WAVES) / 64];
-    const int t = threadIdx.x % THREADS, slot = threadIdx.x / THREADS, wave = threadIdx.x / 64;
+    __shared__ uint32_t slots[2][threads_of(WAVES) / 64];
+    const int t = threadIdx.x % THREADS;
+    const int64_t row = (int64_t)blockIdx.x * TOGETHER + threadIdx.x / THREADS;
+    const bool here = row < a.rows;
+    float v[PIECES][8];
+    uint32_t most = 0;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int c = (p * THREADS + t) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
+        if (!here || c >= a.cols) continue;
+        value8<T, MODE>(a, static_cast<const T*>(a.x) + row * a.pitch, c, v[p]);
+        most = magnitudes(v[p], most);
+    }
+    int turn = 0;
+    most = over_row<WAVES>(most, slots, turn);
+    if (!here) return;
+    const RowScale scale(most);
+    if (t == 0) a.scales[row] = scale.s;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int c = (p * THREADS + t) * 8;
+        if (c < a.code_pitch) *reinterpret_cast<uint2*>(a.codes + row * a.code_pitch + c) = encode8_int(v[p], scale);
+    }
+}
+
+// x times factors: a block goes through per_block rows, the next one's loads under the work on each, with the factors of their group in registers, and leaves the sums
+// of x over its rows (SUMS).
+template <typename T, int WAVES, int PIECES, bool SUMS> __global__ __launch_bounds__(threads_of(WAVES)) void quantize_scaled_rows(QuantizeArgs a) {
+    constexpr int THREADS = 64 * WAVES, TOGETHER = threads_of(WAVES) / THREADS;
+    __shared__ uint32_t slots[2][threads_of(WAVES) / 64];
+    __shared__ __attribute__((aligned(16))) float others[SUMS && TOGETHER > 1 ? (TOGETHER - 1) * PIECES * THREADS * 8 : 4];
+    const int t = threadIdx.x % THREADS, slot = threadIdx.x / THREADS;
     const int64_t first = blockIdx.x * a.per_block, end = first + a.per_block < a.rows ? first + a.per_block : a.rows;
-    float sums[MODE == SCALED ? PIECES : 1][8];
-    if constexpr (MODE == SCALED)
+    float sums[SUMS ? PIECES : 1][8], factor[PIECES][8];
+    Raw8<T> next[PIECES];
+    if constexpr (SUMS)
 #pragma unroll
         for (int p = 0; p < PIECES; ++p)
 #pragma unroll
             for (int i = 0; i < 8; ++i) sums[p][i] = 0.0f;
-    int turn = 0;
-    for (int64_t row = first + slot; row - slot < end; row += TOGETHER) {
-        const bool here = row < end;
-        const T* x = static_cast<const T*>(a.x) + row * a.pitch;
-        const float* factors = a.factors;
-        if (MODE == SCALED && a.offsets && here) factors += (int64_t)group_of(a.offsets, a.groups, row) * a.cols;
-        float v[PIECES][8];
-        uint32_t most = 0;
+    auto load = [&](int64_t row) {                                           // (past the end: the last row once more)
+        const T* x = static_cast<const T*>(a.x) + (row < end ? row : end - 1) * a.pitch;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * THREADS + t) * 8;
+            if (c < a.cols) next[p].load(x, c, a.cols);
+        }
+    };
+    auto load_factors = [&](const float* factors) {
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int c = (p * THREADS + t) * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
-            if (!here || c >= a.cols) continue;
-            float raw[8];
-            value8<T, MODE>(a, x, factors, c, v[p], raw);
+            for (int i = 0; i < 8; ++i) factor[p][i] = 0.0f;
+            if (c < a.cols) load8<float>(factors, c, a.cols, factor[p]);
+        }
+    };
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) next[p].clear();
+    load(first + slot);
+    if (!a.offsets) load_factors(a.factors);
+    int64_t until = -1;                                                      // rows that the factors are for
+    int turn = 0;
+    for (int64_t row = first + slot; row - slot < end; row += TOGETHER) {
+        const bool here = row < end;
+        if (a.offsets && here && row >= until) {                             // (one row for a wavefront or more: no lane of it goes another way)
+            const int g = group_of(a.offsets, a.groups, row);
+            until = g + 1 < a.groups ? a.offsets[g + 1] : a.rows;
+            load_factors(a.factors + (int64_t)g * a.cols);
+        }
+        float v[PIECES][8];
+        uint32_t most = 0;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            next[p].widen(v[p]);
+            if (SUMS && here)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sums[p][i] += v[p][i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[p][i] *= factor[p][i];
             most = magnitudes(v[p], most);
-            if constexpr (MODE == SCALED)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sums[p][i] += raw[i];
         }
-        most = lanes_max<64>(most);
-        if constexpr (WAVES > 1) {                                           // two sets of slots in turn: one barrier a row
-            if (threadIdx.x % 64 == 0) most_of[turn][wave] = most;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                const uint32_t other = most_of[turn][slot * WAVES + w];
-                most = other > most ? other : most;
-            }
-            turn ^= 1;
-        }
+        load(row + TOGETHER);
+        most = over_row<WAVES>(most, slots, turn);
         if (!here) continue;
         const RowScale scale(most);
         if (t == 0) a.scales[row] = scale.s;
@@ -128,9 +178,28 @@ template <typename T, int MODE, int WAVES, int PIECES> __global__ __launch_bound
             if (c < a.code_pitch) *reinterpret_cast<uint2*>(a.codes + row * a.code_pitch + c) = encode8_int(v[p], scale);
         }
     }
-    if constexpr (MODE == SCALED) {
-        if (!a.partial) return;
-        float* to = a.partial + (int64_t)(blockIdx.x * TOGETHER + slot) * a.cols;
+    if constexpr (SUMS) {                                                    // the rows of threads of a block in order
+        if constexpr (TOGETHER > 1) {
+            if (slot)
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4)
+                        *reinterpret_cast<float4*>(&others[((slot - 1) * PIECES + p) * THREADS * 8 + t * 4 + i * THREADS]) =
+                            make_float4(sums[p][i], sums[p][i + 1], sums[p][i + 2], sums[p][i + 3]);
+            __syncthreads();
+            if (slot) return;
+#pragma unroll
+            for (int s = 0; s < TOGETHER - 1; ++s)
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        const float4 more = *reinterpret_cast<const float4*>(&others[(s * PIECES + p) * THREADS * 8 + t * 4 + i * THREADS]);
+                        sums[p][i] += more.x; sums[p][i + 1] += more.y; sums[p][i + 2] += more.z; sums[p][i + 3] += more.w;
+                    }
+        }
+        float* to = a.partial + (int64_t)blockIdx.x * a.cols;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int c = (p * THREADS + t) * 8;
@@ -149,13 +218,24 @@ template <typename T, int MODE> __global__ __launch_bounds__(512) void quantize_
     const int t = threadIdx.x;
     const int64_t first = (int64_t)blockIdx.x * LONG_ROWS, left = a.rows - first;
     const int rows = left < LONG_ROWS ? (int)left : LONG_ROWS;
-    auto factors_of = [&](int64_t row) { return MODE == SCALED && a.offsets ? a.factors + (int64_t)group_of(a.offsets, a.groups, row) * a.cols : a.factors; };
+    auto value = [&](int r, int c, float (&v)[8], float (&raw)[8]) {
+        value8<T, MODE>(a, static_cast<const T*>(a.x) + (first + r) * a.pitch, c, v);
+        if constexpr (MODE == SCALED) {
+            const float* factors = a.offsets ? a.factors + (int64_t)group_of(a.offsets, a.groups, first + r) * a.cols : a.factors;
+            float f[8];
+            load8<float>(factors, c, a.cols, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                raw[i] = v[i];
+                v[i] *= f[i];
+            }
+        }
+    };
     for (int r = 0; r < rows; ++r) {
-        const float* factors = factors_of(first + r);
         uint32_t most = 0;
         for (int c = t * 8; c < a.cols; c += 512 * 8) {
             float v[8], raw[8];
-            value8<T, MODE>(a, static_cast<const T*>(a.x) + (first + r) * a.pitch, factors, c, v, raw);
+            value(r, c, v, raw);
             most = magnitudes(v, most);
         }
         most = lanes_max<64>(most);
@@ -171,7 +251,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(512) void quantize_
             const RowScale scale(most);
             if (c == 0) a.scales[first + r] = scale.s;
             float v[8] = {}, raw[8] = {};
-            if (c < a.cols) value8<T, MODE>(a, static_cast<const T*>(a.x) + (first + r) * a.pitch, factors_of(first + r), c, v, raw);
+            if (c < a.cols) value(r, c, v, raw);
             *reinterpret_cast<uint2*>(a.codes + (first + r) * a.code_pitch + c) = encode8_int(v, scale);
             if constexpr (MODE == SCALED)
 #pragma unroll
@@ -184,39 +264,40 @@ template <typename T, int MODE> __global__ __launch_bounds__(512) void quantize_
     }
 }
 
-// How rows are shared: wavefronts of a row, rows of a block, blocks, and rows of sums that they leave.
+// How rows are shared: wavefronts of a row, rows of a block (SCALED: as many as leave SCALED_BLOCKS), blocks.
 struct Shares {
     int waves, pieces;                                                       // 0 wavefronts: long rows
-    int64_t per_block, blocks, parts;
+    int64_t per_block, blocks;
 };
-Shares shares_of(int64_t rows, int64_t cols, bool sums) {
+#ifndef SB
+#define SB 1024
+#endif
+constexpr int64_t SCALED_BLOCKS = SB;
+Shares shares_of(int64_t rows, int64_t cols, bool scaled) {
     Shares s = {};
     if (cols > 16384) {
         s.per_block = LONG_ROWS;
-        s.blocks = (rows + LONG_ROWS - 1) / LONG_ROWS;
-        s.parts = s.blocks;
-        return s;
+    } else {
+        s.waves = cols <= 2048 ? 1 : cols <= 8192 ? 4 : 8;
+        const int64_t piece = 512 * s.waves;                                 // values that the row's threads have at once
+        s.pieces = cols <= piece ? 1 : cols <= 2 * piece ? 2 : 4;
+        s.per_block = s.waves == 1 ? 4 : 1;
+        if (scaled && rows > SCALED_BLOCKS * s.per_block) s.per_block *= (rows + SCALED_BLOCKS * s.per_block - 1) / (SCALED_BLOCKS * s.per_block);
     }
-    s.waves = cols <= 2048 ? 1 : cols <= 8192 ? 4 : 8;
-    const int64_t piece = 512 * s.waves;                                     // values that the row's threads have at once
-    s.pieces = cols <= piece ? 1 : cols <= 2 * piece ? 2 : 4;
-    const int64_t together = s.waves == 1 ? 4 : 1;
-    // sums: four blocks for each CU at most, a row of sums from each of a block's rows of threads
-    s.per_block = together;
-    if (sums && rows > 1024 * together) s.per_block = (rows + 1024 * together - 1) / (1024 * together) * together;
     s.blocks = (rows + s.per_block - 1) / s.per_block;
-    s.parts = s.blocks * together;
     return s;
 }
 
 template <typename T, int MODE> int launch(QuantizeArgs& a, hipStream_t stream) {
-    const Shares s = shares_of(a.rows, a.cols, a.partial != nullptr);
+    const Shares s = shares_of(a.rows, a.cols, MODE == SCALED);
     a.per_block = s.per_block;
     if (s.blocks >= (int64_t{1} << 31)) return VIOLA_ETOOLARGE;
     const dim3 grid((unsigned)s.blocks);
     auto with = [&](auto waves, auto pieces) {
         constexpr int WAVES = decltype(waves)::value, PIECES = decltype(pieces)::value;
-        VIOLA_LAUNCH((quantize_rows<T, MODE, WAVES, PIECES>), grid, threads_of(WAVES), 0, stream, a);
+        if constexpr (MODE != SCALED) VIOLA_LAUNCH((quantize_rows<T, MODE, WAVES, PIECES>), grid, threads_of(WAVES), 0, stream, a);
+        else if (a.partial) VIOLA_LAUNCH((quantize_scaled_rows<T, WAVES, PIECES, true>), grid, threads_of(WAVES), 0, stream, a);
+        else VIOLA_LAUNCH((quantize_scaled_rows<T, WAVES, PIECES, false>), grid, threads_of(WAVES), 0, stream, a);
     };
     using std::integral_constant;
     const int key = s.waves * 8 + s.pieces;
@@ -241,7 +322,7 @@ struct GatedGradientArgs {
     void* dz;
     const int* total;                                                        // rows in use, on the device; null: all
     int64_t pitch, rows;
-    int cols, activation, whole;
+    int cols, activation, whole;                                             // whole: rows of dz are of whole 16 bytes
 };
 
 template <typename T> __device__ __forceinline__ void store8(T* to, int n, bool whole, const float (&v)[8]) {
@@ -270,9 +351,9 @@ template <typename T> __global__ __launch_bounds__(256) void gated_gradient_kern
         const int c = (int)(i - row * pieces) * 8;
         const T* z = static_cast<const T*>(a.z) + row * a.pitch;
         float g[8], u[8], d[8];
-        load8<T>(z, c, a.cols, a.whole, false, g);
-        load8<T>(z + a.cols, c, a.cols, a.whole, false, u);
-        load8<float>(a.dh + row * a.cols, c, a.cols, a.whole, false, d);
+        load8<T>(z, c, a.cols, g);
+        load8<T>(z + a.cols, c, a.cols, u);
+        load8<float>(a.dh + row * a.cols, c, a.cols, d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float act, derivative;
@@ -287,14 +368,9 @@ template <typename T> __global__ __launch_bounds__(256) void gated_gradient_kern
     }
 }
 
-bool readable8(const void* x, int64_t pitch, int64_t cols, int dtype, bool halves) {
-    const int unit = 16 / viola_dtype_size(dtype);
-    return reinterpret_cast<uintptr_t>(x) % 16 == 0 && pitch % unit == 0 && (!halves || cols % unit == 0);
-}
-
 }  // namespace
 
-extern "C" int64_t viola_int8_sum_parts(int64_t rows, int64_t cols) { return rows <= 0 || cols <= 0 ? 0 : shares_of(rows, cols, true).parts; }
+extern "C" int64_t viola_int8_sum_parts(int64_t rows, int64_t cols) { return rows <= 0 || cols <= 0 ? 0 : shares_of(rows, cols, true).blocks; }
 
 extern "C" int viola_int8_quantize(const void* x, int64_t pitch, int dtype, int64_t rows, int64_t cols, int activation, const float* factors, const int32_t* offsets,
                                    int64_t groups, int8_t* codes, int64_t code_pitch, float* scales, float* partial, viola_stream_t stream_) {
@@ -308,8 +384,6 @@ extern "C" int viola_int8_quantize(const void* x, int64_t pitch, int dtype, int6
     QuantizeArgs a = {};
     a.x = x; a.pitch = pitch; a.rows = rows; a.cols = (int)cols; a.activation = activation; a.groups = (int)groups; a.factors = factors; a.offsets = offsets;
     a.codes = codes; a.code_pitch = code_pitch; a.scales = scales; a.partial = partial;
-    a.whole = readable8(x, pitch, cols, dtype, gated);
-    a.stream_in = false;
     if (dtype == VIOLA_F32) return launch_mode<float>(a, stream);
     return dtype == VIOLA_BF16 ? launch_mode<bf16_t>(a, stream) : launch_mode<f16_t>(a, stream);
 }
@@ -322,7 +396,7 @@ extern "C" int viola_int8_gated_backward(const void* z, int64_t pitch, int dtype
     VIOLA_CHECK_ARG(z && dh && dz);
     GatedGradientArgs a = {};
     a.z = z; a.dh = dh; a.dz = dz; a.total = total; a.pitch = pitch; a.rows = rows; a.cols = (int)cols; a.activation = activation;
-    a.whole = readable8(z, pitch, cols, dtype, true) && cols % 4 == 0 && reinterpret_cast<uintptr_t>(dz) % 16 == 0 && reinterpret_cast<uintptr_t>(dh) % 16 == 0;
+    a.whole = reinterpret_cast<uintptr_t>(dz) % 16 == 0 && cols % (16 / viola_dtype_size(dtype)) == 0;
     const int64_t blocks = (rows * ((cols + 7) / 8) + 255) / 256;
     const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
     if (dtype == VIOLA_F32) VIOLA_LAUNCH((gated_gradient_kernel<float>), grid, 256, 0, stream, a);

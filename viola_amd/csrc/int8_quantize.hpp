@@ -4,27 +4,58 @@
 
 namespace viola {
 
-// Eight values of a row from column c on; zero past the end.
-template <typename T> __device__ __forceinline__ void load8(const T* row, int c, int cols, bool whole, bool stream, float (&v)[8]) {
-    if (whole && c + 8 <= cols) {
-        if constexpr (sizeof(T) == 4) {
-            const uint4 a = stream ? load16<true>(reinterpret_cast<const uint4*>(row + c)) : load16<false>(reinterpret_cast<const uint4*>(row + c));
-            const uint4 b = stream ? load16<true>(reinterpret_cast<const uint4*>(row + c + 4)) : load16<false>(reinterpret_cast<const uint4*>(row + c + 4));
-            v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
-            v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
-        } else {
-            const uint4 a = stream ? load16<true>(reinterpret_cast<const uint4*>(row + c)) : load16<false>(reinterpret_cast<const uint4*>(row + c));
-            const uint32_t words[4] = {a.x, a.y, a.z, a.w};
+// 16 bytes at any address that a value may have: one load all the same, which the hardware cuts at cache lines
+typedef uint32_t loose4 __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ uint4 load16_at(const void* from) {
+    const loose4 w = *static_cast<const loose4*>(from);
+    return make_uint4(w.x, w.y, w.z, w.w);
+}
+
+// Eight values of a row from column c on, as they are stored; zero past the end. Apart from their conversion, so that loads can be under way while other work goes on.
+template <typename T> struct Raw8 {
+    uint4 word[sizeof(T) / 2];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = widen16<T>(words[i] & 0xffffu);
-                v[2 * i + 1] = widen16<T>(words[i] >> 16);
+        for (size_t i = 0; i < sizeof(T) / 2; ++i) word[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const T* row, int c, int cols) {
+        if (c + 8 <= cols) {
+#pragma unroll
+            for (size_t i = 0; i < sizeof(T) / 2; ++i) word[i] = load16_at(row + c + 4 * i);
+            return;
+        }
+        uint32_t w[2 * sizeof(T)];
+#pragma unroll
+        for (int i = 0; i < (int)(2 * sizeof(T)); ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (c + i >= cols) continue;
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(row[c + i]);
+            else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[c + i] << (i % 2 * 16);
+        }
+#pragma unroll
+        for (size_t i = 0; i < sizeof(T) / 2; ++i) word[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+#pragma unroll
+        for (size_t i = 0; i < sizeof(T) / 2; ++i) {
+            const uint32_t w[4] = {word[i].x, word[i].y, word[i].z, word[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(T) == 4) {
+                    v[4 * i + e] = __uint_as_float(w[e]);
+                } else {
+                    v[2 * e] = widen16<T>(w[e] & 0xffffu);
+                    v[2 * e + 1] = widen16<T>(w[e] >> 16);
+                }
             }
         }
-        return;
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f32<T>(row[c + i]) : 0.0f;
+};
+template <typename T> __device__ __forceinline__ void load8(const T* row, int c, int cols, float (&v)[8]) {
+    Raw8<T> raw;
+    raw.load(row, c, cols);
+    raw.widen(v);
 }
 
 __device__ __forceinline__ uint32_t magnitudes(const float (&v)[8], uint32_t most) {
@@ -56,12 +87,12 @@ __device__ __forceinline__ uint2 encode8_int(const float (&v)[8], const RowScale
     float far = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float t = v[i] * r.inverse, b = t + MAGIC;
+        const float b = fmaf(v[i], r.inverse, MAGIC);
         word[i] = __float_as_uint(b);
-        far = fmaxf(far, fabsf(t - (b - MAGIC)));
+        far = fmaxf(far, fabsf(fmaf(v[i], r.inverse, MAGIC - b)));
     }
     // (the rare row that is lifted takes the exact way too, where codes are cut off at 127)
-    if (far > 0.4998f || r.lift != 1.0f) {
+    if (far > 0.49998f || r.lift != 1.0f) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float x = v[i] * r.lift, half = 0.5f * r.lifted;

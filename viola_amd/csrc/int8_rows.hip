@@ -36,7 +36,7 @@ template <typename T> struct FusedRows {
             const int slot = i * ROWS_WAVES + wave, row = slot / parts, c = (slot % parts * WAVE + lane) * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
-            if (row < f.rows && c < f.cols) load8<T>(static_cast<const T*>(f.x) + row * f.pitch, c, f.cols, true, false, v[i]);
+            if (row < f.rows && c < f.cols) load8<T>(static_cast<const T*>(f.x) + row * f.pitch, c, f.cols, v[i]);
         }
     }
     // codes of all rows into LDS (rows `stride` bytes apart, zeros behind the columns, which are a multiple of 16) and their scales
@@ -49,7 +49,7 @@ template <typename T> struct FusedRows {
             if (row >= f.rows) break;
             if (f.activation >= 0 && c < f.cols) {
                 float u[8];
-                load8<T>(static_cast<const T*>(f.x) + row * f.pitch + f.cols, c, f.cols, true, false, u);
+                load8<T>(static_cast<const T*>(f.x) + row * f.pitch + f.cols, c, f.cols, u);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float act, derivative;
@@ -228,7 +228,6 @@ extern "C" int viola_int8_rows_linear(const void* x, int64_t pitch, int dtype, i
     if (m == 0) return 0;
     if (!fused_fits(m, k) || ldb > (int64_t{1} << 22)) return VIOLA_EUNSUPPORTED;
     VIOLA_CHECK_ARG(x && b && sb && out && reinterpret_cast<uintptr_t>(b) % 16 == 0);
-    if (reinterpret_cast<uintptr_t>(x) % 16 || pitch * viola_dtype_size(dtype) % 16) return VIOLA_EUNSUPPORTED;
     Int8Args p = {};
     p.b = b; p.sb = sb; p.bias = bias; p.out = out; p.m = m; p.n = n; p.k = k; p.ldb = ldb; p.ldo = n; p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
     const FusedArgs f = {x, pitch, (int)m, (int)k, activation};
