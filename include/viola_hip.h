@@ -578,7 +578,7 @@ int viola_rows_scatter(const void* x, int64_t pitch, int dtype, int64_t cols, co
  * [viola_int8_sum_parts(rows, cols)][cols] sums of x over rows, for viola_column_reduce.
  * viola_int8_gemm: out[r, c] = (sum_k a[r, k] b[c, k]) sa[r] sb[c] + bias[c], a [m, k] and b [n, k] with rows lda and ldb bytes apart (16-byte aligned, multiples of
  * 16, columns of a beyond k up to the next 16 zero), out [m, n] contiguous. With offsets (int32 [groups + 1] on the device; no bias) rows offsets[g] to offsets[g + 1] take b +
- * g b_stride and sb + g n (sb null: ones), and rows from offsets[groups] on are zero. k <= 2^17, ldb <= 2^22 (VIOLA_EUNSUPPORTED beyond).
+ * g b_stride and sb + g n (sb null: ones), and rows from offsets[groups] on are zero. k <= 2^17, groups <= 1024, ldb <= 2^22 (VIOLA_EUNSUPPORTED beyond).
  * viola_int8_rows_linear: both for a few rows in one launch, out = the product of x's codes (of act(g) u with activation >= 0) with b; m <= 16, m k up to about 32768, k a multiple of 16, rows
  * of x and b 16-byte aligned (VIOLA_EUNSUPPORTED with nothing launched otherwise; the same bits as the two calls).
  * viola_int8_gated_backward: dz [rows, 2 cols] = [dh u act'(g) | dh act(g)], contiguous, of z = [g | u] and dh float [rows, cols]; rows from *total (null: none) on are zero. */

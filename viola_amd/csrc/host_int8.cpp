@@ -95,7 +95,7 @@ Tensor run(const char* name, const Tensor& x, const Tensor& weight, const Tensor
     plan.out_type = type.value_or(plan.x_type);
     TORCH_CHECK(plan.n > 0 && plan.k > 0 && (!grouped || plan.groups > 0), name, ": weight of ", weight.sizes(), " is empty");
     TORCH_CHECK(plan.k <= MOST_K, name, " adds up at most ", MOST_K, " products, got ", plan.k);
-    TORCH_CHECK(plan.groups < (int64_t{1} << 16), name, " takes fewer than 2^16 groups");
+    TORCH_CHECK(plan.groups <= 1024, name, " takes up to 1024 groups, got ", plan.groups);
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) == plan.k * (activation >= 0 ? 2 : 1), name, ": x has to end in ", plan.k * (activation >= 0 ? 2 : 1), " features, got ", x.sizes());
     TORCH_CHECK(!grouped || x.dim() == 2, name, ": x has to be [rows, features], got ", x.sizes());
     TORCH_CHECK(scale.device() == device && scale.scalar_type() == at::kFloat && scale.sizes() == weight.sizes().slice(0, weight.dim() - 1), name,

@@ -19,8 +19,28 @@ struct Int8Args {
 
 constexpr int64_t INT8_MOST_K = 1 << 17;
 
-// Row tile `index` of `rows` rows, counted over the groups (each has whole tiles of its own) and then over the rows behind them: its group (groups: rows that are zero),
-// and its rows [begin, end). False: there are not so many. Every lane of a wavefront has to call it.
+// The rows of group g of the groups' own, and of those behind the last one (g = groups). Offsets that a program made by hand are taken within the rows and in order: a
+// product must stay inside its buffers whatever they hold.
+__device__ __forceinline__ void int8_group_rows(const Int8Args& p, int g, int& from, int& to) {
+    const int m = (int)p.m;
+    from = g <= p.groups ? p.offsets[g] : m;
+    to = g < p.groups ? p.offsets[g + 1] : m;
+    from = from < 0 ? 0 : from < m ? from : m;
+    to = to < from ? from : to < m ? to : m;
+}
+// All row tiles of `rows` rows (each group has whole tiles of its own, the rows behind them too). Every lane of a wavefront has to call it, and the next one.
+__device__ __forceinline__ int int8_count_tiles(const Int8Args& p, int rows) {
+    int tiles = 0;
+    for (int g = threadIdx.x % WAVE; g <= p.groups; g += WAVE) {
+        int from, to;
+        int8_group_rows(p, g, from, to);
+        tiles += (to - from + rows - 1) / rows;
+    }
+#pragma unroll
+    for (int d = 1; d < WAVE; d *= 2) tiles += __shfl_xor(tiles, d, WAVE);
+    return __builtin_amdgcn_readfirstlane(tiles);
+}
+// Row tile `index`: its group (groups: rows that are zero), and its rows [begin, end). False: there are not so many.
 __device__ __forceinline__ bool int8_row_tile(const Int8Args& p, int64_t index, int rows, int& group, int64_t& begin, int64_t& end) {
     if (!p.offsets) {
         group = 0;
@@ -31,12 +51,9 @@ __device__ __forceinline__ bool int8_row_tile(const Int8Args& p, int64_t index, 
     const int lane = threadIdx.x % WAVE;
     int64_t before = 0;                                                      // tiles of the groups so far
     for (int base = 0; base <= p.groups; base += WAVE) {
-        const int g = base + lane;
-        // offsets that a program made by hand are taken within the rows and in order: a product must stay inside its buffers whatever they hold
-        int64_t from = g <= p.groups ? p.offsets[g] : p.m, to = g < p.groups ? p.offsets[g + 1] : p.m;
-        from = from < 0 ? 0 : from < p.m ? from : p.m;
-        to = to < from ? from : to < p.m ? to : p.m;
-        const int tiles = g <= p.groups ? (int)((to - from + rows - 1) / rows) : 0;
+        int from, to;
+        int8_group_rows(p, base + lane, from, to);
+        const int tiles = base + lane <= p.groups ? (to - from + rows - 1) / rows : 0;
         int upto = tiles;
 #pragma unroll
         for (int d = 1; d < WAVE; d *= 2) {
@@ -49,7 +66,7 @@ __device__ __forceinline__ bool int8_row_tile(const Int8Args& p, int64_t index, 
             const int at = __ffsll((long long)past) - 1;
             group = __builtin_amdgcn_readfirstlane(base + at);
             const int skipped = __builtin_amdgcn_readfirstlane(__shfl(upto - tiles, at, WAVE));
-            const int first = __builtin_amdgcn_readfirstlane(__shfl((int)from, at, WAVE)), last = __builtin_amdgcn_readfirstlane(__shfl((int)to, at, WAVE));
+            const int first = __builtin_amdgcn_readfirstlane(__shfl(from, at, WAVE)), last = __builtin_amdgcn_readfirstlane(__shfl(to, at, WAVE));
             begin = first + (want - skipped) * rows;
             end = begin + rows < last ? begin + rows : last;
             return true;

@@ -14,13 +14,26 @@ namespace viola {
 
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
+typedef int loose_words4 __attribute__((ext_vector_type(4), aligned(2)));
+
+// 16 bytes of a row from column `col` on, at any address: one store all the same
+template <typename TO> __device__ __forceinline__ void store_piece(TO* to, int64_t col, int64_t n, const uint4& value) {
+    constexpr int PER = 16 / (int)sizeof(TO);
+    if (col + PER <= n) {
+        __builtin_nontemporal_store(loose_words4{(int)value.x, (int)value.y, (int)value.z, (int)value.w}, reinterpret_cast<loose_words4*>(to));
+    } else {
+        const TO* values = reinterpret_cast<const TO*>(&value);
+        for (int e = 0; e < PER; ++e)
+            if (col + e < n) to[e] = values[e];
+    }
+}
+
 // The finished sums of a wave times their scales plus bias, through its own part of the ring (which every wave has left), out in 16-byte pieces.
 template <typename S, typename TO>
 __device__ __forceinline__ void store_int8_tile(const i32x16 (&total)[S::TN][S::TM], const Int8Args& p, TO* out, int64_t m_begin, int64_t m_end, int64_t n_begin,
                                                 uint8_t* ring, const float* columns) {
     const int lane = threadIdx.x % WAVE, l32 = lane % 32, lhi = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE), wm = wave / S::WN, wn = wave % S::WN;
-    const bool pieces_out = (p.ldo * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     constexpr int PER = 16 / (int)sizeof(TO), COLS_W = 32 * S::TN, PLD = COLS_W + PER, PIECES = COLS_W / PER;
     static_assert(8 * 32 * PLD * (int)sizeof(TO) <= S::STAGES * S::STAGE);
     TO* park = reinterpret_cast<TO*>(ring) + wave * 32 * PLD;
@@ -44,14 +57,7 @@ __device__ __forceinline__ void store_int8_tile(const i32x16 (&total)[S::TN][S::
             const int id = it * WAVE + lane, pr = id / PIECES, pc = id % PIECES;
             const int64_t mrow = row0 + pr, ncol = ncol0 + pc * PER;
             const uint4 value = *reinterpret_cast<const uint4*>(&park[pr * PLD + pc * PER]);
-            if (mrow >= m_end || ncol >= p.n) continue;
-            if (pieces_out && ncol + PER <= p.n) {
-                store_streaming(out + mrow * p.ldo + ncol, value);
-            } else {
-                const TO* values = reinterpret_cast<const TO*>(&value);
-                for (int e = 0; e < PER; ++e)
-                    if (ncol + e < p.n) out[mrow * p.ldo + ncol + e] = values[e];
-            }
+            if (mrow < m_end && ncol < p.n) store_piece(out + mrow * p.ldo + ncol, ncol, p.n, value);
         }
     }
 }
@@ -203,34 +209,37 @@ __device__ __forceinline__ void int8_tile(const Int8Args& p, int group, int64_t 
     else store_int8_tile<S>(total, p, static_cast<f16_t*>(p.out), m_begin, m_end, n_begin, lds, columns);
 }
 
-// Rows that no group has.
-__device__ __forceinline__ void int8_zeros(const Int8Args& p, int64_t m_begin, int64_t m_end, int64_t n_begin, int cols) {
-    const int64_t left = p.n - n_begin;
-    const int here = left < cols ? (int)left : cols;
-    for (int64_t row = m_begin; row < m_end; ++row)
-        for (int c = threadIdx.x; c < here; c += blockDim.x) store_float(p.out, row * p.ldo + n_begin + c, p.out_dtype, 0.0f);
-}
-
-template <typename S> __device__ __forceinline__ void int8_place(const Int8Args& p, int t, uint8_t* lds) {
-    // groups of 8 row tiles, as in pingpong_place
-    const int across = 8 * p.tiles_n, first_m = t / across * 8;
-    const int rows_here = p.tiles_m - first_m < 8 ? p.tiles_m - first_m : 8;
-    const int64_t n_begin = (int64_t)(t % across / rows_here) * S::COLS;
-    int group;
-    int64_t m_begin, m_end;
-    if (!int8_row_tile(p, first_m + t % across % rows_here, S::ROWS, group, m_begin, m_end)) return;
-    if (p.offsets && group == p.groups) int8_zeros(p, m_begin, m_end, n_begin, S::COLS);
-    else int8_tile<S>(p, group, m_begin, m_end, n_begin, lds);
+// Rows that no group has, of one tile
+template <typename S, typename TO> __device__ __forceinline__ void int8_zeros(const Int8Args& p, int64_t m_begin, int64_t m_end, int64_t n_begin) {
+    constexpr int PER = 16 / (int)sizeof(TO), PIECES = S::COLS / PER;
+    for (int i = threadIdx.x; i < S::ROWS * PIECES; i += S::THREADS) {
+        const int64_t row = m_begin + i / PIECES, col = n_begin + i % PIECES * PER;
+        if (row < m_end && col < p.n) store_piece(static_cast<TO*>(p.out) + row * p.ldo + col, col, p.n, make_uint4(0, 0, 0, 0));
+    }
 }
 
 template <typename S, int WAVES_PER_SIMD> __global__ __launch_bounds__(512, WAVES_PER_SIMD) void int8_gemm(Int8Args p) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[int8_lds<S>()];
-    const int t = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;       // contiguous ranges per XCD
-    if (t >= p.tiles_m * p.tiles_n) return;
-    int8_place<S>(p, t, lds);
+    // contiguous ranges for each XCD, of the tiles that there are: the host knows a bound on those of groups
+    const int tiles_m = p.offsets ? int8_count_tiles(p, S::ROWS) : p.tiles_m, each = (tiles_m * p.tiles_n + 7) / 8;
+    const int t = blockIdx.x % 8 * each + blockIdx.x / 8;
+    if ((int)blockIdx.x / 8 >= each || t >= tiles_m * p.tiles_n) return;
+    // groups of 8 row tiles, as in pingpong_place
+    const int across = 8 * p.tiles_n, first_m = t / across * 8;
+    const int rows_here = tiles_m - first_m < 8 ? tiles_m - first_m : 8;
+    const int64_t n_begin = (int64_t)(t % across / rows_here) * S::COLS;
+    int group;
+    int64_t m_begin, m_end;
+    if (!int8_row_tile(p, first_m + t % across % rows_here, S::ROWS, group, m_begin, m_end)) return;
+    if (!p.offsets || group < p.groups) int8_tile<S>(p, group, m_begin, m_end, n_begin, lds);
+    else if (p.out_dtype == VIOLA_F32) int8_zeros<S, float>(p, m_begin, m_end, n_begin);
+    else int8_zeros<S, bf16_t>(p, m_begin, m_end, n_begin);                  // (zero is zero in either type of 16 bits)
 }
 
-using Int8L = PingPongShape<2, 4, 4, 2, 2, 128>;                             // 256 x 256
+// 256 x 256 in four stages of 64 k, or in two of 128 k for long sums (16384 x 4096 -> 11008 668 and 690 us, 32768 rows at 16 experts of 4096 -> 1024 165 and 185, 4096 x 11008 -> 4096
+// 161 and 153)
+using Int8L = PingPongShape<2, 4, 4, 2, 4>;
+using Int8Long = PingPongShape<2, 4, 4, 2, 2, 128>;
 using Int8M = PingPongShape<4, 2, 2, 2, 3, 128>;                             // 256 x 128
 using Int8S = PingPongShape<2, 4, 2, 1, 3, 128>;                             // 128 x 128
 using Int8Pairs = PingPongShape<2, 4, 2, 1, 4>;                              // 128 x 128, two blocks on a CU
@@ -245,17 +254,34 @@ template <typename S, int WAVES_PER_SIMD> static int launch_tiles(const Int8Args
     return viola_launch_status();
 }
 
+// The tile that takes least by estimates in microseconds, fitted to measured times of 20 shapes and within 15 % of most. A round of a tile for each CU takes a fixed part and a time
+// for each chunk of 64 k, which grows with the share of CUs at work as the clock falls: L .42 to .84 + 8.5, M .30 to .47 + 5.3, S .24 to .29 + 4, two S on a CU .25 to
+// .73 + 4. Each group leaves half a row tile unfilled on average. So 8192 x 1024 -> 4096 takes L (47 us; M 57, S 66), 8192 x 4096 -> 1024 M (36; L 49, S 47), 2048 x 2048 ->
+// 2048 S (13; M 17), 9850 x 770 -> 1000 L (19; M 25), 4000 rows at 128 experts of 2048 -> 1024 pairs of S (61; L 69).
+enum Int8TileShape { INT8_L, INT8_M, INT8_S, INT8_PAIRS };
+static Int8TileShape choose_int8_tile(const Int8Args& p) {
+    const double chunks = (double)((p.k + 63) / 64);
+    auto estimate = [&](int rows, int cols, int at_once, double idle, double busy, double fixed) {
+        const int64_t row_tiles = (p.m + rows - 1) / rows + (p.offsets ? (p.groups < p.m ? p.groups : p.m) / 2 : 0), tiles = row_tiles * ((p.n + cols - 1) / cols);
+        const double full = (double)(tiles / at_once), rest = (double)(tiles % at_once) / at_once;
+        return full * (chunks * busy + fixed) + (rest > 0 ? chunks * (idle + (busy - idle) * rest) + fixed : 0.0);
+    };
+    const double time[4] = {estimate(256, 256, 256, 0.42, 0.84, 8.5), estimate(256, 128, 256, 0.30, 0.47, 5.3), estimate(128, 128, 256, 0.24, 0.29, 4.0),
+                            estimate(128, 128, 512, 0.25, 0.73, 4.0)};
+    int best = 0;
+    for (int i = 1; i < 4; ++i) best = time[i] < time[best] ? i : best;
+    return (Int8TileShape)best;
+}
+
 static int launch_int8(const Int8Args& p, hipStream_t stream) {
     const int status = launch_int8_rows(p, stream);
     if (status != VIOLA_EUNSUPPORTED) return status;
-    ScaledTile tile = choose_scaled_tile(p.m, p.n, p.k, false);
-    switch (tile) {
-        case SCALED_TILE_L: return launch_tiles<Int8L, 2>(p, stream);
-        case SCALED_TILE_M: return launch_tiles<Int8M, 2>(p, stream);
-        default: break;
+    switch (choose_int8_tile(p)) {
+        case INT8_L: return p.k > 8192 ? launch_tiles<Int8Long, 2>(p, stream) : launch_tiles<Int8L, 2>(p, stream);
+        case INT8_M: return launch_tiles<Int8M, 2>(p, stream);
+        case INT8_S: return launch_tiles<Int8S, 2>(p, stream);
+        default: return launch_tiles<Int8Pairs, 4>(p, stream);
     }
-    if ((p.m + 127) / 128 * ((p.n + 127) / 128) <= 256) return launch_tiles<Int8S, 2>(p, stream);
-    return launch_tiles<Int8Pairs, 4>(p, stream);
 }
 
 }  // namespace viola
