@@ -108,6 +108,29 @@ def test_linear(tokens, width, out):
     _check_linear(_rows(tokens, width, BF16), w, sw, _rows(1, out, F32, seed=5)[0])
 
 
+@pytest.mark.parametrize("tokens,width,out", [(1, 8192, 40), (2, 4096, 65), (7, 2032, 33), (16, 512, 70), (16, 528, 70), (17, 1024, 130), (20, 1024, 9000), (32, 272, 8200), (48, 512, 700),
+                                              (130, 1024, 520), (512, 128, 768), (512, 128, 769), (513, 128, 700), (300, 9008, 200), (260, 8208, 272), (3000, 128, 3000), (9, 131072, 20)])
+def test_ways_of_a_product(tokens, width, out):
+    """Rows quantized on the way in, few rows, one to four tiles of channels a wavefront, tiles of each size, long sums: on the borders between them."""
+    w, sw = _weights(out, width)
+    _check_linear(_rows(tokens, width, BF16), w, sw * 0.1, _rows(1, out, F32, seed=5)[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("activation", [None, "silu", "gelu"])
+def test_few_rows_are_quantized_as_many(dtype, activation):
+    """The same bits from one launch as from two, at any address of x."""
+    from viola_amd import nn
+    for tokens, width, out in ((1, 1024, 100), (3, 2560, 33), (8, 1024, 64), (15, 48, 17)):
+        w, sw = _weights(out, width)
+        store = _rows(600, 2 * width + 3, dtype).clamp(-30, 30)
+        cols = width * (2 if activation else 1)
+        for first in (0, 1, 3):
+            many = nn.int8_linear(store[:, first:first + cols], w, sw, activation=activation)
+            few = nn.int8_linear(store[:tokens, first:first + cols], w, sw, activation=activation)
+            assert torch.equal(few, many[:tokens])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("result", [None, F32, BF16, F16])
 @pytest.mark.parametrize("tokens,width,out", [(9, 200, 72), (260, 384, 136), (33, 100, 51)])
@@ -161,7 +184,7 @@ def test_longest_sums():
 
 
 GROUPS = [([5], 0), ([0, 0, 3], 0), ([0, 5, 0, 130, 1], 7), ([300, 0, 17, 128, 129, 256], 0), ([0, 0, 0], 20), ([1] * 70 + [0] * 30 + [33] * 31, 3), ([2, 1, 0, 4] * 16, 0),
-          ([700, 20, 900, 0, 500], 200), ([16, 17, 15, 32], 1)]
+          ([700, 20, 900, 0, 500], 200), ([16, 17, 15, 32], 1), ([20, 21, 0, 19] * 40, 30), ([1, 0] * 512, 0), ([3000, 1, 0, 2900], 900), ([33] * 65, 0)]
 
 
 @pytest.mark.parametrize("counts,left", GROUPS)
@@ -264,6 +287,18 @@ def test_wanted_gradients_alone():
         y.sum().backward()
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 8), (3, 1000), (5000, 70), (4100, 520), (2500, 2049), (1100, 4104), (40, 9000), (700, 16384), (33, 16400)])
+def test_bias_gradient(rows, cols):
+    """Sums over rows that one block, several and the longest rows' leave."""
+    from viola_amd import nn
+    w, sw = _weights(cols, 16)
+    bias = torch.zeros(cols, device="cuda", requires_grad=True)
+    dy = _rows(rows, cols, BF16, seed=3)
+    nn.int8_linear(_rows(rows, 16, BF16), w, sw, bias).backward(dy)
+    d = dy.double()
+    assert oi.within(bias.grad, d.sum(0), 2048 * oi.U * d.abs().sum(0))
+
+
 def test_another_stream_and_two_at_once():
     from viola_amd import nn
     w, sw = _weights(512, 1024)
@@ -320,6 +355,8 @@ def test_refusals():
            lambda: nn.int8_linear(x, w, sw, torch.zeros(23, device="cuda")), lambda: nn.int8_linear(x, w, sw.requires_grad_()), lambda: nn.int8_linear(x.double(), w, sw),
            lambda: nn.int8_linear(x, e, se), lambda: nn.int8_linear(x, w, sw.detach(), weight_t=w), lambda: nn.int8_linear(x, w.cpu(), sw.detach()),
            lambda: nn.int8_linear(x, w, sw.detach(), dtype=torch.int8), lambda: nn.int8_linear(x, w, sw.detach(), activation="silu"),
+           lambda: nn.int8_grouped_linear(x, torch.zeros(1025, 4, 32, dtype=torch.int8, device="cuda"), torch.zeros(1025, 4, device="cuda"),
+                                          torch.zeros(1026, dtype=torch.int32, device="cuda")),
            lambda: nn.int8_grouped_linear(x, w, sw.detach(), offsets), lambda: nn.int8_grouped_linear(x, e, se, offsets.long()),
            lambda: nn.int8_grouped_linear(x, e, se, offsets[:3]), lambda: nn.int8_grouped_linear(x, e, se, offsets.cpu()), lambda: nn.int8_grouped_linear(x[None], e, se, offsets),
            lambda: nn.quantize_int8(x[:, :31], activation="silu"), lambda: nn.quantize_int8(x.long()), lambda: nn.quantize_int8(torch.zeros(3, 0, device="cuda"))]
