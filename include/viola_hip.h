@@ -579,6 +579,8 @@ int viola_rows_scatter(const void* x, int64_t pitch, int dtype, int64_t cols, co
  * viola_int8_gemm: out[r, c] = (sum_k a[r, k] b[c, k]) sa[r] sb[c] + bias[c], a [m, k] and b [n, k] with rows lda and ldb bytes apart (16-byte aligned, multiples of
  * 16, columns of a beyond k up to the next 16 zero), out [m, n] contiguous. With offsets (int32 [groups + 1] on the device; no bias) rows offsets[g] to offsets[g + 1] take b +
  * g b_stride and sb + g n (sb null: ones), and rows from offsets[groups] on are zero. k <= 2^17, groups <= 1024, ldb <= 2^22 (VIOLA_EUNSUPPORTED beyond).
+ * viola_int8_gemm_gated_backward: that product dh (n its columns, without channel scales) and viola_int8_gated_backward of it in one, dz [m, 2 n] of z's type; few rows
+ * and k > 2048 take the two calls (VIOLA_EUNSUPPORTED with nothing launched).
  * viola_int8_rows_linear: both for a few rows in one launch, out = the product of x's codes (of act(g) u with activation >= 0) with b; m <= 16, m k up to about 32768, k a multiple of 16, rows
  * of x and b 16-byte aligned (VIOLA_EUNSUPPORTED with nothing launched otherwise; the same bits as the two calls).
  * viola_int8_gated_backward: dz [rows, 2 cols] = [dh u act'(g) | dh act(g)], contiguous, of z = [g | u] and dh float [rows, cols]; rows from *total (null: none) on are zero. */
@@ -587,6 +589,8 @@ int viola_int8_quantize(const void* x, int64_t pitch, int dtype, int64_t rows, i
                         int64_t groups, int8_t* codes, int64_t code_pitch, float* scales, float* partial, viola_stream_t stream);
 int viola_int8_gemm(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, int64_t b_stride, const float* sb, const int32_t* offsets,
                     int64_t groups, int64_t m, int64_t n, int64_t k, const void* bias, int bias_dtype, void* out, int out_dtype, viola_stream_t stream);
+int viola_int8_gemm_gated_backward(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, int64_t b_stride, const int32_t* offsets, int64_t groups,
+                                   int64_t m, int64_t n, int64_t k, const void* z, int64_t z_pitch, int z_dtype, int activation, void* dz, viola_stream_t stream);
 int viola_int8_rows_linear(const void* x, int64_t pitch, int dtype, int64_t m, int64_t k, int activation, const int8_t* b, int64_t ldb, const float* sb, int64_t n,
                            const void* bias, int bias_dtype, void* out, int out_dtype, viola_stream_t stream);
 int viola_int8_gated_backward(const void* z, int64_t pitch, int dtype, int64_t rows, int64_t cols, int activation, const float* dh, const int32_t* total,

@@ -140,7 +140,7 @@ def test_types(dtype, result, tokens, width, out):
 
 
 @pytest.mark.parametrize("activation", ["silu", "gelu", "relu"])
-@pytest.mark.parametrize("tokens,width,out,dtype", [(1, 64, 48, BF16), (37, 129, 65, F16), (300, 1024, 520, BF16), (50, 2056, 40, F32), (3, 16400, 24, BF16)])
+@pytest.mark.parametrize("tokens,width,out,dtype", [(1, 64, 48, BF16), (37, 129, 65, F16), (300, 1024, 520, BF16), (50, 2056, 40, F32), (3, 16400, 24, BF16), (700, 72, 2080, BF16), (700, 333, 65, F32)])
 def test_gated(activation, tokens, width, out, dtype):
     w, sw = _weights(out, width)
     _check_linear(_rows(tokens, 2 * width, dtype).clamp(-30, 30), w, sw * 0.1, activation=activation)

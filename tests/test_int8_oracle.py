@@ -104,6 +104,15 @@ def test_rejected_calls_launch_nothing():
                 dict(offsets=P), dict(offsets=P, groups=2, bias=P), dict(bs=8), dict(groups=-1), dict(m=1 << 31)):
         assert g(**bad) == -1, bad
     assert g(k=(1 << 17) + 1) == -2 and g(ldb=(1 << 22) + 16) == -2 and g(m=0) == 0
+    gb = lambda **c: lib.viola_int8_gemm_gated_backward(*{**dict(a=P, lda=64, sa=P, b=P, ldb=64, bs=0, offsets=None, groups=0, m=1000, n=800, k=64, z=P, zp=1600, zt=BF16, act=0,  # noqa: E731
+                                                                 dz=P), **c}.values(), None)
+    for bad in (dict(act=-1), dict(act=3), dict(zp=1599), dict(n=0), dict(zt=E4M3), dict(z=None), dict(dz=None), dict(lda=48), dict(m=-1), dict(offsets=P), dict(a=P + 4)):
+        assert gb(**bad) == -1, bad
+    assert gb(m=0) == 0 and gb(m=8) == -2 and gb(k=2064, lda=2064, ldb=2064) == -2
+    r = lambda **c: lib.viola_int8_rows_linear(*{**dict(x=P, pitch=64, dtype=BF16, m=4, k=64, act=-1, b=P, ldb=64, sb=P, n=8, bias=None, bt=F32, out=P, ot=BF16), **c}.values(), None)  # noqa: E731
+    for bad in (dict(dtype=E4M3), dict(pitch=63), dict(act=0), dict(act=3), dict(ldb=48), dict(ldb=72), dict(n=0), dict(sb=None), dict(b=P + 8), dict(out=None), dict(bias=P, bt=E4M3)):
+        assert r(**bad) == -1, bad
+    assert r(m=0) == 0 and r(m=17) == -2 and r(k=40) == -2 and r(m=8, k=4096, pitch=4096, ldb=4096) == -2
     b = lambda **c: lib.viola_int8_gated_backward(*{**dict(z=P, pitch=64, dtype=BF16, rows=4, cols=32, act=0, dh=P, total=None, dz=P), **c}.values(), None)  # noqa: E731
     for bad in (dict(dtype=E4M3), dict(pitch=63), dict(act=-1), dict(act=3), dict(dh=None), dict(dz=None), dict(rows=-1)):
         assert b(**bad) == -1, bad

@@ -93,6 +93,7 @@ _SIGNATURES = {
     "viola_rows_scatter": [_p, _l, _i, _l, _p, _p, _l, _i, _p, _p, _l, _p, _l, _p, _p],
     "viola_int8_quantize": [_p, _l, _i, _l, _l, _i, _p, _p, _l, _p, _l, _p, _p, _p],
     "viola_int8_gemm": [_p, _l, _p, _p, _l, _l, _p, _p, _l, _l, _l, _l, _p, _i, _p, _i, _p],
+    "viola_int8_gemm_gated_backward": [_p, _l, _p, _p, _l, _l, _p, _l, _l, _l, _l, _p, _l, _i, _i, _p, _p],
     "viola_int8_rows_linear": [_p, _l, _i, _l, _l, _i, _p, _l, _p, _l, _p, _i, _p, _i, _p],
     "viola_int8_gated_backward": [_p, _l, _i, _l, _l, _i, _p, _p, _p, _p],
     "viola_selftest_fp8": [_p, _p],

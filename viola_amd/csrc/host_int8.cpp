@@ -191,8 +191,6 @@ variable_list ProductBackward::apply(variable_list&& grads) {
     const int64_t pitch = ceil_to(plan.n, 16), parts = needs_bias ? viola_int8_sum_parts(plan.rows, plan.n) : 0;
     Arena temp;
     const int64_t scales_at = temp.take(plan.rows * 4), codes_at = temp.take(plan.rows * pitch), sums_at = temp.take(parts * plan.n * 4);
-    const bool gated = plan.activation >= 0;
-    const int64_t dh_at = gated && needs_x ? temp.take(plan.rows * plan.k * 4) : 0;
     temp.make(device);
     std::vector<int64_t> channel_shape;
     if (plan.groups) channel_shape.push_back(plan.groups);
@@ -213,15 +211,25 @@ variable_list ProductBackward::apply(variable_list&& grads) {
                     (plan.groups ? w.dim() == 3 && w.size(0) == plan.groups : w.dim() == 2), "a tensor saved by ", label, " came back changed");
     const Codes back = has_turned ? Codes(w, stream) : Codes::turned(w, stream);
     result[0] = room(shape, plan.x_type, device);
-    product(plan, temp.as<int8_t>(codes_at), pitch, temp.as<float>(scales_at), back, nullptr, places, Tensor(), plan.k, plan.n,
-            gated ? temp.at(dh_at) : result[0].mutable_data_ptr(), gated ? at::kFloat : plan.x_type, stream);
-    if (gated) {
-        const Tensor z = x.unpack();
-        TORCH_CHECK(z.defined() && z.device() == device && z.scalar_type() == plan.x_type && z.sizes() == at::IntArrayRef(shape), "a tensor saved by ", label, " came back changed");
-        const Rows zr(z);
-        VIOLA_CALL(viola_int8_gated_backward, zr.data(), zr.pitch, code_of(plan.x_type), plan.rows, plan.k, plan.activation, temp.as<float>(dh_at),
-                   plan.groups ? static_cast<const int32_t*>(places.const_data_ptr()) + plan.groups : nullptr, result[0].mutable_data_ptr(), stream);
+    const int8_t* codes = temp.as<int8_t>(codes_at);
+    const float* scales = temp.as<float>(scales_at);
+    if (plan.activation < 0) {
+        product(plan, codes, pitch, scales, back, nullptr, places, Tensor(), plan.k, plan.n, result[0].mutable_data_ptr(), plan.x_type, stream);
+        return result;
     }
+    const Tensor z = x.unpack();
+    TORCH_CHECK(z.defined() && z.device() == device && z.scalar_type() == plan.x_type && z.sizes() == at::IntArrayRef(shape), "a tensor saved by ", label, " came back changed");
+    const Rows zr(z);
+    const int status = VIOLA_TRY(viola_int8_gemm_gated_backward, codes, pitch, scales, back.data(), back.pitch, back.stride, static_cast<const int32_t*>(ptr(places)), plan.groups,
+                                 plan.rows, plan.k, plan.n, zr.data(), zr.pitch, code_of(plan.x_type), plan.activation, result[0].mutable_data_ptr(), stream);
+    if (status != VIOLA_EUNSUPPORTED) {
+        check("viola_int8_gemm_gated_backward", status);
+        return result;
+    }
+    const Tensor dh = room({plan.rows, plan.k}, at::kFloat, device);         // few rows, long sums
+    product(plan, codes, pitch, scales, back, nullptr, places, Tensor(), plan.k, plan.n, dh.mutable_data_ptr(), at::kFloat, stream);
+    VIOLA_CALL(viola_int8_gated_backward, zr.data(), zr.pitch, code_of(plan.x_type), plan.rows, plan.k, plan.activation, static_cast<const float*>(dh.const_data_ptr()),
+               plan.groups ? static_cast<const int32_t*>(places.const_data_ptr()) + plan.groups : nullptr, result[0].mutable_data_ptr(), stream);
     return result;
 }
 

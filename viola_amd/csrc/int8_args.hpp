@@ -15,9 +15,10 @@ struct Int8Args {
     const int* offsets; int groups; int64_t b_stride;                        // bytes from one b to the next
     int bias_dtype, out_dtype;
     int tiles_m, tiles_n;
+    const void* z; int64_t z_pitch; int activation;                          // gated (int8_gemm.hip): out [m, 2 n] = the gradient of z = [g | u] from the product dh; z null: not
 };
 
-constexpr int64_t INT8_MOST_K = 1 << 17;
+constexpr int64_t INT8_MOST_K = 1 << 17, INT8_MOST_GROUPS = 1024;
 
 // The rows of group g of the groups' own, and of those behind the last one (g = groups). Offsets that a program made by hand are taken within the rows and in order: a
 // product must stay inside its buffers whatever they hold.
@@ -78,7 +79,8 @@ __device__ __forceinline__ bool int8_row_tile(const Int8Args& p, int64_t index, 
 // (tiles of rows that a launch has to provide for: each group can leave one unfilled)
 inline int64_t int8_row_tiles(const Int8Args& p, int rows) { return (p.m + rows - 1) / rows + (p.offsets ? p.groups + 1 : 0); }
 
-// VIOLA_EUNSUPPORTED: too many rows. int8_rows.hip
+// Whether the rows are few enough for int8_rows.hip, and the product there
+bool int8_rows_fit(const Int8Args& p);
 int launch_int8_rows(const Int8Args& p, hipStream_t stream);
 
 }  // namespace viola

@@ -9,6 +9,7 @@
 
 #include "gemm_pingpong.hpp"
 #include "int8_args.hpp"
+#include "int8_quantize.hpp"
 
 namespace viola {
 
@@ -62,10 +63,87 @@ __device__ __forceinline__ void store_int8_tile(const i32x16 (&total)[S::TN][S::
     }
 }
 
+// The same for the product dh of a gated activation's backward pass: dz = [dh u act'(g) | dh act(g)], dh in 32 bits from the wave's part of the ring, z read and dz written in
+// pieces of eight columns along the rows. On pairs of blocks, one's activations under the other's products: 32768 rows at 64 experts, 1024 -> 1024, 140 us, as two passes 93 and 65,
+// on tiles of 256 x 256, whose only block does nothing beside it, 158. Sums of more than GATED_MOST_K are two passes: there the larger tiles win more (.6 us for 64 k of
+// 65536 results on a CU) than dh out and back in 32 bits costs.
+template <typename S, typename TO>
+__device__ __forceinline__ void store_int8_gradient(const i32x16 (&total)[S::TN][S::TM], const Int8Args& p, int64_t m_begin, int64_t m_end, int64_t n_begin, uint8_t* ring,
+                                                    const float* columns) {
+    const int lane = threadIdx.x % WAVE, l32 = lane % 32, lhi = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE), wm = wave / S::WN, wn = wave % S::WN;
+    constexpr int COLS_W = 32 * S::TN, PLD = COLS_W + 4, PIECES = COLS_W / 8, TURNS = 32 * PIECES / WAVE;
+    static_assert(8 * 32 * PLD * 4 <= S::STAGES * S::STAGE);
+    float* park = reinterpret_cast<float*>(ring) + wave * 32 * PLD;
+    const int64_t ncol0 = n_begin + wn * COLS_W;
+#pragma unroll
+    for (int j = 0; j < S::TM; ++j) {
+        const int64_t row0 = m_begin + (wm * S::TM + j) * 32;
+        Raw8<TO> g[TURNS], u[TURNS];
+#pragma unroll
+        for (int it = 0; it < TURNS; ++it) {
+            const int id = it * WAVE + lane;
+            const int64_t row = row0 + id / PIECES, col = ncol0 + id % PIECES * 8;
+            const TO* z = static_cast<const TO*>(p.z) + row * p.z_pitch + col;
+            const int left = (int)(p.n - col < 8 ? p.n - col : 8);
+            if (row >= m_end || left <= 0) continue;
+            g[it].load(z, 0, left);
+            u[it].load(z + p.n, 0, left);
+        }
+        const float sa = row0 + l32 < m_end ? p.sa[row0 + l32] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 sb = *reinterpret_cast<const float4*>(&columns[(wn * S::TN + i) * 32 + q * 8 + lhi * 4]);
+                *reinterpret_cast<float4*>(&park[l32 * PLD + i * 32 + q * 8 + lhi * 4]) =
+                    make_float4((float)total[i][j][4 * q] * sa * sb.x, (float)total[i][j][4 * q + 1] * sa * sb.y, (float)total[i][j][4 * q + 2] * sa * sb.z,
+                                (float)total[i][j][4 * q + 3] * sa * sb.w);
+            }
+#pragma unroll
+        for (int it = 0; it < TURNS; ++it) {
+            const int id = it * WAVE + lane;
+            const int64_t row = row0 + id / PIECES, col = ncol0 + id % PIECES * 8;
+            const float4 low = *reinterpret_cast<const float4*>(&park[id / PIECES * PLD + id % PIECES * 8]), high = *reinterpret_cast<const float4*>(&park[id / PIECES * PLD + id % PIECES * 8 + 4]);
+            if (row >= m_end || col >= p.n) continue;
+            const float d[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};
+            float gate[8], up[8];
+            g[it].widen(gate);
+            u[it].widen(up);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float act, derivative;
+                gate_math(p.activation, gate[e], act, derivative);
+                gate[e] = d[e] * up[e] * derivative;
+                up[e] = d[e] * act;
+            }
+            TO* dz = static_cast<TO*>(p.out) + row * p.ldo + col;
+            if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    store_piece(dz + e, col + e, p.n, make_uint4(__float_as_uint(gate[e]), __float_as_uint(gate[e + 1]), __float_as_uint(gate[e + 2]), __float_as_uint(gate[e + 3])));
+                    store_piece(dz + p.n + e, col + e, p.n, make_uint4(__float_as_uint(up[e]), __float_as_uint(up[e + 1]), __float_as_uint(up[e + 2]), __float_as_uint(up[e + 3])));
+                }
+            } else {
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = narrow16<TO>(gate[2 * e]) | narrow16<TO>(gate[2 * e + 1]) << 16;
+                    w[4 + e] = narrow16<TO>(up[2 * e]) | narrow16<TO>(up[2 * e + 1]) << 16;
+                }
+                store_piece(dz, col, p.n, make_uint4(w[0], w[1], w[2], w[3]));
+                store_piece(dz + p.n, col, p.n, make_uint4(w[4], w[5], w[6], w[7]));
+            }
+        }
+    }
+}
+
+constexpr int64_t GATED_MOST_K = 2048;
+
 template <typename S> constexpr int int8_lds() { return S::STAGES * S::STAGE + 2 * S::COLS * 4; }
 
 // Rows [m_begin, m_end) of one group and the columns from n_begin on.
-template <typename S>
+template <typename S, bool GATED>
 __device__ __forceinline__ void int8_tile(const Int8Args& p, int group, int64_t m_begin, int64_t m_end, int64_t n_begin, uint8_t* lds) {
     constexpr int TM = S::TM, TN = S::TN, STAGES = S::STAGES, RING = STAGES * S::STAGE, HALVES = S::HALVES;
     static_assert(S::TEAMS == 1);
@@ -204,21 +282,25 @@ __device__ __forceinline__ void int8_tile(const Int8Args& p, int group, int64_t 
     if (!late) barrier();
     __builtin_amdgcn_s_waitcnt(0x0F70);                                      // the trailing loads must not land in what follows
     __syncthreads();                                                         // every wave has left the ring, and the columns' scales are there
-    if (p.out_dtype == VIOLA_F32) store_int8_tile<S>(total, p, static_cast<float*>(p.out), m_begin, m_end, n_begin, lds, columns);
+    if constexpr (GATED) {
+        if (p.out_dtype == VIOLA_F32) store_int8_gradient<S, float>(total, p, m_begin, m_end, n_begin, lds, columns);
+        else if (p.out_dtype == VIOLA_BF16) store_int8_gradient<S, bf16_t>(total, p, m_begin, m_end, n_begin, lds, columns);
+        else store_int8_gradient<S, f16_t>(total, p, m_begin, m_end, n_begin, lds, columns);
+    } else if (p.out_dtype == VIOLA_F32) store_int8_tile<S>(total, p, static_cast<float*>(p.out), m_begin, m_end, n_begin, lds, columns);
     else if (p.out_dtype == VIOLA_BF16) store_int8_tile<S>(total, p, static_cast<bf16_t*>(p.out), m_begin, m_end, n_begin, lds, columns);
     else store_int8_tile<S>(total, p, static_cast<f16_t*>(p.out), m_begin, m_end, n_begin, lds, columns);
 }
 
 // Rows that no group has, of one tile
-template <typename S, typename TO> __device__ __forceinline__ void int8_zeros(const Int8Args& p, int64_t m_begin, int64_t m_end, int64_t n_begin) {
+template <typename S, typename TO> __device__ __forceinline__ void int8_zeros(const Int8Args& p, int64_t m_begin, int64_t m_end, int64_t n_begin, int64_t shift) {
     constexpr int PER = 16 / (int)sizeof(TO), PIECES = S::COLS / PER;
     for (int i = threadIdx.x; i < S::ROWS * PIECES; i += S::THREADS) {
         const int64_t row = m_begin + i / PIECES, col = n_begin + i % PIECES * PER;
-        if (row < m_end && col < p.n) store_piece(static_cast<TO*>(p.out) + row * p.ldo + col, col, p.n, make_uint4(0, 0, 0, 0));
+        if (row < m_end && col < p.n) store_piece(static_cast<TO*>(p.out) + row * p.ldo + shift + col, col, p.n, make_uint4(0, 0, 0, 0));
     }
 }
 
-template <typename S, int WAVES_PER_SIMD> __global__ __launch_bounds__(512, WAVES_PER_SIMD) void int8_gemm(Int8Args p) {
+template <typename S, int WAVES_PER_SIMD, bool GATED> __global__ __launch_bounds__(512, WAVES_PER_SIMD) void int8_gemm(Int8Args p) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[int8_lds<S>()];
     // contiguous ranges for each XCD, of the tiles that there are: the host knows a bound on those of groups
     const int tiles_m = p.offsets ? int8_count_tiles(p, S::ROWS) : p.tiles_m, each = (tiles_m * p.tiles_n + 7) / 8;
@@ -231,9 +313,12 @@ template <typename S, int WAVES_PER_SIMD> __global__ __launch_bounds__(512, WAVE
     int group;
     int64_t m_begin, m_end;
     if (!int8_row_tile(p, first_m + t % across % rows_here, S::ROWS, group, m_begin, m_end)) return;
-    if (!p.offsets || group < p.groups) int8_tile<S>(p, group, m_begin, m_end, n_begin, lds);
-    else if (p.out_dtype == VIOLA_F32) int8_zeros<S, float>(p, m_begin, m_end, n_begin);
-    else int8_zeros<S, bf16_t>(p, m_begin, m_end, n_begin);                  // (zero is zero in either type of 16 bits)
+    if (!p.offsets || group < p.groups) int8_tile<S, GATED>(p, group, m_begin, m_end, n_begin, lds);
+    else
+        for (int64_t half = 0; half < (GATED ? 2 : 1); ++half) {             // (zero is zero in either type of 16 bits)
+            if (p.out_dtype == VIOLA_F32) int8_zeros<S, float>(p, m_begin, m_end, n_begin, half * p.n);
+            else int8_zeros<S, bf16_t>(p, m_begin, m_end, n_begin, half * p.n);
+        }
 }
 
 // 256 x 256 in four stages of 64 k, or in two of 128 k for long sums (16384 x 4096 -> 11008 668 and 690 us, 32768 rows at 16 experts of 4096 -> 1024 165 and 185, 4096 x 11008 -> 4096
@@ -244,13 +329,14 @@ using Int8M = PingPongShape<4, 2, 2, 2, 3, 128>;                             // 
 using Int8S = PingPongShape<2, 4, 2, 1, 3, 128>;                             // 128 x 128
 using Int8Pairs = PingPongShape<2, 4, 2, 1, 4>;                              // 128 x 128, two blocks on a CU
 
-template <typename S, int WAVES_PER_SIMD> static int launch_tiles(const Int8Args& args, hipStream_t stream) {
+template <typename S, int WAVES_PER_SIMD, bool GATED = false> static int launch_tiles(const Int8Args& args, hipStream_t stream) {
     Int8Args p = args;
     const int64_t tiles_m = int8_row_tiles(p, S::ROWS), tiles_n = (p.n + S::COLS - 1) / S::COLS;
     if (tiles_m * tiles_n >= (int64_t{1} << 30)) return VIOLA_ETOOLARGE;
     p.tiles_m = (int)tiles_m;
     p.tiles_n = (int)tiles_n;
-    VIOLA_LAUNCH((int8_gemm<S, WAVES_PER_SIMD>), dim3((unsigned)((tiles_m * tiles_n + 7) / 8 * 8)), 512, 0, stream, p);
+    const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8));
+    VIOLA_LAUNCH((int8_gemm<S, WAVES_PER_SIMD, GATED>), grid, 512, 0, stream, p);
     return viola_launch_status();
 }
 
@@ -274,8 +360,8 @@ static Int8TileShape choose_int8_tile(const Int8Args& p) {
 }
 
 static int launch_int8(const Int8Args& p, hipStream_t stream) {
-    const int status = launch_int8_rows(p, stream);
-    if (status != VIOLA_EUNSUPPORTED) return status;
+    if (p.z) return launch_tiles<Int8Pairs, 4, true>(p, stream);
+    if (int8_rows_fit(p)) return launch_int8_rows(p, stream);
     switch (choose_int8_tile(p)) {
         case INT8_L: return p.k > 8192 ? launch_tiles<Int8Long, 2>(p, stream) : launch_tiles<Int8L, 2>(p, stream);
         case INT8_M: return launch_tiles<Int8M, 2>(p, stream);
@@ -288,18 +374,43 @@ static int launch_int8(const Int8Args& p, hipStream_t stream) {
 
 using namespace viola;
 
+namespace {
+
+int product(Int8Args p, int64_t groups, hipStream_t stream) {
+    VIOLA_CHECK_ARG(p.m >= 0 && p.n > 0 && p.k > 0 && p.m < (int64_t{1} << 31) && p.n < (int64_t{1} << 30) && groups >= 0 && viola_is_float(p.out_dtype) &&
+                    (!p.bias || viola_is_float(p.bias_dtype)) && (!p.offsets || (groups > 0 && !p.bias)));
+    if (p.k > INT8_MOST_K || groups > INT8_MOST_GROUPS) return VIOLA_EUNSUPPORTED;
+    if (p.m == 0) return 0;
+    VIOLA_CHECK_ARG(p.a && p.sa && p.b && p.out && p.lda >= p.k && p.ldb >= p.k && p.lda % 16 == 0 && p.ldb % 16 == 0 && p.lda <= 2 * INT8_MOST_K && p.b_stride % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0);
+    if (p.ldb > (int64_t{1} << 22)) return VIOLA_EUNSUPPORTED;               // rows of one tile within 32 bits
+    p.k = (p.k + 15) / 16 * 16;
+    p.groups = (int)groups;
+    return launch_int8(p, stream);
+}
+
+}  // namespace
+
 extern "C" int viola_int8_gemm(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, int64_t b_stride, const float* sb, const int32_t* offsets,
                                int64_t groups, int64_t m, int64_t n, int64_t k, const void* bias, int bias_dtype, void* out, int out_dtype, viola_stream_t stream_) {
     hipStream_t stream = viola_enter(stream_);
-    VIOLA_CHECK_ARG(m >= 0 && n > 0 && k > 0 && m < (int64_t{1} << 31) && n < (int64_t{1} << 31) && groups >= 0 && groups < (int64_t{1} << 16) && viola_is_float(out_dtype) &&
-                    (!bias || viola_is_float(bias_dtype)) && (!offsets || (groups > 0 && !bias)));
-    if (k > INT8_MOST_K) return VIOLA_EUNSUPPORTED;
-    if (m == 0) return 0;
-    VIOLA_CHECK_ARG(a && sa && b && out && lda >= k && ldb >= k && lda % 16 == 0 && ldb % 16 == 0 && lda <= 2 * INT8_MOST_K && b_stride % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(b) % 16 == 0);
-    if (ldb > (int64_t{1} << 22)) return VIOLA_EUNSUPPORTED;                  // rows of one tile within 32 bits
     Int8Args p = {};
-    p.a = a; p.b = b; p.sa = sa; p.sb = sb; p.bias = bias; p.out = out; p.m = m; p.n = n; p.k = (k + 15) / 16 * 16;
-    p.lda = lda; p.ldb = ldb; p.ldo = n; p.offsets = offsets; p.groups = (int)groups; p.b_stride = b_stride; p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
-    return launch_int8(p, stream);
+    p.a = a; p.b = b; p.sa = sa; p.sb = sb; p.bias = bias; p.out = out; p.m = m; p.n = n; p.k = k;
+    p.lda = lda; p.ldb = ldb; p.ldo = n; p.offsets = offsets; p.b_stride = b_stride; p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
+    return product(p, groups, stream);
+}
+
+extern "C" int viola_int8_gemm_gated_backward(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, int64_t b_stride, const int32_t* offsets,
+                                              int64_t groups, int64_t m, int64_t n, int64_t k, const void* z, int64_t z_pitch, int z_dtype, int activation, void* dz,
+                                              viola_stream_t stream_) {
+    hipStream_t stream = viola_enter(stream_);
+    VIOLA_CHECK_ARG(activation >= 0 && activation <= VIOLA_RELU && m >= 0 && n > 0 && z_pitch >= 2 * n);
+    Int8Args p = {};
+    p.a = a; p.b = b; p.sa = sa; p.out = dz; p.m = m; p.n = n; p.k = k; p.lda = lda; p.ldb = ldb; p.ldo = 2 * n; p.offsets = offsets; p.b_stride = b_stride;
+    p.out_dtype = z_dtype; p.z = z; p.z_pitch = z_pitch; p.activation = activation;
+    if (m == 0 && viola_is_float(z_dtype)) return 0;
+    VIOLA_CHECK_ARG(z);
+    p.groups = groups > 0 && groups <= INT8_MOST_GROUPS ? (int)groups : 1;
+    if (int8_rows_fit(p) || k > GATED_MOST_K) return VIOLA_EUNSUPPORTED;      // two calls
+    return product(p, groups, stream);
 }

@@ -193,7 +193,7 @@ template <int MT, int NT, typename T> __global__ __launch_bounds__(64 * ROWS_WAV
 
 template <int MT, int NT, typename T> static int launch_rows(const Int8Args& p, const FusedArgs& f, hipStream_t stream) {
     const int64_t tiles = (p.n + 16 * NT - 1) / (16 * NT), row_tiles = int8_row_tiles(p, 16 * MT), steps = (p.k + 127) / 128;
-    if (row_tiles >= 65536) return VIOLA_EUNSUPPORTED;
+    if (row_tiles >= 65536) return VIOLA_ETOOLARGE;                          // (groups and 16 rows each at most: fewer)
     // wavefronts that share a tile: as many as give every SIMD four, at least a step each
     const int64_t real = p.offsets ? p.m / (16 * MT) + (p.groups < p.m ? p.groups : p.m) : row_tiles;       // about
     int ks = ROWS_WAVES;
@@ -208,11 +208,10 @@ template <int MT, int NT, typename T> static int launch_rows(const Int8Args& p, 
 // each 16 or 32 rows read the weights again. us, here and there: 64 x 4096 -> 4096 15 and 22, 128 x 4096 -> 4096 26 and 24, 128 x 4096 -> 1024 9 and 23, 64 x 4096 -> 11008 29 and 24; of groups,
 // 4 rows each of 64 4096 -> 2048 98 and 157, 16 each 158 and 166, 31 each of 128 2048 -> 1024 124 and 89. Four tiles of channels for a wavefront share the loads of x where
 // there are wavefronts enough without them: 32 x 4096 -> 11008 19 and 23 us, 32 x 4096 -> 4096 17 and 11.
+bool int8_rows_fit(const Int8Args& p) { return p.offsets ? p.m <= 16 * (int64_t)p.groups : p.m <= 32 || (p.m <= 512 && p.m * p.n <= 393216); }
 int launch_int8_rows(const Int8Args& p, hipStream_t stream) {
     const FusedArgs none = {};
-    if (p.offsets) return p.m <= 16 * (int64_t)p.groups ? launch_rows<1, 1, void>(p, none, stream) : VIOLA_EUNSUPPORTED;
-    if (p.m > 32 && (p.m > 512 || p.m * p.n > 393216)) return VIOLA_EUNSUPPORTED;
-    if (p.m <= 16) return launch_rows<1, 1, void>(p, none, stream);
+    if (p.offsets || p.m <= 16) return launch_rows<1, 1, void>(p, none, stream);
     return p.n >= 8192 ? launch_rows<2, 4, void>(p, none, stream) : launch_rows<2, 1, void>(p, none, stream);
 }
 
