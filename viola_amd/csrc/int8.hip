@@ -62,6 +62,18 @@ template <typename T, int MODE> __device__ __forceinline__ void value8(const Qua
     }
 }
 
+typedef float loose_floats4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void store_sums(float* to, int c, int cols, const float (&sums)[8]) {
+    if (c + 8 <= cols) {
+        *reinterpret_cast<loose_floats4*>(to + c) = loose_floats4{sums[0], sums[1], sums[2], sums[3]};
+        *reinterpret_cast<loose_floats4*>(to + c + 4) = loose_floats4{sums[4], sums[5], sums[6], sums[7]};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (c + i < cols) to[c + i] = sums[i];
+}
+
 constexpr int threads_of(int waves) { return waves <= 4 ? 256 : 64 * waves; }
 
 // The largest magnitude of a row of WAVES wavefronts, in all of them: two sets of slots in turn, so one barrier a row is enough
@@ -201,12 +213,7 @@ template <typename T, int WAVES, int PIECES, bool SUMS> __global__ __launch_boun
         }
         float* to = a.partial + (int64_t)blockIdx.x * a.cols;
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-            const int c = (p * THREADS + t) * 8;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < a.cols) to[c + i] = sums[p][i];
-        }
+        for (int p = 0; p < PIECES; ++p) store_sums(to, (p * THREADS + t) * 8, a.cols, sums[p]);
     }
 }
 
@@ -257,23 +264,18 @@ template <typename T, int MODE> __global__ __launch_bounds__(512) void quantize_
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sums[i] += raw[i];
         }
-        if (MODE == SCALED && a.partial)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < a.cols) a.partial[(int64_t)blockIdx.x * a.cols + c + i] = sums[i];
+        if (MODE == SCALED && a.partial) store_sums(a.partial + (int64_t)blockIdx.x * a.cols, c, a.cols, sums);
     }
 }
 
-// How rows are shared: wavefronts of a row, rows of a block (SCALED: as many as leave SCALED_BLOCKS), blocks.
+// How rows are shared: wavefronts of a row, rows of a block, blocks. x times factors: as many rows as leave 1024 blocks, or 512 where each leaves a row of sums
+// (8192 x 4096: 21 us, 27 with 512 blocks; with sums and their reduction 30, 35 with 1024).
 struct Shares {
     int waves, pieces;                                                       // 0 wavefronts: long rows
     int64_t per_block, blocks;
 };
-#ifndef SB
-#define SB 1024
-#endif
-constexpr int64_t SCALED_BLOCKS = SB;
-Shares shares_of(int64_t rows, int64_t cols, bool scaled) {
+enum Purpose { ONCE, SCALE, SCALE_AND_SUM };
+Shares shares_of(int64_t rows, int64_t cols, Purpose purpose) {
     Shares s = {};
     if (cols > 16384) {
         s.per_block = LONG_ROWS;
@@ -282,14 +284,15 @@ Shares shares_of(int64_t rows, int64_t cols, bool scaled) {
         const int64_t piece = 512 * s.waves;                                 // values that the row's threads have at once
         s.pieces = cols <= piece ? 1 : cols <= 2 * piece ? 2 : 4;
         s.per_block = s.waves == 1 ? 4 : 1;
-        if (scaled && rows > SCALED_BLOCKS * s.per_block) s.per_block *= (rows + SCALED_BLOCKS * s.per_block - 1) / (SCALED_BLOCKS * s.per_block);
+        const int64_t most = s.per_block * (purpose == SCALE ? 1024 : 512);
+        if (purpose != ONCE && rows > most) s.per_block *= (rows + most - 1) / most;
     }
     s.blocks = (rows + s.per_block - 1) / s.per_block;
     return s;
 }
 
 template <typename T, int MODE> int launch(QuantizeArgs& a, hipStream_t stream) {
-    const Shares s = shares_of(a.rows, a.cols, MODE == SCALED);
+    const Shares s = shares_of(a.rows, a.cols, MODE != SCALED ? ONCE : a.partial ? SCALE_AND_SUM : SCALE);
     a.per_block = s.per_block;
     if (s.blocks >= (int64_t{1} << 31)) return VIOLA_ETOOLARGE;
     const dim3 grid((unsigned)s.blocks);
@@ -370,7 +373,7 @@ template <typename T> __global__ __launch_bounds__(256) void gated_gradient_kern
 
 }  // namespace
 
-extern "C" int64_t viola_int8_sum_parts(int64_t rows, int64_t cols) { return rows <= 0 || cols <= 0 ? 0 : shares_of(rows, cols, true).blocks; }
+extern "C" int64_t viola_int8_sum_parts(int64_t rows, int64_t cols) { return rows <= 0 || cols <= 0 ? 0 : shares_of(rows, cols, SCALE_AND_SUM).blocks; }
 
 extern "C" int viola_int8_quantize(const void* x, int64_t pitch, int dtype, int64_t rows, int64_t cols, int activation, const float* factors, const int32_t* offsets,
                                    int64_t groups, int8_t* codes, int64_t code_pitch, float* scales, float* partial, viola_stream_t stream_) {
