@@ -121,7 +121,7 @@ def test_ways_of_a_product(tokens, width, out):
 def test_few_rows_are_quantized_as_many(dtype, activation):
     """The same bits from one launch as from two, at any address of x."""
     from viola_amd import nn
-    for tokens, width, out in ((1, 1024, 100), (3, 2560, 33), (8, 1024, 64), (15, 48, 17)):
+    for tokens, width, out in ((1, 1024, 100), (3, 2560, 33), (2, 4096, 40), (4, 2032, 65), (8, 1024, 64), (15, 48, 17)):
         w, sw = _weights(out, width)
         store = _rows(600, 2 * width + 3, dtype).clamp(-30, 30)
         cols = width * (2 if activation else 1)
@@ -422,3 +422,109 @@ def test_a_mixture_of_experts(tokens):
             assert oi.within(out_rows[a:b], *oi.forward(z.detach()[a:b], down[e], sdown[e] * 0.05, None, "silu"))
     dx, dl = torch.autograd.grad(y, [x, logits], _rows(tokens, width, BF16, seed=4))
     assert torch.isfinite(dx).all() and torch.isfinite(dl).all() and dx.abs().max() > 0 and (tokens == 1 or dl.abs().max() > 0)
+
+
+@pytest.mark.parametrize("shape,width,inner", [((2, 61), 100, 72), ((3, 400), 128, 160), ((5, 1), 96, 40)])
+def test_a_balanced_mixture_of_experts(shape, width, inner):
+    """A router with a bias and groups over a padded batch, its rows through `Int8Experts`, and back: each step's forward and gradient against the formulas, on what the step was given."""
+    from oracle import routing as ro
+    from viola_amd import nn
+    torch.manual_seed(shape[1])
+    experts, top_k = 32, 6
+    up = nn.Int8Experts.from_float(torch.randn(experts, 2 * inner, width, device="cuda") * 0.1, cache_transpose=True)
+    down = nn.Int8Experts.from_float(torch.randn(experts, width, inner, device="cuda") * 0.1, activation="silu")
+    tokens = shape[0] * shape[1]
+    x = _rows(tokens, width, BF16).reshape(*shape, width).requires_grad_()
+    logits = torch.randn(*shape, experts, device="cuda", requires_grad=True)
+    bias = torch.randn(experts, device="cuda") * 0.1
+    mask = torch.rand(shape, device="cuda") < 0.8
+    mask[0, 0] = True
+    r = nn.route(logits, top_k, score="sigmoid", bias=bias, groups=8, top_groups=4, group_top=2, mask=mask, per_sequence=True)
+    chosen = ro.choose_steered(logits.detach().cpu(), top_k, "sigmoid", mask.cpu(), bias.cpu(), 8, 4, 2)
+    assert torch.equal(r.experts.cpu().long(), chosen)
+    rows = nn.dispatch(x, r)
+    z = up(rows, r.offsets)
+    out_rows = down(z, r.offsets)
+    y = nn.combine(out_rows, r)
+    dy = _rows(tokens, width, BF16, seed=4).reshape(*shape, width)
+    d_rows, dz, d_out, dx, dl = torch.autograd.grad((y, r.balance), (rows, z, out_rows, x, logits), (dy, torch.ones((), device="cuda")))
+    bounds = r.offsets.tolist()
+    for e in range(experts):
+        a, b = bounds[e], bounds[e + 1]
+        if a < b:
+            assert oi.within(z[a:b], *oi.forward(rows.detach()[a:b], up.weight[e], up.weight_scale[e]))
+            assert oi.within(out_rows[a:b], *oi.forward(z.detach()[a:b], down.weight[e], down.weight_scale[e], None, "silu"))
+            assert oi.within(dz[a:b], *oi.backward(d_out[a:b], down.weight[e], down.weight_scale[e], z.detach()[a:b], "silu"))
+            assert oi.within(d_rows[a:b], *oi.backward(dz[a:b], up.weight[e], up.weight_scale[e]))
+    for t in (z, out_rows, dz, d_rows):
+        assert (t[bounds[-1]:] == 0).all()
+    there = r.positions.cpu() >= 0
+    gates, places = r.gates.detach().cpu().double() * there, r.positions.cpu().long().clamp(min=0)
+
+    def sums(t, by):                                                         # top_k products and as many sums in 32 bits
+        picked = t.detach().cpu().double()[places] * by[..., None]
+        return picked.sum(-2), 2 * top_k * oi.U * picked.abs().sum(-2)
+
+    assert oi.within(y.cpu(), *sums(out_rows, gates)) and oi.within(dx.cpu(), *sums(d_rows, there.double()))
+    assert (y[~mask] == 0).all() and (dx[~mask] == 0).all() and (dl[~mask] == 0).all()
+    # a gate's gradient is a dot product of `width` terms; what the logits' makes of its error is at most that error times the gate's slope, which is below one
+    dots = (out_rows.detach().cpu().double()[places] * dy.cpu().double()[..., None, :])
+    dgates, off = dots.sum(-1) * there, ((width + 1) * oi.U * dots.abs().sum(-1) * there).sum(-1, keepdim=True)
+    expected = ro.gradient(logits.detach().cpu(), chosen, "sigmoid", mask.cpu(), True, dloss=1.0, dgates=dgates)
+    spread = (dgates.abs().sum(-1, keepdim=True) + 1.0) * (4 * experts * oi.U)
+    assert ((dl.cpu().double() - expected).abs() <= off + spread).all()
+
+
+def test_a_served_mixture_is_replayed():
+    """A decoding step of router, experts and combine in one graph: new tokens, a new bias and other places by each replay, with eager work in between."""
+    from viola_amd import nn
+    torch.manual_seed(7)
+    experts, width, inner, tokens = 64, 128, 96, 12
+    up = nn.Int8Experts.from_float(torch.randn(experts, 2 * inner, width, device="cuda") * 0.1)
+    down = nn.Int8Experts.from_float(torch.randn(experts, width, inner, device="cuda") * 0.1, activation="silu")
+    head = nn.Int8Linear.from_float(torch.nn.Linear(width, 70, device="cuda"))
+    x, logits, bias = _rows(tokens, width, BF16), torch.randn(tokens, experts, device="cuda"), torch.zeros(experts, device="cuda")
+
+    def step():                                                              # bias of `head` is a parameter: gradients are recorded, and only their pass has to be eager
+        r = nn.route(logits, 8, score="sigmoid", bias=bias, groups=8, top_groups=3, group_top=2)
+        return head(nn.combine(down(up(nn.dispatch(x, r), r.offsets), r.offsets), r)).detach(), r.experts
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for replay in range(4):
+        x.copy_(_rows(tokens, width, BF16, seed=replay + 20))
+        logits.copy_(torch.randn(tokens, experts))
+        bias.copy_(torch.randn(experts) * 0.1)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, step()):
+            assert torch.equal(a, b)
+
+
+def test_a_captured_backward_pass_is_refused():
+    """No eager graph of these leaves is alive, and the capture ends in order: refused by the nodes themselves before they launch anything."""
+    from viola_amd import nn
+    w, sw = _weights(48, 64)
+    x, logits = _rows(20, 64, BF16).requires_grad_(), torch.randn(20, 16, device="cuda", requires_grad=True)
+    bias = torch.zeros(16, device="cuda")
+    dy, dg = _rows(20, 48, BF16, seed=2), torch.ones(20, 4, device="cuda")
+    with torch.no_grad():
+        nn.int8_linear(x, w, sw), nn.route(logits, 4, bias=bias)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        y, gates = nn.int8_linear(x, w, sw), nn.route(logits, 4, bias=bias).gates
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            torch.autograd.grad(y, x, dy)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            torch.autograd.grad(gates, logits, dg)
+    torch.cuda.synchronize()
+    dx, = torch.autograd.grad(nn.int8_linear(x, w, sw), x, dy)
+    assert oi.within(dx, *oi.backward(dy, w, sw))

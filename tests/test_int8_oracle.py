@@ -112,7 +112,7 @@ def test_rejected_calls_launch_nothing():
     r = lambda **c: lib.viola_int8_rows_linear(*{**dict(x=P, pitch=64, dtype=BF16, m=4, k=64, act=-1, b=P, ldb=64, sb=P, n=8, bias=None, bt=F32, out=P, ot=BF16), **c}.values(), None)  # noqa: E731
     for bad in (dict(dtype=E4M3), dict(pitch=63), dict(act=0), dict(act=3), dict(ldb=48), dict(ldb=72), dict(n=0), dict(sb=None), dict(b=P + 8), dict(out=None), dict(bias=P, bt=E4M3)):
         assert r(**bad) == -1, bad
-    assert r(m=0) == 0 and r(m=17) == -2 and r(k=40) == -2 and r(m=8, k=4096, pitch=4096, ldb=4096) == -2
+    assert r(m=0) == 0 and r(m=17) == -2 and r(m=5) == -2 and r(k=40) == -2 and r(m=8, k=4096, pitch=4096, ldb=4096) == -2
     b = lambda **c: lib.viola_int8_gated_backward(*{**dict(z=P, pitch=64, dtype=BF16, rows=4, cols=32, act=0, dh=P, total=None, dz=P), **c}.values(), None)  # noqa: E731
     for bad in (dict(dtype=E4M3), dict(pitch=63), dict(act=-1), dict(act=3), dict(dh=None), dict(dz=None), dict(rows=-1)):
         assert b(**bad) == -1, bad

@@ -127,6 +127,12 @@ inline void check_float(const char* name, const char* what, const Tensor& t, con
 
 // The gradients of these nodes are computed by kernels that autograd does not see.
 inline void check_once(const char* name) { TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), name, " can be differentiated once only (create_graph is not supported)"); }
+// A backward pass under capture ends the process where an eager graph of the same leaves lives (its accumulators stand on another stream), which a node cannot see: refused.
+inline void check_eager(const char* name, const Tensor& t) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    TORCH_CHECK(hipStreamIsCapturing(static_cast<hipStream_t>(stream_of(t)), &status) == hipSuccess, name, " could not ask for the state of its stream");
+    TORCH_CHECK(status == hipStreamCaptureStatusNone, name, ": a backward pass cannot be captured into a graph (a forward pass can)");
+}
 
 // Memory for a result: the allocator at once, without the dispatcher's two rounds (a router has up to eight results and workspaces, and a
 // decoding step's call of it takes as long on the host as on the GPU).

@@ -381,6 +381,7 @@ variable_list RouterBackward::apply(variable_list&& grads) {
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Device device = (d_gates.defined() ? d_gates : d_loss).device();
     const c10::DeviceGuard guard(device);
+    if (plan.groups) check_eager("route with a bias or groups", d_gates.defined() ? d_gates : d_loss);
     const Tensor l = logits.unpack();
     TORCH_CHECK(l.device() == device && l.scalar_type() == type && l.sizes() == at::IntArrayRef(shape), "the logits of a router were moved or replaced between forward and backward");
     result[0] = room(shape, type, device);

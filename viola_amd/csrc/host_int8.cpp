@@ -136,7 +136,7 @@ Tensor run(const char* name, const Tensor& x, const Tensor& weight, const Tensor
             const Tensor channels = scale.contiguous(), b = bias.defined() ? bias.contiguous() : Tensor();
             const float* channel_data = static_cast<const float*>(channels.const_data_ptr());
             int status = VIOLA_EUNSUPPORTED;
-            if (!grouped && plan.rows <= 16) {                               // few rows: quantized on the way into the product
+            if (!grouped && plan.rows <= 4) {                                // few rows: quantized on the way into the product
                 status = VIOLA_TRY(viola_int8_rows_linear, rows.data(), rows.pitch, code_of(plan.x_type), plan.rows, plan.k, activation, w.data(), w.pitch, channel_data, plan.n,
                                    ptr(b), b.defined() ? code_of(b.scalar_type()) : VIOLA_F32, out.mutable_data_ptr(), code_of(plan.out_type), stream);
                 if (status != VIOLA_EUNSUPPORTED) check("viola_int8_rows_linear", status);
@@ -180,6 +180,7 @@ variable_list ProductBackward::apply(variable_list&& grads) {
     const Tensor& dy = grads[0];
     const at::Device device = dy.device();
     const c10::DeviceGuard guard(device);
+    check_eager(label.c_str(), dy);
     const auto options = at::TensorOptions().device(device);
     if (!plan.rows) {
         if (needs_x) result[0] = at::empty(shape, options.dtype(plan.x_type));

@@ -10,7 +10,7 @@ namespace viola {
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int ROWS_WAVES = 4;
-constexpr int FUSED_ROWS = 16;
+constexpr int FUSED_ROWS = 4;
 struct FusedArgs {
     const void* x;
     int64_t pitch;
@@ -21,7 +21,9 @@ struct FusedArgs {
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // The quantizer of a block: rows are cut into parts of 512 values, eight for each lane, and the wavefronts take the parts in turn, FUSED_PIECES each at most. They are
-// loaded before the first weights, so that those are not waited for.
+// loaded before the first weights, so that those are not waited for. Every block makes all of them, so more rows, or wider ones, take longer than as two launches: us with 4096 channels,
+// here and as two, 4 x 1024 6.7 and 8.0, 4 x 2048 8.5 and 10.4, 2 x 4096 12.0 and 11.0 (with 11008 14.7 and 15.8), 8 x 1024 8.1 and 8.3 (with 11008 11.9 and 9.6), 4 x 4096 17.0 and
+// 11.2; with 1024 channels 16 x 256 9.5 and 7.9.
 constexpr int FUSED_PIECES = 4;
 inline bool fused_fits(int64_t rows, int64_t cols) { return rows <= FUSED_ROWS && cols % 16 == 0 && rows * ((cols + 511) / 512) <= ROWS_WAVES * FUSED_PIECES; }
 template <typename T> struct FusedRows {
