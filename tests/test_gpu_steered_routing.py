@@ -219,3 +219,13 @@ def test_large_batches_are_chosen_as_small_ones():
             kept = torch.zeros_like(rank).scatter_(-1, torch.sort(rank, descending=True, stable=True).indices[:, :4], 1.0)
             c = torch.where(kept.repeat_interleave(experts // 8, -1) > 0, c, -math.inf)
             assert torch.equal(torch.sort(c, descending=True, stable=True).indices[:, :6].int(), r.experts)
+
+
+@pytest.mark.parametrize("far", [-86.0, -100.0, -300.0])
+@pytest.mark.parametrize("experts,groups", [(8, 1), (32, 4), (256, 8), (600, 1)])
+def test_scores_below_the_smallest_float(far, experts, groups):
+    """Sigmoids that 32 bits cannot hold beside biases of zero, or of next to nothing, are ordered in 64."""
+    torch.manual_seed(14)
+    logits = far + torch.randn(50, experts)
+    for bias in (torch.zeros(experts), -torch.zeros(experts), torch.randint(-3, 4, (experts,)) * 2.0 ** -149, torch.randn(experts) * 2.0 ** -130):
+        _check(logits, min(6, experts), bias=bias, groups=groups, top_groups=max(1, groups // 2), group_top=2)

@@ -147,7 +147,7 @@ __device__ __forceinline__ double over_wave(double v, int step) {
 }
 
 // The choice of one row in 64 bits, by a whole wavefront that has experts lane, lane + 64, ..; into chosen and values (logits), top_k each. c: [experts] in the
-// wavefront's own LDS. A function of its own, as inlined the exponential's constants stay in registers all through the kernel, which has none to spare.
+// wavefront's own LDS. It runs at the end of a stage, where little else has to be kept in registers.
 struct ExactChoice {
     const void* row;
     const float* bias;
@@ -624,7 +624,7 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                         // Keys give their last bits to say which of the lane's values they are of, are sorted within the lane, and each choice is the largest head, which its
                         // lane takes off its list. (Of 256 experts 38 operations to sort and some 35 for a choice, which otherwise takes 80.)
                         constexpr uint32_t LAST = VALUES - 1;
-                        constexpr float CUT = VALUES * 0x1p-23f;             // of a key without its last bits
+                        constexpr float CUT = VALUES * 0x1p-23f, TINY = 0x1p-126f;           // of a key without its last bits, in a normal number and in a subnormal one
 #pragma unroll
                         for (int i = 0; i < VALUES; ++i) key[i] = open[i] && c[i] > -__builtin_inff() ? (key_of(c[i]) & ~LAST) | (LAST - i) : 0;
                         sort_down(key);
@@ -634,7 +634,7 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                             const uint32_t head = lanes_max<LANES>(key[0]);
                             const float v = value_of(head);
                             // (infinite biases tie: their order is the exact one's too)
-                            near = near || head >= 0xff800000u || (j && head && before - v <= (0x1p-24f + CUT) * (fabsf(before) + fabsf(v)) + 2.0f * NEAR<SIGMOID> * largest);
+                            near = near || head >= 0xff800000u || (j && head && before - v <= (0x1p-24f + CUT) * (fabsf(before) + fabsf(v)) + 2.0f * NEAR<SIGMOID> * largest + TINY);
                             before = v;
                             if (j == a.top_k) break;
                             const int owner = first_lane<LANES>(__ballot(key[0] == head));       // of equal heads the row is near
