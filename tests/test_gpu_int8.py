@@ -528,3 +528,29 @@ def test_a_captured_backward_pass_is_refused():
     torch.cuda.synchronize()
     dx, = torch.autograd.grad(nn.int8_linear(x, w, sw), x, dy)
     assert oi.within(dx, *oi.backward(dy, w, sw))
+
+
+def test_more_rows_than_one_row_of_blocks():
+    """2^26 and some rows of three values: more blocks of the quantizer than a grid has threads for in one dimension."""
+    from viola_amd import nn
+    rows = 2 ** 26 + 37
+    x = torch.randn(rows, 3, device="cuda", dtype=BF16)
+    w, sw = _weights(4, 3)
+    codes, scale = nn.quantize_int8(x)
+    y = nn.int8_linear(x, w, sw)
+    for part in (slice(0, 1000), slice(2 ** 22 - 500, 2 ** 22 + 500), slice(2 ** 25, 2 ** 25 + 1000), slice(rows - 1000, rows)):
+        q, s, _, _ = oi.quantize(x[part].double())
+        assert torch.equal(scale[part].double(), s[:, 0]) and torch.equal(codes[part].double(), q)
+        assert oi.within(y[part], *oi.forward(x[part], w, sw))
+
+
+def test_codes_loaded_on_the_cpu_are_turned_on_the_way():
+    from viola_amd import nn
+    source = nn.Int8Linear.from_float(torch.nn.Linear(40, 24, device="cuda"), cache_transpose=True)
+    layer = nn.Int8Linear(40, 24, cache_transpose=True)
+    layer.load_state_dict({name: t.cpu() for name, t in source.state_dict().items()})
+    assert layer.weight_t is None
+    layer.cuda()
+    assert torch.equal(layer.weight_t, source.weight_t)
+    x = _rows(9, 40, F32)
+    assert torch.equal(layer(x), source(x))

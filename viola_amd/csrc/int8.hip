@@ -98,7 +98,7 @@ template <typename T, int MODE, int WAVES, int PIECES> __global__ __launch_bound
     constexpr int THREADS = 64 * WAVES, TOGETHER = threads_of(WAVES) / THREADS;
     __shared__ uint32_t slots[2][threads_of(WAVES) / 64];
     const int t = threadIdx.x % THREADS;
-    const int64_t row = (int64_t)blockIdx.x * TOGETHER + threadIdx.x / THREADS;
+    const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * TOGETHER + threadIdx.x / THREADS;
     const bool here = row < a.rows;
     float v[PIECES][8];
     uint32_t most = 0;
@@ -292,11 +292,13 @@ Shares shares_of(int64_t rows, int64_t cols, Purpose purpose) {
     return s;
 }
 
+constexpr int64_t MOST_ACROSS = 1 << 20;                                     // blocks in a row of the grid, which takes fewer than 2^32 threads
 template <typename T, int MODE> int launch(QuantizeArgs& a, hipStream_t stream) {
     const Shares s = shares_of(a.rows, a.cols, MODE != SCALED ? ONCE : a.partial ? SCALE_AND_SUM : SCALE);
     a.per_block = s.per_block;
     if (s.blocks >= (int64_t{1} << 31)) return VIOLA_ETOOLARGE;
-    const dim3 grid((unsigned)s.blocks);
+    const int64_t across = MODE == SCALED || s.waves == 0 || s.blocks < MOST_ACROSS ? s.blocks : MOST_ACROSS;
+    const dim3 grid((unsigned)across, (unsigned)((s.blocks + across - 1) / across));
     auto with = [&](auto waves, auto pieces) {
         constexpr int WAVES = decltype(waves)::value, PIECES = decltype(pieces)::value;
         if constexpr (MODE != SCALED) VIOLA_LAUNCH((quantize_rows<T, MODE, WAVES, PIECES>), grid, threads_of(WAVES), 0, stream, a);

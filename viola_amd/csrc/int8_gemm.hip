@@ -333,7 +333,7 @@ using Int8Pairs = PingPongShape<2, 4, 2, 1, 4>;                              // 
 template <typename S, int WAVES_PER_SIMD, bool GATED = false> static int launch_tiles(const Int8Args& args, hipStream_t stream) {
     Int8Args p = args;
     const int64_t tiles_m = int8_row_tiles(p, S::ROWS), tiles_n = (p.n + S::COLS - 1) / S::COLS;
-    if (tiles_m * tiles_n >= (int64_t{1} << 30)) return VIOLA_ETOOLARGE;
+    if (tiles_m * tiles_n >= (int64_t{1} << 32) / 512 - 8) return VIOLA_ETOOLARGE;                // threads of a grid
     p.tiles_m = (int)tiles_m;
     p.tiles_n = (int)tiles_n;
     const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8));

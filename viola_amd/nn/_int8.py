@@ -96,6 +96,8 @@ class _Fixed(nn.Module):
         scale = self.weight_scale
         super()._apply(fn, recurse)
         self.weight_scale = scale.to(self.weight_scale.device)
+        if self.codes_t is None:                                             # loaded on the CPU
+            self._turn()
         return self
 
     def _load_from_state_dict(self, *args, **kwargs):
