@@ -109,7 +109,7 @@ def test_linear(tokens, width, out):
 
 
 @pytest.mark.parametrize("tokens,width,out", [(1, 8192, 40), (2, 4096, 65), (7, 2032, 33), (16, 512, 70), (16, 528, 70), (17, 1024, 130), (20, 1024, 9000), (32, 272, 8200), (48, 512, 700),
-                                              (130, 1024, 520), (512, 128, 768), (512, 128, 769), (513, 128, 700), (300, 9008, 200), (260, 8208, 272), (3000, 128, 3000), (9, 131072, 20)])
+                                              (130, 1024, 520), (512, 128, 768), (512, 128, 769), (513, 128, 700), (300, 9008, 200), (260, 8208, 272), (3000, 128, 3000), (9000, 200, 4200), (9, 131072, 20)])
 def test_ways_of_a_product(tokens, width, out):
     """Rows quantized on the way in, few rows, one to four tiles of channels a wavefront, tiles of each size, long sums: on the borders between them."""
     w, sw = _weights(out, width)

@@ -2,7 +2,7 @@
 //
 // The integers are multiplied by v_mfma_i32_32x32x32_i8, whose 32-bit sums are exact; the scales are applied to the finished sums in registers:
 // out = (sum * sa) * sb + bias, one rounding each. Bound by the matrix pipes (as many operations a cycle as FP8) and, on large products, by the power limit:
-// 16384 x 4096 -> 11008 645 to 680 us (2.2 POP/s), 4096 x 11008 -> 4096 143 (2.6), 8192 x 1024 -> 4096 46 (1.5: the results of a round of tiles leave at its end, 8.5 us of 23).
+// 16384 x 4096 -> 11008 645 to 680 us (2.2 POP/s), 4096 x 11008 -> 4096 143 (2.6), 8192 x 1024 -> 4096 46 (1.5: the results of a round of tiles leave at its end, some 9 us of 23).
 //
 // The tiles are those of gemm_pingpong.hpp: eight wavefronts, two on each SIMD, whose memory work and math alternate; a chunk of 128 k is two pairs of
 // instructions for each 32 x 32 sub-tile where FP8 has one of 64 k, and an operand's 16-byte pieces are in the instruction's own order.
@@ -329,6 +329,7 @@ using Int8Long = PingPongShape<2, 4, 4, 2, 2, 128>;
 using Int8M = PingPongShape<4, 2, 2, 2, 3, 128>;                             // 256 x 128
 using Int8S = PingPongShape<2, 4, 2, 1, 3, 128>;                             // 128 x 128
 using Int8Pairs = PingPongShape<2, 4, 2, 1, 4>;                              // 128 x 128, two blocks on a CU
+using Int8Wide = PingPongShape<4, 2, 2, 2, 3>;                               // 256 x 128, two blocks on a CU
 
 template <typename S, int WAVES_PER_SIMD, bool GATED = false> static int launch_tiles(const Int8Args& args, hipStream_t stream) {
     Int8Args p = args;
@@ -341,11 +342,12 @@ template <typename S, int WAVES_PER_SIMD, bool GATED = false> static int launch_
     return viola_launch_status();
 }
 
-// The tile that takes least by estimates in microseconds, fitted to measured times of 20 shapes and within 15 % of most. A round of a tile for each CU takes a fixed part and a time
-// for each chunk of 64 k, which grows with the share of CUs at work as the clock falls: L .42 to .84 + 8.5, M .30 to .47 + 5.3, S .24 to .29 + 4, two S on a CU .25 to
-// .73 + 4. Each group leaves half a row tile unfilled on average. So 8192 x 1024 -> 4096 takes L (47 us; M 57, S 66), 8192 x 4096 -> 1024 M (36; L 49, S 47), 2048 x 2048 ->
-// 2048 S (13; M 17), 9850 x 770 -> 1000 L (19; M 25), 4000 rows at 128 experts of 2048 -> 1024 pairs of S (61; L 69).
-enum Int8TileShape { INT8_L, INT8_M, INT8_S, INT8_PAIRS };
+// The tile that takes least by estimates in microseconds, fitted to measured times of 30 shapes and within 15 % of most. A round of a tile for each CU takes a fixed part and a time
+// for each chunk of 64 k, which grows with the share of CUs at work as the clock falls: L .42 to .84 + 9.5, M .30 to .47 + 6.3, S .24 to .29 + 4, two S on a CU .25 to
+// .73 + 4, two M 1 to 1.04 + 6.4 (one's ends under the other's products, slower ones: for short sums). Each group leaves half a row tile unfilled on average. So
+// 8192 x 1024 -> 4096 takes L (47 us; M 57, S 66), 8192 x 4096 -> 1024 M (35; L 49, S 47), 2048 x 2048 -> 2048 S (13; M 17), 9850 x 770 -> 1000 L (18; M 25), 4000 rows at 128
+// experts of 2048 -> 1024 pairs of S (61; L 69), 16384 x 512 -> 2048 pairs of M (28; L 33, pairs of S 34).
+enum Int8TileShape { INT8_L, INT8_M, INT8_S, INT8_PAIRS, INT8_WIDE };
 static Int8TileShape choose_int8_tile(const Int8Args& p) {
     const double chunks = (double)((p.k + 63) / 64);
     auto estimate = [&](int rows, int cols, int at_once, double idle, double busy, double fixed) {
@@ -353,10 +355,10 @@ static Int8TileShape choose_int8_tile(const Int8Args& p) {
         const double full = (double)(tiles / at_once), rest = (double)(tiles % at_once) / at_once;
         return full * (chunks * busy + fixed) + (rest > 0 ? chunks * (idle + (busy - idle) * rest) + fixed : 0.0);
     };
-    const double time[4] = {estimate(256, 256, 256, 0.42, 0.84, 8.5), estimate(256, 128, 256, 0.30, 0.47, 5.3), estimate(128, 128, 256, 0.24, 0.29, 4.0),
-                            estimate(128, 128, 512, 0.25, 0.73, 4.0)};
+    const double time[5] = {estimate(256, 256, 256, 0.42, 0.84, 9.5), estimate(256, 128, 256, 0.30, 0.47, 6.3), estimate(128, 128, 256, 0.24, 0.29, 4.0),
+                            estimate(128, 128, 512, 0.25, 0.73, 4.0), estimate(256, 128, 512, 1.0, 1.04, 6.4)};
     int best = 0;
-    for (int i = 1; i < 4; ++i) best = time[i] < time[best] ? i : best;
+    for (int i = 1; i < 5; ++i) best = time[i] < time[best] ? i : best;
     return (Int8TileShape)best;
 }
 
@@ -367,6 +369,7 @@ static int launch_int8(const Int8Args& p, hipStream_t stream) {
         case INT8_L: return p.k > 8192 ? launch_tiles<Int8Long, 2>(p, stream) : launch_tiles<Int8L, 2>(p, stream);
         case INT8_M: return launch_tiles<Int8M, 2>(p, stream);
         case INT8_S: return launch_tiles<Int8S, 2>(p, stream);
+        case INT8_WIDE: return launch_tiles<Int8Wide, 4>(p, stream);
         default: return launch_tiles<Int8Pairs, 4>(p, stream);
     }
 }
