@@ -65,7 +65,7 @@ __device__ __forceinline__ void store_int8_tile(const i32x16 (&total)[S::TN][S::
 }
 
 // The same for the product dh of a gated activation's backward pass: dz = [dh u act'(g) | dh act(g)], dh in 32 bits from the wave's part of the ring, z read and dz written in
-// pieces of eight columns along the rows. On pairs of blocks, one's activations under the other's products: 32768 rows at 64 experts, 1024 -> 1024, 140 us, as two passes 93 and 65,
+// pieces of eight columns along the rows. On pairs of blocks, one's activations under the other's products: 32768 rows at 64 experts, 1024 -> 1024, 102 to 125 us, as two passes 93 and 65,
 // on tiles of 256 x 256, whose only block does nothing beside it, 158. Sums of more than GATED_MOST_K are two passes: there the larger tiles win more (.6 us for 64 k of
 // 65536 results on a CU) than dh out and back in 32 bits costs.
 template <typename S, typename TO>

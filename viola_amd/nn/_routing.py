@@ -62,7 +62,7 @@ def route(logits, top_k, *, score="softmax", normalize=True, scale=1.0, mask=Non
     bias [experts]: the choice is by s + bias instead, s being the softmax's probability or sigmoid(logit); gates and balance remain those of s. A program that balances the load
     moves it after each step, for instance by bias += rate * torch.sign(counts.float().mean() - counts); it has no gradient. An expert whose bias is -inf or NaN is never chosen.
     groups: equal runs of experts (up to 64), of which a token's choice is open to the top_groups (all by default) of largest rank, ties to the lower run; a rank is the sum of the
-    group_top (1 or 2) largest s + bias of a run. Scores are compared as in 64 bits, ties to the lowest index. A row with a NaN logit (with softmax, +inf too) is
+    group_top (1 or 2) largest s + bias of a run; without a bias the choice among their experts is by the logits. Scores are compared as in 64 bits, ties to the lowest index. A row with a NaN logit (with softmax, +inf too) is
     chosen by its logits alone, as without bias and groups."""
     top_groups = groups if top_groups is None else top_groups
     experts, gates, positions, counts, offsets, balance = _lib.host().route(logits, top_k, _score(score), normalize, scale, mask, per_sequence, bias, _groups(groups), top_groups,
