@@ -104,6 +104,7 @@ def test_rejected_calls_launch_nothing():
                 dict(offsets=P), dict(offsets=P, groups=2, bias=P), dict(bs=8), dict(groups=-1), dict(m=1 << 31)):
         assert g(**bad) == -1, bad
     assert g(k=(1 << 17) + 1) == -2 and g(ldb=(1 << 22) + 16) == -2 and g(m=0) == 0
+    assert g(m=(1 << 31) - 1, n=1 << 20) == -3                               # more tiles than a grid has threads for
     gb = lambda **c: lib.viola_int8_gemm_gated_backward(*{**dict(a=P, lda=64, sa=P, b=P, ldb=64, bs=0, offsets=None, groups=0, m=1000, n=800, k=64, z=P, zp=1600, zt=BF16, act=0,  # noqa: E731
                                                                  dz=P), **c}.values(), None)
     for bad in (dict(act=-1), dict(act=3), dict(zp=1599), dict(n=0), dict(zt=E4M3), dict(z=None), dict(dz=None), dict(lda=48), dict(m=-1), dict(offsets=P), dict(a=P + 4)):
