@@ -1,0 +1,52 @@
+"""Corners of nn.route with a bias and groups, against the 64-bit formulas: choices equal, gates, loss and gradient within the bounds of tests/test_gpu_steered_routing.py."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import routing
+from test_gpu_steered_routing import _bias, _check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts", [8, 60, 64, 256, 700])
+@pytest.mark.parametrize("top_k", [1, 3, 6])
+def test_chosen_experts_far_below_the_largest(score, experts, top_k):
+    """A bias of -inf closes each row's likely experts; the gates are the shares of what is left, however small its scores are beside those."""
+    torch.manual_seed(experts)
+    bias = _bias(experts, score, 1e-3)
+    bias[:2] = -math.inf
+    for far in (-60.0, -100.0, -300.0):
+        logits = far + 8 * torch.randn(70, experts)
+        logits[:50, 0] = torch.randn(50)
+        logits[20:60, 1] = 1.0
+        _check(logits, top_k, bias=bias, score=score)                        # (the last rows have no likely expert)
+        _check(logits, min(top_k, experts // 2), bias=bias, score=score, groups=4, top_groups=2, group_top=2, scale=2.5)
+        coarse = (logits / 4).round() * 4                                    # ties: rows that are chosen again in 64 bits
+        _check(coarse, top_k, bias=torch.where(bias == -math.inf, bias, 0.0), score=score)
+        _check(coarse, top_k, bias=bias, score=score, mask=torch.rand(70) < 0.7)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_no_expert_left(score):
+    from viola_amd import nn
+    torch.manual_seed(1)
+    logits = torch.randn(40, 16)
+    logits[:, 3:] -= 200.0
+    bias = torch.full((16,), -math.inf)
+    r = _check(logits, 2, bias=bias, score=score)
+    assert (r.experts == -1).all() and (r.gates == 0).all()
+    bias[7] = 0.0
+    l = logits.cuda().requires_grad_()
+    r = nn.route(l, 2, bias=bias.cuda(), score=score)
+    chosen = routing.choose_steered(logits, 2, score, bias=bias)
+    assert torch.equal(r.experts.cpu().long(), chosen)
+    assert (r.experts[:, 0] == 7).all() and (r.gates[:, 0] == 1).all() and (r.gates[:, 1] == 0).all()
+    # a probability below 2^-126 is 0, which costs the loss at most that times the expert's cost, at most the 16 experts over the tokens' number, for each token of each expert
+    loss, _, _ = routing.balance(logits, chosen, score)
+    assert abs(r.balance.item() - loss.item()) <= 2.0 ** -16 * loss.item() + 16 * 16 * 2.0 ** -126
+    grad, = torch.autograd.grad(r.gates, l, torch.ones_like(r.gates))
+    assert (grad == 0).all()

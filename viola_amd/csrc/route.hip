@@ -96,6 +96,10 @@ __device__ __forceinline__ float near_sigmoid(float l) {
     return (l < 0.0f ? t : 1.0f) * r;
 }
 
+// A bias can leave a row only experts whose scores vanish beside its largest logit's. Where the chosen ones' sum (of u, or of p) is below this, their shares are of scores
+// that have the largest chosen logit for m: of the rest, what is 0 below 2^-126 is below 2^-86 of the sum.
+constexpr float VANISHING = 0x1p-40f;
+
 // VALUES logits of a lane: runs of four, LANES runs apart; -inf beyond the experts
 template <int LANES> __device__ __forceinline__ int expert_of(int i, int lane) { return ((i / 4) * LANES + lane) * 4 + i % 4; }
 
@@ -691,6 +695,27 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                             }
                         }
                     picked = lanes_sum<LANES>(picked);
+                    if constexpr (BIASED) {
+                        const bool vanishing = a.normalize && counted && !near && picked < VANISHING;
+                        if (__any(vanishing)) {
+                            uint32_t top = 0;
+                            for (int j = lane; vanishing && j < a.top_k; j += LANES) {
+                                const int e = chosen[row * a.top_k + j];
+                                const uint32_t k = e >= 0 ? key_of(mine[e]) : 0;
+                                top = k > top ? k : top;
+                            }
+                            const float highest = value_of(lanes_max<LANES>(top));
+                            float again = 0.0f;
+                            for (int j = lane; vanishing && j < a.top_k; j += LANES) {
+                                const int at = row * a.top_k + j, e = chosen[at];
+                                const float value = e >= 0 ? score<SIGMOID>(mine[e], highest) : 0.0f;
+                                values[at] = value;
+                                again += value;
+                            }
+                            again = lanes_sum<LANES>(again);
+                            picked = vanishing ? again : picked;
+                        }
+                    }
                     if (lane == 0) factors[row] = a.scale * (a.normalize ? (counted ? 1.0f / picked : 0.0f) : SIGMOID ? 1.0f : inverse);
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     __builtin_amdgcn_wave_barrier();
@@ -742,17 +767,17 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                     const char* logits = static_cast<const char*>(a.logits) + (base + row) * a.pitch * (a.dtype == VIOLA_F32 ? 4 : 2);
                     choose_exactly<SIGMOID>({logits, odd ? nullptr : a.bias, a.dtype, a.experts, a.top_k, odd ? 1 : a.groups, a.top_groups, a.group_top, m, odd,
                                              reinterpret_cast<double*>(keys), reinterpret_cast<double*>(ranks), chosen + row * a.top_k, values + row * a.top_k});
-                    float picked = 0.0f;
-                    if (of < a.top_k) {
-                        const int at = row * a.top_k + of, e = chosen[at];
-                        const float v = values[at], value = !a.normalize && SIGMOID ? sigmoid_of(v) : score<SIGMOID>(v, m);
-                        values[at] = value;
-                        if (e >= 0) {
-                            picked = value;
-                            atomicOr(&bits[e * WORDS + row / 32], 1u << (row % 32));
-                        }
+                    const int at = row * a.top_k + of, e = of < a.top_k ? chosen[at] : -1;
+                    const float v = e >= 0 ? values[at] : 0.0f;
+                    float value = e < 0 ? 0.0f : !a.normalize && SIGMOID ? sigmoid_of(v) : score<SIGMOID>(v, m);
+                    if (e >= 0) atomicOr(&bits[e * WORDS + row / 32], 1u << (row % 32));
+                    float picked = lanes_sum<64>(value);
+                    if (a.normalize && picked < VANISHING) {
+                        const float highest = value_of(lanes_max<64>(e >= 0 ? key_of(v) : 0));
+                        value = e >= 0 ? score<SIGMOID>(v, highest) : 0.0f;
+                        picked = lanes_sum<64>(value);
                     }
-                    picked = lanes_sum<64>(picked);
+                    if (e >= 0) values[at] = value;
                     if (of == 0) factors[row] = a.scale * (a.normalize ? 1.0f / picked : SIGMOID ? 1.0f : inverse);
                 }
                 __syncthreads();
@@ -957,12 +982,33 @@ template <int LANES, int VALUES, bool SIGMOID> __global__ __launch_bounds__(256)
         if (g.dgates && (a.normalize || !SIGMOID)) {
             if (a.normalize) {                                               // gate_i = scale q_i, q = p / picked: q_i (dgate_i - sum q dgate)
                 picked = lanes_sum<LANES>(picked);
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) from_gates[i] = word[i] == NOT_CHOSEN ? 0.0f : p[i];
+                const bool vanishing = counted && picked < VANISHING;
+                if (__any(vanishing)) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int i = 0; i < VALUES; ++i) {
+                        const uint32_t k = word[i] == NOT_CHOSEN ? 0 : key_of(l[i]);
+                        top = k > top ? k : top;
+                    }
+                    const float highest = value_of(lanes_max<LANES>(top));
+                    float again = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < VALUES; ++i) {
+                        const float u = word[i] == NOT_CHOSEN ? 0.0f : score<SIGMOID>(l[i], highest);
+                        from_gates[i] = vanishing ? u : from_gates[i];
+                        again += u;
+                    }
+                    again = lanes_sum<LANES>(again);
+                    picked = vanishing ? again : picked;
+                }
                 const float inverse = 1.0f / picked;
                 along = 0.0f;
 #pragma unroll
                 for (int i = 0; i < VALUES; ++i) {
                     // the quotient to its last place: of a row's only choice it is 1, whose gradient is 0 and not what rounding leaves of it
-                    const float near = p[i] * inverse, q = fmaf(fmaf(-near, picked, p[i]), inverse, near);
+                    const float near = from_gates[i] * inverse, q = fmaf(fmaf(-near, picked, from_gates[i]), inverse, near);
                     from_gates[i] = word[i] == NOT_CHOSEN ? 0.0f : q;
                     along = fmaf(from_gates[i], part(i), along);
                 }
