@@ -50,3 +50,20 @@ def test_no_expert_left(score):
     assert abs(r.balance.item() - loss.item()) <= 2.0 ** -16 * loss.item() + 16 * 16 * 2.0 ** -126
     grad, = torch.autograd.grad(r.gates, l, torch.ones_like(r.gates))
     assert (grad == 0).all()
+
+
+def test_groups_apart_by_less_than_the_smallest_normal_number():
+    """Sigmoids that 32 bits hold as 0 and biases of a few 2^-149: the order of the groups is that of 64 bits, also where the choices themselves lie far apart."""
+    tiny = 2.0 ** -149
+    _check(torch.tensor([[-99.0, -100.0, -100.0, -100.0]]), 1, bias=torch.tensor([tiny, -1.0, 2 * tiny, -1.0]), groups=2, top_groups=1)
+    _check(torch.tensor([[-100.0, -100.0, -99.0, -100.0]]), 2, bias=torch.tensor([1.0, 3 * tiny, tiny, -1.0]), groups=4, top_groups=2)
+    torch.manual_seed(2)
+    for experts, groups, group_top in ((8, 2, 1), (32, 8, 1), (64, 16, 2), (256, 8, 2), (1024, 64, 2)):
+        size = experts // groups
+        for far in (-87.5, -95.0, -102.0):
+            bias = -torch.rand(groups, size)
+            bias[:, 0] = torch.randint(0, 4, (groups,)) * tiny
+            if group_top == 2:                                               # the second of a run the same everywhere
+                bias[:, 1] = -2.0 ** -60
+                bias[:, 2:] -= 0.5
+            _check(far + torch.randn(60, experts), 1, bias=bias.reshape(-1), groups=groups, top_groups=1, group_top=group_top)

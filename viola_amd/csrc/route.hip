@@ -143,6 +143,8 @@ template <int LANES, int VALUES> __device__ __forceinline__ void load_logits(con
 // logits, as ever, and exact; ranks of single experts are too.
 template <bool SIGMOID> constexpr float NEAR = SIGMOID ? 0x1p-20f : 0x1p-19f;
 constexpr int MOST_GROUPS = 64;
+// Scores below 2^-126 (1 + 2^-16) may be 0 besides: what two of them may be off by, on either side of a comparison or both
+constexpr float FLUSHED = 0x1p-125f;
 
 __device__ __forceinline__ double over_wave(double v, int step) {
     const uint64_t b = __double_as_longlong(v);
@@ -315,7 +317,7 @@ template <int LANES, int VALUES> __device__ __forceinline__ void open_groups(con
         for (int h = 0; h < a.groups; ++h) {
             const float2 other = *reinterpret_cast<const float2*>(&ranks[2 * h]);
             before += other.x > mine.x || (other.x == mine.x && h < g);
-            close = close || (h != g && fabsf(other.x - mine.x) <= near_by * (other.y + mine.y + slack));    // of two without experts: a NaN
+            close = close || (h != g && fabsf(other.x - mine.x) <= near_by * (other.y + mine.y + slack) + 2.0f * FLUSHED);   // of two without experts: a NaN
         }
         kept[t] = before < a.top_groups ? 1.0f : 0.0f;
     }
@@ -628,7 +630,7 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                         // Keys give their last bits to say which of the lane's values they are of, are sorted within the lane, and each choice is the largest head, which its
                         // lane takes off its list. (Of 256 experts 38 operations to sort and some 35 for a choice, which otherwise takes 80.)
                         constexpr uint32_t LAST = VALUES - 1;
-                        constexpr float CUT = VALUES * 0x1p-23f, TINY = 0x1p-126f;           // of a key without its last bits, in a normal number and in a subnormal one
+                        constexpr float CUT = VALUES * 0x1p-23f;             // of a key without its last bits: of a normal number; of a subnormal one VALUES 2^-149
 #pragma unroll
                         for (int i = 0; i < VALUES; ++i) key[i] = open[i] && c[i] > -__builtin_inff() ? (key_of(c[i]) & ~LAST) | (LAST - i) : 0;
                         sort_down(key);
@@ -638,7 +640,7 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                             const uint32_t head = lanes_max<LANES>(key[0]);
                             const float v = value_of(head);
                             // (infinite biases tie: their order is the exact one's too)
-                            near = near || head >= 0xff800000u || (j && head && before - v <= (0x1p-24f + CUT) * (fabsf(before) + fabsf(v)) + 2.0f * NEAR<SIGMOID> * largest + TINY);
+                            near = near || head >= 0xff800000u || (j && head && before - v <= (0x1p-24f + CUT) * (fabsf(before) + fabsf(v)) + 2.0f * NEAR<SIGMOID> * largest + FLUSHED);
                             before = v;
                             if (j == a.top_k) break;
                             const int owner = first_lane<LANES>(__ballot(key[0] == head));       // of equal heads the row is near
