@@ -67,3 +67,20 @@ def test_groups_apart_by_less_than_the_smallest_normal_number():
                 bias[:, 1] = -2.0 ** -60
                 bias[:, 2:] -= 0.5
             _check(far + torch.randn(60, experts), 1, bias=bias.reshape(-1), groups=groups, top_groups=1, group_top=group_top)
+
+
+def test_ranks_that_only_64_bits_hold():
+    """Sums of two biases beyond the largest float: they differ, and are neither infinite nor those of closed runs."""
+    torch.manual_seed(3)
+    low = torch.finfo(torch.float32).min
+    for top_groups in (1, 2, 3):
+        bias = torch.randn(16)
+        bias[:4], bias[4:8], bias[8:12], bias[12:] = -math.inf, low, torch.tensor([low, low, low / 2, low]), low * 0.75
+        _check(torch.randn(40, 16), 3, bias=bias, groups=4, top_groups=top_groups, group_top=2)
+        bias = torch.zeros(16)
+        bias[2:4], bias[4:6], bias[8:10], bias[12:] = 2e38, 3e38, 2.5e38, math.inf
+        _check(torch.randn(40, 16), 3, bias=bias, groups=4, top_groups=top_groups, group_top=2)
+    bias = torch.zeros(12)
+    bias[2:4], bias[4:6], bias[8:10] = 2e38, 3e38, 2.5e38
+    for top_groups in (1, 2):
+        _check(torch.randn(40, 12), 3, bias=bias, groups=3, top_groups=top_groups, group_top=2)

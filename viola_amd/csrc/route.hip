@@ -282,6 +282,7 @@ template <int LANES, int VALUES> __device__ __forceinline__ void open_groups(con
     while (2 * parts * a.groups <= LANES) parts *= 2;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");                   // a row's lanes are of one wavefront, whose LDS accesses stay in order
     __builtin_amdgcn_wave_barrier();
+    bool close = false;
     for (int g0 = 0; g0 < a.groups; g0 += LANES) {
         const int g = g0 + lane / parts;
         float first = -__builtin_inff(), second = first;
@@ -298,13 +299,14 @@ template <int LANES, int VALUES> __device__ __forceinline__ void open_groups(con
         }
         if (g < a.groups && lane % parts == 0) {
             const bool both = a.group_top > 1 && second > -__builtin_inff();
-            ranks[2 * g] = both ? first + second : first;
+            const float rank = both ? first + second : first;
+            close = close || (fabsf(rank) == __builtin_inff() && fabsf(first) != __builtin_inff());      // a sum that only 64 bits hold
+            ranks[2 * g] = rank;
             ranks[2 * g + 1] = both ? fabsf(first) + fabsf(second) : fabsf(first);
         }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    bool close = false;
     constexpr int TURNS = (LANES * VALUES < MOST_GROUPS ? LANES * VALUES : MOST_GROUPS) / LANES > 1 ? (LANES * VALUES < MOST_GROUPS ? LANES * VALUES : MOST_GROUPS) / LANES : 1;
     float kept[TURNS];
 #pragma unroll
