@@ -84,3 +84,28 @@ def test_ranks_that_only_64_bits_hold():
     bias[2:4], bias[4:6], bias[8:10] = 2e38, 3e38, 2.5e38
     for top_groups in (1, 2):
         _check(torch.randn(40, 12), 3, bias=bias, groups=3, top_groups=top_groups, group_top=2)
+
+
+@pytest.mark.parametrize("group_top", [1, 2])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_groups_of_scores_that_are_one_number_in_64_bits(score, group_top):
+    """Without a bias, too, runs are ranked by scores as 64 bits hold them, ties to the lower run: sigmoids of large logits, scores of logits next to zero, scores that vanish."""
+    if group_top == 1 and score == "sigmoid":
+        _check(torch.tensor([[40.0, 1.0, 45.0, 2.0]]), 1, groups=2, top_groups=1)
+    for experts, groups in ((8, 4), (16, 4), (64, 8), (60, 6), (256, 8), (256, 64), (1024, 16)):
+        torch.manual_seed(experts)
+        size = experts // groups
+        for scale, shift in ((1.0, 500.0), (30.0, 0.0), (4.0, 24.0), (4.0, 34.0), (1.0, -90.0), (1e-20, 0.0), (1e-20, -1e-18), (300.0, 0.0), (1.0, -1000.0)):
+            logits = torch.randn(40, experts) * scale + shift
+            logits[:5, 0], logits[3:8, 1::size] = 5.0, -math.inf             # one expert far above the rest in a few rows, experts that are not there in others
+            if score == "sigmoid":
+                logits[:, 5], logits[7, 3] = 36.0, math.inf
+            _check(logits, min(3, size), groups=groups, top_groups=max(1, groups // 3), group_top=min(group_top, size), score=score)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_groups_without_a_bias_at_other_logits(dtype):
+    torch.manual_seed(4)
+    for score in ("softmax", "sigmoid"):
+        for scale in (0.5, 3.0, 8.0):
+            _check((torch.randn(200, 512) * scale).to(dtype), 8, groups=64, top_groups=8, group_top=1, score=score)

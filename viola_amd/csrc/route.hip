@@ -140,7 +140,7 @@ template <int LANES, int VALUES> __device__ __forceinline__ void load_logits(con
 //   softmax  24 2^-24 of the row's largest (the sum of at most 16 values of 64 lanes besides)
 // and the sum with its bias by 2^-24 of itself. Where two that are told apart lie nearer than NEAR times their magnitudes and the row's largest score,
 // the row is chosen again in 64 bits by the whole wavefront: about one row in 150 of 256 experts with sigmoid scores and a bias. Without a bias the choice itself is by
-// logits, as ever, and exact; ranks of single experts are too.
+// logits, as ever, and exact.
 template <bool SIGMOID> constexpr float NEAR = SIGMOID ? 0x1p-20f : 0x1p-19f;
 constexpr int MOST_GROUPS = 64;
 // Scores below 2^-126 (1 + 2^-16) may be 0 besides: what two of them may be off by, on either side of a comparison or both
@@ -273,9 +273,14 @@ template <int LANES> __device__ __forceinline__ int first_lane(uint64_t votes) {
 
 // The runs of experts that a row's choice is open to, of values v (-inf: not there) in the row's part of `keys`; `ranks`: [2 groups]. In each lane whether that of value i is;
 // near: two runs' ranks could be the other way round.
-template <int LANES, int VALUES> __device__ __forceinline__ void open_groups(const RouteArgs& a, const float (&v)[VALUES], int lane, float* keys, float* ranks, float slack,
-                                                                             float near_by, bool (&open)[VALUES], bool& near) {
+// Ranks of single scores without a bias: v are the logits, whose order is that of the scores but where two scores are one number in 64 bits (sigmoids of more than some 24 to 36,
+// logits that differ next to zero only, scores that vanish in 64 bits too); m: what a logit's score is relative to. A sigmoid's relative distance is that of the logits times
+// 1 - s, at least exp(-max(l, 0)) / 2; 64 bits tell apart what is more than 2^-46 of itself.
+template <int LANES, int VALUES, bool BIASED, bool SIGMOID> __device__ __forceinline__ void open_groups(const RouteArgs& a, const float (&v)[VALUES], int lane, float* keys,
+                                                                                                        float* ranks, float slack, float near_by, float m,
+                                                                                                        bool (&open)[VALUES], bool& near) {
     const int size = a.experts / a.groups;
+    const bool single = !BIASED && a.group_top == 1;
 #pragma unroll
     for (int i = 0; i < VALUES; i += 4) *reinterpret_cast<float4*>(&keys[expert_of<LANES>(i, lane)]) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     int parts = 1;                                                           // lanes that share a run
@@ -302,7 +307,7 @@ template <int LANES, int VALUES> __device__ __forceinline__ void open_groups(con
             const float rank = both ? first + second : first;
             close = close || (fabsf(rank) == __builtin_inff() && fabsf(first) != __builtin_inff());      // a sum that only 64 bits hold
             ranks[2 * g] = rank;
-            ranks[2 * g + 1] = both ? fabsf(first) + fabsf(second) : fabsf(first);
+            ranks[2 * g + 1] = single ? SIGMOID ? exp_of(-fmaxf(first, 0.0f)) : 1.0f : both ? fabsf(first) + fabsf(second) : fabsf(first);
         }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -319,7 +324,12 @@ template <int LANES, int VALUES> __device__ __forceinline__ void open_groups(con
         for (int h = 0; h < a.groups; ++h) {
             const float2 other = *reinterpret_cast<const float2*>(&ranks[2 * h]);
             before += other.x > mine.x || (other.x == mine.x && h < g);
-            close = close || (h != g && fabsf(other.x - mine.x) <= near_by * (other.y + mine.y + slack) + 2.0f * FLUSHED);   // of two without experts: a NaN
+            if (single) {
+                const float low = fminf(other.x, mine.x);
+                close = close || (other.x != mine.x && low > -__builtin_inff() && (!(fabsf(other.x - mine.x) * fminf(other.y, mine.y) >= 0x1p-46f) || low - m < -700.0f));
+            } else {
+                close = close || (h != g && fabsf(other.x - mine.x) <= near_by * (other.y + mine.y + slack) + 2.0f * FLUSHED); // of two without experts: a NaN
+            }
         }
         kept[t] = before < a.top_groups ? 1.0f : 0.0f;
     }
@@ -621,12 +631,12 @@ template <int LANES, int VALUES, int MODE, bool SIGMOID> __global__ __launch_bou
                     for (int i = 0; i < VALUES; ++i) {
                         c[i] = u[i] * unit + (BIASED ? bias[expert_of<LANES>(i, lane)] : 0.0f);
                         c[i] = key[i] && c[i] > -__builtin_inff() ? c[i] : -__builtin_inff();
-                        if (!BIASED && a.group_top == 1) c[i] = l[i];        // ranks of single experts, exactly
+                        if (!BIASED && a.group_top == 1) c[i] = l[i];
                         open[i] = true;
                     }
                     if (!BIASED || a.groups > 1) {
-                        open_groups<LANES, VALUES>(a, c, lane, mine, ranks + in_wave * (ranks_of<LANES, VALUES>() / (64 / LANES)), 4.0f * largest, NEAR<SIGMOID>, open, near);
-                        near = near && (BIASED || a.group_top > 1);
+                        open_groups<LANES, VALUES, BIASED, SIGMOID>(a, c, lane, mine, ranks + in_wave * (ranks_of<LANES, VALUES>() / (64 / LANES)), 4.0f * largest, NEAR<SIGMOID>,
+                                                                    SIGMOID ? 0.0f : m, open, near);
                     }
                     if constexpr (BIASED) {
                         // Keys give their last bits to say which of the lane's values they are of, are sorted within the lane, and each choice is the largest head, which its
