@@ -109,3 +109,27 @@ def test_groups_without_a_bias_at_other_logits(dtype):
     for score in ("softmax", "sigmoid"):
         for scale in (0.5, 3.0, 8.0):
             _check((torch.randn(200, 512) * scale).to(dtype), 8, groups=64, top_groups=8, group_top=1, score=score)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_groups", [(512, 64, 8), (256, 32, 5), (64, 16, 8), (1024, 64, 31)])
+@pytest.mark.parametrize("group_top", [1, 2])
+def test_many_groups_of_many_tokens(score, experts, groups, top_groups, group_top):
+    """Runs that 32 bits do not order where it matters, among many where it does not; closed runs, and runs that a lowest bias keeps for the last, in every row."""
+    from viola_amd import nn
+    torch.manual_seed(experts + group_top)
+    size = experts // groups
+    for deviation in (0.5, 3.0):
+        logits = torch.randn(8000, experts, device="cuda") * deviation
+        l = logits.double()
+        s = torch.sigmoid(l) if score == "sigmoid" else torch.softmax(l, -1)
+        bias = torch.randn(experts, device="cuda") * (0.02 if score == "sigmoid" else 0.02 / experts)
+        closed = bias.clone()
+        closed[:size], closed[3 * size:4 * size], closed[5 * size:6 * size] = -math.inf, torch.finfo(torch.float32).min, -math.inf
+        for b in (None, bias, closed):
+            c = s if b is None else s + b.double()
+            rank = c.view(-1, groups, size).topk(group_top, -1).values.sum(-1)
+            kept = torch.zeros_like(rank).scatter_(-1, torch.sort(rank, descending=True, stable=True).indices[:, :top_groups], 1.0)
+            by = torch.where(kept.repeat_interleave(size, -1) > 0, l if b is None else c, -math.inf)
+            r = nn.route(logits, 8, score=score, bias=b, groups=groups, top_groups=top_groups, group_top=group_top)
+            assert torch.equal(torch.sort(by, descending=True, stable=True).indices[:, :8].int(), r.experts)
