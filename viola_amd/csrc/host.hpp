@@ -127,7 +127,8 @@ inline void check_float(const char* name, const char* what, const Tensor& t, con
 
 // The gradients of these nodes are computed by kernels that autograd does not see.
 inline void check_once(const char* name) { TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), name, " can be differentiated once only (create_graph is not supported)"); }
-// A backward pass under capture ends the process where an eager graph of the same leaves lives (its accumulators stand on another stream), which a node cannot see: refused.
+// A backward pass under capture ends the process where an eager graph of the same leaves lives (its accumulators stand on another stream), which a node cannot see: refused, by
+// every node around a block and of 8-bit integers. (Gradients that autograd hands to leaves before it reaches the first of these nodes are out of their sight.)
 inline void check_eager(const char* name, const Tensor& t) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     TORCH_CHECK(hipStreamIsCapturing(static_cast<hipStream_t>(stream_of(t)), &status) == hipSuccess, name, " could not ask for the state of its stream");

@@ -187,6 +187,7 @@ variable_list NormBackward::apply(variable_list&& grads) {
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Device device = (d_out.defined() ? d_out : d_h).device();
     const c10::DeviceGuard guard(device);
+    check_eager("a norm around a block", d_out.defined() ? d_out : d_h);
     Tensor t[INPUTS];
     for (int i = 0; i < INPUTS; ++i) {
         if (!kept[i] || (i == X && !d_h.defined())) continue;
@@ -381,7 +382,7 @@ variable_list RouterBackward::apply(variable_list&& grads) {
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Device device = (d_gates.defined() ? d_gates : d_loss).device();
     const c10::DeviceGuard guard(device);
-    if (plan.groups) check_eager("route with a bias or groups", d_gates.defined() ? d_gates : d_loss);
+    check_eager("the router", d_gates.defined() ? d_gates : d_loss);
     const Tensor l = logits.unpack();
     TORCH_CHECK(l.device() == device && l.scalar_type() == type && l.sizes() == at::IntArrayRef(shape), "the logits of a router were moved or replaced between forward and backward");
     result[0] = room(shape, type, device);
@@ -438,6 +439,7 @@ struct DispatchBackward : public Node {
         if (!grads[0].defined() || !task_should_compute_output(0)) return result;
         at::AutoDispatchBelowADInplaceOrView below;
         const c10::DeviceGuard guard(grads[0].device());
+        check_eager("dispatch", grads[0]);
         const Tensor p = restored(positions, grads[0].device(), at::kInt, places);
         result[0] = room(shape, type, grads[0].device());
         if (result[0].numel()) gather(grads[0], p, Tensor(), result[0]);
@@ -493,6 +495,7 @@ struct CombineBackward : public Node {
         at::AutoDispatchBelowADInplaceOrView below;
         const at::Device device = grads[0].device();
         const c10::DeviceGuard guard(device);
+        check_eager("combine", grads[0]);
         const bool needs_y = task_should_compute_output(0), needs_gates = has_gates && task_should_compute_output(1);
         const Tensor p = restored(positions, device, at::kInt, places), o = restored(offsets, device, at::kInt, {experts});
         const Tensor g = has_gates && needs_y ? restored(gates, device, at::kFloat, places) : Tensor();
