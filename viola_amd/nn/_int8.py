@@ -95,7 +95,8 @@ class _Fixed(nn.Module):
     def _apply(self, fn, recurse=True):
         scale = self.weight_scale
         super()._apply(fn, recurse)
-        self.weight_scale = scale.to(self.weight_scale.device)
+        if self.weight_scale.dtype != scale.dtype:                           # cast: moved alone instead (`to_empty` off the meta device has nothing to move)
+            self.weight_scale = scale.to(self.weight_scale.device)
         if self.codes_t is None:                                             # loaded on the CPU
             self._turn()
         return self
