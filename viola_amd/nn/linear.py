@@ -240,6 +240,13 @@ def _destination(fn, tensor):
     return fn(torch.empty(0, device=tensor.device)).device
 
 
+def _moved(fn, tensor):
+    device = _destination(fn, tensor)
+    if tensor.is_meta and device.type != "meta":                               # `to_empty` (`.to()` has raised by now): memory, and no values yet
+        return torch.empty_like(tensor, device=device)
+    return tensor.to(device)
+
+
 class Linear(nn.Module):
     """y = x W^T + b computed with FP8 GEMMs on the GPU; inputs/outputs are ordinary BF16/FP16/FP32.
 
@@ -429,15 +436,17 @@ class Linear(nn.Module):
             for (owner, key), tensor in zip(slots, held):
                 owner[key] = tensor
         for (owner, key), tensor in zip(slots, held):
-            device = _destination(fn, tensor)
-            if isinstance(tensor, nn.Parameter):                               # the same Parameter object, relocated
-                tensor.data = tensor.data.to(device)
+            moved = _moved(fn, tensor.data)
+            if not isinstance(tensor, nn.Parameter):
+                owner[key] = moved
+            elif tensor.is_meta != moved.is_meta:                              # no Parameter changes between these
+                owner[key] = nn.Parameter(moved, requires_grad=tensor.requires_grad)
+            else:                                                              # the same Parameter object, relocated
+                tensor.data = moved
                 if tensor.grad is not None:
-                    tensor.grad = tensor.grad.to(device)
-            else:
-                owner[key] = tensor.to(device)
+                    tensor.grad = tensor.grad.to(moved.device)
         if self._initial_weight is not None:
-            self._initial_weight = self._initial_weight.to(_destination(fn, self._initial_weight))
+            self._initial_weight = _moved(fn, self._initial_weight)
         self._set_grad_dtype(grad_dtype)
         master = self._master()
         if self._store.pending and master is not None and master.is_cuda and self.weight.is_cuda:
