@@ -581,8 +581,8 @@ int viola_rows_scatter(const void* x, int64_t pitch, int dtype, int64_t cols, co
  * g b_stride and sb + g n (sb null: ones), and rows from offsets[groups] on are zero. k <= 2^17, groups <= 1024, ldb <= 2^22 (VIOLA_EUNSUPPORTED beyond).
  * viola_int8_gemm_gated_backward: that product dh (n its columns, without channel scales) and viola_int8_gated_backward of it in one, dz [m, 2 n] of z's type; few rows
  * and k > 2048 take the two calls (VIOLA_EUNSUPPORTED with nothing launched).
- * viola_int8_rows_linear: both for a few rows in one launch, out = the product of x's codes (of act(g) u with activation >= 0) with b; m <= 4, m k up to about 8192, k a multiple of 16, rows
- * of x and b 16-byte aligned (VIOLA_EUNSUPPORTED with nothing launched otherwise; the same bits as the two calls).
+ * viola_int8_rows_linear: both for a few rows in one launch, out = the product of x's codes (of act(g) u with activation >= 0) with b (the same bits as the two calls); m <= 4, m k up to
+ * about 8192, k a multiple of 16, ldb <= 2^22 (VIOLA_EUNSUPPORTED with nothing launched otherwise). x at any address of its type, rows of b 16-byte aligned (VIOLA_EINVAL otherwise).
  * viola_int8_gated_backward: dz [rows, 2 cols] = [dh u act'(g) | dh act(g)], contiguous, of z = [g | u] and dh float [rows, cols]; rows from *total (null: none) on are zero. */
 int64_t viola_int8_sum_parts(int64_t rows, int64_t cols);
 int viola_int8_quantize(const void* x, int64_t pitch, int dtype, int64_t rows, int64_t cols, int activation, const float* factors, const int32_t* offsets,
