@@ -540,7 +540,8 @@ int viola_norm_backward(const void* x, int64_t x_pitch, int x_dtype, const void*
  * viola_route_steered_forward: the same with a choice by c = s + bias (bias float[experts], null: none; s = p, or sigmoid(logit) for VIOLA_SIGMOID) among the experts of the
  * top_groups of `groups` equal runs of experts (at most 64) whose ranks are largest (ties to the lower run), a rank being the sum of the group_top (1 or 2) largest c of a run;
  * without a bias the choice among them is by the logits. Scores are compared as in 64 bits. An expert whose logit is -inf, or whose c is -inf or NaN, is not chosen; a row with a NaN
- * among its logits (or, for VIOLA_SOFTMAX, +inf) is chosen by the logits alone. Gates and loss are of s. workspace: viola_route_steered_workspace words; backward: viola_route_backward.
+ * among its logits (or, for VIOLA_SOFTMAX, +inf) is chosen by the logits alone. Gates and loss are of s. workspace: viola_route_steered_workspace words; backward: with a bias
+ * viola_route_steered_backward, which has the shares of experts however far below a row's largest logit.
  * viola_balance_forward: loss and counts for choices made elsewhere (int32, or int64 with chosen_wide; indices out of range count nowhere).
  * viola_route_backward: dlogits [tokens, experts], contiguous, of the logits' type from the gates' and / or the loss's gradient (null: none). */
 int64_t viola_route_workspace(int64_t tokens, int64_t experts, int64_t sequence);
@@ -558,6 +559,9 @@ int viola_balance_forward(const void* logits, int64_t pitch, int dtype, int64_t 
 int viola_route_backward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
                          int64_t sequence, const int32_t* chosen, const float* cost, const float* stats, const float* dgates, const float* dloss,
                          void* dlogits, viola_stream_t stream);
+int viola_route_steered_backward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
+                                 int64_t sequence, const int32_t* chosen, const float* cost, const float* stats, const float* dgates, const float* dloss,
+                                 void* dlogits, viola_stream_t stream);
 
 /* Rows of tokens to the experts and back (f32 / bf16 / f16, sums in f32). positions [tokens, top_k]: a row, or negative for none; no row twice.
  * viola_rows_gather: out[t] = sum_j gates[t, j] rows[positions[t, j]] (gates null: ones), out [tokens, cols] contiguous.

@@ -89,6 +89,7 @@ _SIGNATURES = {
     "viola_route_steered_forward": [_p, _l, _i, _l, _l, _i, _i, _i, _f, _p, _i, _i, _i, _p, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p, _l, _p],
     "viola_balance_forward": [_p, _l, _i, _l, _l, _i, _i, _p, _l, _p, _i, _p, _p, _p, _p, _p, _l, _p],
     "viola_route_backward": [_p, _l, _i, _l, _l, _i, _i, _i, _f, _l, _p, _p, _p, _p, _p, _p, _p],
+    "viola_route_steered_backward": [_p, _l, _i, _l, _l, _i, _i, _i, _f, _l, _p, _p, _p, _p, _p, _p, _p],
     "viola_rows_gather": [_p, _l, _l, _i, _l, _p, _p, _l, _i, _p, _p],
     "viola_rows_scatter": [_p, _l, _i, _l, _p, _p, _l, _i, _p, _p, _l, _p, _l, _p, _p],
     "viola_int8_quantize": [_p, _l, _i, _l, _l, _i, _p, _p, _l, _p, _l, _p, _p, _p],

@@ -239,7 +239,7 @@ variable_list NormBackward::apply(variable_list&& grads) {
 struct RouterPlan {
     int64_t tokens = 0, experts = 0, top_k = 0, sequence = 1;
     int score = VIOLA_SOFTMAX;
-    bool normalize = true, given = false;
+    bool normalize = true, given = false, biased = false;
     double scale = 1.0;
     int64_t groups = 0, top_groups = 1, group_top = 1;           // groups 0: the choice is by the logits alone
 };
@@ -285,6 +285,7 @@ Routed router(const char* name, const Tensor& logits, const Tensor& given, const
     if (bias.defined()) {
         check_float(name, "bias", bias, device);
         TORCH_CHECK(bias.sizes() == at::IntArrayRef({plan.experts}), name, ": bias has to be of shape [", plan.experts, "], got ", bias.sizes());
+        plan.biased = true;
         TORCH_CHECK(!bias.requires_grad(), name, ": bias steers a choice, which has no gradient: it cannot require one");
     }
     if (plan.groups) {
@@ -394,9 +395,13 @@ variable_list RouterBackward::apply(variable_list&& grads) {
     const Tensor choice = plan.given ? Tensor() : restored(chosen, device, at::kInt, choices);
     const Tensor dg = d_gates.defined() ? d_gates.contiguous() : Tensor(), dl = d_loss.defined() ? d_loss.contiguous() : Tensor();
     const Rows rows(l);
-    VIOLA_CALL(viola_route_backward, rows.data(), rows.pitch, code_of(type), plan.tokens, plan.experts, (int)plan.top_k, plan.score, plan.normalize, (float)plan.scale,
-               plan.sequence, static_cast<const int*>(ptr(choice)), base, base + stats_at / 4, static_cast<const float*>(ptr(dg)), static_cast<const float*>(ptr(dl)),
-               result[0].mutable_data_ptr(), stream_of(l));
+    const char* const call = plan.biased ? "viola_route_steered_backward" : "viola_route_backward";
+    check(call, timed(call, [&] {
+        return (plan.biased ? viola_route_steered_backward : viola_route_backward)(
+            rows.data(), rows.pitch, code_of(type), plan.tokens, plan.experts, (int)plan.top_k, plan.score, plan.normalize, (float)plan.scale, plan.sequence,
+            static_cast<const int*>(ptr(choice)), base, base + stats_at / 4, static_cast<const float*>(ptr(dg)), static_cast<const float*>(ptr(dl)),
+            result[0].mutable_data_ptr(), stream_of(l));
+    }));
     return result;
 }
 

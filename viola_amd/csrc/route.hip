@@ -935,7 +935,9 @@ struct RouteGradArgs {
 // What stands for "not chosen" among the gates' gradients in LDS: a NaN that none of them is, as theirs are made the usual one.
 constexpr uint32_t NOT_CHOSEN = 0xffffdeadu;
 
-template <int LANES, int VALUES, bool SIGMOID> __global__ __launch_bounds__(256) void route_gradient_kernel(RouteGradArgs g) {
+// FAR: the chosen experts may lie far below a row's largest logit, as a bias has it. (For all rows it takes registers and code: 32752 x 64 softmax 5.5 and 6.0 us, 32768 x 256 sigmoid
+// 25.4 and 27.6.)
+template <int LANES, int VALUES, bool SIGMOID, bool FAR> __global__ __launch_bounds__(256) void route_gradient_kernel(RouteGradArgs g) {
     constexpr int ROWS = 256 / LANES;
     __shared__ uint32_t parts[ROWS][LANES * VALUES];                         // a row's gate gradients by expert; its own lanes' only
     const RouteArgs& a = g.r;
@@ -1009,33 +1011,35 @@ template <int LANES, int VALUES, bool SIGMOID> __global__ __launch_bounds__(256)
         if (g.dgates && (a.normalize || !SIGMOID)) {
             if (a.normalize) {                                               // gate_i = scale q_i, q = p / picked: q_i (dgate_i - sum q dgate)
                 picked = lanes_sum<LANES>(picked);
+                if constexpr (FAR) {
 #pragma unroll
-                for (int i = 0; i < VALUES; ++i) from_gates[i] = word[i] == NOT_CHOSEN ? 0.0f : p[i];
-                const bool vanishing = counted && picked < VANISHING;
-                if (__any(vanishing)) {
-                    uint32_t top = 0;
+                    for (int i = 0; i < VALUES; ++i) from_gates[i] = word[i] == NOT_CHOSEN ? 0.0f : p[i];
+                    const bool vanishing = counted && picked < VANISHING;
+                    if (__any(vanishing)) {
+                        uint32_t top = 0;
 #pragma unroll
-                    for (int i = 0; i < VALUES; ++i) {
-                        const uint32_t k = word[i] == NOT_CHOSEN ? 0 : key_of(l[i]);
-                        top = k > top ? k : top;
+                        for (int i = 0; i < VALUES; ++i) {
+                            const uint32_t k = word[i] == NOT_CHOSEN ? 0 : key_of(l[i]);
+                            top = k > top ? k : top;
+                        }
+                        const float highest = value_of(lanes_max<LANES>(top));
+                        float again = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < VALUES; ++i) {
+                            const float u = word[i] == NOT_CHOSEN ? 0.0f : score<SIGMOID>(l[i], highest);
+                            from_gates[i] = vanishing ? u : from_gates[i];
+                            again += u;
+                        }
+                        again = lanes_sum<LANES>(again);
+                        picked = vanishing ? again : picked;
                     }
-                    const float highest = value_of(lanes_max<LANES>(top));
-                    float again = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < VALUES; ++i) {
-                        const float u = word[i] == NOT_CHOSEN ? 0.0f : score<SIGMOID>(l[i], highest);
-                        from_gates[i] = vanishing ? u : from_gates[i];
-                        again += u;
-                    }
-                    again = lanes_sum<LANES>(again);
-                    picked = vanishing ? again : picked;
                 }
                 const float inverse = 1.0f / picked;
                 along = 0.0f;
 #pragma unroll
                 for (int i = 0; i < VALUES; ++i) {
                     // the quotient to its last place: of a row's only choice it is 1, whose gradient is 0 and not what rounding leaves of it
-                    const float near = from_gates[i] * inverse, q = fmaf(fmaf(-near, picked, from_gates[i]), inverse, near);
+                    const float v = FAR ? from_gates[i] : p[i], near = v * inverse, q = fmaf(fmaf(-near, picked, v), inverse, near);
                     from_gates[i] = word[i] == NOT_CHOSEN ? 0.0f : q;
                     along = fmaf(from_gates[i], part(i), along);
                 }
@@ -1222,10 +1226,8 @@ extern "C" int viola_balance_forward(const void* logits, int64_t pitch, int dtyp
     return forward(a, workspace, workspace_words, stream);
 }
 
-extern "C" int viola_route_backward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
-                                    int64_t sequence, const int32_t* chosen, const float* cost, const float* stats, const float* dgates, const float* dloss,
-                                    void* dlogits, viola_stream_t stream_) {
-    hipStream_t stream = viola_enter(stream_);
+static int gradient(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale, int64_t sequence,
+                    const int32_t* chosen, const float* cost, const float* stats, const float* dgates, const float* dloss, void* dlogits, bool far, hipStream_t stream) {
     RouteGradArgs g = {};
     if (const int status = set_common(g.r, logits, pitch, dtype, tokens, experts, top_k, score, normalize, scale, nullptr, sequence)) return status;
     if (tokens == 0) return 0;
@@ -1240,8 +1242,24 @@ extern "C" int viola_route_backward(const void* logits, int64_t pitch, int dtype
         constexpr int LANES = decltype(lanes)::value, VALUES = decltype(values)::value;
         const int64_t blocks = (tokens + 256 / LANES - 1) / (256 / LANES);
         const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
-        if (g.r.sigmoid) VIOLA_LAUNCH((route_gradient_kernel<LANES, VALUES, true>), grid, 256, 0, stream, g);
-        else VIOLA_LAUNCH((route_gradient_kernel<LANES, VALUES, false>), grid, 256, 0, stream, g);
+        if (far && g.r.sigmoid) VIOLA_LAUNCH((route_gradient_kernel<LANES, VALUES, true, true>), grid, 256, 0, stream, g);
+        else if (far) VIOLA_LAUNCH((route_gradient_kernel<LANES, VALUES, false, true>), grid, 256, 0, stream, g);
+        else if (g.r.sigmoid) VIOLA_LAUNCH((route_gradient_kernel<LANES, VALUES, true, false>), grid, 256, 0, stream, g);
+        else VIOLA_LAUNCH((route_gradient_kernel<LANES, VALUES, false, false>), grid, 256, 0, stream, g);
     });
     return viola_launch_status();
+}
+
+extern "C" int viola_route_backward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
+                                    int64_t sequence, const int32_t* chosen, const float* cost, const float* stats, const float* dgates, const float* dloss,
+                                    void* dlogits, viola_stream_t stream_) {
+    hipStream_t stream = viola_enter(stream_);
+    return gradient(logits, pitch, dtype, tokens, experts, top_k, score, normalize, scale, sequence, chosen, cost, stats, dgates, dloss, dlogits, false, stream);
+}
+
+extern "C" int viola_route_steered_backward(const void* logits, int64_t pitch, int dtype, int64_t tokens, int64_t experts, int top_k, int score, int normalize, float scale,
+                                            int64_t sequence, const int32_t* chosen, const float* cost, const float* stats, const float* dgates, const float* dloss,
+                                            void* dlogits, viola_stream_t stream_) {
+    hipStream_t stream = viola_enter(stream_);
+    return gradient(logits, pitch, dtype, tokens, experts, top_k, score, normalize, scale, sequence, chosen, cost, stats, dgates, dloss, dlogits, normalize && dgates, stream);
 }
