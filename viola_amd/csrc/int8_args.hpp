@@ -20,6 +20,13 @@ struct Int8Args {
 
 constexpr int64_t INT8_MOST_K = 1 << 17, INT8_MOST_GROUPS = 1024;
 
+// A row's scale as it is applied: out = (sum * s) * sb, times lift, plus bias in one rounding. Of a row of values near the largest float sum * s would be infinite before a channel's
+// scale makes it small again, so it is taken 2^64 smaller until then; of every other row lift is 1, and the last step a sum.
+struct RowFactor {
+    float s, lift;
+    __device__ __forceinline__ explicit RowFactor(float sa) : s(sa > 0x1p60f ? sa * 0x1p-64f : sa), lift(sa > 0x1p60f ? 0x1p64f : 1.0f) {}
+};
+
 // The rows of group g of the groups' own, and of those behind the last one (g = groups). Offsets that a program made by hand are taken within the rows and in order: a
 // product must stay inside its buffers whatever they hold.
 __device__ __forceinline__ void int8_group_rows(const Int8Args& p, int g, int& from, int& to) {

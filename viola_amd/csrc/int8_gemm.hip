@@ -43,15 +43,15 @@ __device__ __forceinline__ void store_int8_tile(const i32x16 (&total)[S::TN][S::
 #pragma unroll
     for (int j = 0; j < S::TM; ++j) {
         const int64_t row0 = m_begin + (wm * S::TM + j) * 32;
-        const float sa = row0 + l32 < m_end ? p.sa[row0 + l32] : 0.0f;
+        const RowFactor row(row0 + l32 < m_end ? p.sa[row0 + l32] : 0.0f);
 #pragma unroll
         for (int i = 0; i < S::TN; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int col = (wn * S::TN + i) * 32 + q * 8 + lhi * 4;
                 const float4 sb = *reinterpret_cast<const float4*>(&columns[col]), bias = *reinterpret_cast<const float4*>(&columns[S::COLS + col]);
-                const float v[4] = {(float)total[i][j][4 * q] * sa * sb.x + bias.x, (float)total[i][j][4 * q + 1] * sa * sb.y + bias.y,
-                                    (float)total[i][j][4 * q + 2] * sa * sb.z + bias.z, (float)total[i][j][4 * q + 3] * sa * sb.w + bias.w};
+                const float v[4] = {fmaf((float)total[i][j][4 * q] * row.s * sb.x, row.lift, bias.x), fmaf((float)total[i][j][4 * q + 1] * row.s * sb.y, row.lift, bias.y),
+                                    fmaf((float)total[i][j][4 * q + 2] * row.s * sb.z, row.lift, bias.z), fmaf((float)total[i][j][4 * q + 3] * row.s * sb.w, row.lift, bias.w)};
                 Quad<TO>::store(&park[l32 * PLD + i * 32 + q * 8 + lhi * 4], v);
             }
 #pragma unroll

@@ -176,14 +176,14 @@ template <int MT, int NT, typename T> __global__ __launch_bounds__(64 * ROWS_WAV
         // lane l: row l % 16, channels 4 (l / 16) .. + 3 of the tile
         const int64_t row = m_begin + tile / NT * 16 + l16, col = n0 + tile % NT * 16 + quarter * 4;
         if (row >= m_end || col >= p.n) continue;
-        const float sa = FUSED ? scales[row] : p.sa[row];
+        const RowFactor factor(FUSED ? scales[row] : p.sa[row]);
         float out[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int64_t c = col + r < p.n ? col + r : p.n - 1;
-            out[r] = (float)v[r] * sa;
+            out[r] = (float)v[r] * factor.s;
             if (p.sb) out[r] *= p.sb[(int64_t)group * p.n + c];
-            if (p.bias) out[r] += load_float(p.bias, c, p.bias_dtype);
+            out[r] = fmaf(out[r], factor.lift, p.bias ? load_float(p.bias, c, p.bias_dtype) : -0.0f);
         }
         const int64_t at = row * p.ldo + col;
         if (p.n % 4 == 0 && p.out_dtype == VIOLA_BF16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(f32_to_bf16x2_bits(out[0], out[1]), f32_to_bf16x2_bits(out[2], out[3]));
