@@ -1,8 +1,8 @@
 // Products of 8-bit integers with a scale for each row of either operand (tokens and channels), whole or by groups of rows.
 //
 // The integers are multiplied by v_mfma_i32_32x32x32_i8, whose 32-bit sums are exact; the scales are applied to the finished sums in registers:
-// out = (sum * sa) * sb + bias, one rounding each. Bound by the matrix pipes (as many operations a cycle as FP8) and, on large products, by the power limit:
-// 16384 x 4096 -> 11008 645 to 680 us (2.2 POP/s), 4096 x 11008 -> 4096 143 (2.6), 8192 x 1024 -> 4096 46 (1.5: the results of a round of tiles leave at its end, some 9 us of 23).
+// out = (sum * sa) * sb + bias, one rounding each. Bound by the matrix pipes (as many operations a cycle as FP8; why the first of these takes longer than the same tiles on FP8, 509 us,
+// has not been found): 16384 x 4096 -> 11008 645 to 690 us (2.2 POP/s), 4096 x 11008 -> 4096 143 (2.6), 8192 x 1024 -> 4096 46 (1.5: the results of a round of tiles leave at its end, some 9 us of 23).
 //
 // The tiles are those of gemm_pingpong.hpp: eight wavefronts, two on each SIMD, whose memory work and math alternate; a chunk of 128 k is two pairs of
 // instructions for each 32 x 32 sub-tile where FP8 has one of 64 k, and an operand's 16-byte pieces are in the instruction's own order.

@@ -23,7 +23,7 @@
 // out), and the vector units are busy 70 % of the time. 32768 tokens to eight of 128 experts: choosing 18 us (its logits and results are 4 us of traffic), places and
 // loss 9, gradient 11; two of 16 experts chosen elsewhere, 16384 tokens: 6, 5 and 3.4. Measured and left out, as neither was faster: a lane's logits sorted
 // first (rank and expert as one double), a lane's largest found together with its index. 32 tokens, one block: 8.6 us, of which 4 are any
-// launch, 1.6 the eight choices. Steered, eight of 256 from four of eight groups with a bias: 32768 tokens 61 us, places 15, gradient 26; 32 tokens 12 to 15 and 4.
+// launch, 1.6 the eight choices. Steered, eight of 256 from four of eight groups with a bias: 32768 tokens 60 us, places 15, gradient 27; 32 tokens 12 to 15 and 4.
 #include "block_ops.hpp"
 
 #include <type_traits>
@@ -139,7 +139,7 @@ template <int LANES, int VALUES> __device__ __forceinline__ void load_logits(con
 //            |l - m| 2^-24 u or at most a third of 2^-24 of the largest; the factor exp(min(m, 0)) 4 2^-24 where it is not one; their product)
 //   softmax  24 2^-24 of the row's largest (the sum of at most 16 values of 64 lanes besides)
 // and the sum with its bias by 2^-24 of itself. Where two that are told apart lie nearer than NEAR times their magnitudes and the row's largest score,
-// the row is chosen again in 64 bits by the whole wavefront: about one row in 150 of 256 experts with sigmoid scores and a bias. Without a bias the choice itself is by
+// the row is chosen again in 64 bits by the whole wavefront: two in 1000 of 256 experts with sigmoid scores (logits of deviation 1.3) and a bias. Without a bias the choice itself is by
 // logits, as ever, and exact.
 template <bool SIGMOID> constexpr float NEAR = SIGMOID ? 0x1p-20f : 0x1p-19f;
 constexpr int MOST_GROUPS = 64;
@@ -272,8 +272,8 @@ template <int LANES> __device__ __forceinline__ int first_lane(uint64_t votes) {
 }
 
 // The runs of experts that a row's choice is open to, of values v (-inf: not there) in the row's part of `keys`; `ranks`: [2 groups]. In each lane whether that of value i is;
-// near: a run that is kept and one that is not could be the other way round. (Any two instead: 29 % of the rows of 512 experts in 64 runs, logits of deviation 2, and every row with
-// a run whose experts are all closed; so less than 0.1 %.) What a rank may be off by is on either side of it: least is that of the kept ones, most that of the others.
+// near: a run that is kept and one that is not could be the other way round. (Any two instead: 22 % of the rows of 512 experts in 64 runs, softmax of logits of deviation 2, and every
+// row with a run whose experts are all closed; so 0.02 %.) What a rank may be off by is on either side of it: least is that of the kept ones, most that of the others.
 // Ranks of single scores without a bias: v are the logits, whose order is that of the scores but where two scores are one number in 64 bits (sigmoids of more than some 24 to 36,
 // logits that differ next to zero only, scores that vanish in 64 bits too); m: what a logit's score is relative to. A sigmoid's relative distance is that of the logits times
 // 1 - s, at least exp(-max(l, 0)) / 2; 64 bits tell apart what is more than 2^-46 of itself.
