@@ -6,7 +6,8 @@ The sum over the features is exact, the scales are applied in 32 bits, and the r
 of a gated block gives, and act(g) * u is quantized (gelu is its tanh form, as in `MLP`).
 
 Gradients flow to x and bias as if rounding to integers were the identity, and the gradient is a product of the same kind: dx = (q' @ weight) * s' with
-q', s' = quantize_int8(dy * weight_scale). So adapters, norms and routers beside fixed layers can be trained through them. The reference has no such operators.
+q', s' = quantize_int8(dy * weight_scale). So adapters, norms and routers beside fixed layers can be trained through them. A forward pass can be
+captured into a graph, a backward pass raises there. The reference has no such operators.
 
     up, down = nn.Int8Experts.from_float(fp8_up), nn.Int8Experts.from_float(fp8_down, activation="silu")
     routing = nn.route(logits, 8, score="sigmoid", bias=bias, groups=8, top_groups=4, group_top=2)

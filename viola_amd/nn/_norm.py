@@ -5,8 +5,8 @@
     h   = (n(out) * weight + bias) * (1 + scale) + shift
 
 n divides a row by its root mean square ("rms"), or subtracts its mean first ("layer"). x is the residual stream, y a block's result, h what
-the next block reads. Sums and statistics are in 32 bits whatever the types; h is computed from `out` before that is rounded. The reference
-has no such operator.
+the next block reads. Sums and statistics are in 32 bits whatever the types; h is computed from `out` before that is rounded. A
+forward pass can be captured into a graph, a backward pass raises there. The reference has no such operator.
 """
 
 from .. import _lib

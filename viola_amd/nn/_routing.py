@@ -1,6 +1,6 @@
 """Routing of a mixture of experts, beside the variable-group linear that the experts run on: the router's choice with its gates, places,
 counts and balance loss (`route`), that loss for choices made elsewhere (`balance_loss`), and the rows' way to the experts and back
-(`dispatch`, `combine`). The reference has no such operators.
+(`dispatch`, `combine`). A forward pass can be captured into a graph, a backward pass raises there. The reference has no such operators.
 
     routing = nn.route(logits, 2)                                   # logits [tokens, experts]
     counts = routing.counts.tolist()                                # grouped_linear takes them on the host
